@@ -475,6 +475,106 @@ SH_API int sh_attn_decode_f16_noalloc(sh_ctx *ctx, const float *q, const uint16_
                                       int batch, int heads, int kv_heads, int head_dim,
                                       int max_positions, float scale);
 
+/* ---- typed ops: a KV cache in pages, and sampling -------------------------------
+ * No reference counterpart: what a server of many sequences needs around a
+ * decoder's layers. Only device memory that the caller passes is used (work
+ * buffers too), nothing is allocated and nothing waited for, so every call can
+ * be captured into a graph; a captured call keeps its work buffer, which no
+ * other call may use at the same time. */
+
+/* The cache of a batch of sequences, in pages of a pool that they share.
+ * Position p of sequence b lies in page page_table[b * max_pages + p / page_size],
+ * row p % page_size. In this call sequence b has n = starts[b + 1] - starts[b]
+ * new tokens, in rows starts[b] .. starts[b + 1] - 1 of the call's tensors, and
+ * lengths[b] positions with them: new token i is at position lengths[b] - n + i.
+ * Rows from starts[batch] on belong to no sequence and are left as they are.
+ * Everything the pointers name is in device memory, so that a captured call
+ * replays with other contents. Values outside their ranges do no harm: starts
+ * are taken within 0 .. tokens and ascending, lengths within 0 .. max_pages *
+ * page_size; a position whose table entry is no page (not 0 .. num_pages - 1)
+ * is seen by no token and not stored. page_size: a power of two, 16..65536. */
+typedef struct sh_paged_kv {
+  uint16_t *k, *v; /* [num_pages][kv_heads][page_size][head_dim], 16-byte aligned */
+  const int32_t *page_table; /* [batch][max_pages] */
+  const int32_t *lengths;    /* [batch] */
+  const int32_t *starts;     /* [batch + 1] */
+  int batch, max_pages, num_pages, page_size, kv_heads, head_dim;
+} sh_paged_kv;
+
+/* A linear's rows qkv[token] = q (heads) | k (kv_heads) | v (kv_heads), head_dim
+ * values each, rows ld >= (heads + 2 kv_heads) * head_dim values apart: q and k
+ * normalised per head, x / sqrt(mean(x^2) + eps) * gain (gains fp32, head_dim
+ * values), then rotated by halves at the token's position, angle = position *
+ * theta^(-2i / head_dim) in fp64; q to q[tokens][heads][head_dim], k and v (as
+ * it is) to their pages. fp16 or bf16, rounded once. A token before position 0
+ * is rotated by its negative position and not stored. head_dim 64 or 128; qkv
+ * and q 16-byte aligned, ld a multiple of 8; q must not overlap qkv. Two tokens
+ * of one page row (a page in two tables) leave either's values. */
+SH_API int sh_qk_norm_rope_paged_f16(sh_ctx *ctx, const sh_paged_kv *kv, const uint16_t *qkv,
+                                     const float *q_gain, const float *k_gain, uint16_t *q,
+                                     int tokens, int heads, int ld, float eps, float theta);
+SH_API int sh_qk_norm_rope_paged_bf16(sh_ctx *ctx, const sh_paged_kv *kv, const uint16_t *qkv,
+                                      const float *q_gain, const float *k_gain, uint16_t *q,
+                                      int tokens, int heads, int ld, float eps, float theta);
+
+/* Attention of the new tokens over their sequences' pages (which hold the new
+ * tokens' k and v already), grouped-query: for the token at position pos and
+ * query head h, KV head h / (heads / kv_heads),
+ *   out = sum_p softmax_p(scale q . k[p]) v[p]
+ * over p <= pos, with window > 0 only those with p > pos - window or p < sinks
+ * (window 0: all). A row that sees nothing gets zeros; what stands in places
+ * that a row does not see, NaN and infinities included, does not reach it; a
+ * score of -infinity has no weight. q, out [tokens][heads][head_dim] in the
+ * cache's type, 16-byte aligned, not overlapping; fp32 scores, softmax and sums,
+ * the weights rounded to the type for the product with v. head_dim 64 or 128,
+ * heads / kv_heads <= 128, scale > 0. max_new: the most new tokens of any sequence;
+ * the kernel and the work buffer are chosen by it, more are computed as well. The
+ * work buffer (16-byte aligned) holds at least what sh_attn_paged_workspace
+ * says for the same sizes. */
+SH_API int sh_attn_paged_workspace(const sh_paged_kv *kv, int tokens, int heads, int max_new,
+                                   size_t *bytes);
+SH_API int sh_attn_paged_f16(sh_ctx *ctx, const sh_paged_kv *kv, const uint16_t *q, uint16_t *out,
+                             int tokens, int heads, int max_new, int window, int sinks,
+                             float scale, void *workspace, size_t workspace_bytes);
+SH_API int sh_attn_paged_bf16(sh_ctx *ctx, const sh_paged_kv *kv, const uint16_t *q, uint16_t *out,
+                              int tokens, int heads, int max_new, int window, int sinks,
+                              float scale, void *workspace, size_t workspace_bytes);
+
+/* Pages src[i] to pages dst[i], i < count, in each of `planes` pools (the K and V
+ * pools of every layer) at pool + p * plane_stride bytes, num_pages pages of
+ * page_bytes each. src and dst are device int32; a pair with a number outside
+ * 0 .. num_pages - 1 is skipped. A page may be the source of several; the dst
+ * pages are distinct and none of them a source of another. pool 16-byte aligned,
+ * page_bytes and plane_stride multiples of 16, plane_stride >= num_pages *
+ * page_bytes. */
+SH_API int sh_pages_copy(sh_ctx *ctx, void *pool, int planes, size_t plane_stride, int num_pages,
+                         size_t page_bytes, const int32_t *src, const int32_t *dst, int count);
+
+/* index[r] = a token drawn from the logits x[r][0 .. n - 1] (rows ld values
+ * apart) with the uniform number u[r]:
+ *   the tokens by x, descending (equal values: the smaller index first);
+ *   the first top_k[r] of them (0 or less: all);
+ *   weights w = exp((x - max) / temperature[r]);
+ *   each while the weights before it sum to less than top_p[r] of all (at least
+ *   one token; top_p >= 1 or NaN: all);
+ *   those with w >= min_p[r] (0 or less, or NaN: all; above 1: as 1);
+ *   then, by index, the first whose weights up to it sum to more than u[r] times
+ *   the sum.
+ * temperature 0 (or less, or NaN) is greedy: the first of the largest. The other
+ * parameters are device arrays of one value per row, top_k int32, the rest fp32;
+ * NULL: temperature 1, all tokens; u is needed, taken within 0 .. 1. NaN and
+ * -infinity are never drawn (+infinity shares the weight among its like); a row
+ * of nothing else gives -1. Weights are 42-bit fractions of the largest, from
+ * fp64 exponentials, and their sums exact: a token below 2^-43 of the likeliest
+ * is not drawn, and results do not depend on any order. n <= 2^20, rows <= 2^16.
+ * The work buffer (16-byte aligned) holds at least what
+ * sh_sample_workspace says for the same sizes. */
+SH_API int sh_sample_workspace(int rows, int n, size_t *bytes);
+SH_API int sh_sample_f32(sh_ctx *ctx, const float *x, int rows, int n, int ld,
+                         const float *temperature, const int32_t *top_k, const float *top_p,
+                         const float *min_p, const float *u, int32_t *index, void *workspace,
+                         size_t workspace_bytes);
+
 /* ---- LLM decode (model runners) ------------------------------------------------
  * No reference counterpart. The models: GPT-2 (measured as GPT-2 small, fp16
  * weights) and Qwen3 (the 0.6B shape, FP8-E4M3 weights with per-output-channel

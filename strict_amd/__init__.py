@@ -32,7 +32,7 @@ from ._lib import (SH_ERR_COMPILE, SH_ERR_INVALID_ARGUMENT, SH_ERR_NO_DEVICE, SH
 
 __all__ = [
     "StrictHipError", "CompileError", "Context", "DeviceVariable", "RuntimeCompiler",
-    "KernelFunction", "Module", "Kernel", "device_count", "SAXPY_SOURCE",
+    "KernelFunction", "Module", "Kernel", "device_count", "SAXPY_SOURCE", "PagedKV",
     "ADD", "SUBTRACT", "MULTIPLY", "DIVIDE", "BLUR_CONFIG", "BLUR_REFERENCE",
     "BRIGHTNESS_ALL_CHANNELS",
 ]
@@ -140,6 +140,24 @@ class DeviceVariable:
 
     def __exit__(self, *exc):
         self.free()
+
+
+class PagedKV:
+    """A batch's KV cache in pages (sh_paged_kv): k, v [num_pages, kv_heads,
+    page_size, head_dim] of dtype "f16" or "bf16" (16-bit patterns), page table
+    [batch, max_pages], lengths [batch] (new tokens included) and starts
+    [batch + 1] (rows of the new tokens), all int32 on the device."""
+
+    def __init__(self, k, v, page_table, lengths, starts, *, batch: int, max_pages: int,
+                 num_pages: int, page_size: int, kv_heads: int, head_dim: int, dtype: str = "f16"):
+        if dtype not in ("f16", "bf16"):
+            raise ValueError(f"dtype {dtype!r}: 'f16' or 'bf16'")
+        self.dtype = dtype
+        self.kv_heads, self.head_dim = kv_heads, head_dim
+        self.buffers = (k, v, page_table, lengths, starts)  # kept alive with the struct
+        self.struct = _lib.PagedKv(*(_ptr(b) for b in self.buffers), batch, max_pages, num_pages,
+                                   page_size, kv_heads, head_dim)
+        self.address = ctypes.byref(self.struct)
 
 
 class RuntimeCompiler:
@@ -463,6 +481,53 @@ class Context:
         _check(self._l.sh_attn_decode_f16_noalloc(self.handle, _ptr(q), _ptr(k), _ptr(v),
                                                   _ptr(lengths), _ptr(out), batch, heads,
                                                   kv_heads, head_dim, max_positions, scale))
+
+
+    # -- a KV cache in pages, and sampling --
+    def qk_norm_rope_paged(self, kv: PagedKV, qkv, q_gain, k_gain, q, tokens: int, heads: int,
+                           eps: float, theta: float, ld: int | None = None) -> None:
+        """Rows q | k | v of a linear: q and k normalised per head and rotated at the
+        tokens' positions, q to q [tokens, heads, d], k and v to their pages."""
+        f = (self._l.sh_qk_norm_rope_paged_f16 if kv.dtype == "f16"
+             else self._l.sh_qk_norm_rope_paged_bf16)
+        _check(f(self.handle, kv.address, _ptr(qkv), _ptr(q_gain), _ptr(k_gain), _ptr(q), tokens,
+                 heads, (heads + 2 * kv.kv_heads) * kv.head_dim if ld is None else ld, eps, theta))
+
+    def attn_paged_workspace(self, kv: PagedKV, tokens: int, heads: int, max_new: int) -> int:
+        """Bytes of the work buffer attn_paged takes at these sizes."""
+        n = ctypes.c_size_t(0)
+        _check(self._l.sh_attn_paged_workspace(kv.address, tokens, heads, max_new, ctypes.byref(n)))
+        return n.value
+
+    def attn_paged(self, kv: PagedKV, q, out, tokens: int, heads: int, max_new: int, scale: float,
+                   workspace: DeviceVariable, window: int = 0, sinks: int = 0) -> None:
+        """Attention of the new tokens (q, out [tokens, heads, d] in the cache's type)
+        over their sequences' pages, causal; window > 0: over the last `window`
+        positions and the first `sinks`. max_new: the most new tokens of a sequence."""
+        f = self._l.sh_attn_paged_f16 if kv.dtype == "f16" else self._l.sh_attn_paged_bf16
+        _check(f(self.handle, kv.address, _ptr(q), _ptr(out), tokens, heads, max_new, window, sinks,
+                 scale, _ptr(workspace), workspace.nbytes))
+
+    def pages_copy(self, pool, planes: int, num_pages: int, page_bytes: int, src, dst, count: int,
+                   plane_stride: int | None = None) -> None:
+        """Pages src[i] to dst[i] (device int32) in each of `planes` pools."""
+        _check(self._l.sh_pages_copy(self.handle, _ptr(pool), planes,
+                                     num_pages * page_bytes if plane_stride is None else plane_stride,
+                                     num_pages, page_bytes, _ptr(src), _ptr(dst), count))
+
+    def sample_workspace(self, rows: int, n: int) -> int:
+        """Bytes of the work buffer sample takes at these sizes."""
+        size = ctypes.c_size_t(0)
+        _check(self._l.sh_sample_workspace(rows, n, ctypes.byref(size)))
+        return size.value
+
+    def sample(self, logits, rows: int, n: int, temperature, top_k, top_p, min_p, u, index,
+               workspace: DeviceVariable, ld: int | None = None) -> None:
+        """index[r] = a token drawn from logits [rows, n] (rows ld apart) by each row's
+        temperature, top-k, top-p, min-p (device arrays or None) and uniform number u."""
+        _check(self._l.sh_sample_f32(self.handle, _ptr(logits), rows, n, n if ld is None else ld,
+                                     _ptr(temperature), _ptr(top_k), _ptr(top_p), _ptr(min_p),
+                                     _ptr(u), _ptr(index), _ptr(workspace), workspace.nbytes))
 
 
 class Event:

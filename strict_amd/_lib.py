@@ -92,6 +92,23 @@ class LlmConfig(ctypes.Structure):
     ]
 
 
+class PagedKv(ctypes.Structure):
+    """sh_paged_kv: a batch's KV cache in pages."""
+    _fields_ = [
+        ("k", ctypes.c_void_p),
+        ("v", ctypes.c_void_p),
+        ("page_table", ctypes.c_void_p),
+        ("lengths", ctypes.c_void_p),
+        ("starts", ctypes.c_void_p),
+        ("batch", ctypes.c_int),
+        ("max_pages", ctypes.c_int),
+        ("num_pages", ctypes.c_int),
+        ("page_size", ctypes.c_int),
+        ("kv_heads", ctypes.c_int),
+        ("head_dim", ctypes.c_int),
+    ]
+
+
 _P = ctypes.c_void_p
 _PP = ctypes.POINTER(ctypes.c_void_p)
 _I = ctypes.c_int
@@ -178,6 +195,14 @@ SIGNATURES = {
     "sh_argmax_f32": (_I, [_P, _P, _I, _I, _P]),
     "sh_attn_decode_f16": (_I, [_P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _F]),
     "sh_attn_decode_f16_noalloc": (_I, [_P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _F]),
+    "sh_qk_norm_rope_paged_f16": (_I, [_P, _P, _P, _P, _P, _P, _I, _I, _I, _F, _F]),
+    "sh_qk_norm_rope_paged_bf16": (_I, [_P, _P, _P, _P, _P, _P, _I, _I, _I, _F, _F]),
+    "sh_attn_paged_workspace": (_I, [_P, _I, _I, _I, ctypes.POINTER(_SZ)]),
+    "sh_attn_paged_f16": (_I, [_P, _P, _P, _P, _I, _I, _I, _I, _I, _F, _P, _SZ]),
+    "sh_attn_paged_bf16": (_I, [_P, _P, _P, _P, _I, _I, _I, _I, _I, _F, _P, _SZ]),
+    "sh_pages_copy": (_I, [_P, _P, _I, _SZ, _I, _SZ, _P, _P, _I]),
+    "sh_sample_workspace": (_I, [_I, _I, ctypes.POINTER(_SZ)]),
+    "sh_sample_f32": (_I, [_P, _P, _I, _I, _I, _P, _P, _P, _P, _P, _P, _P, _SZ]),
     "sh_llm_create": (_I, [_P, ctypes.POINTER(LlmConfig), _PP]),
     "sh_llm_destroy": (_I, [_P]),
     "sh_llm_init_random": (_I, [_P, ctypes.c_uint64, _F]),

@@ -1,0 +1,70 @@
+// Device helpers of the operators over a KV cache in pages (paged_ops.hip,
+// paged_attn.hip): the two 16-bit types and their conversions, and the pointer
+// checks that both files' entry points share.
+#pragma once
+
+#include <hip/hip_runtime.h>
+
+#include "common.h"
+#include "paged.h"
+
+namespace sh {
+
+typedef _Float16 pf16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 pbf16x8 __attribute__((ext_vector_type(8)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+
+// (bf16's range is fp32's, so its weights need no scale; fp16 weights are kept
+// 2^14 times as large, which leaves those down to 2^-28 normal.)
+struct PagedF16 {
+  typedef _Float16 Value;
+  typedef pf16x8 Vec;
+  static constexpr float kWeightLog2 = 14.0f;
+  static __device__ __forceinline__ f32x4 mfma16(Vec a, Vec b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+  }
+  static __device__ __forceinline__ f32x16 mfma32(Vec a, Vec b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+  }
+};
+struct PagedBf16 {
+  typedef __bf16 Value;
+  typedef pbf16x8 Vec;
+  static constexpr float kWeightLog2 = 0.0f;
+  static __device__ __forceinline__ f32x4 mfma16(Vec a, Vec b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+  }
+  static __device__ __forceinline__ f32x16 mfma32(Vec a, Vec b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+  }
+};
+
+template <class T>
+__device__ __forceinline__ void unpack8(u32x4 bits, float (&x)[8]) {
+  const typename T::Vec v = __builtin_bit_cast(typename T::Vec, bits);
+#pragma unroll
+  for (int e = 0; e < 8; e++) x[e] = (float)v[e];
+}
+
+template <class T>
+__device__ __forceinline__ u32x4 pack8(const float (&x)[8]) {
+  typename T::Vec v;
+#pragma unroll
+  for (int e = 0; e < 8; e++) v[e] = (typename T::Value)x[e];
+  return __builtin_bit_cast(u32x4, v);
+}
+
+inline int check_paged_pointers(sh_ctx *ctx, const sh_paged_kv *kv) {
+  int rc;
+  const size_t pool = paged_pool_bytes(kv);
+  if ((rc = check_range(ctx, kv->k, pool, "k pages")) || (rc = check_range(ctx, kv->v, pool, "v pages")) ||
+      (rc = check_range(ctx, kv->page_table, (size_t)kv->batch * kv->max_pages * 4, "page_table")) ||
+      (rc = check_range(ctx, kv->lengths, (size_t)kv->batch * 4, "lengths")) ||
+      (rc = check_range(ctx, kv->starts, ((size_t)kv->batch + 1) * 4, "starts")))
+    return rc;
+  if ((reinterpret_cast<uintptr_t>(kv->k) | reinterpret_cast<uintptr_t>(kv->v)) & 15)
+    return fail(SH_ERR_INVALID_ARGUMENT, "k and v pages must be 16-byte aligned");
+  return SH_OK;
+}
+
+}  // namespace sh

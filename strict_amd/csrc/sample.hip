@@ -1,0 +1,804 @@
+// One token per row of logits by temperature, top-k, top-p and min-p
+// (sh_sample_f32; the definition is in strict_hip.h).
+//
+// A token's weight is exp(-y), y = (max - x) / temperature, as a whole number of
+// 2^-42: sums of weights are then exact in 64 bits (at most 2^20 tokens), in any
+// order, and atomics in any order give the same. The order of the tokens is that
+// of 64-bit keys: the value's order above, the complement of the index below.
+//
+// Rows of up to 2,048 logits: one kernel, one workgroup a row. Longer ones in four
+// kernels over (row, split):
+//   max     the splits' largest values; clears the row's histogram
+//   bins    count and weight of the tokens by y in bins of 1/64 (rows with top-k
+//           or top-p only)
+//   gather  from the bins, the bin where top-k (without it, top-p) ends. Up to
+//           2,048 tokens to that bin's end: all of them to a list, from which the
+//           rest is decided. More: only that bin's tokens, and each split's weight
+//           of the kept tokens before them. Without top-k and top-p: each split's
+//           weight of all
+//   draw    a workgroup a row: sorts the list, ends the selection within it, finds
+//           the split, in it the 256 tokens and among them the token that u falls on
+// A list that would not hold the bin's tokens, or top-p after a top-k of more than
+// the list holds: the draw kernel finds the last kept key by its digits, reading
+// the row once per digit.
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+#include <cmath>
+
+#include "common.h"
+#include "sample.h"
+
+namespace sh {
+namespace {
+
+constexpr int kT = 512;
+constexpr int kBins = 2048, kBinsPerUnit = 64;
+constexpr int kList = 2048;
+constexpr int kFraction = 42;       // bits of a weight
+constexpr double kCutoff = 29.9;    // exp(-y) 2^42 is below 1/2 from y = 29.81 on
+constexpr int kSegment = 256;       // tokens that a wave takes at once
+constexpr int kMaxSegments = kMaxSampleN / kSegment;
+constexpr int kMaxSplits = 64;
+
+enum { kAll = 0, kListed = 1, kBinned = 2, kDigits = 3 };
+
+// A row's state between the kernels, in the work buffer.
+struct RowState {
+  unsigned long long mass[kBins];  // weights of the bin's tokens
+  unsigned int count[kBins];
+  unsigned long long list[kList];  // keys
+  unsigned long long split_mass[kMaxSplits];
+  float split_max[kMaxSplits];
+  unsigned int listed;
+  int mode, bin;                   // bin: where the list ends (kAll: past all bins)
+  unsigned int before_count;       // of the tokens in the bins before `bin`
+  unsigned long long before_mass;
+  unsigned long long limit;        // top-p's, 0: none (or, with top-k, not known yet)
+  int k;                           // top-k's, 0: none
+};
+
+struct SampleArgs {
+  const float *x, *temperature, *top_p, *min_p, *u;
+  const int *top_k;
+  int *index;
+  RowState *rows;
+  int n, ld, splits, chunk;
+  double table[64];  // 2^(-j / 64)
+};
+
+struct RowParams {
+  float m;          // largest logit
+  double inv_t;
+  bool greedy;
+  int k;            // 0: all
+  double p, least;  // p >= 1: all; least <= 0: all
+};
+
+__device__ __forceinline__ RowParams row_params(const SampleArgs &a, int row, float m) {
+  RowParams r;
+  const float t = a.temperature ? a.temperature[row] : 1.0f;
+  const int k = a.top_k ? a.top_k[row] : 0;
+  const float p = a.top_p ? a.top_p[row] : 1.0f, least = a.min_p ? a.min_p[row] : 0.0f;
+  r.m = m;
+  r.greedy = !(t > 0.0f) || k == 1;
+  r.inv_t = 1.0 / (double)t;
+  r.k = k > 0 && k < a.n ? k : 0;
+  r.p = p < 1.0f ? (double)p : 1.0;
+  r.least = least > 0.0f ? (double)fminf(least, 1.0f) : 0.0;
+  return r;
+}
+
+// y of a logit (NaN for one that is NaN).
+__device__ __forceinline__ double exponent(const RowParams &r, float x) {
+  return x == r.m ? 0.0 : ((double)r.m - (double)x) * r.inv_t;
+}
+
+// exp(-y), 0 <= y < kCutoff: y = (n + f) ln(2) / 64, the table's 2^(-(n % 64) / 64)
+// and a polynomial of f's part, |f ln(2) / 64| <= 0.0055 (next term 4e-17).
+__device__ __forceinline__ double exp_minus(double y, const double *table) {
+  const double n = rint(y * 92.332482616893656877);
+  double f = fma(n, -1.08304246962491454596e-2, y);  // ln(2) / 64 to 2^-54 of it
+  f = fma(n, -3.62351064663484314921e-19, f);
+  double e = fma(f, -1.0 / 120.0, 1.0 / 24.0);
+  e = fma(f, e, -1.0 / 6.0);
+  e = fma(f, e, 0.5);
+  e = fma(f, e, -1.0);
+  e = fma(f, e, 1.0);
+  const int i = (int)n;
+  return ldexp(e * table[i & 63], -(i >> 6));
+}
+
+// The weight; *e gets exp(-y). 0: never drawn.
+__device__ __forceinline__ unsigned long long weight(double y, const double *table, double *e) {
+  *e = exp_minus(y, table);
+  // 2^52 + w has w in its low bits, rounded to the nearest
+  const double w = fma(*e, (double)(1LL << kFraction), 4503599627370496.0);
+  return __builtin_bit_cast(unsigned long long, w) & ((1ULL << 52) - 1);
+}
+
+__device__ __forceinline__ int bin_of(double y) { return (int)(y * kBinsPerUnit); }
+
+// Order of (value, index), descending; -0 as +0. 0 is no token's key (the value
+// of key 0 would be a NaN).
+__device__ __forceinline__ unsigned long long key_of(float x, int i) {
+  uint32_t u = __builtin_bit_cast(uint32_t, x + 0.0f);
+  u = (u & 0x80000000u) ? ~u : (u | 0x80000000u);
+  return ((unsigned long long)u << 32) | (uint32_t)~i;
+}
+__device__ __forceinline__ int key_index(unsigned long long key) { return (int)~(uint32_t)key; }
+__device__ __forceinline__ float key_value(unsigned long long key) {
+  const uint32_t u = (uint32_t)(key >> 32);
+  return __builtin_bit_cast(float, (u & 0x80000000u) ? (u & 0x7fffffffu) : ~u);
+}
+
+typedef float f32x4_any __attribute__((ext_vector_type(4), aligned(4)));
+
+// Logits i .. i + 3 of a row (-infinity from `end` on).
+__device__ __forceinline__ f32x4 load4(const float *x, int i, int end) {
+  if (i + 4 <= end) return *reinterpret_cast<const f32x4_any *>(x + i);
+  f32x4 v;
+#pragma unroll
+  for (int e = 0; e < 4; e++) v[e] = i + e < end ? x[i + e] : -INFINITY;
+  return v;
+}
+
+__device__ __forceinline__ unsigned long long wave_sum_u64(unsigned long long v) {
+#pragma unroll
+  for (int off = 32; off >= 1; off >>= 1) v += __shfl_xor(v, off, 64);
+  return v;
+}
+
+__device__ __forceinline__ unsigned long long wave_scan_u64(unsigned long long v) {
+#pragma unroll
+  for (int off = 1; off < 64; off *= 2) {
+    const unsigned long long o = __shfl_up(v, off, 64);
+    if ((int)(threadIdx.x & 63) >= off) v += o;
+  }
+  return v;
+}
+
+// Inclusive sum over the workgroup's threads; *total: of all.
+__device__ __forceinline__ unsigned long long block_scan_u64(unsigned long long v, unsigned long long *red,
+                                                             unsigned long long *total) {
+  const int wave = threadIdx.x >> 6;
+  v = wave_scan_u64(v);
+  __syncthreads();  // red's earlier readers are done
+  if ((threadIdx.x & 63) == 63) red[wave] = v;
+  __syncthreads();
+  unsigned long long sum = 0;
+#pragma unroll
+  for (int w = 0; w < kT / 64; w++) {
+    if (w == wave) v += sum;
+    sum += red[w];
+  }
+  *total = sum;
+  return v;
+}
+
+__device__ __forceinline__ float block_max(float v, float *red) {
+#pragma unroll
+  for (int off = 32; off >= 1; off >>= 1) v = fmaxf(v, __shfl_xor(v, off, 64));
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+  __syncthreads();
+  v = red[0];
+#pragma unroll
+  for (int w = 1; w < kT / 64; w++) v = fmaxf(v, red[w]);
+  return v;
+}
+
+__device__ __forceinline__ unsigned long long block_min_u64(unsigned long long v, unsigned long long *red) {
+#pragma unroll
+  for (int off = 32; off >= 1; off >>= 1) {
+    const unsigned long long o = __shfl_xor(v, off, 64);
+    v = o < v ? o : v;
+  }
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+  __syncthreads();
+  v = red[0];
+#pragma unroll
+  for (int w = 1; w < kT / 64; w++) v = red[w] < v ? red[w] : v;
+  return v;
+}
+
+// Weights before p of the total: the smallest whole number not below.
+__device__ __forceinline__ unsigned long long limit_of(double p, unsigned long long total) {
+  const double l = ceil(p * (double)total);
+  return l >= 1.0 ? (unsigned long long)l : 1ULL;  // (at least one token)
+}
+
+// What the weights up to a token must exceed for u to fall on it or before.
+__device__ __forceinline__ unsigned long long target_of(const SampleArgs &a, int row, unsigned long long total) {
+  const float u = a.u[row];
+  const unsigned long long t = u > 0.0f ? (unsigned long long)((double)fminf(u, 1.0f) * (double)total) : 0ULL;
+  return t < total ? t : total - 1;
+}
+
+// ---- the list of candidates, in LDS ------------------------------------------------
+
+struct Candidates {
+  unsigned long long key[kList], mass[kList];
+  unsigned int place[kList];  // index << 11 | position in key
+};
+
+// n values, a power of two of at least 2; `up`: ascending.
+template <class V>
+__device__ __forceinline__ void bitonic_sort(V *v, int n, bool up) {
+  for (int k = 2; k <= n; k *= 2)
+    for (int j = k / 2; j >= 1; j /= 2) {
+      __syncthreads();
+      for (int i = threadIdx.x; i < n / 2; i += kT) {
+        const int lo = (i / j) * 2 * j + i % j, hi = lo + j;
+        const bool asc = ((lo & k) == 0) == up;
+        const V x = v[lo], y = v[hi];
+        if ((x > y) == asc) {
+          v[lo] = y;
+          v[hi] = x;
+        }
+      }
+    }
+  __syncthreads();
+}
+
+__device__ __forceinline__ int power_of_two(int n) {
+  int p = 2;
+  while (p < n) p *= 2;
+  return p;
+}
+
+// Sorts c.key[0 .. n) (the rest up to the power of two is filled with 0) and works
+// out the weights.
+__device__ __forceinline__ void rank_candidates(const RowParams &r, Candidates &c, int n, const double *table) {
+  const int size = power_of_two(n);
+  for (int i = n + threadIdx.x; i < size; i += kT) c.key[i] = 0;
+  bitonic_sort(c.key, size, false);
+  for (int i = threadIdx.x; i < n; i += kT) {
+    double e;
+    c.mass[i] = weight(exponent(r, key_value(c.key[i])), table, &e);
+  }
+  __syncthreads();
+}
+
+// Of n ranked candidates, those before them having weight `before`: how many are
+// kept by the limit (0: all).
+__device__ __forceinline__ int kept_by_limit(const Candidates &c, int n, unsigned long long before,
+                                             unsigned long long limit, unsigned long long *red) {
+  constexpr int kPer = kList / kT;
+  if (limit == 0) return n;
+  unsigned long long sum = 0, total, first = n;
+  const int i0 = threadIdx.x * kPer;
+#pragma unroll
+  for (int e = 0; e < kPer; e++) sum += i0 + e < n ? c.mass[i0 + e] : 0;
+  unsigned long long at = before + block_scan_u64(sum, red, &total) - sum;
+#pragma unroll
+  for (int e = 0; e < kPer; e++)
+    if (i0 + e < n) {
+      if (at >= limit && first == (unsigned long long)n) first = i0 + e;
+      at += c.mass[i0 + e];
+    }
+  return (int)block_min_u64(first, red);
+}
+
+__device__ __forceinline__ unsigned long long total_mass(const Candidates &c, int n, unsigned long long *red) {
+  unsigned long long sum = 0, total;
+  for (int i = threadIdx.x; i < n; i += kT) sum += c.mass[i];
+  block_scan_u64(sum, red, &total);
+  return total;
+}
+
+// Everything from a list of all tokens that may be kept. limit: top-p's, 0: to be
+// worked out of the list's weights (which are then all, or all that top-k keeps).
+__device__ __forceinline__ int draw_listed(const SampleArgs &a, const RowParams &r, int row, Candidates &c, int n,
+                                           unsigned long long limit, const double *table,
+                                           unsigned long long *red) {
+  constexpr int kPer = kList / kT;
+  rank_candidates(r, c, n, table);
+  if (r.k > 0) n = min(n, r.k);
+  if (r.p < 1.0 && limit == 0) limit = limit_of(r.p, total_mass(c, n, red));
+  n = kept_by_limit(c, n, 0, limit, red);
+  for (int i = threadIdx.x; i < n; i += kT) {
+    if (exp_minus(exponent(r, key_value(c.key[i])), table) < r.least) c.mass[i] = 0;
+    c.place[i] = ((unsigned)key_index(c.key[i]) << 11) | (unsigned)i;
+  }
+  const int size = power_of_two(n);
+  for (int i = n + threadIdx.x; i < size; i += kT) c.place[i] = 0xffffffffu;
+  bitonic_sort(c.place, size, true);
+  unsigned long long mass[kPer], sum = 0, total;
+  const int i0 = threadIdx.x * kPer;
+#pragma unroll
+  for (int e = 0; e < kPer; e++) {
+    mass[e] = i0 + e < n ? c.mass[c.place[i0 + e] & (kList - 1)] : 0;
+    sum += mass[e];
+  }
+  unsigned long long at = block_scan_u64(sum, red, &total) - sum, found = ~0ULL;
+  const unsigned long long target = target_of(a, row, total);
+#pragma unroll
+  for (int e = 0; e < kPer; e++) {
+    if (at <= target && target < at + mass[e]) found = c.place[i0 + e] >> 11;
+    at += mass[e];
+  }
+  return (int)block_min_u64(found, red);
+}
+
+// The first position in [begin, end) whose value is m.
+__device__ __forceinline__ int first_of(const float *x, int begin, int end, float m, unsigned long long *red) {
+  unsigned long long found = ~0ULL;
+  for (int i = begin + 4 * (int)threadIdx.x; i < end && found == ~0ULL; i += 4 * kT) {
+    const f32x4 v = load4(x, i, end);
+#pragma unroll
+    for (int e = 3; e >= 0; e--)
+      if (v[e] == m && i + e < end) found = i + e;
+  }
+  return (int)block_min_u64(found, red);
+}
+
+__device__ __forceinline__ void load_table(const SampleArgs &a, double *table) {
+  if (threadIdx.x < 64) table[threadIdx.x] = a.table[threadIdx.x];
+  __syncthreads();
+}
+
+// ---- short rows ---------------------------------------------------------------------
+
+__global__ __launch_bounds__(kT) void sample_short_kernel(const SampleArgs a) {
+  __shared__ Candidates c;
+  __shared__ double table[64];
+  __shared__ unsigned long long red[kT / 64];
+  __shared__ float fred[kT / 64];
+  __shared__ unsigned int listed;
+  const int row = blockIdx.x;
+  const float *x = a.x + (size_t)row * a.ld;
+  load_table(a, table);
+  if (threadIdx.x == 0) listed = 0;
+  const f32x4 v = load4(x, 4 * threadIdx.x, a.n);
+  float m = -INFINITY;
+#pragma unroll
+  for (int e = 0; e < 4; e++) m = fmaxf(m, v[e]);
+  m = block_max(m, fred);
+  const RowParams r = row_params(a, row, m);
+  int found = -1;
+  if (m > -INFINITY) {
+    if (r.greedy) {
+      found = first_of(x, 0, a.n, m, red);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; e++) {
+        const double y = exponent(r, v[e]);
+        if (y < kCutoff) c.key[atomicAdd(&listed, 1u)] = key_of(v[e], 4 * threadIdx.x + e);
+      }
+      __syncthreads();
+      found = draw_listed(a, r, row, c, (int)listed, 0, table, red);
+    }
+  }
+  if (threadIdx.x == 0) a.index[row] = found;
+}
+
+// ---- long rows ----------------------------------------------------------------------
+
+__global__ __launch_bounds__(kT) void sample_max_kernel(const SampleArgs a) {
+  constexpr int kU = 4;
+  __shared__ float red[kT / 64];
+  const int row = blockIdx.x / a.splits, split = blockIdx.x % a.splits;
+  const float *x = a.x + (size_t)row * a.ld;
+  RowState &s = a.rows[row];
+  const int begin = split * a.chunk, end = min(begin + a.chunk, a.n);
+  float m = -INFINITY;
+  for (int i = begin + 4 * (int)threadIdx.x; i < end; i += 4 * kT * kU) {
+    f32x4 v[kU];
+#pragma unroll
+    for (int u = 0; u < kU; u++) v[u] = load4(x, min(i + 4 * kT * u, end), end);
+#pragma unroll
+    for (int u = 0; u < kU; u++) m = fmaxf(fmaxf(fmaxf(m, v[u].x), fmaxf(v[u].y, v[u].z)), v[u].w);
+  }
+  for (int i = split * kT + threadIdx.x; i < kBins; i += a.splits * kT) {
+    s.mass[i] = 0;
+    s.count[i] = 0;
+  }
+  m = block_max(m, red);
+  if (threadIdx.x == 0) {
+    s.split_max[split] = m;
+    if (split == 0) s.listed = 0;
+  }
+}
+
+__device__ __forceinline__ float row_max(const RowState &s, int splits) {
+  float m = -INFINITY;
+  for (int i = 0; i < splits; i++) m = fmaxf(m, s.split_max[i]);
+  return m;
+}
+
+__global__ __launch_bounds__(kT) void sample_bins_kernel(const SampleArgs a) {
+  __shared__ unsigned long long mass[kBins];
+  __shared__ unsigned int count[kBins];
+  __shared__ double table[64];
+  const int row = blockIdx.x / a.splits, split = blockIdx.x % a.splits;
+  const float *x = a.x + (size_t)row * a.ld;
+  RowState &s = a.rows[row];
+  const RowParams r = row_params(a, row, row_max(s, a.splits));
+  if (r.m == -INFINITY || r.greedy || (r.k == 0 && r.p >= 1.0)) return;
+  for (int i = threadIdx.x; i < kBins; i += kT) {
+    mass[i] = 0;
+    count[i] = 0;
+  }
+  load_table(a, table);
+  const int begin = split * a.chunk, end = min(begin + a.chunk, a.n);
+  for (int i = begin + 4 * (int)threadIdx.x; i < end; i += 4 * kT) {
+    const f32x4 v = load4(x, i, end);
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+      const double y = exponent(r, v[e]);
+      if (y < kCutoff) {
+        double ex;
+        const unsigned long long w = weight(y, table, &ex);
+        atomicAdd(&mass[bin_of(y)], w);
+        atomicAdd(&count[bin_of(y)], 1u);
+      }
+    }
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < kBins; i += kT)
+    if (count[i] != 0) {
+      atomicAdd(&s.mass[i], mass[i]);
+      atomicAdd(&s.count[i], count[i]);
+    }
+}
+
+__global__ __launch_bounds__(kT) void sample_gather_kernel(const SampleArgs a) {
+  constexpr int kPer = kBins / kT;
+  __shared__ double table[64];
+  __shared__ unsigned long long red[kT / 64];
+  __shared__ unsigned long long found[4];
+  const int row = blockIdx.x / a.splits, split = blockIdx.x % a.splits, lane = threadIdx.x & 63;
+  const float *x = a.x + (size_t)row * a.ld;
+  RowState &s = a.rows[row];
+  const RowParams r = row_params(a, row, row_max(s, a.splits));
+  if (r.m == -INFINITY || r.greedy) return;
+  load_table(a, table);
+  int mode = kAll, bin = kBins, k = 0;
+  unsigned long long limit = 0, before_mass = 0;
+  unsigned int before_count = 0;
+  if (r.k > 0 || r.p < 1.0) {
+    unsigned long long mass[kPer], masses = 0, counts = 0, total_masses, total_counts;
+    unsigned int count[kPer];
+    const int i0 = threadIdx.x * kPer;
+#pragma unroll
+    for (int e = 0; e < kPer; e++) {
+      mass[e] = s.mass[i0 + e];
+      count[e] = s.count[i0 + e];
+      masses += mass[e];
+      counts += count[e];
+    }
+    unsigned long long m0 = block_scan_u64(masses, red, &total_masses) - masses;
+    unsigned long long c0 = block_scan_u64(counts, red, &total_counts) - counts;
+    k = r.k > 0 && (unsigned long long)r.k < total_counts ? r.k : 0;
+    if (k == 0 && r.p < 1.0) limit = limit_of(r.p, total_masses);
+    if (k > 0 || limit > 0) {
+#pragma unroll
+      for (int e = 0; e < kPer; e++) {
+        // the bin that the k-th token, or the last one within the limit, is in
+        const bool here = k > 0 ? c0 < (unsigned)k && (unsigned)k <= c0 + count[e]
+                                : m0 < limit && limit <= m0 + mass[e];
+        if (here) {
+          found[0] = i0 + e;
+          found[1] = c0;
+          found[2] = m0;
+          found[3] = count[e];
+        }
+        c0 += count[e];
+        m0 += mass[e];
+      }
+      __syncthreads();
+      bin = (int)found[0];
+      before_count = (unsigned)found[1];
+      before_mass = found[2];
+      const unsigned in_bin = (unsigned)found[3];
+      mode = before_count + in_bin <= kList ? kListed
+             : in_bin <= kList && !(k > 0 && r.p < 1.0) ? kBinned
+                                                        : kDigits;
+    }
+  }
+  if (split == 0 && threadIdx.x == 0) {
+    s.mode = mode;
+    s.bin = bin;
+    s.before_count = before_count;
+    s.before_mass = before_mass;
+    s.limit = limit;
+    s.k = k;
+  }
+  if (mode == kDigits) return;
+  const int begin = split * a.chunk, end = min(begin + a.chunk, a.n);
+  unsigned long long sum = 0;
+  for (int i = begin + 4 * (int)threadIdx.x; i - 4 * lane < end; i += 4 * kT) {
+    const f32x4 v = load4(x, min(i, end), end);
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+      const double y = exponent(r, v[e]);
+      const int b = y < kCutoff ? bin_of(y) : kBins + 1;
+      if (mode != kListed && b < bin) {
+        double ex;
+        const unsigned long long w = weight(y, table, &ex);
+        sum += ex >= r.least ? w : 0;
+      }
+      if (mode != kAll) {
+        const bool take = mode == kListed ? b <= bin : b == bin;
+        const unsigned long long takers = __ballot(take);
+        if (takers != 0) {
+          unsigned int at = 0;
+          if (lane == __ffsll(takers) - 1) at = atomicAdd(&s.listed, (unsigned)__popcll(takers));
+          at = __shfl(at, __ffsll(takers) - 1, 64) + __popcll(takers & ((1ULL << lane) - 1));
+          if (take && at < kList) s.list[at] = key_of(v[e], i + e);
+        }
+      }
+    }
+  }
+  if (mode != kListed) {
+    unsigned long long total;
+    block_scan_u64(sum, red, &total);
+    if (threadIdx.x == 0) s.split_mass[split] = total;
+  }
+}
+
+// ---- the draw of long rows ------------------------------------------------------------
+
+struct DrawLds {
+  union {
+    Candidates c;
+    unsigned long long segment[kMaxSegments];
+    struct {
+      unsigned long long amount[256], mass[256];
+    } digits;
+  };
+  double table[64];
+  unsigned long long red[kT / 64], split_mass[kMaxSplits], shared[4];
+};
+
+// A token is kept: by its bin (before `bin`), or its key (`last`: the last kept
+// one's), and min_p. Its weight, or 0.
+__device__ __forceinline__ unsigned long long kept_weight(const RowParams &r, float x, int i, int bin,
+                                                          unsigned long long last, const double *table) {
+  const double y = exponent(r, x);
+  if (!(y < kCutoff)) return 0;
+  if (!(bin_of(y) < bin) && key_of(x, i) < last) return 0;
+  double e;
+  const unsigned long long w = weight(y, table, &e);
+  return e >= r.least ? w : 0;
+}
+
+// The token of [begin, end) on which `target` of the kept weights from `begin` on
+// falls; with pick false only their sum. A segment of 256 tokens per wave and
+// step, its sum in LDS.
+__device__ __forceinline__ unsigned long long segment_sums(const RowParams &r, const float *x, int begin, int end,
+                                                           int bin, unsigned long long last, DrawLds &lds) {
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  const int segments = (end - begin + kSegment - 1) / kSegment;
+  __syncthreads();
+  for (int g = wave; g < segments; g += kT / 64) {
+    const int i = begin + g * kSegment + 4 * lane;
+    const f32x4 v = load4(x, min(i, end), end);
+    unsigned long long sum = 0;
+#pragma unroll
+    for (int e = 0; e < 4; e++) sum += kept_weight(r, v[e], i + e, bin, last, lds.table);
+    sum = wave_sum_u64(sum);
+    if (lane == 0) lds.segment[g] = sum;
+  }
+  __syncthreads();
+  unsigned long long sum = 0, total;
+  for (int g = threadIdx.x; g < segments; g += kT) sum += lds.segment[g];
+  block_scan_u64(sum, lds.red, &total);
+  return total;
+}
+
+__device__ __forceinline__ int pick(const RowParams &r, const float *x, int begin, int end, int bin,
+                                    unsigned long long last, unsigned long long target, DrawLds &lds) {
+  const int segments = (end - begin + kSegment - 1) / kSegment, lane = threadIdx.x & 63;
+  // the segment: each thread looks through a run of them
+  const int per = (segments + kT - 1) / kT, g0 = threadIdx.x * per;
+  unsigned long long sum = 0, total;
+  for (int g = g0; g < min(g0 + per, segments); g++) sum += lds.segment[g];
+  unsigned long long at = block_scan_u64(sum, lds.red, &total) - sum;
+  for (int g = g0; g < min(g0 + per, segments); g++) {
+    const unsigned long long w = lds.segment[g];
+    if (at <= target && target < at + w) {
+      lds.shared[0] = g;
+      lds.shared[1] = at;
+    }
+    at += w;
+  }
+  __syncthreads();
+  if (threadIdx.x < 64) {
+    const int i = begin + (int)lds.shared[0] * kSegment + 4 * lane;
+    const f32x4 v = load4(x, min(i, end), end);
+    unsigned long long w[4], mine = 0;
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+      w[e] = kept_weight(r, v[e], i + e, bin, last, lds.table);
+      mine += w[e];
+    }
+    unsigned long long to = lds.shared[1] + wave_scan_u64(mine) - mine;
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+      if (to <= target && target < to + w[e]) lds.shared[2] = i + e;
+      to += w[e];
+    }
+  }
+  __syncthreads();
+  return (int)lds.shared[2];
+}
+
+// The first key, descending, at which the tokens' counts (by_mass false) or
+// weights up to it and with it reach `limit`, 8 bits of the key at a time;
+// *mass: the weights up to it and with it.
+__device__ unsigned long long key_at(const RowParams &r, const float *x, int n, bool by_mass,
+                                     unsigned long long limit, DrawLds &lds, unsigned long long *mass) {
+  unsigned long long prefix = 0, before = 0, before_mass = 0;
+  for (int shift = 56; shift >= 0; shift -= 8) {
+    __syncthreads();
+    for (int i = threadIdx.x; i < 256; i += kT) lds.digits.amount[i] = lds.digits.mass[i] = 0;
+    __syncthreads();
+    for (int i = threadIdx.x; i < n; i += kT) {
+      const float v = x[i];
+      const double y = exponent(r, v);
+      const unsigned long long key = key_of(v, i);
+      if (!(y < kCutoff) || (shift < 56 && (key >> (shift + 8)) != prefix)) continue;
+      double e;
+      const unsigned long long w = weight(y, lds.table, &e);
+      atomicAdd(&lds.digits.mass[(key >> shift) & 255], w);
+      atomicAdd(&lds.digits.amount[(key >> shift) & 255], by_mass ? w : 1ULL);
+    }
+    __syncthreads();
+    // threads 0 .. 255 hold the digits from 255 down
+    const int d = 255 - (int)threadIdx.x;
+    const unsigned long long amount = d >= 0 ? lds.digits.amount[d] : 0, w = d >= 0 ? lds.digits.mass[d] : 0;
+    unsigned long long total;
+    const unsigned long long c = before + block_scan_u64(amount, lds.red, &total);
+    const unsigned long long m = before_mass + block_scan_u64(w, lds.red, &total);
+    if (d >= 0 && c - amount < limit && limit <= c) {
+      lds.shared[0] = (prefix << 8) | (unsigned)d;
+      lds.shared[1] = c - amount;
+      lds.shared[2] = m - w;
+      lds.shared[3] = m;
+    }
+    __syncthreads();
+    prefix = lds.shared[0];
+    before = lds.shared[1];
+    before_mass = lds.shared[2];
+    *mass = lds.shared[3];
+  }
+  return prefix;
+}
+
+__global__ __launch_bounds__(kT) void sample_draw_kernel(const SampleArgs a) {
+  __shared__ DrawLds lds;
+  const int row = blockIdx.x;
+  const float *x = a.x + (size_t)row * a.ld;
+  const RowState &s = a.rows[row];
+  const RowParams r = row_params(a, row, row_max(s, a.splits));
+  load_table(a, lds.table);
+  int found = -1;
+  if (r.m > -INFINITY && r.greedy) {
+    int split = 0;
+    while (split < a.splits - 1 && s.split_max[split] != r.m) split++;
+    found = first_of(x, split * a.chunk, min((split + 1) * a.chunk, a.n), r.m, lds.red);
+  } else if (r.m > -INFINITY) {
+    const int listed = (int)min(s.listed, (unsigned)kList), mode = s.mode;
+    int bin = s.bin;
+    unsigned long long last = ~0ULL;
+    if (mode == kListed || mode == kBinned) {
+      for (int i = threadIdx.x; i < listed; i += kT) lds.c.key[i] = s.list[i];
+      __syncthreads();
+    }
+    if (mode == kListed) {
+      found = draw_listed(a, r, row, lds.c, listed, s.limit, lds.table, lds.red);
+    } else if (mode == kDigits) {
+      unsigned long long mass = 0, limit = s.limit;
+      last = 0;
+      bin = 0;
+      if (s.k > 0) {
+        last = key_at(r, x, a.n, false, (unsigned long long)s.k, lds, &mass);
+        limit = r.p < 1.0 ? limit_of(r.p, mass) : 0;
+      }
+      if (limit > 0) last = key_at(r, x, a.n, true, limit, lds, &mass);
+      const unsigned long long total = segment_sums(r, x, 0, a.n, bin, last, lds);
+      found = pick(r, x, 0, a.n, bin, last, target_of(a, row, total), lds);
+    } else {
+      for (int i = threadIdx.x; i < a.splits; i += kT) lds.split_mass[i] = s.split_mass[i];
+      __syncthreads();
+      if (mode == kBinned) {
+        rank_candidates(r, lds.c, listed, lds.table);
+        const int kept = s.k > 0 ? min(listed, s.k - (int)s.before_count)
+                                 : kept_by_limit(lds.c, listed, s.before_mass, s.limit, lds.red);
+        last = lds.c.key[max(kept - 1, 0)];
+        for (int i = threadIdx.x; i < kept; i += kT)
+          if (exp_minus(exponent(r, key_value(lds.c.key[i])), lds.table) >= r.least)
+            atomicAdd(&lds.split_mass[key_index(lds.c.key[i]) / a.chunk], lds.c.mass[i]);
+        __syncthreads();
+      }
+      unsigned long long total = 0;
+      for (int i = 0; i < a.splits; i++) total += lds.split_mass[i];
+      unsigned long long target = target_of(a, row, total);
+      int split = 0;
+      while (split < a.splits - 1 && target >= lds.split_mass[split]) target -= lds.split_mass[split++];
+      const int begin = split * a.chunk, end = min(begin + a.chunk, a.n);
+      segment_sums(r, x, begin, end, bin, last, lds);
+      found = pick(r, x, begin, end, bin, last, target, lds);
+    }
+  }
+  if (threadIdx.x == 0) a.index[row] = found;
+}
+
+// Splits of a row: about 1,024 workgroups in all, of at least 2,048 logits each.
+void sample_split(int rows, int n, int *splits, int *chunk) {
+  const int unit = 4 * kT;
+  const long long most = std::min<long long>(kMaxSplits, (n + unit - 1) / unit);
+  const long long want = std::max(1LL, std::min(most, (long long)(1024 + rows - 1) / rows));
+  *chunk = (int)((n + want * unit - 1) / (want * unit)) * unit;
+  *splits = (n + *chunk - 1) / *chunk;
+}
+
+size_t workspace_of(int rows, int n) { return n <= kList ? 16 : (size_t)rows * sizeof(RowState); }
+
+}  // namespace
+}  // namespace sh
+
+using namespace sh;
+
+extern "C" {
+
+SH_API int sh_sample_workspace(int rows, int n, size_t *bytes) {
+  if (!bytes) return fail(SH_ERR_INVALID_ARGUMENT, "bytes is NULL");
+  if (const char *wrong = check_sample_sizes(rows, n, n)) return fail(SH_ERR_INVALID_ARGUMENT, "%s", wrong);
+  *bytes = workspace_of(rows, n);
+  return SH_OK;
+}
+
+SH_API int sh_sample_f32(sh_ctx *ctx, const float *x, int rows, int n, int ld, const float *temperature,
+                         const int32_t *top_k, const float *top_p, const float *min_p, const float *u,
+                         int32_t *index, void *workspace, size_t workspace_bytes) {
+  int rc = enter(ctx);
+  if (rc != SH_OK) return rc;
+  if (const char *wrong = check_sample_sizes(rows, n, ld)) return fail(SH_ERR_INVALID_ARGUMENT, "%s", wrong);
+  if (rows == 0) return SH_OK;
+  const size_t per_row = (size_t)rows * 4, need = workspace_of(rows, n);
+  if ((rc = check_range(ctx, x, ((size_t)(rows - 1) * ld + n) * 4, "x")) ||
+      (temperature && (rc = check_range(ctx, temperature, per_row, "temperature"))) ||
+      (top_k && (rc = check_range(ctx, top_k, per_row, "top_k"))) ||
+      (top_p && (rc = check_range(ctx, top_p, per_row, "top_p"))) ||
+      (min_p && (rc = check_range(ctx, min_p, per_row, "min_p"))) || (rc = check_range(ctx, u, per_row, "u")) ||
+      (rc = check_range(ctx, index, per_row, "index")))
+    return rc;
+  if (workspace_bytes < need)
+    return fail(SH_ERR_INVALID_ARGUMENT, "the work buffer has %zu bytes, %zu are needed", workspace_bytes, need);
+  if ((rc = check_range(ctx, workspace, need, "workspace"))) return rc;
+  if (reinterpret_cast<uintptr_t>(workspace) & 15)
+    return fail(SH_ERR_INVALID_ARGUMENT, "the work buffer must be 16-byte aligned");
+  SampleArgs a;
+  a.x = x;
+  a.temperature = temperature;
+  a.top_k = top_k;
+  a.top_p = top_p;
+  a.min_p = min_p;
+  a.u = u;
+  a.index = index;
+  a.rows = static_cast<RowState *>(workspace);
+  a.n = n;
+  a.ld = ld;
+  for (int j = 0; j < 64; j++) a.table[j] = std::exp2(-j / 64.0);
+  const hipStream_t st = stream_of(ctx);
+  if (n <= kList) {
+    a.splits = 1;
+    a.chunk = n;
+    sample_short_kernel<<<rows, kT, 0, st>>>(a);
+  } else {
+    sample_split(rows, n, &a.splits, &a.chunk);
+    const unsigned grid = (unsigned)rows * (unsigned)a.splits;
+    sample_max_kernel<<<grid, kT, 0, st>>>(a);
+    sample_bins_kernel<<<grid, kT, 0, st>>>(a);
+    sample_gather_kernel<<<grid, kT, 0, st>>>(a);
+    sample_draw_kernel<<<rows, kT, 0, st>>>(a);
+  }
+  const hipError_t e = hipGetLastError();
+  return e == hipSuccess ? SH_OK : hip_fail(e, "sample");
+}
+
+}  // extern "C"
