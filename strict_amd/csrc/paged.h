@@ -255,6 +255,8 @@ SH_HD PieceStep plan_step(const PagedPlan &p, const long long *prefix, int parts
   r.u0 = plan_cut(p, r.tile, r.span.units, x0);
   r.u1 = plan_cut(p, r.tile, r.span.units, x1);
   r.slot = -1;
+  r.run = false;
+  if (r.span.count == 0) return r;  // (no tile: only where sums saturated)
   if (c.count > 1) {
     r.slot = 2 * worker + (r.tile.begin > x0 ? 1 : 0);
     r.run = true;  // (of no units, too: the merge reads every part)
