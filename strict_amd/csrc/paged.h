@@ -65,9 +65,11 @@ struct PagedPlan {
   const int *starts, *lengths;
   int batch, tokens, kv_heads, capacity;
   int per_tile;       // tokens of a tile
-  int unit;           // positions of a unit: a tile is cut at multiples of it
+  int unit;           // positions of a unit, a power of two: a tile is cut at multiples of it
+  int unit_shift;     // its logarithm
   int window, sinks;  // window 0: none
   int workers;
+  double inv_workers; // 1 / workers, rounded up
   int min_piece;      // shortest piece of the line
   int whole_below;    // tiles of at most this cost are not cut
 };
@@ -98,14 +100,35 @@ SH_HD long long plan_prefix(const PagedPlan &p, const PagedSeq &s, int t) {
 
 SH_HD long long plan_add(long long a, long long b) { return a + b < kMaxLine ? a + b : kMaxLine; }
 
-// Cost of a sequence (each KV head's tiles).
-SH_HD long long plan_cost(const PagedPlan &p, const PagedSeq &s) {
-  return plan_prefix(p, s, plan_tiles(p, s)) * p.kv_heads;
+// A sequence on the line: its tiles, and what one KV head's cost together.
+struct PlanSeq {
+  PagedSeq seq;
+  int tiles;
+  long long one;
+};
+
+SH_HD PlanSeq plan_sequence(const PagedPlan &p, int b) {
+  PlanSeq s;
+  s.seq = plan_seq(p, b);
+  s.tiles = plan_tiles(p, s.seq);
+  s.one = plan_prefix(p, s.seq, s.tiles);
+  return s;
 }
 
+// (At least total / workers: inv_workers is rounded up, and what a product in fp64
+// loses of a total below 2^61 is added.)
 SH_HD long long plan_piece(const PagedPlan &p, long long total) {
-  const long long q = plan_div(total + p.workers - 1, p.workers);
+  const long long q = (long long)((double)total * p.inv_workers) + (total >> 50) + 1;
   return q > p.min_piece ? q : p.min_piece;
+}
+
+// Workers for a call: `most`, or fewer where even full tables would not give each of
+// them a shortest piece. A multiple of 8.
+inline int plan_workers(int batch, int kv_heads, int tokens, int capacity, int per_tile, int min_piece, int most) {
+  const double tiles = (double)tokens / per_tile + batch;  // at most, of each KV head
+  const double line = tiles * kv_heads * ((double)capacity + per_tile + kTileFixedCost);
+  const double n = line / min_piece + 8;
+  return n < most ? ((int)n + 7) / 8 * 8 : most;
 }
 
 // A tile and where it lies on the line.
@@ -115,10 +138,9 @@ struct PagedTile {
   long long begin, cost;
 };
 
-// The tile that point x < prefix[parts] of the line lies in. prefix[i]: cost of
-// the sequences before i * per (parts + 1 ascending values, prefix[0] = 0).
-SH_HD PagedTile plan_locate(const PagedPlan &p, const long long *prefix, int parts, int per, long long x) {
-  int lo = 0, hi = parts;  // prefix[lo] <= x < prefix[hi]
+// The last i < parts with prefix[i] <= x (prefix ascends from 0).
+SH_HD int plan_find(const long long *prefix, int parts, long long x) {
+  int lo = 0, hi = parts;
   while (hi - lo > 1) {
     const int mid = (lo + hi) / 2;
     if (prefix[mid] <= x)
@@ -126,35 +148,37 @@ SH_HD PagedTile plan_locate(const PagedPlan &p, const long long *prefix, int par
     else
       hi = mid;
   }
+  return lo;
+}
+
+// The tile that point x of the line lies in. at: cost of the sequences before part *
+// per, the sequence of x among the `per` from there on. seqs: the sequences where
+// per is 1 (worked out again otherwise).
+SH_HD PagedTile plan_locate(const PagedPlan &p, const PlanSeq *seqs, int part, int per, long long at, long long x) {
   PagedTile t;
-  long long at = prefix[lo];
-  const int end = (lo + 1) * per < p.batch ? (lo + 1) * per : p.batch;
-  t.b = lo * per < end ? lo * per : end - 1;
-  t.seq = plan_seq(p, t.b);
-  long long cost = plan_cost(p, t.seq);
-  while (x >= at + cost && t.b + 1 < end) {
-    at += cost;
-    t.seq = plan_seq(p, ++t.b);
-    cost = plan_cost(p, t.seq);
+  const int end = (part + 1) * per < p.batch ? (part + 1) * per : p.batch;
+  t.b = part * per < end ? part * per : end - 1;
+  PlanSeq s = per == 1 ? seqs[t.b] : plan_sequence(p, t.b);
+  while (x >= at + s.one * p.kv_heads && t.b + 1 < end) {
+    at += s.one * p.kv_heads;
+    s = plan_sequence(p, ++t.b);
   }
-  const int tiles = plan_tiles(p, t.seq);
-  const long long one = plan_prefix(p, t.seq, tiles);  // a KV head's
-  long long in = x - at;
-  const long long head = one > 0 ? plan_div(in, one) : 0;
+  t.seq = s.seq;
+  const long long head = p.kv_heads > 1 && s.one > 0 ? plan_div(x - at, s.one) : 0;
   t.kv_head = (int)(head < p.kv_heads ? head : p.kv_heads - 1);
-  at += one * t.kv_head;
-  in = x - at;
-  int a = 0, z = tiles > 1 ? tiles : 1;  // prefix(a) <= in < prefix(z)
+  at += s.one * t.kv_head;
+  int a = 0, z = s.tiles > 1 ? s.tiles : 1;  // prefix(a) <= x - at < prefix(z)
   while (z - a > 1) {
     const int mid = a + (z - a) / 2;
-    if (plan_prefix(p, t.seq, mid) <= in)
+    if (plan_prefix(p, t.seq, mid) <= x - at)
       a = mid;
     else
       z = mid;
   }
   t.tile = a;
-  t.begin = at + plan_prefix(p, t.seq, a);
-  t.cost = plan_prefix(p, t.seq, a + 1) - plan_prefix(p, t.seq, a);
+  const long long before = a > 0 ? plan_prefix(p, t.seq, a) : 0;
+  t.begin = at + before;
+  t.cost = (s.tiles > 1 ? plan_prefix(p, t.seq, a + 1) : s.one) - before;
   return t;
 }
 
@@ -179,12 +203,12 @@ SH_HD TileSpan plan_span(const PagedPlan &p, const PagedTile &t) {
   s.sinks = 0;
   s.gap = 0;
   s.sink_units = 0;
-  s.units = (s.hi + p.unit - 1) / p.unit;
+  s.units = (s.hi + p.unit - 1) >> p.unit_shift;
   if (p.window > 0) {
     const long long lo = (long long)s.pos0 - p.window + 1;
     s.lo = lo > 0 ? (int)lo : 0;
     s.sinks = p.sinks < s.hi ? p.sinks : s.hi;
-    const int su = (s.sinks + p.unit - 1) / p.unit, wu = s.lo / p.unit;
+    const int su = (s.sinks + p.unit - 1) >> p.unit_shift, wu = s.lo >> p.unit_shift;
     if (wu > su) {
       s.sink_units = su;
       s.gap = wu - su;
@@ -201,28 +225,11 @@ SH_HD int span_position(const TileSpan &s, int unit, int j) {
 
 // Units of a tile before point x of its cost: what a cut there leaves on its left.
 SH_HD int plan_cut(const PagedPlan &p, const PagedTile &t, int units, long long x) {
-  const long long in = x <= t.begin ? 0 : x >= t.begin + t.cost ? t.cost : x - t.begin;
-  if (in == t.cost) return units;
+  if (x <= t.begin) return 0;
+  if (x >= t.begin + t.cost) return units;
+  const long long in = x - t.begin;
   if (t.cost <= p.whole_below) return 2 * in >= t.cost ? units : 0;
   return (int)plan_div(in * units, t.cost);
-}
-
-// The cut of tile t by a piece that starts or ends strictly inside it: whether a
-// point k * piece within the tile divides its units, from the first such point on.
-struct TileParts {
-  int first, count;  // pieces that touch the tile; count 1: not cut
-};
-SH_HD TileParts plan_parts(const PagedPlan &p, const PagedTile &t, int units, long long piece) {
-  TileParts r;
-  r.first = (int)plan_div(t.begin, piece);
-  const int last = (int)plan_div(t.begin + t.cost - 1, piece);
-  r.count = 1;
-  for (int w = r.first + 1; w <= last; w++) {
-    const int u = plan_cut(p, t, units, (long long)w * piece);
-    if (u > 0 && u < units) r.count = last - r.first + 1;
-    if (u > 0) break;  // (cuts ascend: one inside comes before any at the end)
-  }
-  return r;
 }
 
 // What a workgroup whose piece starts inside a cut tile leaves for the merge: the
@@ -232,44 +239,54 @@ struct MergeItem {
   int row0, tokens, kv_head;            // first token's row of q / out
 };
 
-// Worker w's step at point x of its piece [x0, x1): the tile there, the units of
-// it that are the worker's and where they go. The next step is at tile.begin +
-// tile.cost. A worker has two slots: 2 w for a tile that its piece starts in, 2 w +
-// 1 for one that its piece ends in.
+// Worker w's step at point x of its piece [x0, x1), x0 = w * piece: the tile there,
+// the units of it that are the worker's and where they go. The next step is at
+// tile.begin + tile.cost. A tile is cut if two pieces' ends lie in it, or one that
+// divides its units. A worker has two slots: 2 w for a cut tile that its piece
+// starts in (or with), 2 w + 1 for one that its piece ends in.
 struct PieceStep {
   PagedTile tile;
   TileSpan span;
   int u0, u1;
-  int slot;      // -1: the whole tile, to the output
-  bool run;      // false: nothing of the tile is this worker's
-  bool more;     // false: sums that saturated, the walk ends
+  int slot;   // -1: the whole tile, to the output
+  bool run;   // false: nothing of the tile is this worker's
+  bool more;  // false: sums that saturated, the walk ends
 };
 
-SH_HD PieceStep plan_step(const PagedPlan &p, const long long *prefix, int parts, int per, long long piece,
-                          int worker, long long x0, long long x1, long long x, MergeItem *item) {
+// The first worker of a tile.
+SH_HD int plan_first(const PagedTile &t, int worker, long long piece, long long x0) {
+  return t.begin >= x0 ? worker : worker - (int)plan_div(x0 - t.begin + piece - 1, piece);
+}
+
+SH_HD PieceStep plan_step(const PagedPlan &p, const PagedTile &t, long long piece, int worker, long long x0,
+                          long long x, MergeItem *item) {
   PieceStep r;
-  r.tile = plan_locate(p, prefix, parts, per, x);
-  r.more = x < r.tile.begin + r.tile.cost;
-  r.span = plan_span(p, r.tile);
-  const TileParts c = plan_parts(p, r.tile, r.span.units, piece);
-  r.u0 = plan_cut(p, r.tile, r.span.units, x0);
-  r.u1 = plan_cut(p, r.tile, r.span.units, x1);
+  r.tile = t;
+  r.span = plan_span(p, t);
+  const long long end = t.begin + t.cost;
+  r.more = x < end;
+  r.u0 = plan_cut(p, t, r.span.units, x0);
+  r.u1 = plan_cut(p, t, r.span.units, x0 + piece);
   r.slot = -1;
   r.run = false;
   if (r.span.count == 0) return r;  // (no tile: only where sums saturated)
-  if (c.count > 1) {
-    r.slot = 2 * worker + (r.tile.begin > x0 ? 1 : 0);
+  const bool left = t.begin < x0, right = end > x0 + piece;
+  bool cut = left && (right || t.begin < x0 - piece);
+  cut = cut || (right && end > x0 + 2 * piece);
+  cut = cut || (left && r.u0 > 0 && r.u0 < r.span.units) || (right && r.u1 > 0 && r.u1 < r.span.units);
+  if (cut) {
+    r.slot = 2 * worker + (t.begin > x0 ? 1 : 0);
     r.run = true;  // (of no units, too: the merge reads every part)
-    if (r.tile.begin < x0 && worker == c.first + 1) {
-      item->parts = c.count;
-      item->first_worker = c.first;
-      item->first_slot = 2 * c.first + (r.tile.begin > (long long)c.first * piece ? 1 : 0);
-      item->row0 = r.tile.seq.row0 + r.span.first;
+    if (left && t.begin >= x0 - piece) {
+      item->first_worker = worker - 1;
+      item->parts = 2 + (right ? (int)plan_div(end - x0 - 1, piece) : 0);
+      item->first_slot = 2 * (worker - 1) + (t.begin > x0 - piece ? 1 : 0);
+      item->row0 = t.seq.row0 + r.span.first;
       item->tokens = r.span.count;
-      item->kv_head = r.tile.kv_head;
+      item->kv_head = t.kv_head;
     }
   } else {
-    r.run = r.span.units > 0 ? r.u0 < r.u1 : worker == c.first;
+    r.run = r.span.units > 0 ? r.u0 < r.u1 : !left;
   }
   return r;
 }

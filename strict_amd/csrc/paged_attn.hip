@@ -5,7 +5,9 @@
 // heads of one KV head, its rows (token, head) numbered token * G + head. A tile
 // that lies in one piece is written to the output; one cut between pieces leaves
 // a part in each of its workgroups' slots (V sums, maximum and sum of weights
-// per row), and a second kernel merges the parts.
+// per row), and a second kernel merges the parts. That kernel also works out again,
+// in fp32 without matrix products, what came out not finite: infinities and NaN in
+// q, K or V, or in places of V that only some of a tile's rows see.
 //
 // Softmax runs over the positions in order with a running maximum, in base 2:
 // s = q.k scale log2(e), weights 2^(s - max) (times 2^14 in fp16).
@@ -22,14 +24,14 @@
 namespace sh {
 namespace {
 
-constexpr int kT = 256;
+constexpr int kT = 256, kMaxT = 512;
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 #define SH_PAGED_LDS __attribute__((address_space(3)))
 
 // Pieces of a call, and the shortest, in positions: three workgroups per CU are
 // resident with the small tiles, two with the large ones.
-constexpr int kSmallRows = 16, kSmallWorkers = 768, kSmallPiece = 256;
-constexpr int kLargeRows = 128, kLargeWorkers = 512, kLargePiece = 512;
+constexpr int kSmallRows = 16, kSmallWorkers = 512, kSmallPiece = 128, kSmallWhole = 192, kSmallMergeRows = 1;
+constexpr int kLargeRows = 128, kLargeWorkers = 512, kLargePiece = 256, kLargeWhole = 1400, kLargeMergeRows = 8;
 
 struct PagedAttnArgs {
   const uint16_t *q, *k, *v;
@@ -37,10 +39,20 @@ struct PagedAttnArgs {
   const int *table;
   PagedPlan plan;
   MergeItem *items;  // [workers]
+  int *groups;       // [workers]: rows to merge of the worker's item, in groups
+  int *redo;         // [workers]: 1: some of the worker's results are not finite
   float *slots;      // [2 workers][rows of a tile][d + 4]
-  int heads, group, max_pages, num_pages, page_shift, tile_rows;
+  int heads, group, group_inv, max_pages, num_pages, page_shift, tile_rows;
   float scale_log2;
 };
+
+// Token of a tile's row (r <= 255, group <= 128: exact), and its row of heads in q
+// and out.
+__device__ __forceinline__ int token_of(const PagedAttnArgs &a, int r) { return (r * a.group_inv) >> 16; }
+__device__ __forceinline__ size_t head_row(const PagedAttnArgs &a, int row0, int kv_head, int r) {
+  const int token = token_of(a, r);
+  return (size_t)(row0 + token) * a.heads + kv_head * a.group + (r - token * a.group);
+}
 
 // Row r of slot s: d V sums, then the row's maximum and sum of weights (and 8
 // bytes that align the next).
@@ -54,7 +66,7 @@ template <class T, int kD>
 __device__ __forceinline__ void store_value(const PagedAttnArgs &a, const PagedTile &t, const TileSpan &s,
                                             int slot, int r, int dim, float acc, float l) {
   if (slot < 0) {
-    const size_t row = (size_t)(t.seq.row0 + s.first + r / a.group) * a.heads + t.kv_head * a.group + r % a.group;
+    const size_t row = head_row(a, t.seq.row0 + s.first, t.kv_head, r);
     reinterpret_cast<typename T::Value *>(a.out)[row * kD + dim] = (typename T::Value)(l == 0.0f ? 0.0f : acc / l);
   } else {
     slot_row<kD>(a, slot, r)[dim] = acc;
@@ -63,23 +75,22 @@ __device__ __forceinline__ void store_value(const PagedAttnArgs &a, const PagedT
 
 __device__ __forceinline__ float exp2_weight(float x) { return __builtin_amdgcn_exp2f(x); }
 
-// Units [u0, u1) of a tile in fp32, a wave per row, a lane per position of 64:
+// A tile in fp32, a wave per row, a lane per position of 64:
 // whatever the values are. A score of -infinity, and a weight that is 0 in fp32,
-// adds nothing. Slow: for parts whose sums by MFMA are not finite.
+// adds nothing. Slow: for tiles whose sums by MFMA are not finite.
 template <class T, int kD>
-__device__ void attn_exact(const PagedAttnArgs &a, const PagedTile &t, const TileSpan &s, int u0, int u1, int slot) {
+__device__ void attn_exact(const PagedAttnArgs &a, const PagedTile &t, const TileSpan &s) {
   typedef typename T::Value Value;
   constexpr int kDims = kD / 64;
   const int lane = threadIdx.x & 63, rows = s.count * a.group;
   const Value *kp = reinterpret_cast<const Value *>(a.k), *vp = reinterpret_cast<const Value *>(a.v);
-  for (int r = threadIdx.x >> 6; r < rows; r += kT / 64) {
-    const int pos = s.pos0 + r / a.group;
-    const Value *q = reinterpret_cast<const Value *>(a.q) +
-                     ((size_t)(t.seq.row0 + s.first + r / a.group) * a.heads + t.kv_head * a.group + r % a.group) * kD;
+  for (int r = threadIdx.x >> 6; r < rows; r += blockDim.x >> 6) {
+    const int pos = s.pos0 + token_of(a, r);
+    const Value *q = reinterpret_cast<const Value *>(a.q) + head_row(a, t.seq.row0 + s.first, t.kv_head, r) * kD;
     float m = -INFINITY, l = 0.0f, acc[kDims];
 #pragma unroll
     for (int j = 0; j < kDims; j++) acc[j] = 0.0f;
-    for (int u = u0; u < u1; u++) {
+    for (int u = 0; u < s.units; u++) {
       const int p0 = span_position(s, a.plan.unit, u), end = min(p0 + a.plan.unit, s.hi);
       for (int pt = p0; pt < end; pt += 64) {
         const int p = pt + lane;
@@ -114,49 +125,82 @@ __device__ void attn_exact(const PagedAttnArgs &a, const PagedTile &t, const Til
       }
     }
 #pragma unroll
-    for (int j = 0; j < kDims; j++) store_value<T, kD>(a, t, s, slot, r, lane + 64 * j, acc[j], l);
-    if (slot >= 0 && lane == 0) {
-      slot_row<kD>(a, slot, r)[kD] = m;
-      slot_row<kD>(a, slot, r)[kD + 1] = l;
-    }
+    for (int j = 0; j < kDims; j++) store_value<T, kD>(a, t, s, -1, r, lane + 64 * j, acc[j], l);
   }
 }
 
-// Prefix sums of the sequences' costs, by threads of `per` sequences each.
-__device__ __forceinline__ void scan_costs(const PagedPlan &p, int per, long long *prefix, long long *waves) {
+// The line's division among the workers, in LDS.
+struct PlanLds {
+  long long prefix[kT + 1], waves[kMaxT / 64];
+  PlanSeq seqs[kT];  // where a thread has one sequence
+};
+
+// Prefix sums of the sequences' costs, by kT threads (of kT or more) of `per`
+// sequences each.
+__device__ __forceinline__ void scan_costs(const PagedPlan &p, int per, PlanLds &lds) {
   const int t = threadIdx.x, lane = t & 63;
   long long sum = 0;
-  for (int b = t * per; b < min((t + 1) * per, p.batch); b++) sum = plan_add(sum, plan_cost(p, plan_seq(p, b)));
+  for (int b = t * per; b < min((t + 1) * per, p.batch); b++) {
+    const PlanSeq s = plan_sequence(p, b);
+    if (per == 1) lds.seqs[t] = s;
+    sum = plan_add(sum, s.one * p.kv_heads);
+  }
 #pragma unroll
   for (int off = 1; off < 64; off *= 2) {
     const long long o = __shfl_up(sum, off, 64);
     if (lane >= off) sum = plan_add(sum, o);
   }
-  if (lane == 63) waves[t >> 6] = sum;
+  if (lane == 63) lds.waves[t >> 6] = sum;
   __syncthreads();
-  for (int w = 0; w < (t >> 6); w++) sum = plan_add(sum, waves[w]);
-  prefix[t + 1] = sum;
-  if (t == 0) prefix[0] = 0;
+  for (int w = 0; w < (t >> 6); w++) sum = plan_add(sum, lds.waves[w]);
+  if (t < kT) lds.prefix[t + 1] = sum;
+  if (t == 0) lds.prefix[0] = 0;
   __syncthreads();
 }
 
-// A worker's piece, tile by tile: part(tile, span, u0, u1, slot).
+// The last i < kT with prefix[i] <= x: how many of the values from prefix[1] on are
+// (a wave looks at all 256 at once).
+__device__ __forceinline__ int find_part(const PlanLds &lds, long long x) {
+  const int lane = threadIdx.x & 63;
+  int n = 0;
+#pragma unroll
+  for (int i = 0; i < kT / 64; i++) n += __popcll(__ballot(lds.prefix[1 + i * 64 + lane] <= x));
+  return min(n, kT - 1);
+}
+
+// A worker's piece, step by step: part(step), which says whether its results are
+// finite. Returns whether all are.
 template <class Part>
-__device__ __forceinline__ void walk_piece(const PagedAttnArgs &a, int worker, Part part) {
-  __shared__ long long prefix[kT + 1], waves[kT / 64];
-  const PagedPlan &p = a.plan;
+__device__ __forceinline__ bool walk_piece(const PagedPlan &p, int worker, PlanLds &lds, MergeItem *item,
+                                           long long *piece_out, Part part) {
   const int per = (p.batch + kT - 1) / kT;
-  scan_costs(p, per, prefix, waves);
-  const long long total = prefix[kT], piece = plan_piece(p, total);
+  scan_costs(p, per, lds);
+  const long long total = lds.prefix[kT], piece = plan_piece(p, total);
   const long long x0 = worker * piece, x1 = min(x0 + piece, total);
-  MergeItem item = {0, 0, 0, 0, 0, 0};
+  *piece_out = piece;
+  bool finite = true;
   for (long long x = x0; x < x1;) {
-    const PieceStep st = plan_step(p, prefix, kT, per, piece, worker, x0, x1, x, &item);
+    const int i = find_part(lds, x);
+    const PagedTile t = plan_locate(p, lds.seqs, i, per, lds.prefix[i], x);
+    const PieceStep st = plan_step(p, t, piece, worker, x0, x, item);
     if (!st.more) break;
-    if (st.run) part(st.tile, st.span, st.u0, st.u1, st.slot);
-    x = st.tile.begin + st.tile.cost;
+    if (st.run && !part(st)) finite = false;
+    x = t.begin + t.cost;
   }
-  if (threadIdx.x == 0) a.items[worker] = item;
+  return finite;
+}
+
+// A worker of the main kernels.
+template <int kMergeRows, class Part>
+__device__ __forceinline__ void work_piece(const PagedAttnArgs &a, int worker, PlanLds &lds, Part part) {
+  MergeItem item = {0, 0, 0, 0, 0, 0};
+  long long piece;
+  const bool finite = walk_piece(a.plan, worker, lds, &item, &piece, part);
+  if (threadIdx.x == 0) {
+    a.items[worker] = item;
+    a.groups[worker] = item.parts > 0 ? (item.tokens * a.group + kMergeRows - 1) / kMergeRows : 0;
+    a.redo[worker] = finite ? 0 : 1;
+  }
 }
 
 __device__ __forceinline__ void wait_lds() {
@@ -177,6 +221,15 @@ __device__ __forceinline__ bool sees(const PagedAttnArgs &a, const TileSpan &s, 
 // Whether any token of the tile does.
 __device__ __forceinline__ bool tile_sees(const PagedAttnArgs &a, const TileSpan &s, int p) {
   return p < s.hi && (a.plan.window == 0 || p >= s.lo || p < s.sinks);
+}
+
+// The larger of a lane's value and lane ^ 32's. (Asm: of the builtin's two results
+// the compiler keeps one, taking them for equal. The operands need to have been
+// written two states before.)
+__device__ __forceinline__ float half_max(float x) {
+  float y = x;
+  asm("s_nop 1\n\tv_permlane32_swap_b32 %0, %1" : "+v"(x), "+v"(y));
+  return fmaxf(x, y);
 }
 
 // ---- tiles of up to 16 rows ------------------------------------------------------------
@@ -205,7 +258,7 @@ struct SmallLds {
 };
 
 template <class T, int kD>
-__device__ __forceinline__ void attn_small(const PagedAttnArgs &a, const PagedTile &t, const TileSpan &s, int u0,
+__device__ __forceinline__ bool attn_small(const PagedAttnArgs &a, const PagedTile &t, const TileSpan &s, int u0,
                                            int u1, int slot, SmallLds<T, kD> &lds) {
   typedef typename T::Vec Vec;
   typedef typename T::Value Value;
@@ -213,9 +266,8 @@ __device__ __forceinline__ void attn_small(const PagedAttnArgs &a, const PagedTi
   constexpr int kRow = kD * 2, kChunks = kD / 8, kVLoads = kUnit * kChunks / 64, kVRows = 64 / kChunks;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int r16 = lane & 15, grp = lane >> 4, rows = s.count * a.group;
-  const int row = min(r16, rows - 1), my_pos = s.pos0 + row / a.group;
-  const uint16_t *qp = a.q + ((size_t)(t.seq.row0 + s.first + row / a.group) * a.heads + t.kv_head * a.group +
-                              row % a.group) * kD + grp * 8;
+  const int row = min(r16, rows - 1), my_pos = s.pos0 + token_of(a, row);
+  const uint16_t *qp = a.q + head_row(a, t.seq.row0 + s.first, t.kv_head, row) * kD + grp * 8;
   const int *table = a.table + (size_t)t.b * a.max_pages;
   const int last_pos = s.pos0 + s.count - 1, page_mask = (1 << a.page_shift) - 1;
   Vec q[kKK];
@@ -262,6 +314,18 @@ __device__ __forceinline__ void attn_small(const PagedAttnArgs &a, const PagedTi
   // chunk c of row r lies at c ^ f(r): a transposing read's 32 lanes (8 rows, 2
   // chunks each) then hit 64 banks
   auto swz = [](int r) { return kD == 128 ? 2 * (r & 7) : 2 * ((r >> 1) & 3); };
+  const int ti = (lane >> 2) & 3, tq = lane & 3;
+  int v_to[2], v_at[kDT];  // (f repeats every 8 rows)
+#pragma unroll
+  for (int u = 0; u < 2; u++) {
+    const int r = u * kVRows + lane / kChunks;
+    v_to[u] = r * kRow + (((lane % kChunks) ^ swz(r)) * 16);
+  }
+#pragma unroll
+  for (int dt = 0; dt < kDT; dt++) {
+    const int r = 4 * grp + ti;
+    v_at[dt] = r * kRow + (((2 * dt + (tq >> 1)) ^ swz(r)) * 16) + (tq & 1) * 8;
+  }
   auto unit = [&](int j, unsigned bad, unsigned *next_bad, int *entries) __attribute__((always_inline)) {
     const int p0 = span_position(s, kUnit, j), next = j + 4;
     f32x4 sc[kBlocks];
@@ -282,11 +346,15 @@ __device__ __forceinline__ void attn_small(const PagedAttnArgs &a, const PagedTi
                        (a.plan.window == 0 || p0 > last_pos - a.plan.window || p0 + kUnit <= s.sinks);
     // V to this wave's LDS rows (LDS works in order: after the last unit's reads);
     // what no row sees as zeros
+    if (!plain) {
+#pragma unroll
+      for (int u = 0; u < kVLoads; u++)
+        if (((bad >> (u * kVRows / 16)) & 1) || !tile_sees(a, s, p0 + u * kVRows + lane / kChunks))
+          vr[u] = u32x4{0, 0, 0, 0};
+    }
 #pragma unroll
     for (int u = 0; u < kVLoads; u++) {
-      const int r = u * kVRows + lane / kChunks, c = lane % kChunks;
-      if (!plain && (((bad >> (u * kVRows / 16)) & 1) || !tile_sees(a, s, p0 + r))) vr[u] = u32x4{0, 0, 0, 0};
-      *reinterpret_cast<u32x4 *>(vl + r * kRow + ((c ^ swz(r)) * 16)) = vr[u];
+      *reinterpret_cast<u32x4 *>(vl + v_to[u & 1] + (u & ~1) * kVRows * kRow) = vr[u];
     }
     if (next < u1) {
       __builtin_amdgcn_sched_barrier(0);
@@ -295,26 +363,32 @@ __device__ __forceinline__ void attn_small(const PagedAttnArgs &a, const PagedTi
       __builtin_amdgcn_sched_barrier(0);
     }
     float mx = -INFINITY;
+    if (!plain) {
+#pragma unroll
+      for (int tt = 0; tt < kBlocks; tt++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+          if (((bad >> tt) & 1) || !sees(a, s, my_pos, p0 + 16 * tt + 4 * grp + e)) sc[tt][e] = -INFINITY;
+        }
+    }
 #pragma unroll
     for (int tt = 0; tt < kBlocks; tt++)
 #pragma unroll
-      for (int e = 0; e < 4; e++) {
-        sc[tt][e] *= a.scale_log2;
-        if (!plain && (((bad >> tt) & 1) || !sees(a, s, my_pos, p0 + 16 * tt + 4 * grp + e))) sc[tt][e] = -INFINITY;
-        mx = fmaxf(mx, sc[tt][e]);
-      }
+      for (int e = 0; e < 4; e++) mx = fmaxf(mx, sc[tt][e]);
     mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
-    mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+    mx = fmaxf(mx, __shfl_xor(mx, 32, 64)) * a.scale_log2;
     const float m = fmaxf(m_run, mx);
     const float corr = m_run == m ? 1.0f : exp2_weight(m_run - m);
     m_run = m;
+    // (a row that has seen nothing yet: its weights are exp2(-infinity))
+    const float off = (m == -INFINITY ? 0.0f : m) - T::kWeightLog2;
     float ls = 0.0f;
     Vec p[kBlocks / 2];
 #pragma unroll
     for (int tt = 0; tt < kBlocks; tt++)
 #pragma unroll
       for (int e = 0; e < 4; e++) {
-        const float w = !plain && sc[tt][e] == -INFINITY ? 0.0f : exp2_weight(sc[tt][e] - (m - T::kWeightLog2));
+        const float w = exp2_weight(fmaf(sc[tt][e], a.scale_log2, -off));
         p[tt / 2][(tt & 1) * 4 + e] = (Value)w;
         ls += w;
       }
@@ -324,18 +398,15 @@ __device__ __forceinline__ void attn_small(const PagedAttnArgs &a, const PagedTi
 #pragma unroll
       for (int e = 0; e < 4; e++) acc[dt][e] *= corr;
     wait_lds();  // this wave's V rows are in LDS
-    const int ti = (lane >> 2) & 3, tq = lane & 3;
 #pragma unroll
     for (int sl = 0; sl < kBlocks / 2; sl++)
 #pragma unroll
       for (int dt = 0; dt < kDT; dt++) {
         s16x4 half[2];
 #pragma unroll
-        for (int q2 = 0; q2 < 2; q2++) {
-          const int r = 32 * sl + 16 * q2 + 4 * grp + ti, c = 2 * dt + (tq >> 1);
-          half[q2] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((SH_PAGED_LDS s16x4 *)(
-              (SH_PAGED_LDS uint8_t *)vl + r * kRow + ((c ^ swz(r)) * 16) + (tq & 1) * 8));
-        }
+        for (int q2 = 0; q2 < 2; q2++)
+          half[q2] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+              (SH_PAGED_LDS s16x4 *)((SH_PAGED_LDS uint8_t *)vl + v_at[dt] + (32 * sl + 16 * q2) * kRow));
         const Vec vf = __builtin_bit_cast(Vec, __builtin_shufflevector(half[0], half[1], 0, 1, 2, 3, 4, 5, 6, 7));
         acc[dt] = T::mfma16(vf, p[sl], acc[dt]);
       }
@@ -385,18 +456,14 @@ __device__ __forceinline__ void attn_small(const PagedAttnArgs &a, const PagedTi
       slot_row<kD>(a, slot, r)[kD + 1] = l;
     }
   }
-  if (__syncthreads_or(finite ? 0 : 1)) {
-    attn_exact<T, kD>(a, t, s, u0, u1, slot);
-    __syncthreads();
-  }
+  return !__syncthreads_or(finite ? 0 : 1);
 }
 
 template <class T, int kD>
-__global__ __launch_bounds__(kT, 3) void paged_small_kernel(const PagedAttnArgs a) {
+__global__ __launch_bounds__(kT, kSmallWorkers / 256) void paged_small_kernel(const PagedAttnArgs a) {
   __shared__ __attribute__((aligned(16))) SmallLds<T, kD> lds;
-  walk_piece(a, blockIdx.x, [&](const PagedTile &t, const TileSpan &s, int u0, int u1, int slot) {
-    attn_small<T, kD>(a, t, s, u0, u1, slot, lds);
-  });
+  __shared__ PlanLds plan;
+  work_piece<kSmallMergeRows>(a, blockIdx.x, plan, [&](const PieceStep &st) { return attn_small<T, kD>(a, st.tile, st.span, st.u0, st.u1, st.slot, lds); });
 }
 
 // ---- tiles of up to 128 rows ------------------------------------------------------------
@@ -410,15 +477,16 @@ __global__ __launch_bounds__(kT, 3) void paged_small_kernel(const PagedAttnArgs 
 //    positions: 4 h + e for e < 4, 8 + 4 h + e - 4 after that), V by transposing reads.
 // A wave skips the units that none of its rows sees.
 constexpr int kLargeUnit = 64;
+constexpr float kSlack = 8.0f;
 
 template <int kD>
 struct LargeLds {
   uint8_t k[2][kLargeUnit * kD * 2], v[2][kLargeUnit * kD * 2];
-  unsigned bad[2][4];  // a 16-position block without a page
+  __attribute__((aligned(16))) unsigned bad[2][4];  // a 16-position block without a page
 };
 
 template <class T, int kD>
-__device__ __forceinline__ void attn_large(const PagedAttnArgs &a, const PagedTile &t, const TileSpan &s, int u0,
+__device__ __forceinline__ bool attn_large(const PagedAttnArgs &a, const PagedTile &t, const TileSpan &s, int u0,
                                            int u1, int slot, LargeLds<kD> &lds) {
   typedef typename T::Vec Vec;
   typedef typename T::Value Value;
@@ -428,12 +496,12 @@ __device__ __forceinline__ void attn_large(const PagedAttnArgs &a, const PagedTi
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int n32 = lane & 31, h = lane >> 5, rows = s.count * a.group;
   const bool active = 32 * wave < rows;  // (of the wave)
-  const int row = min(32 * wave + n32, rows - 1), my_pos = s.pos0 + row / a.group;
-  const int pos_lo = s.pos0 + min(32 * wave, rows - 1) / a.group, pos_hi = s.pos0 + min(32 * wave + 31, rows - 1) / a.group;
+  const int row = min(32 * wave + n32, rows - 1), my_pos = s.pos0 + token_of(a, row);
+  const int pos_lo = s.pos0 + token_of(a, min(32 * wave, rows - 1));
+  const int pos_hi = s.pos0 + token_of(a, min(32 * wave + 31, rows - 1));
   const int *table = a.table + (size_t)t.b * a.max_pages;
   const int page_mask = (1 << a.page_shift) - 1;
-  const uint16_t *qp = a.q + ((size_t)(t.seq.row0 + s.first + row / a.group) * a.heads + t.kv_head * a.group +
-                              row % a.group) * kD + h * 8;
+  const uint16_t *qp = a.q + head_row(a, t.seq.row0 + s.first, t.kv_head, row) * kD + h * 8;
   Vec q[kKK];
 #pragma unroll
   for (int kk = 0; kk < kKK; kk++) q[kk] = *reinterpret_cast<const Vec *>(qp + 16 * kk);
@@ -459,6 +527,7 @@ __device__ __forceinline__ void attn_large(const PagedAttnArgs &a, const PagedTi
   };
   // this wave's 16 rows of K and V of unit j to buffer j & 1. (Inline asm: through the
   // compiler's builtin, later LDS reads would wait for every load in flight.)
+  // Whether there is no page.
   auto load = [&](int j, int e) __attribute__((always_inline)) {
     const int p = span_position(s, kLargeUnit, j) + 16 * wave;
     const int page = paged_page(__builtin_amdgcn_readfirstlane(e), a.num_pages);
@@ -471,6 +540,7 @@ __device__ __forceinline__ void attn_large(const PagedAttnArgs &a, const PagedTi
       asm volatile("global_load_lds_dwordx4 %0, %1" ::"v"(k_off[u]), "s"(kb), "{m0}"(k_lds + to + u * 1024) : "memory");
       asm volatile("global_load_lds_dwordx4 %0, %1" ::"v"(v_off[u]), "s"(vb), "{m0}"(v_lds + to + u * 1024) : "memory");
     }
+    return page < 0;
   };
 
   float m_run = -INFINITY, l_run = 0.0f;
@@ -482,17 +552,27 @@ __device__ __forceinline__ void attn_large(const PagedAttnArgs &a, const PagedTi
 
   __syncthreads();  // the last tile's LDS reads are done
   int entries = 0;
+  bool none = false, none_next = false;  // this wave's 16 positions have no page
   if (u0 < u1) {
-    load(u0, entry(u0));
+    none = load(u0, entry(u0));
     entries = entry(u0 + 1);
   }
-  for (int j = u0; j < u1; j++) {
+  const int ti = (lane >> 2) & 3, tq = lane & 3, side = (lane >> 4) & 1;
+  int v_at[kDB];  // (swz_v repeats every 4 rows, swz_k every 16)
+#pragma unroll
+  for (int db = 0; db < kDB; db++) {
+    const int r = 4 * h + ti, c = 4 * db + 2 * side + (tq >> 1);
+    v_at[db] = r * kRow + ((c ^ swz_v(r)) * 16) + (tq & 1) * 8;
+  }
+  int k_at[kKK];
+#pragma unroll
+  for (int kk = 0; kk < kKK; kk++) k_at[kk] = n32 * kRow + (((2 * kk + h) ^ swz_k(n32)) * 16);
+  for (int j = u0; j < u1; j++, none = none_next) {
     const int p0 = span_position(s, kLargeUnit, j), buf = j & 1;
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     // what no row sees: zeros in V
-    if (__builtin_amdgcn_readfirstlane((int)lds.bad[buf][wave]) || p0 + 16 * wave + 16 > s.hi ||
+    if (none || p0 + 16 * wave + 16 > s.hi ||
         (a.plan.window > 0 && p0 + 16 * wave < s.lo && p0 + 16 * wave + 16 > s.sinks)) {
-      const bool none = lds.bad[buf][wave] != 0;
 #pragma unroll
       for (int u = 0; u < kLoads; u++) {
         const int r = u * kLoadRows + lane / kChunks;
@@ -502,28 +582,48 @@ __device__ __forceinline__ void attn_large(const PagedAttnArgs &a, const PagedTi
     }
     lds_barrier();
     if (j + 1 < u1) {
-      load(j + 1, entries);
+      none_next = load(j + 1, entries);
       entries = entry(j + 2);
     }
     const bool skip = !active || p0 > pos_hi ||
                       (a.plan.window > 0 && p0 + kLargeUnit <= pos_lo - a.plan.window + 1 && p0 >= s.sinks);
     if (skip) continue;
-    const unsigned bad0 = lds.bad[buf][0], bad1 = lds.bad[buf][1], bad2 = lds.bad[buf][2], bad3 = lds.bad[buf][3];
-    const unsigned bad = __builtin_amdgcn_readfirstlane(bad0 | (bad1 << 1) | (bad2 << 2) | (bad3 << 3));
-    const bool plain = bad == 0 && p0 + kLargeUnit <= pos_lo + 1 &&
-                       (a.plan.window == 0 || p0 > pos_hi - a.plan.window || p0 + kLargeUnit <= s.sinks);
+    // all K fragments requested before the first product, V's first half before the
+    // softmax and its second half before the products of the first: the compiler
+    // left to itself reads each just before its use
+    Vec kf[2][kKK];
+    const u32x4 bad4 = *reinterpret_cast<const u32x4 *>(lds.bad[buf]);
+#pragma unroll
+    for (int kk = 0; kk < kKK; kk++)
+#pragma unroll
+      for (int sb = 0; sb < 2; sb++)
+        kf[sb][kk] = *reinterpret_cast<const Vec *>(&lds.k[buf][k_at[kk] + 32 * sb * kRow]);
+    __builtin_amdgcn_sched_barrier(0);
     f32x16 sc[2];
 #pragma unroll
-    for (int sb = 0; sb < 2; sb++) {
+    for (int sb = 0; sb < 2; sb++)
 #pragma unroll
       for (int i = 0; i < 16; i++) sc[sb][i] = 0.0f;
-      const int r = 32 * sb + n32;
 #pragma unroll
-      for (int kk = 0; kk < kKK; kk++) {
-        const Vec kf = *reinterpret_cast<const Vec *>(&lds.k[buf][r * kRow + (((2 * kk + h) ^ swz_k(r)) * 16)]);
-        sc[sb] = T::mfma32(kf, q[kk], sc[sb]);
-      }
-    }
+    for (int kk = 0; kk < kKK; kk++)
+#pragma unroll
+      for (int sb = 0; sb < 2; sb++) sc[sb] = T::mfma32(kf[sb][kk], q[kk], sc[sb]);
+    __builtin_amdgcn_sched_barrier(0);
+    s16x4 vh[4][kDB][2];
+    auto read_v = [&](int ks) __attribute__((always_inline)) {
+#pragma unroll
+      for (int db = 0; db < kDB; db++)
+#pragma unroll
+        for (int q2 = 0; q2 < 2; q2++)
+          vh[ks][db][q2] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+              (SH_PAGED_LDS s16x4 *)((SH_PAGED_LDS uint8_t *)lds.v[buf] + v_at[db] + (16 * ks + 8 * q2) * kRow));
+    };
+    read_v(0);
+    read_v(1);
+    __builtin_amdgcn_sched_barrier(0);
+    const unsigned bad = __builtin_amdgcn_readfirstlane(bad4.x | (bad4.y << 1) | (bad4.z << 2) | (bad4.w << 3));
+    const bool plain = bad == 0 && p0 + kLargeUnit <= pos_lo + 1 &&
+                       (a.plan.window == 0 || p0 > pos_hi - a.plan.window || p0 + kLargeUnit <= s.sinks);
     if (!plain) {
 #pragma unroll
       for (int sb = 0; sb < 2; sb++)
@@ -538,8 +638,10 @@ __device__ __forceinline__ void attn_large(const PagedAttnArgs &a, const PagedTi
     for (int sb = 0; sb < 2; sb++)
 #pragma unroll
       for (int i = 0; i < 16; i++) mx = fmaxf(mx, sc[sb][i]);
-    mx = fmaxf(mx, __shfl_xor(mx, 32, 64)) * a.scale_log2;
-    if (__any(mx > m_run)) {
+    mx = half_max(mx) * a.scale_log2;
+    // the sums are rescaled only once a row's maximum has grown by 2^kSlack: until
+    // then its weights are up to 2^kSlack times as large
+    if (__any(mx > m_run + kSlack)) {
       const float m = fmaxf(m_run, mx);
       const float corr = m_run == m ? 1.0f : exp2_weight(m_run - m);
       m_run = m;
@@ -562,19 +664,16 @@ __device__ __forceinline__ void attn_large(const PagedAttnArgs &a, const PagedTi
         ls += w;
       }
     l_run += ls;
-    const int ti = (lane >> 2) & 3, tq = lane & 3, side = (lane >> 4) & 1;
+    __builtin_amdgcn_sched_barrier(0);
+    read_v(2);
+    read_v(3);
+    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int ks = 0; ks < 4; ks++)
 #pragma unroll
       for (int db = 0; db < kDB; db++) {
-        s16x4 half[2];
-#pragma unroll
-        for (int q2 = 0; q2 < 2; q2++) {
-          const int r = 16 * ks + 8 * q2 + 4 * h + ti, c = 4 * db + 2 * side + (tq >> 1);
-          half[q2] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((SH_PAGED_LDS s16x4 *)(
-              (SH_PAGED_LDS uint8_t *)lds.v[buf] + r * kRow + ((c ^ swz_v(r)) * 16) + (tq & 1) * 8));
-        }
-        const Vec vf = __builtin_bit_cast(Vec, __builtin_shufflevector(half[0], half[1], 0, 1, 2, 3, 4, 5, 6, 7));
+        const Vec vf = __builtin_bit_cast(
+            Vec, __builtin_shufflevector(vh[ks][db][0], vh[ks][db][1], 0, 1, 2, 3, 4, 5, 6, 7));
         acc[db] = T::mfma32(vf, p[ks], acc[db]);
       }
   }
@@ -583,8 +682,7 @@ __device__ __forceinline__ void attn_large(const PagedAttnArgs &a, const PagedTi
   if (32 * wave + n32 < rows) {
     finite = l_run < INFINITY;
     const float inv = l_run == 0.0f ? 0.0f : 1.0f / l_run;
-    uint16_t *op = a.out + ((size_t)(t.seq.row0 + s.first + row / a.group) * a.heads + t.kv_head * a.group +
-                            row % a.group) * kD;
+    uint16_t *op = a.out + head_row(a, t.seq.row0 + s.first, t.kv_head, row) * kD;
     float *sp = slot_row<kD>(a, max(slot, 0), row);
 #pragma unroll
     for (int db = 0; db < kDB; db++)
@@ -606,43 +704,161 @@ __device__ __forceinline__ void attn_large(const PagedAttnArgs &a, const PagedTi
       sp[kD + 1] = l_run;
     }
   }
-  if (__syncthreads_or(finite ? 0 : 1)) attn_exact<T, kD>(a, t, s, u0, u1, slot);
+  return !__syncthreads_or(finite ? 0 : 1);
 }
 
 template <class T, int kD>
 __global__ __launch_bounds__(kT, 2) void paged_large_kernel(const PagedAttnArgs a) {
   __shared__ __attribute__((aligned(16))) LargeLds<kD> lds;
+  __shared__ PlanLds plan;
   // consecutive pieces to one XCD: they share K and V
-  const int worker = (blockIdx.x & 7) * (kLargeWorkers / 8) + (blockIdx.x >> 3);
-  walk_piece(a, worker, [&](const PagedTile &t, const TileSpan &s, int u0, int u1, int slot) {
-    attn_large<T, kD>(a, t, s, u0, u1, slot, lds);
-  });
+  const int worker = (blockIdx.x & 7) * (a.plan.workers >> 3) + (blockIdx.x >> 3);
+  work_piece<kLargeMergeRows>(a, worker, plan, [&](const PieceStep &st) { return attn_large<T, kD>(a, st.tile, st.span, st.u0, st.u1, st.slot, lds); });
 }
 
-// grid (workers): the parts of the tile whose first inner cut is at this
-// worker's start, against their common maximum. (A part that saw nothing, of
-// maximum -infinity, has no weight.)
-template <class T, int kD>
-__global__ __launch_bounds__(kT) void paged_merge_kernel(const PagedAttnArgs a) {
-  const MergeItem it = a.items[blockIdx.x];
-  const int dim = threadIdx.x % kD;
-  for (int r = threadIdx.x / kD; it.parts > 0 && r < it.tokens * a.group; r += kT / kD) {
-    float top = -INFINITY, num = 0.0f, den = 0.0f;
-    for (int j = 0; j < it.parts; j++) {
-      const float *p = slot_row<kD>(a, j == 0 ? it.first_slot : 2 * (it.first_worker + j), r);
-      const float m = p[kD], old = top;
-      if (m == -INFINITY && p[kD + 1] == 0.0f) continue;
-      top = fmaxf(top, m);
-      const float c = old == top ? 1.0f : exp2_weight(old - top), w = m == top ? 1.0f : exp2_weight(m - top);
-      num = num * c;
-      den = den * c;
-      if (w != 0.0f || p[kD + 1] != p[kD + 1]) {  // (a part of NaN scores stays NaN)
-        num = fmaf(w, p[dim], num);
-        den = fmaf(w, p[kD + 1], den);
+// ---- the merge ---------------------------------------------------------------------------
+//
+// out = sum_j 2^(m_j - M) acc_j / sum_j 2^(m_j - M) l_j, M = max_j m_j, over the
+// parts j of a cut tile. The rows of all cut tiles are numbered through, in groups of
+// kRows (a prefix sum over the workers' items), and a group taken by kWaves waves:
+// one wave for 8 rows of large tiles, which have two or three parts, eight for a row
+// of small ones, whose parts may be spread over all workers (of 8 times kWaves parts
+// all loads are requested at once).
+// Tiles with a part that is not finite are left to workgroup w of the first such
+// worker w, which works them out in fp32, and its whole tiles too.
+struct MergeLds {
+  union {
+    int prefix[kT + 1];
+    PlanLds plan;
+  };
+  int waves[kMaxT / 64];
+};
+
+template <class T, int kD, int kThreads, int kWaves, int kRows>
+__global__ __launch_bounds__(kThreads) void paged_merge_kernel(const PagedAttnArgs a) {
+  constexpr int kStep = 8 / kRows, kDims = kD / 64;
+  typedef float Dims __attribute__((ext_vector_type(kDims)));
+  __shared__ MergeLds lds;
+  __shared__ Dims num_part[kWaves][64];
+  __shared__ float top_part[kWaves], den_part[kWaves];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  // threads of two workers each
+  static_assert(kSmallWorkers <= 2 * kT && kLargeWorkers <= 2 * kT, "two items per thread");
+  const int workers = a.plan.workers;
+  int sum = 0;
+  if (tid < kT)
+    for (int w = 2 * tid; w < min(2 * tid + 2, workers); w++) sum += a.groups[w];
+#pragma unroll
+  for (int off = 1; off < 64; off *= 2) {
+    const int o = __shfl_up(sum, off, 64);
+    if (lane >= off) sum += o;
+  }
+  if (lane == 63) lds.waves[wave] = sum;
+  __syncthreads();
+  for (int w = 0; w < wave; w++) sum += lds.waves[w];
+  if (tid < kT) lds.prefix[tid + 1] = sum;
+  if (tid == 0) lds.prefix[0] = 0;
+  __syncthreads();
+  const int total = lds.prefix[kT];
+  constexpr int kAtOnce = kThreads / 64 / kWaves;
+  for (int unit = blockIdx.x * kAtOnce + (kAtOnce > 1 ? wave / kWaves : 0); unit < total; unit += gridDim.x * kAtOnce) {
+    int n = 0;
+#pragma unroll
+    for (int i = 0; i < kT / 64; i++) n += __popcll(__ballot(lds.prefix[1 + i * 64 + lane] <= unit));
+    n = __builtin_amdgcn_readfirstlane(n);
+    int g = unit - lds.prefix[n], w = 2 * n;
+    if (g >= a.groups[w]) g -= a.groups[w++];
+    const MergeItem it = a.items[w];
+    const int r0 = g * kRows, rows = it.tokens * a.group;
+    const int part0 = kWaves == 1 ? 0 : wave;
+    float top[kRows], den[kRows];
+    Dims num[kRows];
+#pragma unroll
+    for (int i = 0; i < kRows; i++) {
+      top[i] = -INFINITY;
+      den[i] = 0.0f;
+      num[i] = 0.0f;
+    }
+    bool redo = false;
+    for (int j0 = part0; j0 < it.parts; j0 += kWaves * kStep) {
+      Dims x[kRows][kStep];
+      float m[kRows][kStep], l[kRows][kStep];
+#pragma unroll
+      for (int u = 0; u < kStep; u++) {
+        const int j = min(j0 + kWaves * u, it.parts - 1), slot = j == 0 ? it.first_slot : 2 * (it.first_worker + j);
+#pragma unroll
+        for (int i = 0; i < kRows; i++) {
+          const float *p = slot_row<kD>(a, slot, min(r0 + i, rows - 1));
+          x[i][u] = *reinterpret_cast<const Dims *>(p + lane * kDims);
+          m[i][u] = p[kD];
+          l[i][u] = p[kD + 1];
+        }
+        redo = redo || a.redo[it.first_worker + j] != 0;
+      }
+#pragma unroll
+      for (int i = 0; i < kRows; i++) {
+        float t = top[i];
+#pragma unroll
+        for (int u = 0; u < kStep; u++)
+          if (j0 + kWaves * u < it.parts) t = fmaxf(t, m[i][u]);
+        const float c = t == top[i] ? 1.0f : exp2_weight(top[i] - t);
+        top[i] = t;
+        num[i] *= c;
+        den[i] *= c;
+#pragma unroll
+        for (int u = 0; u < kStep; u++) {
+          const float f = m[i][u] == -INFINITY || j0 + kWaves * u >= it.parts ? 0.0f : exp2_weight(m[i][u] - t);
+          num[i] += f * x[i][u];
+          den[i] = fmaf(f, l[i][u], den[i]);
+        }
       }
     }
-    const size_t row = (size_t)(it.row0 + r / a.group) * a.heads + it.kv_head * a.group + r % a.group;
-    reinterpret_cast<typename T::Value *>(a.out)[row * kD + dim] = (typename T::Value)(den == 0.0f ? 0.0f : num / den);
+    if constexpr (kWaves > 1) {
+      static_assert(kRows == 1, "the waves' sums are of one row");
+      num_part[wave][lane] = num[0];
+      if (lane == 0) {
+        top_part[wave] = top[0];
+        den_part[wave] = den[0];
+      }
+      redo = __syncthreads_or(redo ? 1 : 0);
+      float t = top_part[0];
+#pragma unroll
+      for (int w2 = 1; w2 < kWaves; w2++) t = fmaxf(t, top_part[w2]);
+      num[0] = 0.0f;
+      den[0] = 0.0f;
+#pragma unroll
+      for (int w2 = 0; w2 < kWaves; w2++) {
+        const float f = top_part[w2] == -INFINITY ? 0.0f : exp2_weight(top_part[w2] - t);
+        num[0] += f * num_part[w2][lane];
+        den[0] = fmaf(f, den_part[w2], den[0]);
+      }
+      __syncthreads();
+    }
+    if (redo || (kWaves > 1 && wave != 0)) continue;
+#pragma unroll
+    for (int i = 0; i < kRows; i++) {
+      if (r0 + i >= rows) break;
+      const float inv = den[i] == 0.0f ? 0.0f : 1.0f / den[i];
+      typename T::Value *o =
+          reinterpret_cast<typename T::Value *>(a.out) + head_row(a, it.row0, it.kv_head, r0 + i) * kD + lane * kDims;
+#pragma unroll
+      for (int e = 0; e < kDims; e++) o[e] = (typename T::Value)(num[i][e] * inv);
+    }
+  }
+
+  for (int w = blockIdx.x; w < workers; w += gridDim.x) {
+    if (a.redo[w] == 0) continue;
+    __syncthreads();  // lds.prefix is read
+    MergeItem unused;
+    long long piece;
+    walk_piece(a.plan, w, lds.plan, &unused, &piece, [&](const PieceStep &st) {
+      if (st.slot >= 0)  // a cut tile is the first flagged worker's
+        for (int j = plan_first(st.tile, w, piece, w * piece); j < w; j++)
+          if (a.redo[j] != 0) return true;
+      attn_exact<T, kD>(a, st.tile, st.span);
+      return true;
+    });
+    __syncthreads();
   }
 }
 
@@ -654,7 +870,7 @@ bool small_tiles(int group, int max_new) { return group <= kSmallRows && (long l
 size_t workspace_of(const sh_paged_kv *kv, int heads, int max_new) {
   const bool small = small_tiles(heads / kv->kv_heads, max_new);
   const size_t workers = small ? kSmallWorkers : kLargeWorkers, rows = small ? kSmallRows : kLargeRows;
-  return workers * sizeof(MergeItem) + 2 * workers * rows * (kv->head_dim + 4) * 4;
+  return workers * (sizeof(MergeItem) + 2 * sizeof(int)) + 2 * workers * rows * (kv->head_dim + 4) * 4;
 }
 
 int check_attn_sizes(const sh_paged_kv *kv, int tokens, int heads, int max_new) {
@@ -663,6 +879,17 @@ int check_attn_sizes(const sh_paged_kv *kv, int tokens, int heads, int max_new) 
     return fail(SH_ERR_UNSUPPORTED, "paged head_dim %d (64 or 128 are built)", kv->head_dim);
   if (max_new < 0) return fail(SH_ERR_INVALID_ARGUMENT, "max_new must not be negative");
   return SH_OK;
+}
+
+template <class T, int kD>
+void launch(hipStream_t st, const PagedAttnArgs &a, bool small) {
+  if (small) {
+    paged_small_kernel<T, kD><<<a.plan.workers, kT, 0, st>>>(a);
+    paged_merge_kernel<T, kD, 512, 8, kSmallMergeRows><<<a.plan.workers, 512, 0, st>>>(a);
+  } else {
+    paged_large_kernel<T, kD><<<a.plan.workers, kT, 0, st>>>(a);
+    paged_merge_kernel<T, kD, kT, 1, kLargeMergeRows><<<a.plan.workers, kT, 0, st>>>(a);
+  }
 }
 
 template <class T>
@@ -695,15 +922,13 @@ int attn_paged(sh_ctx *ctx, const sh_paged_kv *kv, const uint16_t *q, uint16_t *
   a.table = kv->page_table;
   a.heads = heads;
   a.group = heads / kv->kv_heads;
+  a.group_inv = (65536 + a.group - 1) / a.group;
   a.max_pages = kv->max_pages;
   a.num_pages = kv->num_pages;
   a.page_shift = __builtin_ctz((unsigned)kv->page_size);
   const bool small = small_tiles(a.group, max_new);
-  const int workers = small ? kSmallWorkers : kLargeWorkers;
   a.tile_rows = small ? kSmallRows : kLargeRows;
   a.scale_log2 = scale * 1.44269504f;
-  a.items = static_cast<MergeItem *>(workspace);
-  a.slots = reinterpret_cast<float *>(a.items + workers);
   PagedPlan &p = a.plan;
   p.starts = kv->starts;
   p.lengths = kv->lengths;
@@ -713,25 +938,23 @@ int attn_paged(sh_ctx *ctx, const sh_paged_kv *kv, const uint16_t *q, uint16_t *
   p.capacity = kv->max_pages * kv->page_size;
   p.per_tile = a.tile_rows / a.group;
   p.unit = small ? 32 * 128 / kv->head_dim : kLargeUnit;
+  p.unit_shift = __builtin_ctz((unsigned)p.unit);
   p.window = window;
   p.sinks = sinks;
-  p.workers = workers;
   p.min_piece = small ? kSmallPiece : kLargePiece;
-  p.whole_below = 0;
+  p.workers = plan_workers(p.batch, p.kv_heads, tokens, p.capacity, p.per_tile, p.min_piece,
+                           small ? kSmallWorkers : kLargeWorkers);
+  p.inv_workers = std::nextafter(1.0 / p.workers, 2.0);
+  a.items = static_cast<MergeItem *>(workspace);
+  a.groups = reinterpret_cast<int *>(a.items + p.workers);
+  a.redo = a.groups + p.workers;
+  a.slots = reinterpret_cast<float *>(a.redo + p.workers);
+  p.whole_below = small ? kSmallWhole : kLargeWhole;
   const hipStream_t st = stream_of(ctx);
-  if (kv->head_dim == 64) {
-    if (small)
-      paged_small_kernel<T, 64><<<workers, kT, 0, st>>>(a);
-    else
-      paged_large_kernel<T, 64><<<workers, kT, 0, st>>>(a);
-    paged_merge_kernel<T, 64><<<workers, kT, 0, st>>>(a);
-  } else {
-    if (small)
-      paged_small_kernel<T, 128><<<workers, kT, 0, st>>>(a);
-    else
-      paged_large_kernel<T, 128><<<workers, kT, 0, st>>>(a);
-    paged_merge_kernel<T, 128><<<workers, kT, 0, st>>>(a);
-  }
+  if (kv->head_dim == 64)
+    launch<T, 64>(st, a, small);
+  else
+    launch<T, 128>(st, a, small);
   const hipError_t e = hipGetLastError();
   return e == hipSuccess ? SH_OK : hip_fail(e, "attn_paged");
 }

@@ -15,11 +15,12 @@ typedef __bf16 pbf16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
 // (bf16's range is fp32's, so its weights need no scale; fp16 weights are kept
-// 2^14 times as large, which leaves those down to 2^-28 normal.)
+// 2^7 times as large, which leaves those down to 2^-21 normal and those of a
+// maximum that lags behind by up to 2^8 finite.)
 struct PagedF16 {
   typedef _Float16 Value;
   typedef pf16x8 Vec;
-  static constexpr float kWeightLog2 = 14.0f;
+  static constexpr float kWeightLog2 = 7.0f;
   static __device__ __forceinline__ f32x4 mfma16(Vec a, Vec b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
   }

@@ -2,6 +2,7 @@
 // every unit of every tile once, that what is written for the merge is what it
 // reads, and that nothing indexes out of range whatever the device data are; and of
 // the argument checks of the paged operators and of sampling.
+#include <cmath>
 #include <cstdio>
 #include <cstdlib>
 #include <cstring>
@@ -30,7 +31,7 @@ static std::vector<long long> prefix_of(const PagedPlan &p, int per) {
   std::vector<long long> prefix(kParts + 1, 0);
   for (int t = 0; t < kParts; t++) {
     long long sum = 0;
-    for (int b = t * per; b < (t + 1) * per && b < p.batch; b++) sum = plan_add(sum, plan_cost(p, plan_seq(p, b)));
+    for (int b = t * per; b < (t + 1) * per && b < p.batch; b++) sum = plan_add(sum, plan_sequence(p, b).one * p.kv_heads);
     prefix[t + 1] = plan_add(prefix[t], sum);
   }
   return prefix;
@@ -47,6 +48,14 @@ static void walk(const PagedPlan &p, bool orderly, int group) {
   const int per = (p.batch + kParts - 1) / kParts;
   const std::vector<long long> prefix = prefix_of(p, per);
   const long long total = prefix[kParts], piece = plan_piece(p, total);
+  CHECK(piece * p.workers >= total);
+  // the workers that the host gives a call with these sizes have room for it, too
+  PagedPlan q = p;
+  q.workers = plan_workers(p.batch, p.kv_heads, p.tokens, p.capacity, p.per_tile, p.min_piece, 768);
+  q.inv_workers = std::nextafter(1.0 / q.workers, 2.0);
+  CHECK(q.workers > 0 && q.workers <= 768 && q.workers % 8 == 0 && plan_piece(q, total) * q.workers >= total);
+  std::vector<PlanSeq> seqs(kParts);
+  for (int b = 0; b < kParts && b < p.batch; b++) seqs[b] = plan_sequence(p, b);
   std::map<std::tuple<int, int, int>, Written> tiles;
   std::vector<MergeItem> items(p.workers);
   std::map<int, std::tuple<int, int, int>> slot_owner;
@@ -55,7 +64,10 @@ static void walk(const PagedPlan &p, bool orderly, int group) {
     const long long x0 = w * piece, x1 = x0 + piece < total ? x0 + piece : total;
     long long steps = 0;
     for (long long x = x0; x < x1;) {
-      const PieceStep s = plan_step(p, prefix.data(), kParts, per, piece, w, x0, x1, x, &item);
+      const int part = plan_find(prefix.data(), kParts, x);
+      const PagedTile tile = plan_locate(p, seqs.data(), part, per, prefix[part], x);
+      const PieceStep s = plan_step(p, tile, piece, w, x0, x, &item);
+      if (orderly) CHECK(plan_first(tile, w, piece, x0) == (int)(tile.begin / piece));
       CHECK(s.tile.b >= 0 && s.tile.b < p.batch);
       CHECK(s.tile.kv_head >= 0 && s.tile.kv_head < p.kv_heads);
       CHECK(s.span.count >= 0 && s.span.count <= p.per_tile);
@@ -168,10 +180,12 @@ int main() {
     const int group = 1 + upto(round % 5 == 0 ? 127 : 15);
     const int rows = group > 16 ? 128 : (round & 1) ? 16 : 128;
     p.per_tile = rows / group;
-    p.unit = 64 << upto(2);
+    p.unit_shift = 6 + upto(2);
+    p.unit = 1 << p.unit_shift;
     p.window = round % 3 == 0 ? 1 + upto(p.capacity) : 0;
     p.sinks = upto(round % 2 ? 8 : p.capacity);
-    p.workers = 8 << upto(6);
+    p.workers = 8 * (1 + upto(99));
+    p.inv_workers = std::nextafter(1.0 / p.workers, 2.0);
     p.min_piece = 64 << upto(3);
     p.whole_below = round % 2 ? 0 : upto(2000);
     std::vector<int> starts(p.batch + 1), lengths(p.batch);
@@ -195,8 +209,10 @@ int main() {
     p.capacity = kMaxPagedPositions;
     p.per_tile = 1;
     p.unit = 64;
+    p.unit_shift = 6;
     p.window = p.sinks = 0;
     p.workers = 64;
+    p.inv_workers = std::nextafter(1.0 / 64, 2.0);
     p.min_piece = 256;
     p.whole_below = 0;
     std::vector<int> starts(p.batch + 1), lengths(p.batch, kMaxPagedPositions);
@@ -210,7 +226,9 @@ int main() {
     const long long piece = plan_piece(p, prefix[kParts]);
     for (int w = 0; w < p.workers; w++) {
       MergeItem item = {0, 0, 0, 0, 0, 0};
-      const PieceStep s = plan_step(p, prefix.data(), kParts, per, piece, w, w * piece, (w + 1) * piece, w * piece, &item);
+      const int part = plan_find(prefix.data(), kParts, w * piece);
+      const PagedTile tile = plan_locate(p, nullptr, part, per, prefix[part], w * piece);
+      const PieceStep s = plan_step(p, tile, piece, w, w * piece, w * piece, &item);
       CHECK(s.tile.b >= 0 && s.tile.b < p.batch && s.tile.kv_head < p.kv_heads);
       CHECK(s.u0 >= 0 && s.u1 <= s.span.units);
     }

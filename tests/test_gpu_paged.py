@@ -99,12 +99,12 @@ def attention_oracle(c, q, window, sinks, scale):
                         some = w > 0
                         ref[row, h] = w[some] @ vs[some] if not np.isnan(w).any() else np.nan
                         # a score: d products and sums, the scale; its weight: that, 2^x, its rounding to 16 bits
-                        # (or below fp16's 2^-28); the sums: a rounding and a rescaling per position; the output's
+                        # (below fp16's 2^-14, at 2^7 times the weight, by up to 2^-25: 2^-32 of it); the sums: a rounding and a rescaling per position; the output's
                         a = w[some] @ np.abs(vs[some])
                         ds = scale * (np.abs(ks[some]) @ np.abs(q[row, h])).max(initial=0.0) * (c.d + 4) * F
                         n = len(s)
                         tol[row, h] = (u * np.abs(ref[row, h]) + u * a * (1 + u) + a * (2 * ds + (2 * n + 16) * F)
-                                       + n * 2.0 ** -39 * np.abs(vs).max() + 2.0 ** -25)
+                                       + n * 2.0 ** -32 * np.abs(vs).max() + 2.0 ** -25)
     return ref, tol
 
 
