@@ -115,11 +115,19 @@ SH_HD PlanSeq plan_sequence(const PagedPlan &p, int b) {
   return s;
 }
 
+// The cost of the sequence's last tile, its largest.
+SH_HD long long plan_last(const PagedPlan &p, const PlanSeq &s) {
+  return s.tiles > 1 ? s.one - plan_prefix(p, s.seq, s.tiles - 1) : s.one;
+}
+
 // (At least total / workers: inv_workers is rounded up, and what a product in fp64
-// loses of a total below 2^61 is added.)
-SH_HD long long plan_piece(const PagedPlan &p, long long total) {
+// loses of a total below 2^61 is added.) A piece that is somewhat shorter than the
+// largest tile becomes as long: most tiles then fit one and need no merge. Of 448
+// tiles of one cost over 512 workers: 87 -> 73 us a call.
+SH_HD long long plan_piece(const PagedPlan &p, long long total, long long largest) {
   const long long q = (long long)((double)total * p.inv_workers) + (total >> 50) + 1;
-  return q > p.min_piece ? q : p.min_piece;
+  const long long r = q < largest && 8 * q >= 5 * largest ? largest : q;
+  return r > p.min_piece ? r : p.min_piece;
 }
 
 // Workers for a call: `most`, or fewer where even full tables would not give each of
@@ -152,13 +160,16 @@ SH_HD int plan_find(const long long *prefix, int parts, long long x) {
 }
 
 // The tile that point x of the line lies in. at: cost of the sequences before part *
-// per, the sequence of x among the `per` from there on. seqs: the sequences where
-// per is 1 (worked out again otherwise).
-SH_HD PagedTile plan_locate(const PagedPlan &p, const PlanSeq *seqs, int part, int per, long long at, long long x) {
+// per, of which `s` is the first (plan_part_first), the sequence of x among the `per`
+// from there on.
+SH_HD int plan_part_first(const PagedPlan &p, int part, int per) {
+  const int end = (part + 1) * per < p.batch ? (part + 1) * per : p.batch;
+  return part * per < end ? part * per : end - 1;
+}
+SH_HD PagedTile plan_locate(const PagedPlan &p, PlanSeq s, int part, int per, long long at, long long x) {
   PagedTile t;
   const int end = (part + 1) * per < p.batch ? (part + 1) * per : p.batch;
-  t.b = part * per < end ? part * per : end - 1;
-  PlanSeq s = per == 1 ? seqs[t.b] : plan_sequence(p, t.b);
+  t.b = plan_part_first(p, part, per);
   while (x >= at + s.one * p.kv_heads && t.b + 1 < end) {
     at += s.one * p.kv_heads;
     s = plan_sequence(p, ++t.b);

@@ -28,10 +28,15 @@ constexpr int kT = 256, kMaxT = 512;
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 #define SH_PAGED_LDS __attribute__((address_space(3)))
 
-// Pieces of a call, and the shortest, in positions: three workgroups per CU are
-// resident with the small tiles, two with the large ones.
-constexpr int kSmallRows = 16, kSmallWorkers = 512, kSmallPiece = 128, kSmallWhole = 192, kSmallMergeRows = 1;
-constexpr int kLargeRows = 128, kLargeWorkers = 512, kLargePiece = 256, kLargeWhole = 1400, kLargeMergeRows = 8;
+// How a call is divided: rows of a tile, pieces at most (as many as workgroups are
+// resident), the shortest piece and the tiles that are not cut, in positions.
+struct Variant {
+  int rows, workers, min_piece, whole_below;
+};
+constexpr Variant kSmall = {16, 512, 128, 192}, kLarge = {128, 512, 256, 256};
+constexpr int kMaxWorkers = 512;
+// Rows that the merge kernel takes at once.
+constexpr int kSmallMergeRows = 1, kLargeMergeRows = 4;
 
 struct PagedAttnArgs {
   const uint16_t *q, *k, *v;
@@ -75,6 +80,16 @@ __device__ __forceinline__ void store_value(const PagedAttnArgs &a, const PagedT
 
 __device__ __forceinline__ float exp2_weight(float x) { return __builtin_amdgcn_exp2f(x); }
 
+// What a token at position `pos` sees of the positions from p on: i of them on if
+// i <= last and (i >= first or i < sinks). (As limits of i, which the compiler has as
+// constants: as positions it would keep all of them in registers.)
+struct Sees {
+  int last, first, sinks;
+  __device__ __forceinline__ Sees(const PagedAttnArgs &a, const TileSpan &s, int pos, int p)
+      : last(pos - p), first(a.plan.window == 0 ? -p : pos - a.plan.window + 1 - p), sinks(s.sinks - p) {}
+  __device__ __forceinline__ bool operator()(int i) const { return i <= last && (i >= first || i < sinks); }
+};
+
 // A tile in fp32, a wave per row, a lane per position of 64:
 // whatever the values are. A score of -infinity, and a weight that is 0 in fp32,
 // adds nothing. Slow: for tiles whose sums by MFMA are not finite.
@@ -94,7 +109,7 @@ __device__ void attn_exact(const PagedAttnArgs &a, const PagedTile &t, const Til
       const int p0 = span_position(s, a.plan.unit, u), end = min(p0 + a.plan.unit, s.hi);
       for (int pt = p0; pt < end; pt += 64) {
         const int p = pt + lane;
-        bool seen = p < end && p <= pos && (a.plan.window == 0 || p > pos - a.plan.window || p < s.sinks);
+        bool seen = p < end && Sees(a, s, pos, p)(0);
         long long at = 0;  // of the position's k and v
         if (seen) {
           const int page = paged_page(a.table[(size_t)t.b * a.max_pages + (p >> a.page_shift)], a.num_pages);
@@ -131,31 +146,43 @@ __device__ void attn_exact(const PagedAttnArgs &a, const PagedTile &t, const Til
 
 // The line's division among the workers, in LDS.
 struct PlanLds {
-  long long prefix[kT + 1], waves[kMaxT / 64];
+  long long prefix[kT + 1], waves[kMaxT / 64], largest[kMaxT / 64];
   PlanSeq seqs[kT];  // where a thread has one sequence
+  long long x, piece;  // the next step's point (here and not in registers)
 };
 
 // Prefix sums of the sequences' costs, by kT threads (of kT or more) of `per`
 // sequences each.
 __device__ __forceinline__ void scan_costs(const PagedPlan &p, int per, PlanLds &lds) {
   const int t = threadIdx.x, lane = t & 63;
-  long long sum = 0;
+  long long sum = 0, largest = 0;
   for (int b = t * per; b < min((t + 1) * per, p.batch); b++) {
     const PlanSeq s = plan_sequence(p, b);
     if (per == 1) lds.seqs[t] = s;
     sum = plan_add(sum, s.one * p.kv_heads);
+    largest = max(largest, plan_last(p, s));
   }
 #pragma unroll
   for (int off = 1; off < 64; off *= 2) {
-    const long long o = __shfl_up(sum, off, 64);
+    const long long o = __shfl_up(sum, off, 64), l = __shfl_up(largest, off, 64);
     if (lane >= off) sum = plan_add(sum, o);
+    if (lane >= off) largest = max(largest, l);
   }
-  if (lane == 63) lds.waves[t >> 6] = sum;
+  if (lane == 63) {
+    lds.waves[t >> 6] = sum;
+    lds.largest[t >> 6] = largest;
+  }
   __syncthreads();
   for (int w = 0; w < (t >> 6); w++) sum = plan_add(sum, lds.waves[w]);
   if (t < kT) lds.prefix[t + 1] = sum;
   if (t == 0) lds.prefix[0] = 0;
   __syncthreads();
+}
+
+// A value that is the same in every lane, as the compiler cannot know of one from LDS.
+__device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
+__device__ __forceinline__ long long uniform(long long x) {
+  return (long long)(((uint64_t)(uint32_t)uniform((int)(x >> 32)) << 32) | (uint32_t)uniform((int)x));
 }
 
 // The last i < kT with prefix[i] <= x: how many of the values from prefix[1] on are
@@ -172,20 +199,41 @@ __device__ __forceinline__ int find_part(const PlanLds &lds, long long x) {
 // finite. Returns whether all are.
 template <class Part>
 __device__ __forceinline__ bool walk_piece(const PagedPlan &p, int worker, PlanLds &lds, MergeItem *item,
-                                           long long *piece_out, Part part) {
+                                           Part part) {
   const int per = (p.batch + kT - 1) / kT;
   scan_costs(p, per, lds);
-  const long long total = lds.prefix[kT], piece = plan_piece(p, total);
-  const long long x0 = worker * piece, x1 = min(x0 + piece, total);
-  *piece_out = piece;
+  if (threadIdx.x == 0) {
+    long long largest = 0;
+    for (int w = 0; w < kT / 64; w++) largest = max(largest, lds.largest[w]);
+    lds.piece = plan_piece(p, lds.prefix[kT], largest);
+    lds.x = worker * lds.piece;
+  }
+  __syncthreads();
   bool finite = true;
-  for (long long x = x0; x < x1;) {
-    const int i = find_part(lds, x);
-    const PagedTile t = plan_locate(p, lds.seqs, i, per, lds.prefix[i], x);
-    const PieceStep st = plan_step(p, t, piece, worker, x0, x, item);
+  while (true) {
+    const long long total = uniform(lds.prefix[kT]), piece = uniform(lds.piece), x0 = worker * piece;
+    const long long x = uniform(lds.x);
+    if (x >= min(x0 + piece, total)) break;
+    const int i = uniform(find_part(lds, x)), b = plan_part_first(p, i, per);
+    PlanSeq first;
+    if (per == 1) {
+      const PlanSeq &f = lds.seqs[b];
+      first = {{uniform(f.seq.row0), uniform(f.seq.n), uniform(f.seq.len)}, uniform(f.tiles), uniform(f.one)};
+    } else {
+      first = plan_sequence(p, b);
+    }
+    const PagedTile t = plan_locate(p, first, i, per, uniform(lds.prefix[i]), x);
+    PieceStep st = plan_step(p, t, piece, worker, x0, x, item);
+    // (64-bit comparisons are vector instructions, and what is selected by them too)
+    for (int *v : {&st.tile.seq.row0, &st.tile.seq.n, &st.tile.seq.len, &st.tile.b, &st.tile.kv_head, &st.tile.tile,
+                   &st.span.first, &st.span.count, &st.span.pos0, &st.span.lo, &st.span.hi, &st.span.sinks,
+                   &st.span.units, &st.span.sink_units, &st.span.gap, &st.u0, &st.u1, &st.slot})
+      *v = uniform(*v);
+    __syncthreads();  // lds.x is read
+    if (threadIdx.x == 0) lds.x = t.begin + t.cost;
+    __syncthreads();
     if (!st.more) break;
-    if (st.run && !part(st)) finite = false;
-    x = t.begin + t.cost;
+    if (st.run && !part(st, piece)) finite = false;
   }
   return finite;
 }
@@ -194,8 +242,7 @@ __device__ __forceinline__ bool walk_piece(const PagedPlan &p, int worker, PlanL
 template <int kMergeRows, class Part>
 __device__ __forceinline__ void work_piece(const PagedAttnArgs &a, int worker, PlanLds &lds, Part part) {
   MergeItem item = {0, 0, 0, 0, 0, 0};
-  long long piece;
-  const bool finite = walk_piece(a.plan, worker, lds, &item, &piece, part);
+  const bool finite = walk_piece(a.plan, worker, lds, &item, part);
   if (threadIdx.x == 0) {
     a.items[worker] = item;
     a.groups[worker] = item.parts > 0 ? (item.tokens * a.group + kMergeRows - 1) / kMergeRows : 0;
@@ -214,10 +261,6 @@ __device__ __forceinline__ void lds_barrier() {
   __atomic_signal_fence(__ATOMIC_SEQ_CST);
 }
 
-// Whether token position `pos` sees position p of the tile's span.
-__device__ __forceinline__ bool sees(const PagedAttnArgs &a, const TileSpan &s, int pos, int p) {
-  return p <= pos && (a.plan.window == 0 || p > pos - a.plan.window || p < s.sinks);
-}
 // Whether any token of the tile does.
 __device__ __forceinline__ bool tile_sees(const PagedAttnArgs &a, const TileSpan &s, int p) {
   return p < s.hi && (a.plan.window == 0 || p >= s.lo || p < s.sinks);
@@ -231,6 +274,23 @@ __device__ __forceinline__ float half_max(float x) {
   asm("s_nop 1\n\tv_permlane32_swap_b32 %0, %1" : "+v"(x), "+v"(y));
   return fmaxf(x, y);
 }
+
+// x *= f where `really` is not 0 (the same in every lane), in place, x in the
+// registers named. (Asm, with the branch inside: of a branch around the products the
+// compiler keeps both versions of an accumulator and moves one to the other. The
+// pauses are what a product's result and its next addend need, which the compiler
+// does not add for asm.)
+#define SH_SCALE(x, f, really, r0, r1, r2, r3, r4, r5, r6, r7, r8, r9, ra, rb, rc, rd, re, rf)                      \
+  asm volatile("s_cmp_eq_u32 %2, 0\n\ts_cbranch_scc1 .Lpaged_scale%=\n\ts_nop 15\n\ts_nop 3\n\t"                    \
+               "v_mul_f32 v" #r0 ", %1, v" #r0 "\n\tv_mul_f32 v" #r1 ", %1, v" #r1 "\n\tv_mul_f32 v" #r2 ", %1, v" #r2   \
+               "\n\tv_mul_f32 v" #r3 ", %1, v" #r3 "\n\tv_mul_f32 v" #r4 ", %1, v" #r4 "\n\tv_mul_f32 v" #r5 ", %1, v" #r5 \
+               "\n\tv_mul_f32 v" #r6 ", %1, v" #r6 "\n\tv_mul_f32 v" #r7 ", %1, v" #r7 "\n\tv_mul_f32 v" #r8 ", %1, v" #r8 \
+               "\n\tv_mul_f32 v" #r9 ", %1, v" #r9 "\n\tv_mul_f32 v" #ra ", %1, v" #ra "\n\tv_mul_f32 v" #rb ", %1, v" #rb \
+               "\n\tv_mul_f32 v" #rc ", %1, v" #rc "\n\tv_mul_f32 v" #rd ", %1, v" #rd "\n\tv_mul_f32 v" #re ", %1, v" #re \
+               "\n\tv_mul_f32 v" #rf ", %1, v" #rf "\n\ts_nop 3\n.Lpaged_scale%=:"                                  \
+               : "+{v[" #r0 ":" #rf "]}"(x)                                                                          \
+               : "v"(f), "s"(really)                                                                                \
+               : "scc")
 
 // ---- tiles of up to 16 rows ------------------------------------------------------------
 //
@@ -252,9 +312,9 @@ template <class T, int kD>
 struct SmallLds {
   union {
     uint8_t v[4][kSmallUnit<kD> * kD * 2];
-    float acc[4][kSmallRows][kD];
+    float acc[4][kSmall.rows][kD];
   };
-  float stat[4][kSmallRows][2];
+  float stat[4][kSmall.rows][2];
 };
 
 template <class T, int kD>
@@ -364,12 +424,12 @@ __device__ __forceinline__ bool attn_small(const PagedAttnArgs &a, const PagedTi
     }
     float mx = -INFINITY;
     if (!plain) {
+      const Sees seen(a, s, my_pos, p0 + 4 * grp);
 #pragma unroll
       for (int tt = 0; tt < kBlocks; tt++)
 #pragma unroll
-        for (int e = 0; e < 4; e++) {
-          if (((bad >> tt) & 1) || !sees(a, s, my_pos, p0 + 16 * tt + 4 * grp + e)) sc[tt][e] = -INFINITY;
-        }
+        for (int e = 0; e < 4; e++)
+          if (((bad >> tt) & 1) || !seen(16 * tt + e)) sc[tt][e] = -INFINITY;
     }
 #pragma unroll
     for (int tt = 0; tt < kBlocks; tt++)
@@ -460,10 +520,10 @@ __device__ __forceinline__ bool attn_small(const PagedAttnArgs &a, const PagedTi
 }
 
 template <class T, int kD>
-__global__ __launch_bounds__(kT, kSmallWorkers / 256) void paged_small_kernel(const PagedAttnArgs a) {
+__global__ __launch_bounds__(kT, kSmall.workers / 256) void paged_small_kernel(const PagedAttnArgs a) {
   __shared__ __attribute__((aligned(16))) SmallLds<T, kD> lds;
   __shared__ PlanLds plan;
-  work_piece<kSmallMergeRows>(a, blockIdx.x, plan, [&](const PieceStep &st) { return attn_small<T, kD>(a, st.tile, st.span, st.u0, st.u1, st.slot, lds); });
+  work_piece<kSmallMergeRows>(a, blockIdx.x, plan, [&](const PieceStep &st, long long) { return attn_small<T, kD>(a, st.tile, st.span, st.u0, st.u1, st.slot, lds); });
 }
 
 // ---- tiles of up to 128 rows ------------------------------------------------------------
@@ -475,7 +535,6 @@ __global__ __launch_bounds__(kT, kSmallWorkers / 256) void paged_small_kernel(co
 //  - scores as K x q, 32 x 32 positions and rows, K fragments from LDS;
 //  - V sums as V^T x P with the k slots numbered as P has them (slot (h, e) of 16
 //    positions: 4 h + e for e < 4, 8 + 4 h + e - 4 after that), V by transposing reads.
-// A wave skips the units that none of its rows sees.
 constexpr int kLargeUnit = 64;
 constexpr float kSlack = 8.0f;
 
@@ -510,13 +569,11 @@ __device__ __forceinline__ bool attn_large(const PagedAttnArgs &a, const PagedTi
   // hit all banks, and 32 lanes of a transposing read of V (4 rows, 4 chunks each)
   auto swz_k = [](int r) { return kD == 128 ? r & 15 : (r >> 1) & 7; };
   auto swz_v = [](int r) { return kD == 128 ? 4 * (r & 3) : 4 * ((r >> 1) & 1); };
-  uint32_t k_off[kLoads], v_off[kLoads];
-#pragma unroll
-  for (int u = 0; u < kLoads; u++) {
-    const int r = u * kLoadRows + lane / kChunks, c = lane % kChunks;
-    k_off[u] = r * kRow + ((c ^ swz_k(r)) * 16);
-    v_off[u] = r * kRow + ((c ^ swz_v(r)) * 16);
-  }
+  // (both f only flip bits of the chunk that a load, a step kk or a block db counts
+  // up, so that one offset each serves all of them)
+  const int load_row = lane / kChunks, load_chunk = lane % kChunks;
+  const uint32_t k_off = load_row * kRow + ((load_chunk ^ swz_k(load_row)) * 16);
+  const uint32_t v_off = load_row * kRow + ((load_chunk ^ swz_v(load_row)) * 16);
   const uint32_t k_lds = (uint32_t)(uintptr_t)(SH_PAGED_LDS uint8_t *)lds.k[0];
   const uint32_t v_lds = (uint32_t)(uintptr_t)(SH_PAGED_LDS uint8_t *)lds.v[0];
   constexpr uint32_t kBuffer = kLargeUnit * kD * 2, kWave = 16 * kRow;
@@ -525,22 +582,36 @@ __device__ __forceinline__ bool attn_large(const PagedAttnArgs &a, const PagedTi
     const int p = span_position(s, kLargeUnit, min(j, u1 - 1)) + 16 * wave;
     return table[min(p >> a.page_shift, a.max_pages - 1)];
   };
-  // this wave's 16 rows of K and V of unit j to buffer j & 1. (Inline asm: through the
-  // compiler's builtin, later LDS reads would wait for every load in flight.)
-  // Whether there is no page.
-  auto load = [&](int j, int e) __attribute__((always_inline)) {
+  // this wave's 16 rows of K and V of unit j (their addresses; whether there is no
+  // page), then load u of them to buffer j & 1, or nothing. (Inline asm: through the
+  // compiler's builtin, later LDS reads would wait for every load in flight. The branch
+  // is inside, so that the products around it stay one block to the scheduler.)
+  uint64_t k_from = 0, v_from = 0;
+  uint32_t to = 0;
+  auto place = [&](int j, int e) __attribute__((always_inline)) {
     const int p = span_position(s, kLargeUnit, j) + 16 * wave;
     const int page = paged_page(__builtin_amdgcn_readfirstlane(e), a.num_pages);
     if (lane == 0) lds.bad[j & 1][wave] = page < 0 ? 1 : 0;
     const size_t at = ((((size_t)max(page, 0) * a.plan.kv_heads + t.kv_head) << a.page_shift) + (p & page_mask)) * kRow;
-    const uint64_t kb = (uint64_t)(uintptr_t)a.k + at, vb = (uint64_t)(uintptr_t)a.v + at;
-    const uint32_t to = (j & 1) * kBuffer + wave * kWave;
-#pragma unroll
-    for (int u = 0; u < kLoads; u++) {
-      asm volatile("global_load_lds_dwordx4 %0, %1" ::"v"(k_off[u]), "s"(kb), "{m0}"(k_lds + to + u * 1024) : "memory");
-      asm volatile("global_load_lds_dwordx4 %0, %1" ::"v"(v_off[u]), "s"(vb), "{m0}"(v_lds + to + u * 1024) : "memory");
-    }
+    k_from = (uint64_t)(uintptr_t)a.k + at;
+    v_from = (uint64_t)(uintptr_t)a.v + at;
+    to = (j & 1) * kBuffer + wave * kWave;
     return page < 0;
+  };
+  auto load = [&](int u, int really) __attribute__((always_inline)) {
+    asm volatile(
+        "s_cmp_eq_u32 %6, 0\n\t"
+        "s_cbranch_scc1 .Lpaged_load%=\n\t"
+        "s_mov_b32 m0, %4\n\t"
+        "s_nop 0\n\t"
+        "global_load_lds_dwordx4 %0, %2\n\t"
+        "s_mov_b32 m0, %5\n\t"
+        "s_nop 0\n\t"
+        "global_load_lds_dwordx4 %1, %3\n"
+        ".Lpaged_load%=:"
+        ::"v"(k_off ^ (64 * u)), "v"(v_off), "s"(k_from + u * 1024), "s"(v_from + u * 1024),
+        "s"(k_lds + to + u * 1024), "s"(v_lds + to + u * 1024), "s"(uniform(really))
+        : "memory", "scc");
   };
 
   float m_run = -INFINITY, l_run = 0.0f;
@@ -552,52 +623,67 @@ __device__ __forceinline__ bool attn_large(const PagedAttnArgs &a, const PagedTi
 
   __syncthreads();  // the last tile's LDS reads are done
   int entries = 0;
-  bool none = false, none_next = false;  // this wave's 16 positions have no page
+  bool none = false;  // this wave's 16 positions have no page
   if (u0 < u1) {
-    none = load(u0, entry(u0));
+    none = place(u0, entry(u0));
+#pragma unroll
+    for (int u = 0; u < kLoads; u++) load(u, 1);
     entries = entry(u0 + 1);
   }
   const int ti = (lane >> 2) & 3, tq = lane & 3, side = (lane >> 4) & 1;
-  int v_at[kDB];  // (swz_v repeats every 4 rows, swz_k every 16)
-#pragma unroll
-  for (int db = 0; db < kDB; db++) {
-    const int r = 4 * h + ti, c = 4 * db + 2 * side + (tq >> 1);
-    v_at[db] = r * kRow + ((c ^ swz_v(r)) * 16) + (tq & 1) * 8;
-  }
-  int k_at[kKK];
-#pragma unroll
-  for (int kk = 0; kk < kKK; kk++) k_at[kk] = n32 * kRow + (((2 * kk + h) ^ swz_k(n32)) * 16);
-  for (int j = u0; j < u1; j++, none = none_next) {
-    const int p0 = span_position(s, kLargeUnit, j), buf = j & 1;
+  const int v_at0 = (4 * h + ti) * kRow + (((2 * side + (tq >> 1)) ^ swz_v(4 * h + ti)) * 16) + (tq & 1) * 8;
+  const int k_at0 = n32 * kRow + ((h ^ swz_k(n32)) * 16);
+  // the loads of unit j are here and what no row sees is zeros in V
+  auto arrive = [&](int j) __attribute__((always_inline)) {
+    const int p = span_position(s, kLargeUnit, j) + 16 * wave;
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    // what no row sees: zeros in V
-    if (none || p0 + 16 * wave + 16 > s.hi ||
-        (a.plan.window > 0 && p0 + 16 * wave < s.lo && p0 + 16 * wave + 16 > s.sinks)) {
+    if (none || p + 16 > s.hi || (a.plan.window > 0 && p < s.lo && p + 16 > s.sinks)) {
 #pragma unroll
       for (int u = 0; u < kLoads; u++) {
-        const int r = u * kLoadRows + lane / kChunks;
-        if (none || !tile_sees(a, s, p0 + 16 * wave + r))
-          *reinterpret_cast<u32x4 *>(&lds.v[buf][wave * kWave + u * 1024 + lane * 16]) = u32x4{0, 0, 0, 0};
+        if (none || !tile_sees(a, s, p + u * kLoadRows + load_row))
+          *reinterpret_cast<u32x4 *>(&lds.v[j & 1][wave * kWave + u * 1024 + lane * 16]) = u32x4{0, 0, 0, 0};
       }
     }
     lds_barrier();
-    if (j + 1 < u1) {
-      none_next = load(j + 1, entries);
-      entries = entry(j + 2);
-    }
-    const bool skip = !active || p0 > pos_hi ||
-                      (a.plan.window > 0 && p0 + kLargeUnit <= pos_lo - a.plan.window + 1 && p0 >= s.sinks);
-    if (skip) continue;
-    // all K fragments requested before the first product, V's first half before the
-    // softmax and its second half before the products of the first: the compiler
-    // left to itself reads each just before its use
-    Vec kf[2][kKK];
-    const u32x4 bad4 = *reinterpret_cast<const u32x4 *>(lds.bad[buf]);
+  };
+  if (!active) {  // a wave without rows loads its part
+    for (int j = u0; j < u1; j++) {
+      arrive(j);
+      if (j + 1 < u1) {
+        none = place(j + 1, entries);
 #pragma unroll
-    for (int kk = 0; kk < kKK; kk++)
+        for (int u = 0; u < kLoads; u++) load(u, 1);
+        entries = entry(j + 2);
+      }
+    }
+  }
+  for (int j = active ? u0 : u1; j < u1; j++) {
+    const int p0 = span_position(s, kLargeUnit, j), buf = j & 1, more = j + 1 < u1 ? 1 : 0;
+    arrive(j);
+    // Fragments are requested ahead of the products that take them (the compiler left
+    // to itself reads each just before its use), and the next unit's loads spread over
+    // the products of the scores (requested together they held the wave up for a fifth
+    // of the unit).
+    Vec kf[2][kKK];
+    s16x4 vh[4][kDB][2];
+    const int k_at = k_at0 + buf * (int)kBuffer, v_at = v_at0 + buf * (int)kBuffer;
+    auto read_v = [&](int ks) __attribute__((always_inline)) {
+#pragma unroll
+      for (int db = 0; db < kDB; db++)
+#pragma unroll
+        for (int q2 = 0; q2 < 2; q2++)
+          vh[ks][db][q2] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+              (SH_PAGED_LDS s16x4 *)((SH_PAGED_LDS uint8_t *)lds.v[0] + (v_at ^ (64 * db)) + (16 * ks + 8 * q2) * kRow));
+    };
+    auto read_k = [&](int kk) __attribute__((always_inline)) {
 #pragma unroll
       for (int sb = 0; sb < 2; sb++)
-        kf[sb][kk] = *reinterpret_cast<const Vec *>(&lds.k[buf][k_at[kk] + 32 * sb * kRow]);
+        kf[sb][kk] = *reinterpret_cast<const Vec *>(lds.k[0] + (k_at ^ (32 * kk)) + 32 * sb * kRow);
+    };
+    constexpr int kAhead = 4;
+#pragma unroll
+    for (int kk = 0; kk < kAhead; kk++) read_k(kk);
+    const u32x4 bad4 = *reinterpret_cast<const u32x4 *>(lds.bad[buf]);
     __builtin_amdgcn_sched_barrier(0);
     f32x16 sc[2];
 #pragma unroll
@@ -605,19 +691,20 @@ __device__ __forceinline__ bool attn_large(const PagedAttnArgs &a, const PagedTi
 #pragma unroll
       for (int i = 0; i < 16; i++) sc[sb][i] = 0.0f;
 #pragma unroll
-    for (int kk = 0; kk < kKK; kk++)
+    for (int kk = 0; kk < kKK; kk++) {
 #pragma unroll
       for (int sb = 0; sb < 2; sb++) sc[sb] = T::mfma32(kf[sb][kk], q[kk], sc[sb]);
-    __builtin_amdgcn_sched_barrier(0);
-    s16x4 vh[4][kDB][2];
-    auto read_v = [&](int ks) __attribute__((always_inline)) {
-#pragma unroll
-      for (int db = 0; db < kDB; db++)
-#pragma unroll
-        for (int q2 = 0; q2 < 2; q2++)
-          vh[ks][db][q2] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-              (SH_PAGED_LDS s16x4 *)((SH_PAGED_LDS uint8_t *)lds.v[buf] + v_at[db] + (16 * ks + 8 * q2) * kRow));
-    };
+      __builtin_amdgcn_sched_barrier(0);
+      if (kk + kAhead < kKK) read_k(kk + kAhead);
+      if (kk == 0) none = place(min(j + 1, u1 - 1), entries);
+      if (kk % 2 == 1) load(kk / 2, more);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    static_assert(kLoads == kKK / 2, "a pair of loads every other step");
+    // (a wave in its softmax before one in its products, which take turns: 610 -> 599 us
+    // for 8,192 tokens over 12,288 positions)
+    __builtin_amdgcn_s_setprio(1);
+    entries = entry(j + 2);
     read_v(0);
     read_v(1);
     __builtin_amdgcn_sched_barrier(0);
@@ -625,13 +712,12 @@ __device__ __forceinline__ bool attn_large(const PagedAttnArgs &a, const PagedTi
     const bool plain = bad == 0 && p0 + kLargeUnit <= pos_lo + 1 &&
                        (a.plan.window == 0 || p0 > pos_hi - a.plan.window || p0 + kLargeUnit <= s.sinks);
     if (!plain) {
+      const Sees seen(a, s, my_pos, p0 + 4 * h);
 #pragma unroll
       for (int sb = 0; sb < 2; sb++)
 #pragma unroll
-        for (int i = 0; i < 16; i++) {
-          const int key = 32 * sb + 8 * (i / 4) + 4 * h + i % 4;
-          if (((bad >> (2 * sb + i / 8)) & 1) || !sees(a, s, my_pos, p0 + key)) sc[sb][i] = -INFINITY;
-        }
+        for (int i = 0; i < 16; i++)
+          if (((bad >> (2 * sb + i / 8)) & 1) || !seen(32 * sb + 8 * (i / 4) + i % 4)) sc[sb][i] = -INFINITY;
     }
     float mx = -INFINITY;
 #pragma unroll
@@ -639,17 +725,18 @@ __device__ __forceinline__ bool attn_large(const PagedAttnArgs &a, const PagedTi
 #pragma unroll
       for (int i = 0; i < 16; i++) mx = fmaxf(mx, sc[sb][i]);
     mx = half_max(mx) * a.scale_log2;
-    // the sums are rescaled only once a row's maximum has grown by 2^kSlack: until
-    // then its weights are up to 2^kSlack times as large
-    if (__any(mx > m_run + kSlack)) {
-      const float m = fmaxf(m_run, mx);
-      const float corr = m_run == m ? 1.0f : exp2_weight(m_run - m);
-      m_run = m;
-      l_run *= corr;
-#pragma unroll
-      for (int db = 0; db < kDB; db++)
-#pragma unroll
-        for (int i = 0; i < 16; i++) acc[db][i] *= corr;
+    // the sums are rescaled only once a row's maximum has grown by 2^kSlack: until then
+    // its weights are up to 2^kSlack times as large
+    const int grown = uniform(__any(mx > m_run + kSlack) ? 1 : 0);
+    const float m = grown ? fmaxf(m_run, mx) : m_run;
+    const float corr = m_run == m ? 1.0f : exp2_weight(m_run - m);
+    m_run = m;
+    l_run *= corr;
+    SH_SCALE(acc[0], corr, grown, 64, 65, 66, 67, 68, 69, 70, 71, 72, 73, 74, 75, 76, 77, 78, 79);
+    SH_SCALE(acc[1], corr, grown, 80, 81, 82, 83, 84, 85, 86, 87, 88, 89, 90, 91, 92, 93, 94, 95);
+    if constexpr (kDB == 4) {
+      SH_SCALE(acc[2], corr, grown, 96, 97, 98, 99, 100, 101, 102, 103, 104, 105, 106, 107, 108, 109, 110, 111);
+      SH_SCALE(acc[3], corr, grown, 112, 113, 114, 115, 116, 117, 118, 119, 120, 121, 122, 123, 124, 125, 126, 127);
     }
     // (a row that has seen nothing yet: its weights are exp2(-infinity))
     const float off = (m_run == -INFINITY ? 0.0f : m_run) - T::kWeightLog2;
@@ -668,6 +755,7 @@ __device__ __forceinline__ bool attn_large(const PagedAttnArgs &a, const PagedTi
     read_v(2);
     read_v(3);
     __builtin_amdgcn_sched_barrier(0);
+    __builtin_amdgcn_s_setprio(0);
 #pragma unroll
     for (int ks = 0; ks < 4; ks++)
 #pragma unroll
@@ -708,12 +796,14 @@ __device__ __forceinline__ bool attn_large(const PagedAttnArgs &a, const PagedTi
 }
 
 template <class T, int kD>
-__global__ __launch_bounds__(kT, 2) void paged_large_kernel(const PagedAttnArgs a) {
+__global__ __launch_bounds__(kT, kLarge.workers / 256) void paged_large_kernel(const PagedAttnArgs a) {
   __shared__ __attribute__((aligned(16))) LargeLds<kD> lds;
   __shared__ PlanLds plan;
   // consecutive pieces to one XCD: they share K and V
   const int worker = (blockIdx.x & 7) * (a.plan.workers >> 3) + (blockIdx.x >> 3);
-  work_piece<kLargeMergeRows>(a, worker, plan, [&](const PieceStep &st) { return attn_large<T, kD>(a, st.tile, st.span, st.u0, st.u1, st.slot, lds); });
+  work_piece<kLargeMergeRows>(a, worker, plan, [&](const PieceStep &st, long long) {
+    return attn_large<T, kD>(a, st.tile, st.span, st.u0, st.u1, st.slot, lds);
+  });
 }
 
 // ---- the merge ---------------------------------------------------------------------------
@@ -734,16 +824,16 @@ struct MergeLds {
   int waves[kMaxT / 64];
 };
 
-template <class T, int kD, int kThreads, int kWaves, int kRows>
+template <class T, int kD, int kThreads, int kWaves, int kRows, int kStep>
 __global__ __launch_bounds__(kThreads) void paged_merge_kernel(const PagedAttnArgs a) {
-  constexpr int kStep = 8 / kRows, kDims = kD / 64;
+  constexpr int kDims = kD / 64;
   typedef float Dims __attribute__((ext_vector_type(kDims)));
   __shared__ MergeLds lds;
   __shared__ Dims num_part[kWaves][64];
   __shared__ float top_part[kWaves], den_part[kWaves];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   // threads of two workers each
-  static_assert(kSmallWorkers <= 2 * kT && kLargeWorkers <= 2 * kT, "two items per thread");
+  static_assert(kMaxWorkers <= 2 * kT, "two items per thread");
   const int workers = a.plan.workers;
   int sum = 0;
   if (tid < kT)
@@ -850,8 +940,7 @@ __global__ __launch_bounds__(kThreads) void paged_merge_kernel(const PagedAttnAr
     if (a.redo[w] == 0) continue;
     __syncthreads();  // lds.prefix is read
     MergeItem unused;
-    long long piece;
-    walk_piece(a.plan, w, lds.plan, &unused, &piece, [&](const PieceStep &st) {
+    walk_piece(a.plan, w, lds.plan, &unused, [&](const PieceStep &st, long long piece) {
       if (st.slot >= 0)  // a cut tile is the first flagged worker's
         for (int j = plan_first(st.tile, w, piece, w * piece); j < w; j++)
           if (a.redo[j] != 0) return true;
@@ -865,12 +954,13 @@ __global__ __launch_bounds__(kThreads) void paged_merge_kernel(const PagedAttnAr
 // ---- the entry points ---------------------------------------------------------------
 
 // Small tiles where every sequence's new tokens fit one.
-bool small_tiles(int group, int max_new) { return group <= kSmallRows && (long long)group * max_new <= kSmallRows; }
+Variant variant_of(int group, int max_new) {
+  return group <= kSmall.rows && (long long)group * max_new <= kSmall.rows ? kSmall : kLarge;
+}
 
 size_t workspace_of(const sh_paged_kv *kv, int heads, int max_new) {
-  const bool small = small_tiles(heads / kv->kv_heads, max_new);
-  const size_t workers = small ? kSmallWorkers : kLargeWorkers, rows = small ? kSmallRows : kLargeRows;
-  return workers * (sizeof(MergeItem) + 2 * sizeof(int)) + 2 * workers * rows * (kv->head_dim + 4) * 4;
+  const Variant v = variant_of(heads / kv->kv_heads, max_new);
+  return v.workers * (sizeof(MergeItem) + 2 * sizeof(int)) + (size_t)2 * v.workers * v.rows * (kv->head_dim + 4) * 4;
 }
 
 int check_attn_sizes(const sh_paged_kv *kv, int tokens, int heads, int max_new) {
@@ -882,14 +972,15 @@ int check_attn_sizes(const sh_paged_kv *kv, int tokens, int heads, int max_new) 
 }
 
 template <class T, int kD>
-void launch(hipStream_t st, const PagedAttnArgs &a, bool small) {
-  if (small) {
-    paged_small_kernel<T, kD><<<a.plan.workers, kT, 0, st>>>(a);
-    paged_merge_kernel<T, kD, 512, 8, kSmallMergeRows><<<a.plan.workers, 512, 0, st>>>(a);
-  } else {
-    paged_large_kernel<T, kD><<<a.plan.workers, kT, 0, st>>>(a);
-    paged_merge_kernel<T, kD, kT, 1, kLargeMergeRows><<<a.plan.workers, kT, 0, st>>>(a);
+void launch(hipStream_t st, const PagedAttnArgs &a) {
+  const int workers = a.plan.workers;
+  if (a.tile_rows == kSmall.rows) {
+    paged_small_kernel<T, kD><<<workers, kT, 0, st>>>(a);
+    paged_merge_kernel<T, kD, 512, 8, kSmallMergeRows, 8><<<workers, 512, 0, st>>>(a);
+    return;
   }
+  paged_large_kernel<T, kD><<<workers, kT, 0, st>>>(a);
+  paged_merge_kernel<T, kD, kT, 1, kLargeMergeRows, 4><<<std::max(workers, 1024), kT, 0, st>>>(a);
 }
 
 template <class T>
@@ -926,8 +1017,8 @@ int attn_paged(sh_ctx *ctx, const sh_paged_kv *kv, const uint16_t *q, uint16_t *
   a.max_pages = kv->max_pages;
   a.num_pages = kv->num_pages;
   a.page_shift = __builtin_ctz((unsigned)kv->page_size);
-  const bool small = small_tiles(a.group, max_new);
-  a.tile_rows = small ? kSmallRows : kLargeRows;
+  const Variant v = variant_of(a.group, max_new);
+  a.tile_rows = v.rows;
   a.scale_log2 = scale * 1.44269504f;
   PagedPlan &p = a.plan;
   p.starts = kv->starts;
@@ -937,24 +1028,23 @@ int attn_paged(sh_ctx *ctx, const sh_paged_kv *kv, const uint16_t *q, uint16_t *
   p.kv_heads = kv->kv_heads;
   p.capacity = kv->max_pages * kv->page_size;
   p.per_tile = a.tile_rows / a.group;
-  p.unit = small ? 32 * 128 / kv->head_dim : kLargeUnit;
+  p.unit = v.rows == kSmall.rows ? 32 * 128 / kv->head_dim : kLargeUnit;
   p.unit_shift = __builtin_ctz((unsigned)p.unit);
   p.window = window;
   p.sinks = sinks;
-  p.min_piece = small ? kSmallPiece : kLargePiece;
-  p.workers = plan_workers(p.batch, p.kv_heads, tokens, p.capacity, p.per_tile, p.min_piece,
-                           small ? kSmallWorkers : kLargeWorkers);
+  p.min_piece = v.min_piece;
+  p.workers = plan_workers(p.batch, p.kv_heads, tokens, p.capacity, p.per_tile, p.min_piece, v.workers);
   p.inv_workers = std::nextafter(1.0 / p.workers, 2.0);
   a.items = static_cast<MergeItem *>(workspace);
   a.groups = reinterpret_cast<int *>(a.items + p.workers);
   a.redo = a.groups + p.workers;
   a.slots = reinterpret_cast<float *>(a.redo + p.workers);
-  p.whole_below = small ? kSmallWhole : kLargeWhole;
+  p.whole_below = v.whole_below;
   const hipStream_t st = stream_of(ctx);
   if (kv->head_dim == 64)
-    launch<T, 64>(st, a, small);
+    launch<T, 64>(st, a);
   else
-    launch<T, 128>(st, a, small);
+    launch<T, 128>(st, a);
   const hipError_t e = hipGetLastError();
   return e == hipSuccess ? SH_OK : hip_fail(e, "attn_paged");
 }

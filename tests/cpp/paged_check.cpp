@@ -2,6 +2,7 @@
 // every unit of every tile once, that what is written for the merge is what it
 // reads, and that nothing indexes out of range whatever the device data are; and of
 // the argument checks of the paged operators and of sampling.
+#include <algorithm>
 #include <cmath>
 #include <cstdio>
 #include <cstdlib>
@@ -27,11 +28,18 @@ static long long failures = 0;
 
 static constexpr int kParts = 256;
 
-static std::vector<long long> prefix_of(const PagedPlan &p, int per) {
+static std::vector<long long> prefix_of(const PagedPlan &p, int per, long long *largest) {
+  *largest = 0;
   std::vector<long long> prefix(kParts + 1, 0);
   for (int t = 0; t < kParts; t++) {
     long long sum = 0;
-    for (int b = t * per; b < (t + 1) * per && b < p.batch; b++) sum = plan_add(sum, plan_sequence(p, b).one * p.kv_heads);
+    for (int b = t * per; b < (t + 1) * per && b < p.batch; b++) {
+      const PlanSeq s = plan_sequence(p, b);
+      sum = plan_add(sum, s.one * p.kv_heads);
+      for (int i = 0; i < s.tiles && i < 50; i++)
+        CHECK(plan_prefix(p, s.seq, i + 1) - plan_prefix(p, s.seq, i) <= plan_last(p, s));
+      *largest = std::max(*largest, plan_last(p, s));
+    }
     prefix[t + 1] = plan_add(prefix[t], sum);
   }
   return prefix;
@@ -46,16 +54,15 @@ struct Written {
 // orderly: starts ascend, so that every tile is there once.
 static void walk(const PagedPlan &p, bool orderly, int group) {
   const int per = (p.batch + kParts - 1) / kParts;
-  const std::vector<long long> prefix = prefix_of(p, per);
-  const long long total = prefix[kParts], piece = plan_piece(p, total);
+  long long largest;
+  const std::vector<long long> prefix = prefix_of(p, per, &largest);
+  const long long total = prefix[kParts], piece = plan_piece(p, total, largest);
   CHECK(piece * p.workers >= total);
   // the workers that the host gives a call with these sizes have room for it, too
   PagedPlan q = p;
   q.workers = plan_workers(p.batch, p.kv_heads, p.tokens, p.capacity, p.per_tile, p.min_piece, 768);
   q.inv_workers = std::nextafter(1.0 / q.workers, 2.0);
-  CHECK(q.workers > 0 && q.workers <= 768 && q.workers % 8 == 0 && plan_piece(q, total) * q.workers >= total);
-  std::vector<PlanSeq> seqs(kParts);
-  for (int b = 0; b < kParts && b < p.batch; b++) seqs[b] = plan_sequence(p, b);
+  CHECK(q.workers > 0 && q.workers <= 768 && q.workers % 8 == 0 && plan_piece(q, total, largest) * q.workers >= total);
   std::map<std::tuple<int, int, int>, Written> tiles;
   std::vector<MergeItem> items(p.workers);
   std::map<int, std::tuple<int, int, int>> slot_owner;
@@ -65,7 +72,7 @@ static void walk(const PagedPlan &p, bool orderly, int group) {
     long long steps = 0;
     for (long long x = x0; x < x1;) {
       const int part = plan_find(prefix.data(), kParts, x);
-      const PagedTile tile = plan_locate(p, seqs.data(), part, per, prefix[part], x);
+      const PagedTile tile = plan_locate(p, plan_sequence(p, plan_part_first(p, part, per)), part, per, prefix[part], x);
       const PieceStep s = plan_step(p, tile, piece, w, x0, x, &item);
       if (orderly) CHECK(plan_first(tile, w, piece, x0) == (int)(tile.begin / piece));
       CHECK(s.tile.b >= 0 && s.tile.b < p.batch);
@@ -220,14 +227,15 @@ int main() {
     p.starts = starts.data();
     p.lengths = lengths.data();
     const int per = (p.batch + kParts - 1) / kParts;
-    const std::vector<long long> prefix = prefix_of(p, per);
+    long long largest;
+    const std::vector<long long> prefix = prefix_of(p, per, &largest);
     CHECK(prefix[kParts] == kMaxLine);
     for (int t = 0; t < kParts; t++) CHECK(prefix[t] <= prefix[t + 1]);
-    const long long piece = plan_piece(p, prefix[kParts]);
+    const long long piece = plan_piece(p, prefix[kParts], largest);
     for (int w = 0; w < p.workers; w++) {
       MergeItem item = {0, 0, 0, 0, 0, 0};
       const int part = plan_find(prefix.data(), kParts, w * piece);
-      const PagedTile tile = plan_locate(p, nullptr, part, per, prefix[part], w * piece);
+      const PagedTile tile = plan_locate(p, plan_sequence(p, plan_part_first(p, part, per)), part, per, prefix[part], w * piece);
       const PieceStep s = plan_step(p, tile, piece, w, w * piece, w * piece, &item);
       CHECK(s.tile.b >= 0 && s.tile.b < p.batch && s.tile.kv_head < p.kv_heads);
       CHECK(s.u0 >= 0 && s.u1 <= s.span.units);
