@@ -8,6 +8,7 @@
 // anything, and a page number out of range makes its positions invisible.
 #pragma once
 
+#include <cmath>
 #include <cstddef>
 #include <cstdint>
 
@@ -23,13 +24,6 @@ namespace sh {
 
 constexpr int kMaxPagedTokens = 1 << 22, kMaxPagedBatch = 1 << 16, kMaxPagedKvHeads = 1 << 10;
 constexpr int kMaxPagedPositions = 1 << 28;  // max_pages * page_size
-
-// a / b for 0 <= a, 0 < b; most are small, and a 64-bit division is some hundred
-// instructions.
-SH_HD long long plan_div(long long a, long long b) {
-  if (((a | b) >> 31) == 0) return (long long)((uint32_t)a / (uint32_t)b);
-  return a / b;
-}
 
 SH_HD int clamp_int(int v, int lo, int hi) { return v < lo ? lo : v > hi ? hi : v; }
 
@@ -69,14 +63,23 @@ struct PagedPlan {
   int unit_shift;     // its logarithm
   int window, sinks;  // window 0: none
   int workers;
-  double inv_workers; // 1 / workers, rounded up
+  double inv_workers; // 1 / workers
   int min_piece;      // shortest piece of the line
   int whole_below;    // tiles of at most this cost are not cut
 };
 
 constexpr int kTileFixedCost = 64;  // of a tile, in positions
-// Sums saturate here, far above any call's (starts out of order could pass 2^63).
-constexpr long long kMaxLine = 1LL << 61;
+// Places on the line are whole numbers below 2^53 in fp64, of which every operation
+// below is exact and one instruction (of a 64-bit integer product or comparison it
+// takes several, of a division some hundred: planning took 5 us of a kernel with
+// those). The line of a call is at most kMaxLine (check_paged_sizes); sums over starts
+// out of order, which may count tokens twice, stop there.
+typedef double Line;
+constexpr Line kMaxLine = 4503599627370496.0;  // 2^52
+
+// floor(a / b): exact, as a quotient that rounds to a whole number it is below
+// differs from it by less than 1 / a of it.
+SH_HD Line plan_div(Line a, Line b) { return floor(a / b); }
 
 SH_HD PagedSeq plan_seq(const PagedPlan &p, int b) {
   return paged_seq(p.starts[b], p.starts[b + 1], p.lengths[b], p.tokens, p.capacity);
@@ -86,25 +89,25 @@ SH_HD int plan_tiles(const PagedPlan &p, const PagedSeq &s) { return (s.n + p.pe
 
 // Cost of the sequence's first t tiles: tile i sees up to c + (i + 1) per_tile
 // positions, or with a window no more than sinks + window + per_tile.
-SH_HD long long plan_prefix(const PagedPlan &p, const PagedSeq &s, int t) {
-  const long long c = s.len > s.n ? s.len - s.n : 0, R = p.per_tile;
-  long long m = t, cap = 0;
+SH_HD Line plan_prefix(const PagedPlan &p, const PagedSeq &s, int t) {
+  const Line c = s.len > s.n ? s.len - s.n : 0, R = p.per_tile;
+  Line m = t, cap = 0;
   if (p.window > 0) {
     const int sinks = p.sinks < s.len ? p.sinks : s.len;
-    cap = (long long)sinks + p.window + R;
+    cap = (Line)sinks + p.window + R;
     m = cap > c ? plan_div(cap - c, R) : 0;
     m = m < t ? m : t;
   }
-  return (long long)t * kTileFixedCost + m * c + R * m * (m + 1) / 2 + (t - m) * cap;
+  return t * (Line)kTileFixedCost + m * c + R * m * (m + 1) * 0.5 + (t - m) * cap;
 }
 
-SH_HD long long plan_add(long long a, long long b) { return a + b < kMaxLine ? a + b : kMaxLine; }
+SH_HD Line plan_add(Line a, Line b) { return a + b < kMaxLine ? a + b : kMaxLine; }
 
 // A sequence on the line: its tiles, and what one KV head's cost together.
 struct PlanSeq {
   PagedSeq seq;
   int tiles;
-  long long one;
+  Line one;
 };
 
 SH_HD PlanSeq plan_sequence(const PagedPlan &p, int b) {
@@ -116,17 +119,16 @@ SH_HD PlanSeq plan_sequence(const PagedPlan &p, int b) {
 }
 
 // The cost of the sequence's last tile, its largest.
-SH_HD long long plan_last(const PagedPlan &p, const PlanSeq &s) {
+SH_HD Line plan_last(const PagedPlan &p, const PlanSeq &s) {
   return s.tiles > 1 ? s.one - plan_prefix(p, s.seq, s.tiles - 1) : s.one;
 }
 
-// (At least total / workers: inv_workers is rounded up, and what a product in fp64
-// loses of a total below 2^61 is added.) A piece that is somewhat shorter than the
-// largest tile becomes as long: most tiles then fit one and need no merge. Of 448
-// tiles of one cost over 512 workers: 87 -> 73 us a call.
-SH_HD long long plan_piece(const PagedPlan &p, long long total, long long largest) {
-  const long long q = (long long)((double)total * p.inv_workers) + (total >> 50) + 1;
-  const long long r = q < largest && 8 * q >= 5 * largest ? largest : q;
+// (At least total / workers, with room for the roundings.) A piece that is somewhat
+// shorter than the largest tile becomes as long: most tiles then fit one and need no
+// merge. Of 448 tiles of one cost over 512 workers: 87 -> 73 us a call.
+SH_HD Line plan_piece(const PagedPlan &p, Line total, Line largest) {
+  const Line q = floor(total * p.inv_workers) + 2;
+  const Line r = q < largest && 8 * q >= 5 * largest ? largest : q;
   return r > p.min_piece ? r : p.min_piece;
 }
 
@@ -143,11 +145,11 @@ inline int plan_workers(int batch, int kv_heads, int tokens, int capacity, int p
 struct PagedTile {
   PagedSeq seq;
   int b, kv_head, tile;
-  long long begin, cost;
+  Line begin, cost;
 };
 
 // The last i < parts with prefix[i] <= x (prefix ascends from 0).
-SH_HD int plan_find(const long long *prefix, int parts, long long x) {
+SH_HD int plan_find(const Line *prefix, int parts, Line x) {
   int lo = 0, hi = parts;
   while (hi - lo > 1) {
     const int mid = (lo + hi) / 2;
@@ -166,7 +168,7 @@ SH_HD int plan_part_first(const PagedPlan &p, int part, int per) {
   const int end = (part + 1) * per < p.batch ? (part + 1) * per : p.batch;
   return part * per < end ? part * per : end - 1;
 }
-SH_HD PagedTile plan_locate(const PagedPlan &p, PlanSeq s, int part, int per, long long at, long long x) {
+SH_HD PagedTile plan_locate(const PagedPlan &p, PlanSeq s, int part, int per, Line at, Line x) {
   PagedTile t;
   const int end = (part + 1) * per < p.batch ? (part + 1) * per : p.batch;
   t.b = plan_part_first(p, part, per);
@@ -175,8 +177,8 @@ SH_HD PagedTile plan_locate(const PagedPlan &p, PlanSeq s, int part, int per, lo
     s = plan_sequence(p, ++t.b);
   }
   t.seq = s.seq;
-  const long long head = p.kv_heads > 1 && s.one > 0 ? plan_div(x - at, s.one) : 0;
-  t.kv_head = (int)(head < p.kv_heads ? head : p.kv_heads - 1);
+  const Line head = p.kv_heads > 1 && s.one > 0 ? plan_div(x - at, s.one) : 0;
+  t.kv_head = head < p.kv_heads ? (int)head : p.kv_heads - 1;
   at += s.one * t.kv_head;
   int a = 0, z = s.tiles > 1 ? s.tiles : 1;  // prefix(a) <= x - at < prefix(z)
   while (z - a > 1) {
@@ -187,7 +189,7 @@ SH_HD PagedTile plan_locate(const PagedPlan &p, PlanSeq s, int part, int per, lo
       z = mid;
   }
   t.tile = a;
-  const long long before = a > 0 ? plan_prefix(p, t.seq, a) : 0;
+  const Line before = a > 0 ? plan_prefix(p, t.seq, a) : 0;
   t.begin = at + before;
   t.cost = (s.tiles > 1 ? plan_prefix(p, t.seq, a + 1) : s.one) - before;
   return t;
@@ -235,10 +237,10 @@ SH_HD int span_position(const TileSpan &s, int unit, int j) {
 }
 
 // Units of a tile before point x of its cost: what a cut there leaves on its left.
-SH_HD int plan_cut(const PagedPlan &p, const PagedTile &t, int units, long long x) {
+SH_HD int plan_cut(const PagedPlan &p, const PagedTile &t, int units, Line x) {
   if (x <= t.begin) return 0;
   if (x >= t.begin + t.cost) return units;
-  const long long in = x - t.begin;
+  const Line in = x - t.begin;
   if (t.cost <= p.whole_below) return 2 * in >= t.cost ? units : 0;
   return (int)plan_div(in * units, t.cost);
 }
@@ -265,16 +267,16 @@ struct PieceStep {
 };
 
 // The first worker of a tile.
-SH_HD int plan_first(const PagedTile &t, int worker, long long piece, long long x0) {
+SH_HD int plan_first(const PagedTile &t, int worker, Line piece, Line x0) {
   return t.begin >= x0 ? worker : worker - (int)plan_div(x0 - t.begin + piece - 1, piece);
 }
 
-SH_HD PieceStep plan_step(const PagedPlan &p, const PagedTile &t, long long piece, int worker, long long x0,
-                          long long x, MergeItem *item) {
+SH_HD PieceStep plan_step(const PagedPlan &p, const PagedTile &t, Line piece, int worker, Line x0, Line x,
+                          MergeItem *item) {
   PieceStep r;
   r.tile = t;
   r.span = plan_span(p, t);
-  const long long end = t.begin + t.cost;
+  const Line end = t.begin + t.cost;
   r.more = x < end;
   r.u0 = plan_cut(p, t, r.span.units, x0);
   r.u1 = plan_cut(p, t, r.span.units, x0 + piece);
@@ -318,6 +320,9 @@ inline const char *check_paged_sizes(const sh_paged_kv *kv, int tokens, int head
   if (kv->num_pages < 1) return "num_pages must be positive";
   if (kv->max_pages < 1 || kv->max_pages > kMaxPagedPositions / kv->page_size)
     return "max_pages must be positive and max_pages * page_size at most 2^28";
+  // (what an attention call may cost: kMaxLine, in tiles of one token)
+  if (((double)tokens + kv->batch) * kv->kv_heads * ((double)kv->max_pages * kv->page_size + 512.0) > kMaxLine)
+    return "(tokens + batch) * kv_heads * max_pages * page_size exceeds 2^52";
   return nullptr;
 }
 

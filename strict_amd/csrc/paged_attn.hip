@@ -35,8 +35,6 @@ struct Variant {
 };
 constexpr Variant kSmall = {16, 512, 128, 192}, kLarge = {128, 512, 256, 256};
 constexpr int kMaxWorkers = 512;
-// Rows that the merge kernel takes at once.
-constexpr int kSmallMergeRows = 1, kLargeMergeRows = 4;
 
 struct PagedAttnArgs {
   const uint16_t *q, *k, *v;
@@ -46,7 +44,7 @@ struct PagedAttnArgs {
   MergeItem *items;  // [workers]
   int *groups;       // [workers]: rows to merge of the worker's item, in groups
   int *redo;         // [workers]: 1: some of the worker's results are not finite
-  float *slots;      // [2 workers][rows of a tile][d + 4]
+  float *slots;      // [2 workers][rows of a tile * (d + 2)]
   int heads, group, group_inv, max_pages, num_pages, page_shift, tile_rows;
   float scale_log2;
 };
@@ -59,11 +57,22 @@ __device__ __forceinline__ size_t head_row(const PagedAttnArgs &a, int row0, int
   return (size_t)(row0 + token) * a.heads + kv_head * a.group + (r - token * a.group);
 }
 
-// Row r of slot s: d V sums, then the row's maximum and sum of weights (and 8
-// bytes that align the next).
+// A slot: the V sums, then every row's maximum and sum of weights. The V sums of
+// small tiles lie row by row, those of large ones as the lanes hold them (4 values
+// per lane, a KiB at once): written row by row, 16 bytes a row, they took as long as
+// six units.
 template <int kD>
-__device__ __forceinline__ float *slot_row(const PagedAttnArgs &a, int slot, int r) {
-  return a.slots + ((size_t)slot * a.tile_rows + r) * (kD + 4);
+__device__ __forceinline__ float *slot_of(const PagedAttnArgs &a, int slot) {
+  return a.slots + (size_t)slot * a.tile_rows * (kD + 2);
+}
+template <int kD>
+__device__ __forceinline__ float *slot_stats(const PagedAttnArgs &a, int slot, int r) {
+  return slot_of<kD>(a, slot) + a.tile_rows * kD + 2 * r;
+}
+// Values 4 i .. 4 i + 3 of block db of the wave's accumulators.
+template <int kD>
+__device__ __forceinline__ f32x4 *slot_large(const PagedAttnArgs &a, int slot, int wave, int db, int i) {
+  return reinterpret_cast<f32x4 *>(slot_of<kD>(a, slot)) + ((wave * (kD / 32) + db) * 4 + i) * 64 + (threadIdx.x & 63);
 }
 
 // Where the results of a tile's part go: the output (slot -1) or a slot.
@@ -74,7 +83,7 @@ __device__ __forceinline__ void store_value(const PagedAttnArgs &a, const PagedT
     const size_t row = head_row(a, t.seq.row0 + s.first, t.kv_head, r);
     reinterpret_cast<typename T::Value *>(a.out)[row * kD + dim] = (typename T::Value)(l == 0.0f ? 0.0f : acc / l);
   } else {
-    slot_row<kD>(a, slot, r)[dim] = acc;
+    slot_of<kD>(a, slot)[r * kD + dim] = acc;
   }
 }
 
@@ -146,29 +155,46 @@ __device__ void attn_exact(const PagedAttnArgs &a, const PagedTile &t, const Til
 
 // The line's division among the workers, in LDS.
 struct PlanLds {
-  long long prefix[kT + 1], waves[kMaxT / 64], largest[kMaxT / 64];
+  Line prefix[kT + 1], waves[kMaxT / 64], largest[kMaxT / 64];
   PlanSeq seqs[kT];  // where a thread has one sequence
-  long long x, piece;  // the next step's point (here and not in registers)
+  Line x, piece;     // the next step's point (here and not in registers)
 };
 
+template <int kCtrl, int kRowMask>
+__device__ __forceinline__ Line dpp_line(Line v) {
+  const uint64_t u = __builtin_bit_cast(uint64_t, v);
+  const uint32_t lo = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)u, kCtrl, kRowMask, 0xf, false);
+  const uint32_t hi = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)(u >> 32), kCtrl, kRowMask, 0xf, false);
+  return __builtin_bit_cast(Line, ((uint64_t)hi << 32) | lo);
+}
+
+// Sum (maximum) of lanes 0 .. own, by lane moves (row_shr:1, 2, 4, 8, row_bcast:15,
+// 31; a lane that gets nothing gets 0): a fifth of the time of LDS permutes.
+template <class Op>
+__device__ __forceinline__ Line wave_scan_line(Line v, Op op) {
+  v = op(v, dpp_line<0x111, 0xf>(v));
+  v = op(v, dpp_line<0x112, 0xf>(v));
+  v = op(v, dpp_line<0x114, 0xf>(v));
+  v = op(v, dpp_line<0x118, 0xf>(v));
+  v = op(v, dpp_line<0x142, 0xa>(v));
+  v = op(v, dpp_line<0x143, 0xc>(v));
+  return v;
+}
+
 // Prefix sums of the sequences' costs, by kT threads (of kT or more) of `per`
-// sequences each.
+// sequences each, and the largest tile's cost per wave.
 __device__ __forceinline__ void scan_costs(const PagedPlan &p, int per, PlanLds &lds) {
-  const int t = threadIdx.x, lane = t & 63;
-  long long sum = 0, largest = 0;
+  const int t = threadIdx.x;
+  Line sum = 0, largest = 0;
   for (int b = t * per; b < min((t + 1) * per, p.batch); b++) {
     const PlanSeq s = plan_sequence(p, b);
     if (per == 1) lds.seqs[t] = s;
     sum = plan_add(sum, s.one * p.kv_heads);
-    largest = max(largest, plan_last(p, s));
+    largest = fmax(largest, plan_last(p, s));
   }
-#pragma unroll
-  for (int off = 1; off < 64; off *= 2) {
-    const long long o = __shfl_up(sum, off, 64), l = __shfl_up(largest, off, 64);
-    if (lane >= off) sum = plan_add(sum, o);
-    if (lane >= off) largest = max(largest, l);
-  }
-  if (lane == 63) {
+  sum = wave_scan_line(sum, [](Line x, Line y) { return plan_add(x, y); });
+  largest = wave_scan_line(largest, [](Line x, Line y) { return fmax(x, y); });
+  if ((t & 63) == 63) {
     lds.waves[t >> 6] = sum;
     lds.largest[t >> 6] = largest;
   }
@@ -181,13 +207,14 @@ __device__ __forceinline__ void scan_costs(const PagedPlan &p, int per, PlanLds 
 
 // A value that is the same in every lane, as the compiler cannot know of one from LDS.
 __device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
-__device__ __forceinline__ long long uniform(long long x) {
-  return (long long)(((uint64_t)(uint32_t)uniform((int)(x >> 32)) << 32) | (uint32_t)uniform((int)x));
+__device__ __forceinline__ Line uniform(Line x) {
+  const uint64_t u = __builtin_bit_cast(uint64_t, x);
+  return __builtin_bit_cast(Line, ((uint64_t)(uint32_t)uniform((int)(u >> 32)) << 32) | (uint32_t)uniform((int)u));
 }
 
 // The last i < kT with prefix[i] <= x: how many of the values from prefix[1] on are
 // (a wave looks at all 256 at once).
-__device__ __forceinline__ int find_part(const PlanLds &lds, long long x) {
+__device__ __forceinline__ int find_part(const PlanLds &lds, Line x) {
   const int lane = threadIdx.x & 63;
   int n = 0;
 #pragma unroll
@@ -198,37 +225,29 @@ __device__ __forceinline__ int find_part(const PlanLds &lds, long long x) {
 // A worker's piece, step by step: part(step), which says whether its results are
 // finite. Returns whether all are.
 template <class Part>
-__device__ __forceinline__ bool walk_piece(const PagedPlan &p, int worker, PlanLds &lds, MergeItem *item,
-                                           Part part) {
+__device__ __forceinline__ bool walk_piece(const PagedPlan &p, int worker, PlanLds &lds, MergeItem *item, Part part) {
   const int per = (p.batch + kT - 1) / kT;
   scan_costs(p, per, lds);
   if (threadIdx.x == 0) {
-    long long largest = 0;
-    for (int w = 0; w < kT / 64; w++) largest = max(largest, lds.largest[w]);
+    Line largest = 0;
+    for (int w = 0; w < kT / 64; w++) largest = fmax(largest, lds.largest[w]);
     lds.piece = plan_piece(p, lds.prefix[kT], largest);
     lds.x = worker * lds.piece;
   }
   __syncthreads();
   bool finite = true;
   while (true) {
-    const long long total = uniform(lds.prefix[kT]), piece = uniform(lds.piece), x0 = worker * piece;
-    const long long x = uniform(lds.x);
-    if (x >= min(x0 + piece, total)) break;
+    const Line total = lds.prefix[kT], piece = lds.piece, x = lds.x, x0 = worker * piece;
+    if (uniform(x >= fmin(x0 + piece, total) ? 1 : 0)) break;
     const int i = uniform(find_part(lds, x)), b = plan_part_first(p, i, per);
-    PlanSeq first;
-    if (per == 1) {
-      const PlanSeq &f = lds.seqs[b];
-      first = {{uniform(f.seq.row0), uniform(f.seq.n), uniform(f.seq.len)}, uniform(f.tiles), uniform(f.one)};
-    } else {
-      first = plan_sequence(p, b);
-    }
-    const PagedTile t = plan_locate(p, first, i, per, uniform(lds.prefix[i]), x);
+    const PagedTile t = plan_locate(p, per == 1 ? lds.seqs[b] : plan_sequence(p, b), i, per, lds.prefix[i], x);
     PieceStep st = plan_step(p, t, piece, worker, x0, x, item);
-    // (64-bit comparisons are vector instructions, and what is selected by them too)
     for (int *v : {&st.tile.seq.row0, &st.tile.seq.n, &st.tile.seq.len, &st.tile.b, &st.tile.kv_head, &st.tile.tile,
                    &st.span.first, &st.span.count, &st.span.pos0, &st.span.lo, &st.span.hi, &st.span.sinks,
                    &st.span.units, &st.span.sink_units, &st.span.gap, &st.u0, &st.u1, &st.slot})
       *v = uniform(*v);
+    st.run = uniform(st.run ? 1 : 0) != 0;
+    st.more = uniform(st.more ? 1 : 0) != 0;
     __syncthreads();  // lds.x is read
     if (threadIdx.x == 0) lds.x = t.begin + t.cost;
     __syncthreads();
@@ -239,13 +258,14 @@ __device__ __forceinline__ bool walk_piece(const PagedPlan &p, int worker, PlanL
 }
 
 // A worker of the main kernels.
-template <int kMergeRows, class Part>
+// kMergeRows: rows of an item's group, kMergeCols: groups that share rows.
+template <int kMergeRows, int kMergeCols, class Part>
 __device__ __forceinline__ void work_piece(const PagedAttnArgs &a, int worker, PlanLds &lds, Part part) {
   MergeItem item = {0, 0, 0, 0, 0, 0};
   const bool finite = walk_piece(a.plan, worker, lds, &item, part);
   if (threadIdx.x == 0) {
     a.items[worker] = item;
-    a.groups[worker] = item.parts > 0 ? (item.tokens * a.group + kMergeRows - 1) / kMergeRows : 0;
+    a.groups[worker] = item.parts > 0 ? (item.tokens * a.group + kMergeRows - 1) / kMergeRows * kMergeCols : 0;
     a.redo[worker] = finite ? 0 : 1;
   }
 }
@@ -512,8 +532,8 @@ __device__ __forceinline__ bool attn_small(const PagedAttnArgs &a, const PagedTi
     finite = finite && __builtin_fabsf(sum) < INFINITY && l < INFINITY;
     store_value<T, kD>(a, t, s, slot, r, dim, sum, l);
     if (slot >= 0 && dim == 0) {
-      slot_row<kD>(a, slot, r)[kD] = m;
-      slot_row<kD>(a, slot, r)[kD + 1] = l;
+      slot_stats<kD>(a, slot, r)[0] = m;
+      slot_stats<kD>(a, slot, r)[1] = l;
     }
   }
   return !__syncthreads_or(finite ? 0 : 1);
@@ -523,7 +543,7 @@ template <class T, int kD>
 __global__ __launch_bounds__(kT, kSmall.workers / 256) void paged_small_kernel(const PagedAttnArgs a) {
   __shared__ __attribute__((aligned(16))) SmallLds<T, kD> lds;
   __shared__ PlanLds plan;
-  work_piece<kSmallMergeRows>(a, blockIdx.x, plan, [&](const PieceStep &st, long long) { return attn_small<T, kD>(a, st.tile, st.span, st.u0, st.u1, st.slot, lds); });
+  work_piece<1, 1>(a, blockIdx.x, plan, [&](const PieceStep &st, Line) { return attn_small<T, kD>(a, st.tile, st.span, st.u0, st.u1, st.slot, lds); });
 }
 
 // ---- tiles of up to 128 rows ------------------------------------------------------------
@@ -767,30 +787,27 @@ __device__ __forceinline__ bool attn_large(const PagedAttnArgs &a, const PagedTi
   }
   l_run += __shfl_xor(l_run, 32, 64);
   bool finite = true;
-  if (32 * wave + n32 < rows) {
-    finite = l_run < INFINITY;
-    const float inv = l_run == 0.0f ? 0.0f : 1.0f / l_run;
-    uint16_t *op = a.out + head_row(a, t.seq.row0 + s.first, t.kv_head, row) * kD;
-    float *sp = slot_row<kD>(a, max(slot, 0), row);
+  const bool there = 32 * wave + n32 < rows;
+  if (there) finite = l_run < INFINITY;
+  const float inv = l_run == 0.0f ? 0.0f : 1.0f / l_run;
+  uint16_t *op = a.out + head_row(a, t.seq.row0 + s.first, t.kv_head, row) * kD;
 #pragma unroll
-    for (int db = 0; db < kDB; db++)
+  for (int db = 0; db < kDB; db++)
 #pragma unroll
-      for (int i = 0; i < 4; i++) {
-        const f32x4 x = {acc[db][4 * i], acc[db][4 * i + 1], acc[db][4 * i + 2], acc[db][4 * i + 3]};
-        const int dim = 32 * db + 8 * i + 4 * h;
+    for (int i = 0; i < 4; i++) {
+      const f32x4 x = {acc[db][4 * i], acc[db][4 * i + 1], acc[db][4 * i + 2], acc[db][4 * i + 3]};
 #pragma unroll
-        for (int e = 0; e < 4; e++) finite = finite && __builtin_fabsf(x[e]) < INFINITY;
-        if (slot < 0) {
-          const Quad o = {(Value)(x[0] * inv), (Value)(x[1] * inv), (Value)(x[2] * inv), (Value)(x[3] * inv)};
-          *reinterpret_cast<Quad *>(op + dim) = o;
-        } else {
-          *reinterpret_cast<f32x4 *>(sp + dim) = x;
-        }
+      for (int e = 0; e < 4; e++) finite = finite && (!there || __builtin_fabsf(x[e]) < INFINITY);
+      if (slot >= 0) {
+        if (active) *slot_large<kD>(a, slot, wave, db, i) = x;
+      } else if (there) {
+        const Quad o = {(Value)(x[0] * inv), (Value)(x[1] * inv), (Value)(x[2] * inv), (Value)(x[3] * inv)};
+        *reinterpret_cast<Quad *>(op + 32 * db + 8 * i + 4 * h) = o;
       }
-    if (slot >= 0 && h == 0) {
-      sp[kD] = m_run;
-      sp[kD + 1] = l_run;
     }
+  if (slot >= 0 && there && h == 0) {
+    slot_stats<kD>(a, slot, row)[0] = m_run;
+    slot_stats<kD>(a, slot, row)[1] = l_run;
   }
   return !__syncthreads_or(finite ? 0 : 1);
 }
@@ -801,7 +818,7 @@ __global__ __launch_bounds__(kT, kLarge.workers / 256) void paged_large_kernel(c
   __shared__ PlanLds plan;
   // consecutive pieces to one XCD: they share K and V
   const int worker = (blockIdx.x & 7) * (a.plan.workers >> 3) + (blockIdx.x >> 3);
-  work_piece<kLargeMergeRows>(a, worker, plan, [&](const PieceStep &st, long long) {
+  work_piece<32, kD / 32>(a, worker, plan, [&](const PieceStep &st, Line) {
     return attn_large<T, kD>(a, st.tile, st.span, st.u0, st.u1, st.slot, lds);
   });
 }
@@ -809,11 +826,10 @@ __global__ __launch_bounds__(kT, kLarge.workers / 256) void paged_large_kernel(c
 // ---- the merge ---------------------------------------------------------------------------
 //
 // out = sum_j 2^(m_j - M) acc_j / sum_j 2^(m_j - M) l_j, M = max_j m_j, over the
-// parts j of a cut tile. The rows of all cut tiles are numbered through, in groups of
-// kRows (a prefix sum over the workers' items), and a group taken by kWaves waves:
-// one wave for 8 rows of large tiles, which have two or three parts, eight for a row
-// of small ones, whose parts may be spread over all workers (of 8 times kWaves parts
-// all loads are requested at once).
+// parts j of a cut tile. The cut tiles' work is numbered through in groups (a prefix
+// sum over the workers' items): of small tiles a row, whose parts, perhaps spread over
+// all workers, are taken by 8 waves, 8 at once in each; of large tiles, of two or three
+// parts mostly, 32 rows by 32 dims a wave, as the main kernel's lanes held them.
 // Tiles with a part that is not finite are left to workgroup w of the first such
 // worker w, which works them out in fp32, and its whole tiles too.
 struct MergeLds {
@@ -824,20 +840,28 @@ struct MergeLds {
   int waves[kMaxT / 64];
 };
 
-template <class T, int kD, int kThreads, int kWaves, int kRows, int kStep>
-__global__ __launch_bounds__(kThreads) void paged_merge_kernel(const PagedAttnArgs a) {
-  constexpr int kDims = kD / 64;
-  typedef float Dims __attribute__((ext_vector_type(kDims)));
-  __shared__ MergeLds lds;
-  __shared__ Dims num_part[kWaves][64];
-  __shared__ float top_part[kWaves], den_part[kWaves];
-  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  // threads of two workers each
+// Group `unit`'s item, and which of its groups. False: there are fewer.
+__device__ __forceinline__ bool find_item(const PagedAttnArgs &a, const MergeLds &lds, int unit, MergeItem *it, int *g) {
+  const int lane = threadIdx.x & 63;
+  if (unit >= uniform(lds.prefix[kT])) return false;
+  int n = 0;
+#pragma unroll
+  for (int i = 0; i < kT / 64; i++) n += __popcll(__ballot(lds.prefix[1 + i * 64 + lane] <= unit));
+  n = uniform(n);
+  int w = 2 * n;
+  *g = unit - uniform(lds.prefix[n]);
+  if (*g >= a.groups[w]) *g -= a.groups[w++];
+  *it = a.items[w];
+  return true;
+}
+
+// Prefix sums of the items' groups, by threads of two workers each.
+__device__ __forceinline__ void scan_items(const PagedAttnArgs &a, MergeLds &lds) {
   static_assert(kMaxWorkers <= 2 * kT, "two items per thread");
-  const int workers = a.plan.workers;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   int sum = 0;
   if (tid < kT)
-    for (int w = 2 * tid; w < min(2 * tid + 2, workers); w++) sum += a.groups[w];
+    for (int w = 2 * tid; w < min(2 * tid + 2, a.plan.workers); w++) sum += a.groups[w];
 #pragma unroll
   for (int off = 1; off < 64; off *= 2) {
     const int o = __shfl_up(sum, off, 64);
@@ -849,98 +873,16 @@ __global__ __launch_bounds__(kThreads) void paged_merge_kernel(const PagedAttnAr
   if (tid < kT) lds.prefix[tid + 1] = sum;
   if (tid == 0) lds.prefix[0] = 0;
   __syncthreads();
-  const int total = lds.prefix[kT];
-  constexpr int kAtOnce = kThreads / 64 / kWaves;
-  for (int unit = blockIdx.x * kAtOnce + (kAtOnce > 1 ? wave / kWaves : 0); unit < total; unit += gridDim.x * kAtOnce) {
-    int n = 0;
-#pragma unroll
-    for (int i = 0; i < kT / 64; i++) n += __popcll(__ballot(lds.prefix[1 + i * 64 + lane] <= unit));
-    n = __builtin_amdgcn_readfirstlane(n);
-    int g = unit - lds.prefix[n], w = 2 * n;
-    if (g >= a.groups[w]) g -= a.groups[w++];
-    const MergeItem it = a.items[w];
-    const int r0 = g * kRows, rows = it.tokens * a.group;
-    const int part0 = kWaves == 1 ? 0 : wave;
-    float top[kRows], den[kRows];
-    Dims num[kRows];
-#pragma unroll
-    for (int i = 0; i < kRows; i++) {
-      top[i] = -INFINITY;
-      den[i] = 0.0f;
-      num[i] = 0.0f;
-    }
-    bool redo = false;
-    for (int j0 = part0; j0 < it.parts; j0 += kWaves * kStep) {
-      Dims x[kRows][kStep];
-      float m[kRows][kStep], l[kRows][kStep];
-#pragma unroll
-      for (int u = 0; u < kStep; u++) {
-        const int j = min(j0 + kWaves * u, it.parts - 1), slot = j == 0 ? it.first_slot : 2 * (it.first_worker + j);
-#pragma unroll
-        for (int i = 0; i < kRows; i++) {
-          const float *p = slot_row<kD>(a, slot, min(r0 + i, rows - 1));
-          x[i][u] = *reinterpret_cast<const Dims *>(p + lane * kDims);
-          m[i][u] = p[kD];
-          l[i][u] = p[kD + 1];
-        }
-        redo = redo || a.redo[it.first_worker + j] != 0;
-      }
-#pragma unroll
-      for (int i = 0; i < kRows; i++) {
-        float t = top[i];
-#pragma unroll
-        for (int u = 0; u < kStep; u++)
-          if (j0 + kWaves * u < it.parts) t = fmaxf(t, m[i][u]);
-        const float c = t == top[i] ? 1.0f : exp2_weight(top[i] - t);
-        top[i] = t;
-        num[i] *= c;
-        den[i] *= c;
-#pragma unroll
-        for (int u = 0; u < kStep; u++) {
-          const float f = m[i][u] == -INFINITY || j0 + kWaves * u >= it.parts ? 0.0f : exp2_weight(m[i][u] - t);
-          num[i] += f * x[i][u];
-          den[i] = fmaf(f, l[i][u], den[i]);
-        }
-      }
-    }
-    if constexpr (kWaves > 1) {
-      static_assert(kRows == 1, "the waves' sums are of one row");
-      num_part[wave][lane] = num[0];
-      if (lane == 0) {
-        top_part[wave] = top[0];
-        den_part[wave] = den[0];
-      }
-      redo = __syncthreads_or(redo ? 1 : 0);
-      float t = top_part[0];
-#pragma unroll
-      for (int w2 = 1; w2 < kWaves; w2++) t = fmaxf(t, top_part[w2]);
-      num[0] = 0.0f;
-      den[0] = 0.0f;
-#pragma unroll
-      for (int w2 = 0; w2 < kWaves; w2++) {
-        const float f = top_part[w2] == -INFINITY ? 0.0f : exp2_weight(top_part[w2] - t);
-        num[0] += f * num_part[w2][lane];
-        den[0] = fmaf(f, den_part[w2], den[0]);
-      }
-      __syncthreads();
-    }
-    if (redo || (kWaves > 1 && wave != 0)) continue;
-#pragma unroll
-    for (int i = 0; i < kRows; i++) {
-      if (r0 + i >= rows) break;
-      const float inv = den[i] == 0.0f ? 0.0f : 1.0f / den[i];
-      typename T::Value *o =
-          reinterpret_cast<typename T::Value *>(a.out) + head_row(a, it.row0, it.kv_head, r0 + i) * kD + lane * kDims;
-#pragma unroll
-      for (int e = 0; e < kDims; e++) o[e] = (typename T::Value)(num[i][e] * inv);
-    }
-  }
+}
 
-  for (int w = blockIdx.x; w < workers; w += gridDim.x) {
+// The flagged workers' tiles.
+template <class T, int kD>
+__device__ __forceinline__ void redo_tiles(const PagedAttnArgs &a, MergeLds &lds) {
+  for (int w = blockIdx.x; w < a.plan.workers; w += gridDim.x) {
     if (a.redo[w] == 0) continue;
     __syncthreads();  // lds.prefix is read
     MergeItem unused;
-    walk_piece(a.plan, w, lds.plan, &unused, [&](const PieceStep &st, long long piece) {
+    walk_piece(a.plan, w, lds.plan, &unused, [&](const PieceStep &st, Line piece) {
       if (st.slot >= 0)  // a cut tile is the first flagged worker's
         for (int j = plan_first(st.tile, w, piece, w * piece); j < w; j++)
           if (a.redo[j] != 0) return true;
@@ -949,6 +891,138 @@ __global__ __launch_bounds__(kThreads) void paged_merge_kernel(const PagedAttnAr
     });
     __syncthreads();
   }
+}
+
+__device__ __forceinline__ int part_slot(const MergeItem &it, int j) {
+  return j == 0 ? it.first_slot : 2 * (it.first_worker + j);
+}
+
+constexpr int kMergeT = 512;
+template <class T, int kD>
+__global__ __launch_bounds__(kMergeT) void paged_merge_small_kernel(const PagedAttnArgs a) {
+  constexpr int kWaves = kMergeT / 64, kStep = 8, kDims = kD / 64;
+  typedef float Dims __attribute__((ext_vector_type(kDims)));
+  __shared__ MergeLds lds;
+  __shared__ Dims num_part[kWaves][64];
+  __shared__ float top_part[kWaves], den_part[kWaves];
+  const int lane = threadIdx.x & 63, wave = uniform((int)threadIdx.x >> 6);
+  scan_items(a, lds);
+  MergeItem it;
+  int r;
+  for (int unit = blockIdx.x; find_item(a, lds, unit, &it, &r); unit += gridDim.x) {
+    float top = -INFINITY, den = 0.0f;
+    Dims num = 0.0f;
+    bool redo = false;
+    for (int j0 = wave; j0 < it.parts; j0 += kWaves * kStep) {
+      Dims x[kStep];
+      float m[kStep], l[kStep], t = top;
+#pragma unroll
+      for (int u = 0; u < kStep; u++) {
+        const int j = min(j0 + kWaves * u, it.parts - 1), slot = part_slot(it, j);
+        x[u] = *reinterpret_cast<const Dims *>(slot_of<kD>(a, slot) + r * kD + lane * kDims);
+        m[u] = slot_stats<kD>(a, slot, r)[0];
+        l[u] = slot_stats<kD>(a, slot, r)[1];
+        redo = redo || a.redo[it.first_worker + j] != 0;
+      }
+#pragma unroll
+      for (int u = 0; u < kStep; u++)
+        if (j0 + kWaves * u < it.parts) t = fmaxf(t, m[u]);
+      const float c = t == top ? 1.0f : exp2_weight(top - t);
+      top = t;
+      num *= c;
+      den *= c;
+#pragma unroll
+      for (int u = 0; u < kStep; u++) {
+        const float f = m[u] == -INFINITY || j0 + kWaves * u >= it.parts ? 0.0f : exp2_weight(m[u] - t);
+        num += f * x[u];
+        den = fmaf(f, l[u], den);
+      }
+    }
+    num_part[wave][lane] = num;
+    if (lane == 0) {
+      top_part[wave] = top;
+      den_part[wave] = den;
+    }
+    redo = __syncthreads_or(redo ? 1 : 0);
+    if (wave == 0 && !redo) {
+      float t = top_part[0];
+#pragma unroll
+      for (int w = 1; w < kWaves; w++) t = fmaxf(t, top_part[w]);
+      num = 0.0f;
+      den = 0.0f;
+#pragma unroll
+      for (int w = 0; w < kWaves; w++) {
+        const float f = top_part[w] == -INFINITY ? 0.0f : exp2_weight(top_part[w] - t);
+        num += f * num_part[w][lane];
+        den = fmaf(f, den_part[w], den);
+      }
+      const float inv = den == 0.0f ? 0.0f : 1.0f / den;
+      typename T::Value *o =
+          reinterpret_cast<typename T::Value *>(a.out) + head_row(a, it.row0, it.kv_head, r) * kD + lane * kDims;
+#pragma unroll
+      for (int e = 0; e < kDims; e++) o[e] = (typename T::Value)(num[e] * inv);
+    }
+    __syncthreads();  // the parts are read
+  }
+  redo_tiles<T, kD>(a, lds);
+}
+
+template <class T, int kD>
+__global__ __launch_bounds__(kT) void paged_merge_large_kernel(const PagedAttnArgs a) {
+  constexpr int kStep = 3, kDB = kD / 32;
+  typedef typename T::Value Value;
+  typedef Value Quad __attribute__((ext_vector_type(4)));
+  __shared__ MergeLds lds;
+  const int lane = threadIdx.x & 63, n32 = lane & 31, h = lane >> 5;
+  scan_items(a, lds);
+  MergeItem it;
+  int g;
+  for (int unit = blockIdx.x * (kT / 64) + uniform((int)threadIdx.x >> 6); find_item(a, lds, unit, &it, &g);
+       unit += gridDim.x * (kT / 64)) {
+    const int db = g % kDB, wave = g / kDB, rows = it.tokens * a.group, row = min(32 * wave + n32, rows - 1);
+    float top = -INFINITY, den = 0.0f;
+    f32x4 num[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) num[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+    bool redo = false;
+    for (int j0 = 0; j0 < it.parts; j0 += kStep) {
+      f32x4 x[kStep][4];
+      float m[kStep], l[kStep], t = top;
+#pragma unroll
+      for (int u = 0; u < kStep; u++) {
+        const int j = min(j0 + u, it.parts - 1), slot = part_slot(it, j);
+#pragma unroll
+        for (int i = 0; i < 4; i++) x[u][i] = *slot_large<kD>(a, slot, wave, db, i);
+        m[u] = slot_stats<kD>(a, slot, row)[0];
+        l[u] = slot_stats<kD>(a, slot, row)[1];
+        redo = redo || a.redo[it.first_worker + j] != 0;
+      }
+#pragma unroll
+      for (int u = 0; u < kStep; u++)
+        if (j0 + u < it.parts) t = fmaxf(t, m[u]);
+      const float c = t == top ? 1.0f : exp2_weight(top - t);
+      top = t;
+      den *= c;
+#pragma unroll
+      for (int i = 0; i < 4; i++) num[i] *= c;
+#pragma unroll
+      for (int u = 0; u < kStep; u++) {
+        const float f = m[u] == -INFINITY || j0 + u >= it.parts ? 0.0f : exp2_weight(m[u] - t);
+        den = fmaf(f, l[u], den);
+#pragma unroll
+        for (int i = 0; i < 4; i++) num[i] += f * x[u][i];
+      }
+    }
+    if (redo || 32 * wave + n32 >= rows) continue;
+    const float inv = den == 0.0f ? 0.0f : 1.0f / den;
+    uint16_t *op = a.out + head_row(a, it.row0, it.kv_head, row) * kD + 32 * db + 4 * h;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      const Quad o = {(Value)(num[i][0] * inv), (Value)(num[i][1] * inv), (Value)(num[i][2] * inv), (Value)(num[i][3] * inv)};
+      *reinterpret_cast<Quad *>(op + 8 * i) = o;
+    }
+  }
+  redo_tiles<T, kD>(a, lds);
 }
 
 // ---- the entry points ---------------------------------------------------------------
@@ -960,7 +1034,7 @@ Variant variant_of(int group, int max_new) {
 
 size_t workspace_of(const sh_paged_kv *kv, int heads, int max_new) {
   const Variant v = variant_of(heads / kv->kv_heads, max_new);
-  return v.workers * (sizeof(MergeItem) + 2 * sizeof(int)) + (size_t)2 * v.workers * v.rows * (kv->head_dim + 4) * 4;
+  return v.workers * (sizeof(MergeItem) + 2 * sizeof(int)) + (size_t)2 * v.workers * v.rows * (kv->head_dim + 2) * 4;
 }
 
 int check_attn_sizes(const sh_paged_kv *kv, int tokens, int heads, int max_new) {
@@ -976,11 +1050,11 @@ void launch(hipStream_t st, const PagedAttnArgs &a) {
   const int workers = a.plan.workers;
   if (a.tile_rows == kSmall.rows) {
     paged_small_kernel<T, kD><<<workers, kT, 0, st>>>(a);
-    paged_merge_kernel<T, kD, 512, 8, kSmallMergeRows, 8><<<workers, 512, 0, st>>>(a);
+    paged_merge_small_kernel<T, kD><<<workers, kMergeT, 0, st>>>(a);
     return;
   }
   paged_large_kernel<T, kD><<<workers, kT, 0, st>>>(a);
-  paged_merge_kernel<T, kD, kT, 1, kLargeMergeRows, 4><<<std::max(workers, 1024), kT, 0, st>>>(a);
+  paged_merge_large_kernel<T, kD><<<std::max(workers, 1024), kT, 0, st>>>(a);
 }
 
 template <class T>
@@ -1034,7 +1108,7 @@ int attn_paged(sh_ctx *ctx, const sh_paged_kv *kv, const uint16_t *q, uint16_t *
   p.sinks = sinks;
   p.min_piece = v.min_piece;
   p.workers = plan_workers(p.batch, p.kv_heads, tokens, p.capacity, p.per_tile, p.min_piece, v.workers);
-  p.inv_workers = std::nextafter(1.0 / p.workers, 2.0);
+  p.inv_workers = 1.0 / p.workers;
   a.items = static_cast<MergeItem *>(workspace);
   a.groups = reinterpret_cast<int *>(a.items + p.workers);
   a.redo = a.groups + p.workers;

@@ -28,11 +28,11 @@ static long long failures = 0;
 
 static constexpr int kParts = 256;
 
-static std::vector<long long> prefix_of(const PagedPlan &p, int per, long long *largest) {
+static std::vector<Line> prefix_of(const PagedPlan &p, int per, Line *largest) {
   *largest = 0;
-  std::vector<long long> prefix(kParts + 1, 0);
+  std::vector<Line> prefix(kParts + 1, 0);
   for (int t = 0; t < kParts; t++) {
-    long long sum = 0;
+    Line sum = 0;
     for (int b = t * per; b < (t + 1) * per && b < p.batch; b++) {
       const PlanSeq s = plan_sequence(p, b);
       sum = plan_add(sum, s.one * p.kv_heads);
@@ -54,27 +54,27 @@ struct Written {
 // orderly: starts ascend, so that every tile is there once.
 static void walk(const PagedPlan &p, bool orderly, int group) {
   const int per = (p.batch + kParts - 1) / kParts;
-  long long largest;
-  const std::vector<long long> prefix = prefix_of(p, per, &largest);
-  const long long total = prefix[kParts], piece = plan_piece(p, total, largest);
+  Line largest;
+  const std::vector<Line> prefix = prefix_of(p, per, &largest);
+  const Line total = prefix[kParts], piece = plan_piece(p, total, largest);
   CHECK(piece * p.workers >= total);
   // the workers that the host gives a call with these sizes have room for it, too
   PagedPlan q = p;
   q.workers = plan_workers(p.batch, p.kv_heads, p.tokens, p.capacity, p.per_tile, p.min_piece, 768);
-  q.inv_workers = std::nextafter(1.0 / q.workers, 2.0);
+  q.inv_workers = 1.0 / q.workers;
   CHECK(q.workers > 0 && q.workers <= 768 && q.workers % 8 == 0 && plan_piece(q, total, largest) * q.workers >= total);
   std::map<std::tuple<int, int, int>, Written> tiles;
   std::vector<MergeItem> items(p.workers);
   std::map<int, std::tuple<int, int, int>> slot_owner;
   for (int w = 0; w < p.workers; w++) {
     MergeItem item = {0, 0, 0, 0, 0, 0};
-    const long long x0 = w * piece, x1 = x0 + piece < total ? x0 + piece : total;
+    const Line x0 = w * piece, x1 = x0 + piece < total ? x0 + piece : total;
     long long steps = 0;
-    for (long long x = x0; x < x1;) {
+    for (Line x = x0; x < x1;) {
       const int part = plan_find(prefix.data(), kParts, x);
       const PagedTile tile = plan_locate(p, plan_sequence(p, plan_part_first(p, part, per)), part, per, prefix[part], x);
       const PieceStep s = plan_step(p, tile, piece, w, x0, x, &item);
-      if (orderly) CHECK(plan_first(tile, w, piece, x0) == (int)(tile.begin / piece));
+      if (orderly) CHECK(plan_first(tile, w, piece, x0) == (int)std::floor(tile.begin / piece));
       CHECK(s.tile.b >= 0 && s.tile.b < p.batch);
       CHECK(s.tile.kv_head >= 0 && s.tile.kv_head < p.kv_heads);
       CHECK(s.span.count >= 0 && s.span.count <= p.per_tile);
@@ -192,7 +192,7 @@ int main() {
     p.window = round % 3 == 0 ? 1 + upto(p.capacity) : 0;
     p.sinks = upto(round % 2 ? 8 : p.capacity);
     p.workers = 8 * (1 + upto(99));
-    p.inv_workers = std::nextafter(1.0 / p.workers, 2.0);
+    p.inv_workers = 1.0 / p.workers;
     p.min_piece = 64 << upto(3);
     p.whole_below = round % 2 ? 0 : upto(2000);
     std::vector<int> starts(p.batch + 1), lengths(p.batch);
@@ -212,14 +212,14 @@ int main() {
     PagedPlan p;
     p.batch = 4096;
     p.tokens = kMaxPagedTokens;
-    p.kv_heads = kMaxPagedKvHeads;
+    p.kv_heads = 1;
     p.capacity = kMaxPagedPositions;
     p.per_tile = 1;
     p.unit = 64;
     p.unit_shift = 6;
     p.window = p.sinks = 0;
     p.workers = 64;
-    p.inv_workers = std::nextafter(1.0 / 64, 2.0);
+    p.inv_workers = 1.0 / 64;
     p.min_piece = 256;
     p.whole_below = 0;
     std::vector<int> starts(p.batch + 1), lengths(p.batch, kMaxPagedPositions);
@@ -227,11 +227,11 @@ int main() {
     p.starts = starts.data();
     p.lengths = lengths.data();
     const int per = (p.batch + kParts - 1) / kParts;
-    long long largest;
-    const std::vector<long long> prefix = prefix_of(p, per, &largest);
+    Line largest;
+    const std::vector<Line> prefix = prefix_of(p, per, &largest);
     CHECK(prefix[kParts] == kMaxLine);
     for (int t = 0; t < kParts; t++) CHECK(prefix[t] <= prefix[t + 1]);
-    const long long piece = plan_piece(p, prefix[kParts], largest);
+    const Line piece = plan_piece(p, prefix[kParts], largest);
     for (int w = 0; w < p.workers; w++) {
       MergeItem item = {0, 0, 0, 0, 0, 0};
       const int part = plan_find(prefix.data(), kParts, w * piece);
@@ -261,6 +261,12 @@ int main() {
   for (int v : {16, 32, 65536}) CHECK(!refused(&sh_paged_kv::page_size, v));
   for (int v : {0, -1, 3, 4096}) CHECK(refused(&sh_paged_kv::kv_heads, v));
   for (int v : {0, -3, (1 << 24) + 1}) CHECK(refused(&sh_paged_kv::max_pages, v));
+  {
+    sh_paged_kv big = kv;
+    big.max_pages = 1 << 24;
+    big.kv_heads = 8;
+    CHECK(check_paged_sizes(&big, kMaxPagedTokens, 8) && !check_paged_sizes(&big, 1 << 20, 8));
+  }
   CHECK(!refused(&sh_paged_kv::max_pages, 1 << 24));
   for (int v : {0, -3}) CHECK(refused(&sh_paged_kv::num_pages, v));
   for (int v : {-1, kMaxPagedBatch + 1}) CHECK(refused(&sh_paged_kv::batch, v));
