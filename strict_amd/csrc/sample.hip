@@ -220,20 +220,25 @@ __device__ __forceinline__ unsigned long long target_of(const SampleArgs &a, int
 
 struct Candidates {
   unsigned long long key[kList], mass[kList];
-  unsigned int place[kList];  // index << 11 | position in key
+  unsigned long long bucket[1024];  // weights by ten bits of the index
 };
 
-// n values, a power of two of at least 2; `up`: ascending.
-template <class V>
-__device__ __forceinline__ void bitonic_sort(V *v, int n, bool up) {
+// n values, a power of two of at least 2, descending. A wave's pairs of a distance of
+// up to 64 lie in 128 values that no other wave touches meanwhile: of the 66 passes
+// over 2,048 values, 10 need barriers.
+__device__ __forceinline__ void bitonic_sort(unsigned long long *v, int n) {
+  bool apart = true;  // the last pass crossed the waves' values
   for (int k = 2; k <= n; k *= 2)
     for (int j = k / 2; j >= 1; j /= 2) {
-      __syncthreads();
+      if (apart || j > 64)
+        __syncthreads();
+      else
+        __builtin_amdgcn_wave_barrier();
+      apart = j > 64;
       for (int i = threadIdx.x; i < n / 2; i += kT) {
-        const int lo = (i / j) * 2 * j + i % j, hi = lo + j;
-        const bool asc = ((lo & k) == 0) == up;
-        const V x = v[lo], y = v[hi];
-        if ((x > y) == asc) {
+        const int lo = (i & ~(j - 1)) * 2 + (i & (j - 1)), hi = lo + j;
+        const unsigned long long x = v[lo], y = v[hi];
+        if ((x < y) == ((lo & k) == 0)) {
           v[lo] = y;
           v[hi] = x;
         }
@@ -253,7 +258,7 @@ __device__ __forceinline__ int power_of_two(int n) {
 __device__ __forceinline__ void rank_candidates(const RowParams &r, Candidates &c, int n, const double *table) {
   const int size = power_of_two(n);
   for (int i = n + threadIdx.x; i < size; i += kT) c.key[i] = 0;
-  bitonic_sort(c.key, size, false);
+  bitonic_sort(c.key, size);
   for (int i = threadIdx.x; i < n; i += kT) {
     double e;
     c.mass[i] = weight(exponent(r, key_value(c.key[i])), table, &e);
@@ -288,38 +293,48 @@ __device__ __forceinline__ unsigned long long total_mass(const Candidates &c, in
   return total;
 }
 
+// The bucket (of 1,024, ~0: none) on which `target` of the listed weights falls, in
+// c.bucket[1] what of it is left there.
+template <class Of>
+__device__ __forceinline__ unsigned pick_bucket(Candidates &c, int n, unsigned long long target,
+                                                unsigned long long *red, Of of) {
+  __syncthreads();  // the last buckets are read
+  for (int i = threadIdx.x; i < 1024; i += kT) c.bucket[i] = 0;
+  __syncthreads();
+  for (int i = threadIdx.x; i < n; i += kT) {
+    const unsigned b = of((unsigned)key_index(c.key[i]));
+    if (b != ~0u && c.mass[i] != 0) atomicAdd(&c.bucket[b], c.mass[i]);
+  }
+  __syncthreads();
+  const unsigned long long w0 = c.bucket[2 * threadIdx.x], w1 = c.bucket[2 * threadIdx.x + 1];
+  unsigned long long total;
+  const unsigned long long at = block_scan_u64(w0 + w1, red, &total) - (w0 + w1);  // (every bucket is read)
+  if (at <= target && target < at + w0 + w1) {
+    const bool second = target >= at + w0;
+    c.bucket[0] = 2 * threadIdx.x + (second ? 1 : 0);
+    c.bucket[1] = target - at - (second ? w0 : 0);
+  }
+  __syncthreads();
+  return (unsigned)c.bucket[0];
+}
+
 // Everything from a list of all tokens that may be kept. limit: top-p's, 0: to be
 // worked out of the list's weights (which are then all, or all that top-k keeps).
 __device__ __forceinline__ int draw_listed(const SampleArgs &a, const RowParams &r, int row, Candidates &c, int n,
                                            unsigned long long limit, const double *table,
                                            unsigned long long *red) {
-  constexpr int kPer = kList / kT;
   rank_candidates(r, c, n, table);
   if (r.k > 0) n = min(n, r.k);
   if (r.p < 1.0 && limit == 0) limit = limit_of(r.p, total_mass(c, n, red));
   n = kept_by_limit(c, n, 0, limit, red);
-  for (int i = threadIdx.x; i < n; i += kT) {
+  for (int i = threadIdx.x; i < n; i += kT)
     if (exp_minus(exponent(r, key_value(c.key[i])), table) < r.least) c.mass[i] = 0;
-    c.place[i] = ((unsigned)key_index(c.key[i]) << 11) | (unsigned)i;
-  }
-  const int size = power_of_two(n);
-  for (int i = n + threadIdx.x; i < size; i += kT) c.place[i] = 0xffffffffu;
-  bitonic_sort(c.place, size, true);
-  unsigned long long mass[kPer], sum = 0, total;
-  const int i0 = threadIdx.x * kPer;
-#pragma unroll
-  for (int e = 0; e < kPer; e++) {
-    mass[e] = i0 + e < n ? c.mass[c.place[i0 + e] & (kList - 1)] : 0;
-    sum += mass[e];
-  }
-  unsigned long long at = block_scan_u64(sum, red, &total) - sum, found = ~0ULL;
-  const unsigned long long target = target_of(a, row, total);
-#pragma unroll
-  for (int e = 0; e < kPer; e++) {
-    if (at <= target && target < at + mass[e]) found = c.place[i0 + e] >> 11;
-    at += mass[e];
-  }
-  return (int)block_min_u64(found, red);
+  __syncthreads();
+  // the token in the order of the indices: its upper ten bits, then its lower ten
+  unsigned long long target = target_of(a, row, total_mass(c, n, red));
+  const unsigned above = pick_bucket(c, n, target, red, [](unsigned i) { return i >> 10; });
+  target = c.bucket[1];
+  return (int)(above << 10 | pick_bucket(c, n, target, red, [above](unsigned i) { return (i >> 10) == above ? i & 1023 : ~0u; }));
 }
 
 // The first position in [begin, end) whose value is m.
@@ -403,9 +418,27 @@ __global__ __launch_bounds__(kT) void sample_max_kernel(const SampleArgs a) {
 }
 
 __device__ __forceinline__ float row_max(const RowState &s, int splits) {
-  float m = -INFINITY;
-  for (int i = 0; i < splits; i++) m = fmaxf(m, s.split_max[i]);
+  const int lane = threadIdx.x & 63;
+  float m = lane < splits ? s.split_max[lane] : -INFINITY;
+#pragma unroll
+  for (int off = 32; off >= 1; off >>= 1) m = fmaxf(m, __shfl_xor(m, off, 64));
   return m;
+}
+
+// use(v, i) of the row's values v[0 .. 3] at i .. i + 3, i from begin + 4 thread on, all
+// lanes of a wave together; four vectors requested at once.
+template <class Use>
+__device__ __forceinline__ void each4(const float *x, int begin, int end, Use use) {
+  constexpr int kU = 4;
+  const int lane = threadIdx.x & 63;
+  for (int i = begin + 4 * (int)threadIdx.x; i - 4 * lane < end; i += 4 * kT * kU) {
+    f32x4 v[kU];
+#pragma unroll
+    for (int u = 0; u < kU; u++) v[u] = load4(x, min(i + 4 * kT * u, end), end);
+#pragma unroll
+    for (int u = 0; u < kU; u++)
+      if (i + 4 * kT * u - 4 * lane < end) use(v[u], i + 4 * kT * u);
+  }
 }
 
 __global__ __launch_bounds__(kT) void sample_bins_kernel(const SampleArgs a) {
@@ -423,23 +456,24 @@ __global__ __launch_bounds__(kT) void sample_bins_kernel(const SampleArgs a) {
   }
   load_table(a, table);
   const int begin = split * a.chunk, end = min(begin + a.chunk, a.n);
-  for (int i = begin + 4 * (int)threadIdx.x; i < end; i += 4 * kT) {
-    const f32x4 v = load4(x, i, end);
+  const bool weighed = r.k == 0;  // (where top-k ends, the counts say)
+  each4(x, begin, end, [&](f32x4 v, int) {
 #pragma unroll
     for (int e = 0; e < 4; e++) {
       const double y = exponent(r, v[e]);
       if (y < kCutoff) {
-        double ex;
-        const unsigned long long w = weight(y, table, &ex);
-        atomicAdd(&mass[bin_of(y)], w);
+        if (weighed) {
+          double ex;
+          atomicAdd(&mass[bin_of(y)], weight(y, table, &ex));
+        }
         atomicAdd(&count[bin_of(y)], 1u);
       }
     }
-  }
+  });
   __syncthreads();
   for (int i = threadIdx.x; i < kBins; i += kT)
     if (count[i] != 0) {
-      atomicAdd(&s.mass[i], mass[i]);
+      if (weighed) atomicAdd(&s.mass[i], mass[i]);
       atomicAdd(&s.count[i], count[i]);
     }
 }
@@ -448,12 +482,14 @@ __global__ __launch_bounds__(kT) void sample_gather_kernel(const SampleArgs a) {
   constexpr int kPer = kBins / kT;
   __shared__ double table[64];
   __shared__ unsigned long long red[kT / 64];
-  __shared__ unsigned long long found[4];
-  const int row = blockIdx.x / a.splits, split = blockIdx.x % a.splits, lane = threadIdx.x & 63;
+  __shared__ unsigned long long found[4], list[kList];
+  __shared__ unsigned int listed, listed_at;
+  const int row = blockIdx.x / a.splits, split = blockIdx.x % a.splits;
   const float *x = a.x + (size_t)row * a.ld;
   RowState &s = a.rows[row];
   const RowParams r = row_params(a, row, row_max(s, a.splits));
   if (r.m == -INFINITY || r.greedy) return;
+  if (threadIdx.x == 0) listed = 0;
   load_table(a, table);
   int mode = kAll, bin = kBins, k = 0;
   unsigned long long limit = 0, before_mass = 0;
@@ -471,9 +507,10 @@ __global__ __launch_bounds__(kT) void sample_gather_kernel(const SampleArgs a) {
     }
     unsigned long long m0 = block_scan_u64(masses, red, &total_masses) - masses;
     unsigned long long c0 = block_scan_u64(counts, red, &total_counts) - counts;
-    k = r.k > 0 && (unsigned long long)r.k < total_counts ? r.k : 0;
-    if (k == 0 && r.p < 1.0) limit = limit_of(r.p, total_masses);
-    if (k > 0 || limit > 0) {
+    // (fewer tokens than top-k have a weight: it ends with the last of them)
+    k = r.k > 0 ? (int)min((unsigned long long)r.k, total_counts) : 0;
+    if (k == 0) limit = limit_of(r.p, total_masses);
+    {
 #pragma unroll
       for (int e = 0; e < kPer; e++) {
         // the bin that the k-th token, or the last one within the limit, is in
@@ -508,9 +545,13 @@ __global__ __launch_bounds__(kT) void sample_gather_kernel(const SampleArgs a) {
   }
   if (mode == kDigits) return;
   const int begin = split * a.chunk, end = min(begin + a.chunk, a.n);
+  // below this value no token is in the bins up to `bin` (a bin's width and a half
+  // more than y's roundings could make of it): most of the row is passed over by it
+  const float least = mode == kAll ? -INFINITY : (float)((double)r.m - (bin + 1.5) / (kBinsPerUnit * r.inv_t));
   unsigned long long sum = 0;
-  for (int i = begin + 4 * (int)threadIdx.x; i - 4 * lane < end; i += 4 * kT) {
-    const f32x4 v = load4(x, min(i, end), end);
+  each4(x, begin, end, [&](f32x4 v, int i) {
+    const float top = fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w));
+    if (__ballot(!(top < least)) == 0) return;  // (an infinite temperature below infinity: NaN)
 #pragma unroll
     for (int e = 0; e < 4; e++) {
       const double y = exponent(r, v[e]);
@@ -520,17 +561,19 @@ __global__ __launch_bounds__(kT) void sample_gather_kernel(const SampleArgs a) {
         const unsigned long long w = weight(y, table, &ex);
         sum += ex >= r.least ? w : 0;
       }
-      if (mode != kAll) {
-        const bool take = mode == kListed ? b <= bin : b == bin;
-        const unsigned long long takers = __ballot(take);
-        if (takers != 0) {
-          unsigned int at = 0;
-          if (lane == __ffsll(takers) - 1) at = atomicAdd(&s.listed, (unsigned)__popcll(takers));
-          at = __shfl(at, __ffsll(takers) - 1, 64) + __popcll(takers & ((1ULL << lane) - 1));
-          if (take && at < kList) s.list[at] = key_of(v[e], i + e);
-        }
+      // (the bins' counts say that the list holds them all)
+      if (mode != kAll && (mode == kListed ? b <= bin : b == bin)) {
+        const unsigned int at = atomicAdd(&listed, 1u);
+        if (at < kList) list[at] = key_of(v[e], i + e);
       }
     }
+  });
+  if (mode != kAll) {
+    __syncthreads();
+    if (threadIdx.x == 0 && listed > 0) listed_at = atomicAdd(&s.listed, listed);
+    __syncthreads();
+    for (unsigned int i = threadIdx.x; i < min(listed, (unsigned)kList); i += kT)
+      if (listed_at + i < kList) s.list[listed_at + i] = list[i];
   }
   if (mode != kListed) {
     unsigned long long total;
