@@ -1,7 +1,7 @@
 // One token per row of logits by temperature, top-k, top-p and min-p
 // (sh_sample_f32; the definition is in strict_hip.h).
 //
-// A token's weight is exp(-y), y = (max - x) / temperature, as a whole number of
+// A token's weight is exp(-(max - x) / temperature) = 2^-t as a whole number of
 // 2^-42: sums of weights are then exact in 64 bits (at most 2^20 tokens), in any
 // order, and atomics in any order give the same. The order of the tokens is that
 // of 64-bit keys: the value's order above, the complement of the index below.
@@ -9,8 +9,8 @@
 // Rows of up to 2,048 logits: one kernel, one workgroup a row. Longer ones in four
 // kernels over (row, split):
 //   max     the splits' largest values; clears the row's histogram
-//   bins    count and weight of the tokens by y in bins of 1/64 (rows with top-k
-//           or top-p only)
+//   bins    count of the tokens by t in bins of 1/46, or their weight, where top-p is
+//           without top-k; other rows pass
 //   gather  from the bins, the bin where top-k (without it, top-p) ends. Up to
 //           2,048 tokens to that bin's end: all of them to a list, from which the
 //           rest is decided. More: only that bin's tokens, and each split's weight
@@ -33,10 +33,10 @@ namespace sh {
 namespace {
 
 constexpr int kT = 512;
-constexpr int kBins = 2048, kBinsPerUnit = 64;
+constexpr int kBins = 2048, kBinsPerUnit = 46;
 constexpr int kList = 2048;
 constexpr int kFraction = 42;       // bits of a weight
-constexpr double kCutoff = 29.9;    // exp(-y) 2^42 is below 1/2 from y = 29.81 on
+constexpr float kCutoff = 43.1f;    // 2^-t 2^42 is below 1/2 from t = 43 on
 constexpr int kSegment = 256;       // tokens that a wave takes at once
 constexpr int kMaxSegments = kMaxSampleN / kSegment;
 constexpr int kMaxSplits = 64;
@@ -69,7 +69,9 @@ struct SampleArgs {
 
 struct RowParams {
   float m;          // largest logit
-  double inv_t;
+  float half_m;
+  double inv_t;     // log2(e) / temperature
+  float inv_2t;     // twice that in fp32
   bool greedy;
   int k;            // 0: all
   double p, least;  // p >= 1: all; least <= 0: all
@@ -82,42 +84,44 @@ __device__ __forceinline__ RowParams row_params(const SampleArgs &a, int row, fl
   const float p = a.top_p ? a.top_p[row] : 1.0f, least = a.min_p ? a.min_p[row] : 0.0f;
   r.m = m;
   r.greedy = !(t > 0.0f) || k == 1;
-  r.inv_t = 1.0 / (double)t;
+  r.half_m = 0.5f * m;
+  r.inv_t = 1.4426950408889634074 / (double)t;
+  r.inv_2t = fminf((float)(2.0 * r.inv_t), 3.40282347e+38f);
   r.k = k > 0 && k < a.n ? k : 0;
   r.p = p < 1.0f ? (double)p : 1.0;
   r.least = least > 0.0f ? (double)fminf(least, 1.0f) : 0.0;
   return r;
 }
 
-// y of a logit (NaN for one that is NaN).
-__device__ __forceinline__ double exponent(const RowParams &r, float x) {
-  return x == r.m ? 0.0 : ((double)r.m - (double)x) * r.inv_t;
+// t of a logit to fp32 (NaN for one that is NaN): descends with the logit, which is
+// all that the bins need. (Halves, as the difference may exceed fp32's range.)
+__device__ __forceinline__ float exponent(const RowParams &r, float x) {
+  return x == r.m ? 0.0f : (r.half_m - 0.5f * x) * r.inv_2t;
 }
 
-// exp(-y), 0 <= y < kCutoff: y = (n + f) ln(2) / 64, the table's 2^(-(n % 64) / 64)
-// and a polynomial of f's part, |f ln(2) / 64| <= 0.0055 (next term 4e-17).
-__device__ __forceinline__ double exp_minus(double y, const double *table) {
-  const double n = rint(y * 92.332482616893656877);
-  double f = fma(n, -1.08304246962491454596e-2, y);  // ln(2) / 64 to 2^-54 of it
-  f = fma(n, -3.62351064663484314921e-19, f);
-  double e = fma(f, -1.0 / 120.0, 1.0 / 24.0);
-  e = fma(f, e, -1.0 / 6.0);
-  e = fma(f, e, 0.5);
-  e = fma(f, e, -1.0);
+// 2^-t, 0 <= t: t = n / 64 + f, the table's 2^-((n % 64) / 64) and a polynomial of f,
+// |f| <= 1 / 128 (next term 4e-17).
+__device__ __forceinline__ double exp_minus(double t, const double *table) {
+  const double n = rint(t * 64.0), f = fma(n, -1.0 / 64.0, t);
+  double e = fma(f, -1.33335581464284434e-3, 9.61812910762847716e-3);  // ln(2)^k / k!
+  e = fma(f, e, -5.55041086648215800e-2);
+  e = fma(f, e, 2.40226506959100712e-1);
+  e = fma(f, e, -6.93147180559945309e-1);
   e = fma(f, e, 1.0);
   const int i = (int)n;
   return ldexp(e * table[i & 63], -(i >> 6));
 }
 
-// The weight; *e gets exp(-y). 0: never drawn.
-__device__ __forceinline__ unsigned long long weight(double y, const double *table, double *e) {
-  *e = exp_minus(y, table);
+// A logit's weight; *kept: whether min_p keeps it. 0: never drawn.
+__device__ __forceinline__ unsigned long long weight(const RowParams &r, float x, const double *table, bool *kept) {
+  const double e = exp_minus(x == r.m ? 0.0 : ((double)r.m - (double)x) * r.inv_t, table);
+  *kept = e >= r.least;
   // 2^52 + w has w in its low bits, rounded to the nearest
-  const double w = fma(*e, (double)(1LL << kFraction), 4503599627370496.0);
+  const double w = fma(e, (double)(1LL << kFraction), 4503599627370496.0);
   return __builtin_bit_cast(unsigned long long, w) & ((1ULL << 52) - 1);
 }
 
-__device__ __forceinline__ int bin_of(double y) { return (int)(y * kBinsPerUnit); }
+__device__ __forceinline__ int bin_of(float t) { return (int)(t * (float)kBinsPerUnit); }
 
 // Order of (value, index), descending; -0 as +0. 0 is no token's key (the value
 // of key 0 would be a NaN).
@@ -143,18 +147,22 @@ __device__ __forceinline__ f32x4 load4(const float *x, int i, int end) {
   return v;
 }
 
-__device__ __forceinline__ unsigned long long wave_sum_u64(unsigned long long v) {
-#pragma unroll
-  for (int off = 32; off >= 1; off >>= 1) v += __shfl_xor(v, off, 64);
-  return v;
+template <int kCtrl, int kRowMask>
+__device__ __forceinline__ unsigned long long dpp_u64(unsigned long long v) {
+  const uint32_t lo = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)v, kCtrl, kRowMask, 0xf, false);
+  const uint32_t hi = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)(v >> 32), kCtrl, kRowMask, 0xf, false);
+  return ((unsigned long long)hi << 32) | lo;
 }
 
+// Inclusive sum over the wave's lanes (row_shr:1, 2, 4, 8, row_bcast:15, 31; a lane
+// that gets nothing gets 0): a fifth of the time of LDS permutes.
 __device__ __forceinline__ unsigned long long wave_scan_u64(unsigned long long v) {
-#pragma unroll
-  for (int off = 1; off < 64; off *= 2) {
-    const unsigned long long o = __shfl_up(v, off, 64);
-    if ((int)(threadIdx.x & 63) >= off) v += o;
-  }
+  v += dpp_u64<0x111, 0xf>(v);
+  v += dpp_u64<0x112, 0xf>(v);
+  v += dpp_u64<0x114, 0xf>(v);
+  v += dpp_u64<0x118, 0xf>(v);
+  v += dpp_u64<0x142, 0xa>(v);
+  v += dpp_u64<0x143, 0xc>(v);
   return v;
 }
 
@@ -253,16 +261,32 @@ __device__ __forceinline__ int power_of_two(int n) {
   return p;
 }
 
-// Sorts c.key[0 .. n) (the rest up to the power of two is filled with 0) and works
-// out the weights.
+__device__ __forceinline__ unsigned long long key_weight(const RowParams &r, unsigned long long key,
+                                                         const double *table, bool *kept) {
+  const float x = key_value(key);
+  return weight(r, x, table, kept);
+}
+
+// Sorts c.key[0 .. n) (the keys are there) and works out the weights.
+constexpr int kCounted = 256;
 __device__ __forceinline__ void rank_candidates(const RowParams &r, Candidates &c, int n, const double *table) {
-  const int size = power_of_two(n);
-  for (int i = n + threadIdx.x; i < size; i += kT) c.key[i] = 0;
-  bitonic_sort(c.key, size);
-  for (int i = threadIdx.x; i < n; i += kT) {
-    double e;
-    c.mass[i] = weight(exponent(r, key_value(c.key[i])), table, &e);
+  bool kept;
+  if (n <= kCounted) {  // every key's place by counting the larger ones
+    const unsigned long long key = (int)threadIdx.x < n ? c.key[threadIdx.x] : 0;
+    int place = 0;
+    if (((int)threadIdx.x & ~63) < n) {
+#pragma unroll 8
+      for (int i = 0; i < n; i++) place += c.key[i] > key;
+    }
+    __syncthreads();
+    if ((int)threadIdx.x < n) c.key[place] = key;
+    __syncthreads();
+  } else {
+    const int size = power_of_two(n);
+    for (int i = n + threadIdx.x; i < size; i += kT) c.key[i] = 0;
+    bitonic_sort(c.key, size);
   }
+  for (int i = threadIdx.x; i < n; i += kT) c.mass[i] = key_weight(r, c.key[i], table, &kept);
   __syncthreads();
 }
 
@@ -327,9 +351,14 @@ __device__ __forceinline__ int draw_listed(const SampleArgs &a, const RowParams 
   if (r.k > 0) n = min(n, r.k);
   if (r.p < 1.0 && limit == 0) limit = limit_of(r.p, total_mass(c, n, red));
   n = kept_by_limit(c, n, 0, limit, red);
-  for (int i = threadIdx.x; i < n; i += kT)
-    if (exp_minus(exponent(r, key_value(c.key[i])), table) < r.least) c.mass[i] = 0;
-  __syncthreads();
+  if (r.least > 0.0) {
+    bool kept;
+    for (int i = threadIdx.x; i < n; i += kT) {
+      key_weight(r, c.key[i], table, &kept);
+      if (!kept) c.mass[i] = 0;
+    }
+    __syncthreads();
+  }
   // the token in the order of the indices: its upper ten bits, then its lower ten
   unsigned long long target = target_of(a, row, total_mass(c, n, red));
   const unsigned above = pick_bucket(c, n, target, red, [](unsigned i) { return i >> 10; });
@@ -379,8 +408,8 @@ __global__ __launch_bounds__(kT) void sample_short_kernel(const SampleArgs a) {
     } else {
 #pragma unroll
       for (int e = 0; e < 4; e++) {
-        const double y = exponent(r, v[e]);
-        if (y < kCutoff) c.key[atomicAdd(&listed, 1u)] = key_of(v[e], 4 * threadIdx.x + e);
+        const float t = exponent(r, v[e]);
+        if (t < kCutoff) c.key[atomicAdd(&listed, 1u)] = key_of(v[e], 4 * threadIdx.x + e);
       }
       __syncthreads();
       found = draw_listed(a, r, row, c, (int)listed, 0, table, red);
@@ -460,14 +489,16 @@ __global__ __launch_bounds__(kT) void sample_bins_kernel(const SampleArgs a) {
   each4(x, begin, end, [&](f32x4 v, int) {
 #pragma unroll
     for (int e = 0; e < 4; e++) {
-      const double y = exponent(r, v[e]);
-      if (y < kCutoff) {
-        if (weighed) {
-          double ex;
-          atomicAdd(&mass[bin_of(y)], weight(y, table, &ex));
-        }
-        atomicAdd(&count[bin_of(y)], 1u);
+      const float t = exponent(r, v[e]);
+      if (!(t < kCutoff)) continue;
+      if (!weighed) {
+        atomicAdd(&count[bin_of(t)], 1u);
+        continue;
       }
+      bool kept;
+      const unsigned long long w = weight(r, v[e], table, &kept);
+      atomicAdd(&mass[bin_of(t)], w);
+      atomicAdd(&count[bin_of(t)], 1u);
     }
   });
   __syncthreads();
@@ -547,19 +578,21 @@ __global__ __launch_bounds__(kT) void sample_gather_kernel(const SampleArgs a) {
   const int begin = split * a.chunk, end = min(begin + a.chunk, a.n);
   // below this value no token is in the bins up to `bin` (a bin's width and a half
   // more than y's roundings could make of it): most of the row is passed over by it
-  const float least = mode == kAll ? -INFINITY : (float)((double)r.m - (bin + 1.5) / (kBinsPerUnit * r.inv_t));
+  const float least = mode == kAll || (r.k == 0 && bin == kBins - 1)
+                          ? -INFINITY
+                          : (float)((double)r.m - (bin + 1.5) / (kBinsPerUnit * r.inv_t));
   unsigned long long sum = 0;
   each4(x, begin, end, [&](f32x4 v, int i) {
     const float top = fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w));
     if (__ballot(!(top < least)) == 0) return;  // (an infinite temperature below infinity: NaN)
 #pragma unroll
     for (int e = 0; e < 4; e++) {
-      const double y = exponent(r, v[e]);
-      const int b = y < kCutoff ? bin_of(y) : kBins + 1;
+      const float t = exponent(r, v[e]);
+      const int b = t < kCutoff ? bin_of(t) : kBins + 1;
       if (mode != kListed && b < bin) {
-        double ex;
-        const unsigned long long w = weight(y, table, &ex);
-        sum += ex >= r.least ? w : 0;
+        bool kept;
+        const unsigned long long w = weight(r, v[e], table, &kept);
+        sum += kept ? w : 0;
       }
       // (the bins' counts say that the list holds them all)
       if (mode != kAll && (mode == kListed ? b <= bin : b == bin)) {
@@ -600,12 +633,12 @@ struct DrawLds {
 // one's), and min_p. Its weight, or 0.
 __device__ __forceinline__ unsigned long long kept_weight(const RowParams &r, float x, int i, int bin,
                                                           unsigned long long last, const double *table) {
-  const double y = exponent(r, x);
-  if (!(y < kCutoff)) return 0;
-  if (!(bin_of(y) < bin) && key_of(x, i) < last) return 0;
-  double e;
-  const unsigned long long w = weight(y, table, &e);
-  return e >= r.least ? w : 0;
+  const float t = exponent(r, x);
+  if (!(t < kCutoff)) return 0;
+  if (!(bin_of(t) < bin) && key_of(x, i) < last) return 0;
+  bool kept;
+  const unsigned long long w = weight(r, x, table, &kept);
+  return kept ? w : 0;
 }
 
 // The token of [begin, end) on which `target` of the kept weights from `begin` on
@@ -622,8 +655,8 @@ __device__ __forceinline__ unsigned long long segment_sums(const RowParams &r, c
     unsigned long long sum = 0;
 #pragma unroll
     for (int e = 0; e < 4; e++) sum += kept_weight(r, v[e], i + e, bin, last, lds.table);
-    sum = wave_sum_u64(sum);
-    if (lane == 0) lds.segment[g] = sum;
+    sum = wave_scan_u64(sum);
+    if (lane == 63) lds.segment[g] = sum;
   }
   __syncthreads();
   unsigned long long sum = 0, total;
@@ -681,11 +714,11 @@ __device__ unsigned long long key_at(const RowParams &r, const float *x, int n, 
     __syncthreads();
     for (int i = threadIdx.x; i < n; i += kT) {
       const float v = x[i];
-      const double y = exponent(r, v);
+      const float t = exponent(r, v);
       const unsigned long long key = key_of(v, i);
-      if (!(y < kCutoff) || (shift < 56 && (key >> (shift + 8)) != prefix)) continue;
-      double e;
-      const unsigned long long w = weight(y, lds.table, &e);
+      if (!(t < kCutoff) || (shift < 56 && (key >> (shift + 8)) != prefix)) continue;
+      bool kept;
+      const unsigned long long w = weight(r, v, lds.table, &kept);
       atomicAdd(&lds.digits.mass[(key >> shift) & 255], w);
       atomicAdd(&lds.digits.amount[(key >> shift) & 255], by_mass ? w : 1ULL);
     }
@@ -752,9 +785,11 @@ __global__ __launch_bounds__(kT) void sample_draw_kernel(const SampleArgs a) {
         const int kept = s.k > 0 ? min(listed, s.k - (int)s.before_count)
                                  : kept_by_limit(lds.c, listed, s.before_mass, s.limit, lds.red);
         last = lds.c.key[max(kept - 1, 0)];
-        for (int i = threadIdx.x; i < kept; i += kT)
-          if (exp_minus(exponent(r, key_value(lds.c.key[i])), lds.table) >= r.least)
-            atomicAdd(&lds.split_mass[key_index(lds.c.key[i]) / a.chunk], lds.c.mass[i]);
+        for (int i = threadIdx.x; i < kept; i += kT) {
+          bool above;
+          const unsigned long long w = key_weight(r, lds.c.key[i], lds.table, &above);
+          if (above) atomicAdd(&lds.split_mass[key_index(lds.c.key[i]) / a.chunk], w);
+        }
         __syncthreads();
       }
       unsigned long long total = 0;
