@@ -322,7 +322,7 @@ inline const char *check_paged_sizes(const sh_paged_kv *kv, int tokens, int head
     return "max_pages must be positive and max_pages * page_size at most 2^28";
   // (what an attention call may cost: kMaxLine, in tiles of one token)
   if (((double)tokens + kv->batch) * kv->kv_heads * ((double)kv->max_pages * kv->page_size + 512.0) > kMaxLine)
-    return "(tokens + batch) * kv_heads * max_pages * page_size exceeds 2^52";
+    return "(tokens + batch) * kv_heads * (max_pages * page_size + 512) exceeds 2^52";
   return nullptr;
 }
 

@@ -207,10 +207,6 @@ __device__ __forceinline__ void scan_costs(const PagedPlan &p, int per, PlanLds 
 
 // A value that is the same in every lane, as the compiler cannot know of one from LDS.
 __device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
-__device__ __forceinline__ Line uniform(Line x) {
-  const uint64_t u = __builtin_bit_cast(uint64_t, x);
-  return __builtin_bit_cast(Line, ((uint64_t)(uint32_t)uniform((int)(u >> 32)) << 32) | (uint32_t)uniform((int)u));
-}
 
 // The last i < kT with prefix[i] <= x: how many of the values from prefix[1] on are
 // (a wave looks at all 256 at once).
