@@ -1,0 +1,322 @@
+"""The operators over a KV cache in pages as a server uses them together: sequences
+that start, fork, end and move in the pool, steps captured into a graph, two
+contexts at once. Values are checked against the formulas in 64 bits (as in
+test_gpu_paged.py, whose tolerances these are)."""
+import ctypes
+import threading
+
+import numpy as np
+import pytest
+
+import strict_amd
+import test_gpu_paged as paged
+import test_gpu_sample as sampling
+from strict_amd.paged import OutOfPages, PagedCache
+
+pytestmark = pytest.mark.gpu
+
+THREAD_LOCAL = 1  # hipStreamCaptureModeThreadLocal
+EPS, THETA = float(np.float32(1e-6)), 1e4
+
+
+@pytest.fixture(scope="module")
+def hip():
+    return ctypes.CDLL("libamdhip64.so")
+
+
+class Server:
+    """A cache of `layers` layers with what each sequence's tokens were: k as the
+    device stored it (checked when it was written), v as it was given."""
+
+    def __init__(self, ctx, seed, dtype, layers, heads, kv_heads, d, vocab, **cache):
+        self.rng, self.ctx, self.dtype, self.vocab = np.random.default_rng(seed), ctx, dtype, vocab
+        self.heads, self.kv_heads, self.d = heads, kv_heads, d
+        self.cache = PagedCache(ctx, layers, kv_heads, d, dtype=dtype, **cache)
+        ctx.memset(self.cache.pool, 0xff)  # NaN wherever nothing was written
+        self.said = [[([], []) for _ in range(layers)] for _ in range(cache["rows"])]  # [row][layer]
+        self.gains = [(1 + self.rng.normal(0, 0.3, d)).astype(np.float32) for _ in range(2)]
+        self.gain_bufs = [ctx.upload(g) for g in self.gains]
+
+    def plane(self, layer, which):
+        t = self.cache.table
+        shape = (t.num_pages, self.kv_heads, t.page_size, self.d)
+        nbytes = t.num_pages * self.cache.page_bytes
+        return self.cache.pool.view((2 * layer + which) * nbytes, nbytes, np.int16, shape).to_host()
+
+    def fork(self, row, to):
+        self.cache.fork(row, to)
+        self.said[to] = [(list(k), list(v)) for k, v in self.said[row]]
+
+    def free(self, row):
+        self.cache.free(row)
+        self.said[row] = [([], []) for _ in self.said[row]]
+
+    def step(self, new, window=0, sinks=0):
+        """A step of all layers, each operator checked; returns the sampled tokens."""
+        ctx, rng, d = self.ctx, self.rng, self.d
+        tokens, all_heads = self.cache.step(new), self.heads + 2 * self.kv_heads
+        table, rows = self.cache.table, sorted(r for r, n in new.items() if n)
+        max_new = max(new.values())
+        q = ctx.alloc(tokens * self.heads * d * 2).view(0, tokens * self.heads * d * 2, np.int16, (tokens, self.heads, d))
+        out = ctx.upload(paged.to16(np.full((tokens, self.heads, d), 0.5), self.dtype))
+        work = ctx.alloc(ctx.attn_paged_workspace(self.cache.kv[0], tokens, self.heads, max_new))
+        scale = float(np.float32(d ** -0.5))
+        for layer, kv in enumerate(self.cache.kv):
+            bits = paged.to16(rng.normal(0, 1.5, (tokens, all_heads, d)), self.dtype)
+            qkv = ctx.upload(bits)
+            ctx.qk_norm_rope_paged(kv, qkv, *self.gain_bufs, q, tokens, self.heads, EPS, THETA)
+            ctx.attn_paged(kv, q, out, tokens, self.heads, max_new, scale, work, window, sinks)
+            ctx.sync()
+            kd, vd = self.plane(layer, 0), self.plane(layer, 1)
+            x, got_q, got = paged.from16(bits, self.dtype), paged.from16(q.to_host(), self.dtype), paged.from16(out.to_host(), self.dtype)
+            u, at = paged.U[self.dtype], 0
+            for row in rows:
+                n, length = new[row], table.lengths[row]
+                pos = np.arange(length - n, length)
+                page, slot = np.array(table.pages[row])[pos // table.page_size], pos % table.page_size
+                mine = slice(at, at + n)
+                for part, gain, stored in ((x[mine, :self.heads], self.gains[0], got_q[mine]),
+                                           (x[mine, self.heads:self.heads + self.kv_heads], self.gains[1],
+                                            paged.from16(kd[page, :, slot], self.dtype))):
+                    ref, size = paged.norm_rope_oracle(part, gain.astype(np.float64), pos.astype(np.float64), EPS, THETA)
+                    assert (np.abs(stored - ref) <= u * np.abs(ref) + 32 * paged.F * size + 2.0 ** -25).all()
+                ks, vs = self.said[row][layer]
+                ks.extend(kd[page, :, slot])
+                vs.extend(bits[mine, self.heads + self.kv_heads:])
+                assert len(ks) == length
+                # the whole sequence is where the table says, as it was written
+                pos = np.arange(length)
+                page, slot = np.array(table.pages[row])[pos // table.page_size], pos % table.page_size
+                assert (kd[page, :, slot] == np.array(ks)).all() and (vd[page, :, slot] == np.array(vs)).all()
+                seq = History(self, row, layer, n)
+                ref, tol = paged.attention_oracle(seq, got_q[mine], window, sinks, scale)
+                assert (np.abs(got[mine] - ref) <= tol).all(), (row, layer)
+                at += n
+            qkv.free()
+        logits = rng.normal(0, 2.5, (tokens, self.vocab)).astype(np.float32)
+        u = rng.random(tokens).astype(np.float32)
+        t, k, p = (np.resize(v, tokens) for v in (np.float32([0.7, 0.0, 1.3]), np.int32([50, 0, 0]), np.float32([1, 0.9, 0.8])))
+        sampling.check(ctx, logits, t, k, p, None, u)
+        for b in (q, out, work):
+            b.free()
+
+    def dispose(self):
+        self.cache.dispose()
+        for b in self.gain_bufs:
+            b.free()
+
+
+class History:
+    """A sequence as attention_oracle takes one: its tokens in one page."""
+
+    def __init__(self, server, row, layer, n):
+        ks, vs = server.said[row][layer]
+        self.dtype, self.heads, self.kv_heads, self.d = server.dtype, server.heads, server.kv_heads, server.d
+        self.batch, self.new, self.lengths, self.starts = 1, [n], [len(ks)], [0]
+        self.k, self.v = (np.array(x).swapaxes(0, 1) for x in (ks, vs))
+
+    def gathered(self, bits, b, kv_head):
+        return paged.from16(bits[kv_head], self.dtype), np.ones(bits.shape[1], bool)
+
+
+@pytest.mark.parametrize("dtype,heads,kv_heads,d,page", [("f16", 8, 2, 64, 16), ("bf16", 4, 4, 128, 32)])
+def test_a_server(ctx, dtype, heads, kv_heads, d, page):
+    # prompts, decode, a fork whose rows part, an end, a compaction, a late prompt
+    s = Server(ctx, 1, dtype, 2, heads, kv_heads, d, 2500, rows=4, max_pages=300 // page, num_pages=700 // page,
+               page_size=page)
+    s.step({0: 100, 2: 37})
+    s.step({0: 1, 2: 1, 3: 150})
+    s.fork(0, 1)
+    for _ in range(3):
+        s.step({0: 1, 1: 1, 2: 1, 3: 1})
+    assert s.cache.table.pages[0][-1] != s.cache.table.pages[1][-1]
+    s.free(0)
+    s.free(2)
+    s.step({1: 1, 3: 1})
+    before = s.cache.table.array()
+    assert s.cache.compact() > 0 and (before != s.cache.table.array()).any()
+    s.step({1: 1, 3: 1})
+    s.step({1: 2, 0: 130, 3: 1}, window=40, sinks=4)
+    with pytest.raises(OutOfPages):
+        s.cache.step({2: 301})
+    s.step({0: 1, 1: 1, 3: 1}, window=40, sinks=4)
+    s.dispose()
+
+
+def test_rows_that_share_a_page_in_the_middle(ctx):
+    # forks of a fork that part at once: one copy each but for the last holder
+    s = Server(ctx, 2, "f16", 1, 2, 1, 64, 300, rows=4, max_pages=8, num_pages=20, page_size=16)
+    s.step({0: 21})
+    for to in (1, 2, 3):
+        s.fork(to - 1, to)
+    s.step({0: 1, 1: 3, 2: 16, 3: 1})
+    s.step({0: 1, 1: 1, 2: 1, 3: 1})
+    s.dispose()
+
+
+class Step:
+    """One step's operators on buffers that stay: head norms and pages, attention,
+    a page copy, and a token from the attention's values as logits."""
+
+    def __init__(self, ctx, seed, new, lengths, heads=4, kv_heads=2, d=64, page=16, work=None):
+        self.ctx = ctx
+        self.c = c = paged.Case(ctx, seed, "f16", new, lengths, heads, kv_heads, d, page, rows_behind=0, spare=2, extra_entries=4)
+        # (every entry a page of its own, so that lengths may grow)
+        c.num_pages = c.batch * c.max_pages + 2
+        order = c.rng.permutation(c.num_pages - 2).astype(np.int32)
+        c.table = order.reshape(c.batch, c.max_pages)
+        shape = (c.num_pages, kv_heads, page, d)
+        c.k, c.v = (paged.to16(c.rng.normal(0, 1, shape), "f16") for _ in range(2))
+        self.kv = c.upload()
+        self.max_new = max(new)
+        self.vocab = heads * d * c.tokens // 2
+        self.bufs = dict(
+            qkv=ctx.empty((c.tokens, heads + 2 * kv_heads, d), np.int16), q=ctx.empty((c.tokens, heads, d), np.int16),
+            out=ctx.empty((c.tokens, heads, d), np.int16), gain=ctx.upload(np.ones(d, np.float32)),
+            src=ctx.upload(np.array([order[0]], np.int32)), dst=ctx.upload(np.array([c.num_pages - 1], np.int32)),
+            k=ctx.upload(np.array([40, 0], np.int32)), p=ctx.upload(np.array([1, 0.9], np.float32)),
+            u=ctx.upload(np.array([0.3, 0.6], np.float32)), index=ctx.empty(2, np.int32),
+            logits=ctx.empty((2, 5000), np.float32))
+        need = max(ctx.attn_paged_workspace(self.kv, c.tokens, heads, self.max_new), ctx.sample_workspace(2, 5000))
+        self.mine = work is None
+        self.work = ctx.alloc(need) if work is None else work
+        assert self.work.nbytes >= need
+
+    def inputs(self, seed, more):
+        """New tokens' values and lengths, as the next step has them."""
+        rng, c, b = np.random.default_rng(seed), self.c, self.bufs
+        b["qkv"].copy_from_host(paged.to16(rng.normal(0, 1.5, b["qkv"].shape), "f16"))
+        b["logits"].copy_from_host(rng.normal(0, 2, (2, 5000)).astype(np.float32))
+        c.buffers[0].copy_from_host(c.k)
+        c.buffers[1].copy_from_host(c.v)
+        c.buffers[3].copy_from_host(np.array([min(l + more, c.max_pages * c.page) for l in c.lengths], np.int32))
+
+    def run(self):
+        ctx, c, b = self.ctx, self.c, self.bufs
+        ctx.qk_norm_rope_paged(self.kv, b["qkv"], b["gain"], b["gain"], b["q"], c.tokens, c.heads, EPS, THETA)
+        ctx.attn_paged(self.kv, b["q"], b["out"], c.tokens, c.heads, self.max_new, 0.125, self.work, 90, 4)
+        ctx.pages_copy(c.buffers[0], 1, c.num_pages, c.kv_heads * c.page * c.d * 2, b["src"], b["dst"], 1)
+        ctx.sample(b["logits"], 2, 5000, None, b["k"], b["p"], None, b["u"], b["index"], self.work)
+
+    def results(self):
+        self.ctx.sync()
+        return [x.to_host().copy() for x in (self.bufs["q"], self.bufs["out"], self.bufs["index"], *self.c.buffers[:2])]
+
+    def clear(self):
+        self.ctx.memset(self.bufs["out"], 0xff)
+        self.ctx.memset(self.bufs["index"], 0xff)
+
+    def free(self):
+        for b in self.bufs.values():
+            b.free()
+        self.c.free()
+        if self.mine:
+            self.work.free()
+
+
+def same(a, b):
+    return all(np.array_equal(x, y) for x, y in zip(a, b))
+
+
+class Captured:
+    def __init__(self, hip, ctx, step):
+        self.hip, self.ctx = hip, ctx
+        stream, graph, self.run = ctypes.c_void_p(ctx.stream()), ctypes.c_void_p(), ctypes.c_void_p()
+        assert hip.hipStreamBeginCapture(stream, THREAD_LOCAL) == 0
+        try:
+            step.run()
+        finally:
+            ended = hip.hipStreamEndCapture(stream, ctypes.byref(graph))
+        assert ended == 0
+        assert hip.hipGraphInstantiate(ctypes.byref(self.run), graph, None, None, ctypes.c_size_t(0)) == 0
+        assert hip.hipGraphDestroy(graph) == 0
+
+    def launch(self):
+        assert self.hip.hipGraphLaunch(self.run, ctypes.c_void_p(self.ctx.stream())) == 0
+
+    def destroy(self):
+        assert self.hip.hipGraphExecDestroy(self.run) == 0
+
+
+@pytest.mark.parametrize("new,lengths", [([1, 1, 1], [300, 40, 17]), ([30, 1, 90], [400, 40, 90])])
+def test_captured_steps(hip, new, lengths):
+    # replays with other values and lengths, with eager steps in between, repeat the eager results
+    with strict_amd.Context(0) as ctx:
+        step, other = Step(ctx, 3, new, lengths), Step(ctx, 4, [1, 9], [100, 9])
+        other.inputs(0, 0)
+        other.run()
+        first = other.results()
+        graph = Captured(hip, ctx, step)
+        for i in range(5):
+            step.inputs(i, 7 * i)
+            step.run()
+            eager = step.results()
+            step.inputs(i, 7 * i)
+            step.clear()
+            if i % 2:
+                other.inputs(0, 0)
+                other.run()  # (nothing waits between)
+            graph.launch()
+            assert same(step.results(), eager), i
+            assert same(other.results(), first), i
+        graph.destroy()
+        step.free()
+        other.free()
+
+
+def test_two_graphs_of_one_work_buffer(hip):
+    # in turn on one stream
+    with strict_amd.Context(0) as ctx:
+        work = ctx.alloc(64 << 20)
+        steps = [Step(ctx, 5, [1, 1], [500, 90], work=work), Step(ctx, 6, [140, 3], [300, 60], work=work)]
+        want, graphs = [], []
+        for s in steps:
+            s.inputs(1, 0)
+            s.run()
+            want.append(s.results())
+            graphs.append(Captured(hip, ctx, s))
+        for _ in range(3):
+            for s in steps:
+                s.inputs(1, 0)
+                s.clear()
+            for g in graphs + graphs[::-1]:
+                g.launch()
+            for s, w in zip(steps, want):
+                assert same(s.results(), w)
+        for g in graphs:
+            g.destroy()
+        for s in steps:
+            s.free()
+        work.free()
+
+
+def test_contexts_at_once():
+    # a thread and a stream each, buffers of its own: as alone
+    def work(i, results):
+        with strict_amd.Context(0) as ctx:
+            step = Step(ctx, 10 + i, [1, 60 + i, 5], [900, 61 + i, 400])
+            got = []
+            for j in range(6):
+                step.inputs(j, j)
+                step.run()
+                got.append(step.results())
+            step.free()
+            results[i] = got
+    alone, together = {}, {}
+    for i in range(3):
+        work(i, alone)
+    threads = [threading.Thread(target=work, args=(i, together)) for i in range(3)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    for i in range(3):
+        assert all(same(a, b) for a, b in zip(alone[i], together[i])), i
+
+
+def test_a_page_in_several_tables_and_twice_in_one(ctx):
+    # what is only read may be shared in any way
+    c = paged.Case(ctx, 21, "bf16", [1, 1, 40], [100, 100, 140], 4, 2, 64, 16)
+    c.table[1, :6] = c.table[0, :6]
+    c.table[2, 1:4] = c.table[2, 0]
+    paged.check_attention(c)
