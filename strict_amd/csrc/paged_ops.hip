@@ -71,7 +71,9 @@ __device__ __forceinline__ int find_seq(const int *__restrict__ starts, int batc
 // A wave takes 4 * kHeadsAt heads of one token: q heads, then k, then v. A head is
 // d / 16 lanes wide, 8 values of its first half and the 8 that rotate with them in
 // each lane, all loads requested at once. The factors, one pair of them per lane,
-// are worked out meanwhile and go round through LDS. Bound by the rows' bytes.
+// are worked out meanwhile and go round through LDS. Bound by the rows' bytes: 152 MB
+// of bf16 rows of 32 heads of 128 in and out in 25 us, 6.0 TB/s. (Stores that the
+// caches need not keep: 36 us with ordinary ones. Loads of that kind as well: 28.)
 template <class T, int kD>
 __global__ __launch_bounds__(kT) void norm_rope_kernel(const NormRopeArgs a) {
   constexpr int kLanes = kD / 16, kHeadsAt = 64 / kLanes, kSteps = 4, kHalf = kD / 2;
@@ -137,8 +139,8 @@ __global__ __launch_bounds__(kT) void norm_rope_kernel(const NormRopeArgs a) {
     else
       to = (is_k ? a.k : a.v) +
            ((((size_t)page * a.kv_heads + (h - a.heads - (is_k ? 0 : a.kv_heads))) << a.page_shift) + in_page) * kD;
-    *reinterpret_cast<u32x4 *>(to + part * 8) = o1;
-    *reinterpret_cast<u32x4 *>(to + part * 8 + kHalf) = o2;
+    __builtin_nontemporal_store(o1, reinterpret_cast<u32x4 *>(to + part * 8));
+    __builtin_nontemporal_store(o2, reinterpret_cast<u32x4 *>(to + part * 8 + kHalf));
   }
 }
 
@@ -201,7 +203,8 @@ int norm_rope(sh_ctx *ctx, const sh_paged_kv *kv, const uint16_t *qkv, const flo
 constexpr int kCopyVectors = 4;  // of 16 bytes per thread
 
 // grid (chunks of a page, pages, planes): 16 KiB of one page, all of a thread's
-// loads requested before its first store.
+// loads requested before its first store. Bound by the bytes: 257 MB both ways in 45 us,
+// 5.7 TB/s (as accesses that the caches keep: 51).
 __global__ __launch_bounds__(kT) void pages_copy_kernel(uint8_t *pool, size_t plane_stride, int num_pages,
                                                         uint32_t page_vectors, int chunks,
                                                         const int *__restrict__ src,
@@ -215,10 +218,10 @@ __global__ __launch_bounds__(kT) void pages_copy_kernel(uint8_t *pool, size_t pl
   const uint32_t at = (uint32_t)chunk * (kT * kCopyVectors) + threadIdx.x;
   u32x4 v[kCopyVectors];
 #pragma unroll
-  for (int u = 0; u < kCopyVectors; u++) v[u] = s[min(at + u * kT, page_vectors - 1)];
+  for (int u = 0; u < kCopyVectors; u++) v[u] = __builtin_nontemporal_load(s + min(at + u * kT, page_vectors - 1));
 #pragma unroll
   for (int u = 0; u < kCopyVectors; u++)
-    if (at + u * kT < page_vectors) d[at + u * kT] = v[u];
+    if (at + u * kT < page_vectors) __builtin_nontemporal_store(v[u], d + at + u * kT);
 }
 
 }  // namespace
