@@ -157,7 +157,6 @@ __device__ void attn_exact(const PagedAttnArgs &a, const PagedTile &t, const Til
 struct PlanLds {
   Line prefix[kT + 1], waves[kMaxT / 64], largest[kMaxT / 64];
   PlanSeq seqs[kT];  // where a thread has one sequence
-  Line x, piece;     // the next step's point (here and not in registers)
 };
 
 template <int kCtrl, int kRowMask>
@@ -207,6 +206,10 @@ __device__ __forceinline__ void scan_costs(const PagedPlan &p, int per, PlanLds 
 
 // A value that is the same in every lane, as the compiler cannot know of one from LDS.
 __device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
+__device__ __forceinline__ Line uniform(Line x) {
+  const uint64_t u = __builtin_bit_cast(uint64_t, x);
+  return __builtin_bit_cast(Line, ((uint64_t)(uint32_t)uniform((int)(u >> 32)) << 32) | (uint32_t)uniform((int)u));
+}
 
 // The last i < kT with prefix[i] <= x: how many of the values from prefix[1] on are
 // (a wave looks at all 256 at once).
@@ -224,17 +227,14 @@ template <class Part>
 __device__ __forceinline__ bool walk_piece(const PagedPlan &p, int worker, PlanLds &lds, MergeItem *item, Part part) {
   const int per = (p.batch + kT - 1) / kT;
   scan_costs(p, per, lds);
-  if (threadIdx.x == 0) {
-    Line largest = 0;
-    for (int w = 0; w < kT / 64; w++) largest = fmax(largest, lds.largest[w]);
-    lds.piece = plan_piece(p, lds.prefix[kT], largest);
-    lds.x = worker * lds.piece;
-  }
-  __syncthreads();
+  Line largest = 0;
+#pragma unroll
+  for (int w = 0; w < kT / 64; w++) largest = fmax(largest, lds.largest[w]);
+  const Line total = uniform(lds.prefix[kT]), piece = uniform(plan_piece(p, total, largest)), x0 = worker * piece;
+  const Line end = uniform(fmin(x0 + piece, total));
   bool finite = true;
-  while (true) {
-    const Line total = lds.prefix[kT], piece = lds.piece, x = lds.x, x0 = worker * piece;
-    if (uniform(x >= fmin(x0 + piece, total) ? 1 : 0)) break;
+  Line x = x0;
+  while (uniform(x < end ? 1 : 0)) {
     const int i = uniform(find_part(lds, x)), b = plan_part_first(p, i, per);
     const PagedTile t = plan_locate(p, per == 1 ? lds.seqs[b] : plan_sequence(p, b), i, per, lds.prefix[i], x);
     PieceStep st = plan_step(p, t, piece, worker, x0, x, item);
@@ -244,9 +244,7 @@ __device__ __forceinline__ bool walk_piece(const PagedPlan &p, int worker, PlanL
       *v = uniform(*v);
     st.run = uniform(st.run ? 1 : 0) != 0;
     st.more = uniform(st.more ? 1 : 0) != 0;
-    __syncthreads();  // lds.x is read
-    if (threadIdx.x == 0) lds.x = t.begin + t.cost;
-    __syncthreads();
+    x = uniform(t.begin + t.cost);
     if (!st.more) break;
     if (st.run && !part(st, piece)) finite = false;
   }
@@ -833,7 +831,9 @@ __global__ __launch_bounds__(kT, kLarge.workers / 256) void paged_large_kernel(c
 // worker w, which works them out in fp32, and its whole tiles too.
 struct MergeLds {
   union {
-    int prefix[kT + 1];
+    struct {
+      int prefix[kT + 1], first[kT];  // of worker 2 i: the groups before its, and its groups
+    };
     PlanLds plan;
   };
   int waves[kMaxT / 64];
@@ -849,7 +849,11 @@ __device__ __forceinline__ bool find_item(const PagedAttnArgs &a, const MergeLds
   n = uniform(n);
   int w = 2 * n;
   *g = unit - uniform(lds.prefix[n]);
-  if (*g >= a.groups[w]) *g -= a.groups[w++];
+  const int first = uniform(lds.first[n]);
+  if (*g >= first) {
+    *g -= first;
+    w++;
+  }
   *it = a.items[w];
   return true;
 }
@@ -857,39 +861,47 @@ __device__ __forceinline__ bool find_item(const PagedAttnArgs &a, const MergeLds
 // Prefix sums of the items' groups, by threads of two workers each.
 __device__ __forceinline__ void scan_items(const PagedAttnArgs &a, MergeLds &lds) {
   static_assert(kMaxWorkers <= 2 * kT, "two items per thread");
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  int sum = 0;
-  if (tid < kT)
-    for (int w = 2 * tid; w < min(2 * tid + 2, a.plan.workers); w++) sum += a.groups[w];
-#pragma unroll
-  for (int off = 1; off < 64; off *= 2) {
-    const int o = __shfl_up(sum, off, 64);
-    if (lane >= off) sum += o;
-  }
-  if (lane == 63) lds.waves[wave] = sum;
+  const int tid = threadIdx.x, wave = tid >> 6;
+  int2 two = make_int2(0, 0);  // (workers are a multiple of 8)
+  if (2 * tid < a.plan.workers) two = reinterpret_cast<const int2 *>(a.groups)[tid];
+  int sum = two.x + two.y;
+  sum += __builtin_amdgcn_update_dpp(0, sum, 0x111, 0xf, 0xf, false);  // (as in wave_scan_line)
+  sum += __builtin_amdgcn_update_dpp(0, sum, 0x112, 0xf, 0xf, false);
+  sum += __builtin_amdgcn_update_dpp(0, sum, 0x114, 0xf, 0xf, false);
+  sum += __builtin_amdgcn_update_dpp(0, sum, 0x118, 0xf, 0xf, false);
+  sum += __builtin_amdgcn_update_dpp(0, sum, 0x142, 0xa, 0xf, false);
+  sum += __builtin_amdgcn_update_dpp(0, sum, 0x143, 0xc, 0xf, false);
+  if ((tid & 63) == 63) lds.waves[wave] = sum;
   __syncthreads();
-  for (int w = 0; w < wave; w++) sum += lds.waves[w];
-  if (tid < kT) lds.prefix[tid + 1] = sum;
+  if (tid < kT) {
+#pragma unroll
+    for (int w = 0; w < kT / 64; w++) sum += w < wave ? lds.waves[w] : 0;
+    lds.prefix[tid + 1] = sum;
+    lds.first[tid] = two.x;
+  }
   if (tid == 0) lds.prefix[0] = 0;
   __syncthreads();
 }
 
 // The flagged workers' tiles.
 template <class T, int kD>
-__device__ __forceinline__ void redo_tiles(const PagedAttnArgs &a, MergeLds &lds) {
-  for (int w = blockIdx.x; w < a.plan.workers; w += gridDim.x) {
-    if (a.redo[w] == 0) continue;
-    __syncthreads();  // lds.prefix is read
-    MergeItem unused;
-    walk_piece(a.plan, w, lds.plan, &unused, [&](const PieceStep &st, Line piece) {
-      if (st.slot >= 0)  // a cut tile is the first flagged worker's
-        for (int j = plan_first(st.tile, w, piece, w * piece); j < w; j++)
-          if (a.redo[j] != 0) return true;
-      attn_exact<T, kD>(a, st.tile, st.span);
-      return true;
-    });
-    __syncthreads();
-  }
+__device__ __forceinline__ void redo_tiles(const PagedAttnArgs &a, MergeLds &lds, int flagged) {
+  const int w = blockIdx.x;
+  if (flagged == 0) return;
+  __syncthreads();  // lds.prefix is read
+  MergeItem unused;
+  walk_piece(a.plan, w, lds.plan, &unused, [&](const PieceStep &st, Line piece) {
+    if (st.slot >= 0)  // a cut tile is the first flagged worker's
+      for (int j = plan_first(st.tile, w, piece, w * piece); j < w; j++)
+        if (a.redo[j] != 0) return true;
+    attn_exact<T, kD>(a, st.tile, st.span);
+    return true;
+  });
+}
+
+// (read at once, for the end; there are as many workgroups as workers, or more)
+__device__ __forceinline__ int redo_flag(const PagedAttnArgs &a) {
+  return (int)blockIdx.x < a.plan.workers ? a.redo[blockIdx.x] : 0;
 }
 
 __device__ __forceinline__ int part_slot(const MergeItem &it, int j) {
@@ -905,6 +917,7 @@ __global__ __launch_bounds__(kMergeT) void paged_merge_small_kernel(const PagedA
   __shared__ Dims num_part[kWaves][64];
   __shared__ float top_part[kWaves], den_part[kWaves];
   const int lane = threadIdx.x & 63, wave = uniform((int)threadIdx.x >> 6);
+  const int flagged = redo_flag(a);
   scan_items(a, lds);
   MergeItem it;
   int r;
@@ -963,7 +976,7 @@ __global__ __launch_bounds__(kMergeT) void paged_merge_small_kernel(const PagedA
     }
     __syncthreads();  // the parts are read
   }
-  redo_tiles<T, kD>(a, lds);
+  redo_tiles<T, kD>(a, lds, flagged);
 }
 
 template <class T, int kD>
@@ -973,6 +986,7 @@ __global__ __launch_bounds__(kT) void paged_merge_large_kernel(const PagedAttnAr
   typedef Value Quad __attribute__((ext_vector_type(4)));
   __shared__ MergeLds lds;
   const int lane = threadIdx.x & 63, n32 = lane & 31, h = lane >> 5;
+  const int flagged = redo_flag(a);
   scan_items(a, lds);
   MergeItem it;
   int g;
@@ -1021,7 +1035,7 @@ __global__ __launch_bounds__(kT) void paged_merge_large_kernel(const PagedAttnAr
       *reinterpret_cast<Quad *>(op + 8 * i) = o;
     }
   }
-  redo_tiles<T, kD>(a, lds);
+  redo_tiles<T, kD>(a, lds, flagged);
 }
 
 // ---- the entry points ---------------------------------------------------------------
