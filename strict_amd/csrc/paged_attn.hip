@@ -927,25 +927,39 @@ __global__ __launch_bounds__(kMergeT) void paged_merge_small_kernel(const PagedA
     bool redo = false;
     for (int j0 = wave; j0 < it.parts; j0 += kWaves * kStep) {
       Dims x[kStep];
+      // (the maxima and sums of the wave's parts by a lane each; a load more for each
+      // part, and for those that are not there, was 2 us of 9)
+      const int mine = j0 + kWaves * lane;
+      float my_m = -INFINITY, my_l = 0.0f;
+      int not_finite = 0;
+      if (lane < kStep && mine < it.parts) {
+        const f32x2 stat = *reinterpret_cast<const f32x2 *>(slot_stats<kD>(a, part_slot(it, mine), r));
+        my_m = stat.x;
+        my_l = stat.y;
+        not_finite = a.redo[it.first_worker + mine];
+      }
+#pragma unroll
+      for (int u = 0; u < kStep; u++) {
+        x[u] = 0.0f;
+        const int j = j0 + kWaves * u;
+        if (j < it.parts)
+          x[u] = *reinterpret_cast<const Dims *>(slot_of<kD>(a, part_slot(it, j)) + r * kD + lane * kDims);
+      }
+      redo = redo || __any(not_finite != 0);
       float m[kStep], l[kStep], t = top;
 #pragma unroll
       for (int u = 0; u < kStep; u++) {
-        const int j = min(j0 + kWaves * u, it.parts - 1), slot = part_slot(it, j);
-        x[u] = *reinterpret_cast<const Dims *>(slot_of<kD>(a, slot) + r * kD + lane * kDims);
-        m[u] = slot_stats<kD>(a, slot, r)[0];
-        l[u] = slot_stats<kD>(a, slot, r)[1];
-        redo = redo || a.redo[it.first_worker + j] != 0;
+        m[u] = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, my_m), u));
+        l[u] = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, my_l), u));
+        t = fmaxf(t, m[u]);
       }
-#pragma unroll
-      for (int u = 0; u < kStep; u++)
-        if (j0 + kWaves * u < it.parts) t = fmaxf(t, m[u]);
       const float c = t == top ? 1.0f : exp2_weight(top - t);
       top = t;
       num *= c;
       den *= c;
 #pragma unroll
       for (int u = 0; u < kStep; u++) {
-        const float f = m[u] == -INFINITY || j0 + kWaves * u >= it.parts ? 0.0f : exp2_weight(m[u] - t);
+        const float f = m[u] == -INFINITY ? 0.0f : exp2_weight(m[u] - t);
         num += f * x[u];
         den = fmaf(f, l[u], den);
       }
@@ -1003,16 +1017,22 @@ __global__ __launch_bounds__(kT) void paged_merge_large_kernel(const PagedAttnAr
       float m[kStep], l[kStep], t = top;
 #pragma unroll
       for (int u = 0; u < kStep; u++) {
-        const int j = min(j0 + u, it.parts - 1), slot = part_slot(it, j);
+        const int j = j0 + u, slot = part_slot(it, j);
+        m[u] = -INFINITY;
+        l[u] = 0.0f;
 #pragma unroll
-        for (int i = 0; i < 4; i++) x[u][i] = *slot_large<kD>(a, slot, wave, db, i);
-        m[u] = slot_stats<kD>(a, slot, row)[0];
-        l[u] = slot_stats<kD>(a, slot, row)[1];
-        redo = redo || a.redo[it.first_worker + j] != 0;
+        for (int i = 0; i < 4; i++) x[u][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+        if (j < it.parts) {
+          const f32x2 stat = *reinterpret_cast<const f32x2 *>(slot_stats<kD>(a, slot, row));
+          m[u] = stat.x;
+          l[u] = stat.y;
+#pragma unroll
+          for (int i = 0; i < 4; i++) x[u][i] = *slot_large<kD>(a, slot, wave, db, i);
+          redo = redo || a.redo[it.first_worker + j] != 0;
+        }
       }
 #pragma unroll
-      for (int u = 0; u < kStep; u++)
-        if (j0 + u < it.parts) t = fmaxf(t, m[u]);
+      for (int u = 0; u < kStep; u++) t = fmaxf(t, m[u]);
       const float c = t == top ? 1.0f : exp2_weight(top - t);
       top = t;
       den *= c;
@@ -1020,7 +1040,7 @@ __global__ __launch_bounds__(kT) void paged_merge_large_kernel(const PagedAttnAr
       for (int i = 0; i < 4; i++) num[i] *= c;
 #pragma unroll
       for (int u = 0; u < kStep; u++) {
-        const float f = m[u] == -INFINITY || j0 + u >= it.parts ? 0.0f : exp2_weight(m[u] - t);
+        const float f = m[u] == -INFINITY ? 0.0f : exp2_weight(m[u] - t);
         den = fmaf(f, l[u], den);
 #pragma unroll
         for (int i = 0; i < 4; i++) num[i] += f * x[u][i];
