@@ -13,11 +13,11 @@
 //           without top-k; other rows pass
 //   gather  from the bins, the bin where top-k (without it, top-p) ends. Up to
 //           2,048 tokens to that bin's end: all of them to a list, from which the
-//           rest is decided. More: only that bin's tokens, and each split's weight
-//           of the kept tokens before them. Without top-k and top-p: each split's
-//           weight of all
-//   draw    a workgroup a row: sorts the list, ends the selection within it, finds
-//           the split, in it the 256 tokens and among them the token that u falls on
+//           rest is decided. More: only that bin's tokens, and the weight of the
+//           kept tokens before them in each run of 512. Without top-k and top-p: that
+//           of all tokens
+//   draw    a workgroup a row: ends the selection within the list, finds the run and
+//           in it the token that u falls on
 // A list that would not hold the bin's tokens, or top-p after a top-k of more than
 // the list holds: the draw kernel finds the last kept key by its digits, reading
 // the row once per digit.
@@ -39,6 +39,8 @@ constexpr int kFraction = 42;       // bits of a weight
 constexpr float kCutoff = 43.1f;    // 2^-t 2^42 is below 1/2 from t = 43 on
 constexpr int kSegment = 256;       // tokens that a wave takes at once
 constexpr int kMaxSegments = kMaxSampleN / kSegment;
+constexpr int kRun = 2 * kSegment;  // of the gathering kernel
+constexpr int kMaxRuns = kMaxSampleN / kRun;
 constexpr int kMaxSplits = 64;
 
 enum { kAll = 0, kListed = 1, kBinned = 2, kDigits = 3 };
@@ -48,7 +50,7 @@ struct RowState {
   unsigned long long mass[kBins];  // weights of the bin's tokens
   unsigned int count[kBins];
   unsigned long long list[kList];  // keys
-  unsigned long long split_mass[kMaxSplits];
+  unsigned long long run_mass[kMaxRuns];  // weight of the kept tokens before `bin`
   float split_max[kMaxSplits];
   unsigned int listed;
   int mode, bin;                   // bin: where the list ends (kAll: past all bins)
@@ -228,38 +230,10 @@ __device__ __forceinline__ unsigned long long target_of(const SampleArgs &a, int
 
 struct Candidates {
   unsigned long long key[kList], mass[kList];
-  unsigned long long bucket[1024];  // weights by ten bits of the index
+  unsigned long long bucket[1024];  // weights by ten bits of the index, or of the key
+  unsigned int held[1024];          // tokens by ten bits of the key
+  unsigned int high, low;
 };
-
-// n values, a power of two of at least 2, descending. A wave's pairs of a distance of
-// up to 64 lie in 128 values that no other wave touches meanwhile: of the 66 passes
-// over 2,048 values, 10 need barriers.
-__device__ __forceinline__ void bitonic_sort(unsigned long long *v, int n) {
-  bool apart = true;  // the last pass crossed the waves' values
-  for (int k = 2; k <= n; k *= 2)
-    for (int j = k / 2; j >= 1; j /= 2) {
-      if (apart || j > 64)
-        __syncthreads();
-      else
-        __builtin_amdgcn_wave_barrier();
-      apart = j > 64;
-      for (int i = threadIdx.x; i < n / 2; i += kT) {
-        const int lo = (i & ~(j - 1)) * 2 + (i & (j - 1)), hi = lo + j;
-        const unsigned long long x = v[lo], y = v[hi];
-        if ((x < y) == ((lo & k) == 0)) {
-          v[lo] = y;
-          v[hi] = x;
-        }
-      }
-    }
-  __syncthreads();
-}
-
-__device__ __forceinline__ int power_of_two(int n) {
-  int p = 2;
-  while (p < n) p *= 2;
-  return p;
-}
 
 __device__ __forceinline__ unsigned long long key_weight(const RowParams &r, unsigned long long key,
                                                          const double *table, bool *kept) {
@@ -267,67 +241,118 @@ __device__ __forceinline__ unsigned long long key_weight(const RowParams &r, uns
   return weight(r, x, table, kept);
 }
 
-// Sorts c.key[0 .. n) (the keys are there) and works out the weights.
-constexpr int kCounted = 256;
-__device__ __forceinline__ void rank_candidates(const RowParams &r, Candidates &c, int n, const double *table) {
+__device__ __forceinline__ void weigh_candidates(const RowParams &r, Candidates &c, int n, const double *table) {
   bool kept;
-  if (n <= kCounted) {  // every key's place by counting the larger ones
-    const unsigned long long key = (int)threadIdx.x < n ? c.key[threadIdx.x] : 0;
-    int place = 0;
-    if (((int)threadIdx.x & ~63) < n) {
-#pragma unroll 8
-      for (int i = 0; i < n; i++) place += c.key[i] > key;
-    }
-    __syncthreads();
-    if ((int)threadIdx.x < n) c.key[place] = key;
-    __syncthreads();
-  } else {
-    const int size = power_of_two(n);
-    for (int i = n + threadIdx.x; i < size; i += kT) c.key[i] = 0;
-    bitonic_sort(c.key, size);
-  }
   for (int i = threadIdx.x; i < n; i += kT) c.mass[i] = key_weight(r, c.key[i], table, &kept);
   __syncthreads();
 }
 
-// Of n ranked candidates, those before them having weight `before`: how many are
-// kept by the limit (0: all).
-__device__ __forceinline__ int kept_by_limit(const Candidates &c, int n, unsigned long long before,
-                                             unsigned long long limit, unsigned long long *red) {
-  constexpr int kPer = kList / kT;
-  if (limit == 0) return n;
-  unsigned long long sum = 0, total, first = n;
-  const int i0 = threadIdx.x * kPer;
-#pragma unroll
-  for (int e = 0; e < kPer; e++) sum += i0 + e < n ? c.mass[i0 + e] : 0;
-  unsigned long long at = before + block_scan_u64(sum, red, &total) - sum;
-#pragma unroll
-  for (int e = 0; e < kPer; e++)
-    if (i0 + e < n) {
-      if (at >= limit && first == (unsigned long long)n) first = i0 + e;
-      at += c.mass[i0 + e];
+// The first of n keys, descending, at which `before` and the keys' counts (by_mass
+// false) or weights up to it and with it reach `limit`, which all of them do. By ten
+// bits of the keys at a time, from the first in which they differ on, until one key is
+// left: two or three rounds mostly, where a sort of 2,048 keys took 66 passes (16 rows
+// of 151,936 with top-k 1,000 and top-p 48 -> 40 us a call). Up to 256 keys are compared
+// with each other (top-k 50: 26 us, by rounds 30).
+constexpr int kCounted = 256;
+__device__ __forceinline__ unsigned long long last_key(Candidates &c, int n, bool by_mass, unsigned long long before,
+                                                       unsigned long long limit, unsigned long long *red) {
+  __syncthreads();  // the last buckets are read
+  if (n <= kCounted) {  // each key's sum by itself
+    if (((int)threadIdx.x & ~63) < n) {
+      const int mine = min((int)threadIdx.x, n - 1);
+      const unsigned long long key = c.key[mine], own = by_mass ? c.mass[mine] : 1;
+      unsigned long long sum = before;
+#pragma unroll 8
+      for (int i = 0; i < n; i++) sum += c.key[i] >= key ? (by_mass ? c.mass[i] : 1) : 0;
+      if (sum >= limit && sum - own < limit) c.bucket[0] = key;
     }
-  return (int)block_min_u64(first, red);
+    __syncthreads();
+    return c.bucket[0];
+  }
+  if (threadIdx.x == 0) {
+    c.high = 0;
+    c.low = ~0u;
+  }
+  __syncthreads();
+  unsigned high = 0, low = ~0u;
+  for (int i = threadIdx.x; i < n; i += kT) {
+    const unsigned value = (unsigned)(c.key[i] >> 32);
+    high = max(high, value);
+    low = min(low, value);
+  }
+  if (high >= low) {  // (the thread has a key)
+    atomicMax(&c.high, high);
+    atomicMin(&c.low, low);
+  }
+  __syncthreads();
+  high = c.high;
+  const unsigned differ = high ^ c.low;
+  // the keys from bit `known` on are `prefix`, the next digit starts at `shift` (of one
+  // value: the keys' lower halves are complements of numbers below 2^20)
+  int known = differ != 0 ? 64 - __clz(differ) : 20, shift = known - 10;
+  unsigned long long prefix =
+      known < 64 ? (((unsigned long long)high << 32) | (differ != 0 ? 0u : ~0u)) >> known : 0;
+  while (true) {
+    for (int i = threadIdx.x; i < 1024; i += kT) {
+      c.bucket[i] = 0;
+      c.held[i] = 0;
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < n; i += kT) {
+      const unsigned long long key = c.key[i];
+      if (known < 64 && (key >> known) != prefix) continue;
+      const unsigned d = (unsigned)(key >> shift) & 1023;
+      atomicAdd(&c.held[d], 1u);
+      if (by_mass) atomicAdd(&c.bucket[d], c.mass[i]);
+    }
+    __syncthreads();
+    // this thread's digits, descending
+    const int d0 = 1023 - 2 * threadIdx.x, d1 = d0 - 1;
+    const unsigned n0 = c.held[d0], n1 = c.held[d1];
+    const unsigned long long w0 = by_mass ? c.bucket[d0] : n0, w1 = by_mass ? c.bucket[d1] : n1;
+    unsigned long long total;
+    const unsigned long long at = before + block_scan_u64(w0 + w1, red, &total) - (w0 + w1);  // (all are read)
+    if (at < limit && limit <= at + w0 + w1) {
+      const bool second = limit > at + w0;
+      c.bucket[0] = second ? d1 : d0;
+      c.bucket[1] = at + (second ? w0 : 0);
+      c.bucket[2] = second ? n1 : n0;
+    }
+    __syncthreads();
+    prefix = prefix << (known - shift) | (c.bucket[0] & ((1ULL << (known - shift)) - 1));
+    before = c.bucket[1];
+    const bool one = c.bucket[2] == 1;
+    known = shift;
+    __syncthreads();
+    if (one || known == 0) break;
+    shift = max(shift - 10, 0);
+  }
+  for (int i = threadIdx.x; i < n; i += kT)
+    if ((c.key[i] >> known) == prefix) c.bucket[0] = c.key[i];
+  __syncthreads();
+  return c.bucket[0];
 }
 
-__device__ __forceinline__ unsigned long long total_mass(const Candidates &c, int n, unsigned long long *red) {
+// Of the keys from `last` on.
+__device__ __forceinline__ unsigned long long total_mass(const Candidates &c, int n, unsigned long long last,
+                                                         unsigned long long *red) {
   unsigned long long sum = 0, total;
-  for (int i = threadIdx.x; i < n; i += kT) sum += c.mass[i];
+  for (int i = threadIdx.x; i < n; i += kT) sum += c.key[i] >= last ? c.mass[i] : 0;
   block_scan_u64(sum, red, &total);
   return total;
 }
 
-// The bucket (of 1,024, ~0: none) on which `target` of the listed weights falls, in
-// c.bucket[1] what of it is left there.
+// The bucket (of 1,024, ~0: none) on which `target` of the listed weights (of keys
+// from `last` on) falls, in c.bucket[1] what of it is left there.
 template <class Of>
-__device__ __forceinline__ unsigned pick_bucket(Candidates &c, int n, unsigned long long target,
+__device__ __forceinline__ unsigned pick_bucket(Candidates &c, int n, unsigned long long last, unsigned long long target,
                                                 unsigned long long *red, Of of) {
   __syncthreads();  // the last buckets are read
   for (int i = threadIdx.x; i < 1024; i += kT) c.bucket[i] = 0;
   __syncthreads();
   for (int i = threadIdx.x; i < n; i += kT) {
     const unsigned b = of((unsigned)key_index(c.key[i]));
-    if (b != ~0u && c.mass[i] != 0) atomicAdd(&c.bucket[b], c.mass[i]);
+    if (b != ~0u && c.key[i] >= last && c.mass[i] != 0) atomicAdd(&c.bucket[b], c.mass[i]);
   }
   __syncthreads();
   const unsigned long long w0 = c.bucket[2 * threadIdx.x], w1 = c.bucket[2 * threadIdx.x + 1];
@@ -347,10 +372,10 @@ __device__ __forceinline__ unsigned pick_bucket(Candidates &c, int n, unsigned l
 __device__ __forceinline__ int draw_listed(const SampleArgs &a, const RowParams &r, int row, Candidates &c, int n,
                                            unsigned long long limit, const double *table,
                                            unsigned long long *red) {
-  rank_candidates(r, c, n, table);
-  if (r.k > 0) n = min(n, r.k);
-  if (r.p < 1.0 && limit == 0) limit = limit_of(r.p, total_mass(c, n, red));
-  n = kept_by_limit(c, n, 0, limit, red);
+  weigh_candidates(r, c, n, table);
+  unsigned long long last = 0;  // the last kept key
+  if (r.k > 0 && r.k < n) last = last_key(c, n, false, 0, r.k, red);
+  if (r.p < 1.0) last = last_key(c, n, true, 0, limit != 0 ? limit : limit_of(r.p, total_mass(c, n, last, red)), red);
   if (r.least > 0.0) {
     bool kept;
     for (int i = threadIdx.x; i < n; i += kT) {
@@ -360,10 +385,10 @@ __device__ __forceinline__ int draw_listed(const SampleArgs &a, const RowParams 
     __syncthreads();
   }
   // the token in the order of the indices: its upper ten bits, then its lower ten
-  unsigned long long target = target_of(a, row, total_mass(c, n, red));
-  const unsigned above = pick_bucket(c, n, target, red, [](unsigned i) { return i >> 10; });
+  unsigned long long target = target_of(a, row, total_mass(c, n, last, red));
+  const unsigned above = pick_bucket(c, n, last, target, red, [](unsigned i) { return i >> 10; });
   target = c.bucket[1];
-  return (int)(above << 10 | pick_bucket(c, n, target, red, [above](unsigned i) { return (i >> 10) == above ? i & 1023 : ~0u; }));
+  return (int)(above << 10 | pick_bucket(c, n, last, target, red, [above](unsigned i) { return (i >> 10) == above ? i & 1023 : ~0u; }));
 }
 
 // The first position in [begin, end) whose value is m.
@@ -581,37 +606,44 @@ __global__ __launch_bounds__(kT) void sample_gather_kernel(const SampleArgs a) {
   const float least = mode == kAll || (r.k == 0 && bin == kBins - 1)
                           ? -INFINITY
                           : (float)((double)r.m - (bin + 1.5) / (kBinsPerUnit * r.inv_t));
-  unsigned long long sum = 0;
-  each4(x, begin, end, [&](f32x4 v, int i) {
-    const float top = fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w));
-    if (__ballot(!(top < least)) == 0) return;  // (an infinite temperature below infinity: NaN)
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  for (int i0 = begin + wave * kRun; i0 < end; i0 += kT / 64 * kRun) {
+    unsigned long long sum = 0;
+    f32x4 vs[kRun / kSegment];
 #pragma unroll
-    for (int e = 0; e < 4; e++) {
-      const float t = exponent(r, v[e]);
-      const int b = t < kCutoff ? bin_of(t) : kBins + 1;
-      if (mode != kListed && b < bin) {
-        bool kept;
-        const unsigned long long w = weight(r, v[e], table, &kept);
-        sum += kept ? w : 0;
-      }
-      // (the bins' counts say that the list holds them all)
-      if (mode != kAll && (mode == kListed ? b <= bin : b == bin)) {
-        const unsigned int at = atomicAdd(&listed, 1u);
-        if (at < kList) list[at] = key_of(v[e], i + e);
+    for (int u = 0; u < kRun / kSegment; u++) vs[u] = load4(x, min(i0 + u * kSegment + 4 * lane, end), end);
+#pragma unroll
+    for (int u = 0; u < kRun / kSegment; u++) {
+      const f32x4 v = vs[u];
+      const float top = fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w));
+      if (__ballot(!(top < least)) == 0) continue;  // (an infinite temperature below infinity: NaN)
+#pragma unroll
+      for (int e = 0; e < 4; e++) {
+        const float t = exponent(r, v[e]);
+        const int b = t < kCutoff ? bin_of(t) : kBins + 1;
+        if (mode != kListed && b < bin) {
+          bool kept;
+          const unsigned long long w = weight(r, v[e], table, &kept);
+          sum += kept ? w : 0;
+        }
+        // (the bins' counts say that the list holds them all)
+        if (mode != kAll && (mode == kListed ? b <= bin : b == bin)) {
+          const unsigned int at = atomicAdd(&listed, 1u);
+          if (at < kList) list[at] = key_of(v[e], i0 + u * kSegment + 4 * lane + e);
+        }
       }
     }
-  });
+    if (mode != kListed) {
+      sum = wave_scan_u64(sum);
+      if (lane == 63) s.run_mass[i0 / kRun] = sum;
+    }
+  }
   if (mode != kAll) {
     __syncthreads();
     if (threadIdx.x == 0 && listed > 0) listed_at = atomicAdd(&s.listed, listed);
     __syncthreads();
     for (unsigned int i = threadIdx.x; i < min(listed, (unsigned)kList); i += kT)
       if (listed_at + i < kList) s.list[listed_at + i] = list[i];
-  }
-  if (mode != kListed) {
-    unsigned long long total;
-    block_scan_u64(sum, red, &total);
-    if (threadIdx.x == 0) s.split_mass[split] = total;
   }
 }
 
@@ -626,7 +658,7 @@ struct DrawLds {
     } digits;
   };
   double table[64];
-  unsigned long long red[kT / 64], split_mass[kMaxSplits], shared[4];
+  unsigned long long red[kT / 64], run_mass[kMaxRuns], shared[4];
 };
 
 // A token is kept: by its bin (before `bin`), or its key (`last`: the last kept
@@ -697,6 +729,46 @@ __device__ __forceinline__ int pick(const RowParams &r, const float *x, int begi
       if (to <= target && target < to + w[e]) lds.shared[2] = i + e;
       to += w[e];
     }
+  }
+  __syncthreads();
+  return (int)lds.shared[2];
+}
+
+// The token that u falls on, from the runs' weights.
+__device__ __forceinline__ int pick_in_run(const SampleArgs &a, const RowParams &r, const float *x, int row, int bin,
+                                           unsigned long long last, DrawLds &lds) {
+  constexpr int kPer = kMaxRuns / kT;
+  static_assert(kMaxRuns % kT == 0 && kRun <= 4 * kT, "some runs per thread, then four tokens");
+  unsigned long long total, sum = 0;
+  const int g0 = kPer * (int)threadIdx.x;
+#pragma unroll
+  for (int e = 0; e < kPer; e++) sum += lds.run_mass[g0 + e];
+  unsigned long long at = block_scan_u64(sum, lds.red, &total) - sum;
+  const unsigned long long target = target_of(a, row, total);
+#pragma unroll
+  for (int e = 0; e < kPer; e++) {
+    const unsigned long long w = lds.run_mass[g0 + e];
+    if (at <= target && target < at + w) {
+      lds.shared[0] = g0 + e;
+      lds.shared[1] = at;
+    }
+    at += w;
+  }
+  __syncthreads();
+  const int i = (int)lds.shared[0] * kRun + 4 * (int)threadIdx.x;
+  const int end = min((int)(lds.shared[0] + 1) * kRun, a.n);
+  const f32x4 v = load4(x, min(i, end), end);
+  unsigned long long w[4], mine = 0;
+#pragma unroll
+  for (int e = 0; e < 4; e++) {
+    w[e] = kept_weight(r, v[e], i + e, bin, last, lds.table);
+    mine += w[e];
+  }
+  at = lds.shared[1] + block_scan_u64(mine, lds.red, &sum) - mine;
+#pragma unroll
+  for (int e = 0; e < 4; e++) {
+    if (at <= target && target < at + w[e]) lds.shared[2] = i + e;
+    at += w[e];
   }
   __syncthreads();
   return (int)lds.shared[2];
@@ -778,28 +850,20 @@ __global__ __launch_bounds__(kT) void sample_draw_kernel(const SampleArgs a) {
       const unsigned long long total = segment_sums(r, x, 0, a.n, bin, last, lds);
       found = pick(r, x, 0, a.n, bin, last, target_of(a, row, total), lds);
     } else {
-      for (int i = threadIdx.x; i < a.splits; i += kT) lds.split_mass[i] = s.split_mass[i];
+      for (int i = threadIdx.x; i < kMaxRuns; i += kT) lds.run_mass[i] = i * kRun < a.n ? s.run_mass[i] : 0;
       __syncthreads();
       if (mode == kBinned) {
-        rank_candidates(r, lds.c, listed, lds.table);
-        const int kept = s.k > 0 ? min(listed, s.k - (int)s.before_count)
-                                 : kept_by_limit(lds.c, listed, s.before_mass, s.limit, lds.red);
-        last = lds.c.key[max(kept - 1, 0)];
-        for (int i = threadIdx.x; i < kept; i += kT) {
+        weigh_candidates(r, lds.c, listed, lds.table);
+        last = s.k > 0 ? last_key(lds.c, listed, false, s.before_count, s.k, lds.red)
+                       : last_key(lds.c, listed, true, s.before_mass, s.limit, lds.red);
+        for (int i = threadIdx.x; i < listed; i += kT) {
           bool above;
-          const unsigned long long w = key_weight(r, lds.c.key[i], lds.table, &above);
-          if (above) atomicAdd(&lds.split_mass[key_index(lds.c.key[i]) / a.chunk], w);
+          const unsigned long long key = lds.c.key[i], w = key_weight(r, key, lds.table, &above);
+          if (above && key >= last) atomicAdd(&lds.run_mass[key_index(key) / kRun], w);
         }
         __syncthreads();
       }
-      unsigned long long total = 0;
-      for (int i = 0; i < a.splits; i++) total += lds.split_mass[i];
-      unsigned long long target = target_of(a, row, total);
-      int split = 0;
-      while (split < a.splits - 1 && target >= lds.split_mass[split]) target -= lds.split_mass[split++];
-      const int begin = split * a.chunk, end = min(begin + a.chunk, a.n);
-      segment_sums(r, x, begin, end, bin, last, lds);
-      found = pick(r, x, begin, end, bin, last, target, lds);
+      found = pick_in_run(a, r, x, row, bin, last, lds);
     }
   }
   if (threadIdx.x == 0) a.index[row] = found;
