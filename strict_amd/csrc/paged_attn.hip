@@ -29,11 +29,14 @@ typedef short s16x4 __attribute__((ext_vector_type(4)));
 #define SH_PAGED_LDS __attribute__((address_space(3)))
 
 // How a call is divided: rows of a tile, pieces at most (as many as workgroups are
-// resident), the shortest piece and the tiles that are not cut, in positions.
+// resident), the shortest piece and the tiles that are not cut, in positions. (One
+// token over 777 positions 14.2 us a call; with shortest pieces of twice and four times
+// that 15.0 and 16.1. 8 sequences of up to 200 tokens of 12 heads of 64: 28.0, 29.6 and
+// 37.5. Tiles left whole up to half or twice as many positions: within 5 % either way.)
 struct Variant {
   int rows, workers, min_piece, whole_below;
 };
-constexpr Variant kSmall = {16, 512, 128, 192}, kLarge = {128, 512, 256, 256};
+constexpr Variant kSmall = {16, 512, 64, 192}, kLarge = {128, 512, 128, 256};
 constexpr int kMaxWorkers = 512;
 
 struct PagedAttnArgs {
@@ -319,6 +322,8 @@ __device__ __forceinline__ float half_max(float x) {
 //    4 g + e of the first 16 for e < 4, of the second for e >= 4); V goes through
 //    LDS rows as it is and comes back by transposing reads.
 // A unit's 16-position blocks lie in one page each (pages of 16 and more).
+// 48 ragged sequences of up to 4,352 positions (626 MB of bf16): 101 us here and 6 in
+// the merge, 6.2 TB/s of a copy's 6.4.
 template <int kD>
 constexpr int kSmallUnit = 32 * 128 / kD;
 
@@ -552,6 +557,9 @@ __global__ __launch_bounds__(kT, kSmall.workers / 256) void paged_small_kernel(c
 //  - scores as K x q, 32 x 32 positions and rows, K fragments from LDS;
 //  - V sums as V^T x P with the k slots numbered as P has them (slot (h, e) of 16
 //    positions: 4 h + e for e < 4, 8 + 4 h + e - 4 after that), V by transposing reads.
+// 8,192 tokens over 12,288 positions, 16 heads of 128 (550 GFLOP): 600 us, 917 TFLOP/s,
+// where a large product reaches 1,228; matrix cores busy 41 % of the time, vector units
+// (the softmax) 40 %, mostly in turn.
 constexpr int kLargeUnit = 64;
 constexpr float kSlack = 8.0f;
 
@@ -1060,7 +1068,10 @@ __global__ __launch_bounds__(kT) void paged_merge_large_kernel(const PagedAttnAr
 
 // ---- the entry points ---------------------------------------------------------------
 
-// Small tiles where every sequence's new tokens fit one.
+// Small tiles where every sequence's new tokens fit one. (Small and large, us a call, 16
+// sequences of up to 4,096 positions, 8 KV heads of 2 query heads: of 2 tokens 42 and 55,
+// 8 tokens, which is 16 rows, 55 and 59, 16 tokens 87 and 60. 48 sequences of one token
+// 110 and 135.)
 Variant variant_of(int group, int max_new) {
   return group <= kSmall.rows && (long long)group * max_new <= kSmall.rows ? kSmall : kLarge;
 }
