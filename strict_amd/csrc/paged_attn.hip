@@ -1108,8 +1108,9 @@ int attn_paged(sh_ctx *ctx, const sh_paged_kv *kv, const uint16_t *q, uint16_t *
   if (rc != SH_OK) return rc;
   if ((rc = check_attn_sizes(kv, tokens, heads, max_new))) return rc;
   if (window < 0 || sinks < 0) return fail(SH_ERR_INVALID_ARGUMENT, "window and sinks must not be negative");
-  if (!(scale > 0.0f) || !std::isfinite(scale))
-    return fail(SH_ERR_INVALID_ARGUMENT, "scale must be positive and finite");
+  // (times log2(e) it has to be finite)
+  if (!(scale > 0.0f) || !(scale <= 0x1p127f))
+    return fail(SH_ERR_INVALID_ARGUMENT, "scale must be positive and at most 2^127");
   if (tokens == 0 || kv->batch == 0) return SH_OK;
   const size_t bytes = (size_t)tokens * heads * kv->head_dim * 2, need = workspace_of(kv, heads, max_new);
   if ((rc = check_paged_pointers(ctx, kv)) || (rc = check_range(ctx, q, bytes, "q")) ||
@@ -1123,6 +1124,12 @@ int attn_paged(sh_ctx *ctx, const sh_paged_kv *kv, const uint16_t *q, uint16_t *
   if ((rc = check_range(ctx, workspace, need, "workspace"))) return rc;
   if (reinterpret_cast<uintptr_t>(workspace) & 15)
     return fail(SH_ERR_INVALID_ARGUMENT, "the work buffer must be 16-byte aligned");
+  const size_t pool = paged_pool_bytes(kv);
+  if (ranges_overlap(workspace, need, q, bytes) || ranges_overlap(workspace, need, out, bytes) ||
+      ranges_overlap(workspace, need, kv->k, pool) || ranges_overlap(workspace, need, kv->v, pool))
+    return fail(SH_ERR_INVALID_ARGUMENT, "the work buffer overlaps a tensor of the call");
+  if (ranges_overlap(out, bytes, kv->k, pool) || ranges_overlap(out, bytes, kv->v, pool))
+    return fail(SH_ERR_INVALID_ARGUMENT, "out overlaps the cache");
   PagedAttnArgs a;
   a.q = q;
   a.k = kv->k;

@@ -166,6 +166,11 @@ int norm_rope(sh_ctx *ctx, const sh_paged_kv *kv, const uint16_t *qkv, const flo
   if ((reinterpret_cast<uintptr_t>(qkv) | reinterpret_cast<uintptr_t>(q)) & 15)
     return fail(SH_ERR_INVALID_ARGUMENT, "qkv and q must be 16-byte aligned");
   if (ranges_overlap(qkv, in_bytes, q, q_bytes)) return fail(SH_ERR_INVALID_ARGUMENT, "q overlaps qkv");
+  const size_t pool = paged_pool_bytes(kv);
+  if (ranges_overlap(kv->k, pool, kv->v, pool)) return fail(SH_ERR_INVALID_ARGUMENT, "the k and v pages overlap");
+  if (ranges_overlap(kv->k, pool, q, q_bytes) || ranges_overlap(kv->v, pool, q, q_bytes) ||
+      ranges_overlap(kv->k, pool, qkv, in_bytes) || ranges_overlap(kv->v, pool, qkv, in_bytes))
+    return fail(SH_ERR_INVALID_ARGUMENT, "the cache overlaps q or qkv");
   NormRopeArgs a;
   a.qkv = qkv;
   a.q_gain = q_gain;

@@ -917,6 +917,9 @@ SH_API int sh_sample_f32(sh_ctx *ctx, const float *x, int rows, int n, int ld, c
   if ((rc = check_range(ctx, workspace, need, "workspace"))) return rc;
   if (reinterpret_cast<uintptr_t>(workspace) & 15)
     return fail(SH_ERR_INVALID_ARGUMENT, "the work buffer must be 16-byte aligned");
+  const uintptr_t w0 = reinterpret_cast<uintptr_t>(workspace), x0 = reinterpret_cast<uintptr_t>(x);
+  if (n > kList && w0 < x0 + ((size_t)(rows - 1) * ld + n) * 4 && x0 < w0 + need)
+    return fail(SH_ERR_INVALID_ARGUMENT, "the work buffer overlaps x");
   SampleArgs a;
   a.x = x;
   a.temperature = temperature;

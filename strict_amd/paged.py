@@ -36,10 +36,15 @@ class PageTable:
     def free_pages(self) -> int:
         return len(self._free)
 
+    def _check(self, row: int) -> None:
+        if not 0 <= row < len(self.pages):
+            raise IndexError(f"row {row} of {len(self.pages)}")
+
     def extend(self, new) -> list:
         """Room for new[row] more tokens in every row named in the mapping, all or none."""
         plan, need = [], 0
         for row, n in new.items():
+            self._check(row)
             if n < 0:
                 raise ValueError("a negative number of tokens")
             pages, length = self.pages[row], self.lengths[row]
@@ -76,6 +81,8 @@ class PageTable:
 
     def fork(self, row: int, to: int) -> None:
         """Row `to`, which must be empty, continues from the same tokens as `row`."""
+        self._check(row)
+        self._check(to)
         if self.pages[to] or self.lengths[to]:
             raise ValueError(f"row {to} is not empty")
         self.pages[to] = list(self.pages[row])
@@ -85,6 +92,7 @@ class PageTable:
 
     def free(self, row: int) -> None:
         """Ends row's sequence; pages that no other row holds are free again."""
+        self._check(row)
         for page in self.pages[row]:
             self.holders[page] -= 1
             if self.holders[page] == 0:

@@ -320,3 +320,57 @@ def test_a_page_in_several_tables_and_twice_in_one(ctx):
     c.table[1, :6] = c.table[0, :6]
     c.table[2, 1:4] = c.table[2, 0]
     paged.check_attention(c)
+
+
+@pytest.mark.parametrize("new", [[1, 1], [40, 7]])
+@pytest.mark.parametrize("window,sinks", [(2 ** 31 - 1, 0), (2 ** 31 - 1, 2 ** 31 - 1), (1, 2 ** 31 - 1)])
+def test_largest_windows_and_sinks(ctx, new, window, sinks):
+    # rows before position 0 among them
+    c = paged.Case(ctx, 22, "f16", new, [200, 7], 4, 2, 64, 16)
+    c.lengths[1] = min(5, new[1])
+    paged.check_attention(c, window=window, sinks=sinks)
+
+
+def refused(call, text):
+    with pytest.raises(strict_amd.StrictHipError) as e:
+        call()
+    assert e.value.status == strict_amd.SH_ERR_INVALID_ARGUMENT and text in e.value.message, e.value.message
+
+
+def test_tensors_that_overlap(ctx):
+    c = paged.Case(ctx, 23, "f16", [1], [20], 4, 2, 64, 16)
+    kv = c.upload()
+    need = ctx.attn_paged_workspace(kv, c.tokens, 4, 1)
+    nbytes = c.tokens * 4 * 64 * 2
+    big = ctx.alloc(need + 4 * nbytes)
+    work, inside, behind = big.view(0, need), big.view(need - 16, nbytes), big.view(need + nbytes, nbytes)
+    attn = lambda q, out, work, scale=1.0, kv=kv: (  # noqa: E731
+        lambda: ctx.attn_paged(kv, q, out, c.tokens, 4, 1, scale, work))
+    refused(attn(inside, behind, work), "work buffer overlaps")
+    refused(attn(behind, inside, work), "work buffer overlaps")
+    refused(attn(behind, c.buffers[0], work), "out overlaps the cache")
+    refused(attn(behind, c.buffers[1], work), "out overlaps the cache")
+    pool = ctx.alloc(need + c.buffers[0].nbytes)
+    low = strict_amd.PagedKV(pool, *c.buffers[1:], batch=1, max_pages=c.max_pages, num_pages=c.num_pages, page_size=16,
+                             kv_heads=2, head_dim=64, dtype="f16")
+    refused(attn(behind, big.view(need + 2 * nbytes, nbytes), pool, kv=low), "work buffer overlaps")
+    refused(attn(behind, big.view(need + 2 * nbytes, nbytes), work, 3e38), "scale")
+    gain = ctx.upload(np.ones(64, np.float32))
+    qkv = ctx.alloc(c.tokens * 8 * 64 * 2)
+    same = strict_amd.PagedKV(c.buffers[0], c.buffers[0], *c.buffers[2:], batch=1, max_pages=c.max_pages,
+                              num_pages=c.num_pages, page_size=16, kv_heads=2, head_dim=64, dtype="f16")
+    rope = lambda kv, qkv, q: (lambda: ctx.qk_norm_rope_paged(kv, qkv, gain, gain, q, c.tokens, 4, 1e-6, 1e4))  # noqa: E731
+    refused(rope(same, qkv, behind), "k and v pages overlap")
+    refused(rope(kv, qkv, c.buffers[1]), "cache overlaps")
+    refused(rope(kv, c.buffers[0], behind), "cache overlaps")
+    for b in (big, pool, gain, qkv):
+        b.free()
+    c.free()
+    need = ctx.sample_workspace(2, 4000)
+    big = ctx.alloc(need + 64000)
+    small = ctx.upload(np.zeros(2, np.float32))
+    index = ctx.empty(2, np.int32)
+    refused(lambda: ctx.sample(big.view(need - 64, 32000), 2, 4000, None, None, None, None, small, index, big.view(0, need)),
+            "work buffer overlaps x")
+    for b in (big, small, index):
+        b.free()

@@ -131,3 +131,14 @@ def test_full_last_page_stays_shared():
     t.fork(0, 1)
     assert t.extend({0: 1, 1: 1}) == []
     assert t.pages == [[0, 1, 2], [0, 1, 3]]
+
+
+@pytest.mark.parametrize("row", [-1, 2])
+def test_rows_that_are_not_there(row):
+    t = PageTable(2, 4, 8, 4)
+    t.extend({0: 5, 1: 5})
+    before = t.array()
+    for call in (lambda: t.extend({0: 1, row: 1}), lambda: t.free(row), lambda: t.fork(0, row), lambda: t.fork(row, 1)):
+        with pytest.raises(IndexError):
+            call()
+    assert (t.array() == before).all() and t.lengths == [5, 5]
