@@ -224,23 +224,34 @@ __device__ __forceinline__ int find_part(const PlanLds &lds, Line x) {
   return min(n, kT - 1);
 }
 
+// The worker that a workgroup is, if workgroups of one XCD are to be consecutive
+// workers, which share K and V. Of fewer pieces than workers each XCD takes an eighth
+// (448 tiles on 512: 66.4 -> 64.0 us a call; 8 sequences of up to 200 tokens 28 -> 27).
+__device__ __forceinline__ int worker_by_xcd(const PagedPlan &p, Line total, Line piece) {
+  const int used = min((int)plan_div(total + piece - 1, piece), p.workers), per = (used + 7) >> 3;
+  const int xcd = blockIdx.x & 7, i = blockIdx.x >> 3;
+  return i < per ? xcd * per + i : 8 * i + xcd;
+}
+
 // A worker's piece, step by step: part(step), which says whether its results are
-// finite. Returns whether all are.
-template <class Part>
-__device__ __forceinline__ bool walk_piece(const PagedPlan &p, int worker, PlanLds &lds, MergeItem *item, Part part) {
+// finite. Returns whether all are. kByXcd: *worker is to be found.
+template <bool kByXcd, class Part>
+__device__ __forceinline__ bool walk_piece(const PagedPlan &p, int *worker, PlanLds &lds, MergeItem *item, Part part) {
   const int per = (p.batch + kT - 1) / kT;
   scan_costs(p, per, lds);
   Line largest = 0;
 #pragma unroll
   for (int w = 0; w < kT / 64; w++) largest = fmax(largest, lds.largest[w]);
-  const Line total = uniform(lds.prefix[kT]), piece = uniform(plan_piece(p, total, largest)), x0 = worker * piece;
-  const Line end = uniform(fmin(x0 + piece, total));
+  const Line total = uniform(lds.prefix[kT]), piece = uniform(plan_piece(p, total, largest));
+  const int me = kByXcd ? uniform(worker_by_xcd(p, total, piece)) : *worker;
+  *worker = me;
+  const Line x0 = me * piece, end = uniform(fmin(x0 + piece, total));
   bool finite = true;
   Line x = x0;
   while (uniform(x < end ? 1 : 0)) {
     const int i = uniform(find_part(lds, x)), b = plan_part_first(p, i, per);
     const PagedTile t = plan_locate(p, per == 1 ? lds.seqs[b] : plan_sequence(p, b), i, per, lds.prefix[i], x);
-    PieceStep st = plan_step(p, t, piece, worker, x0, x, item);
+    PieceStep st = plan_step(p, t, piece, me, x0, x, item);
     for (int *v : {&st.tile.seq.row0, &st.tile.seq.n, &st.tile.seq.len, &st.tile.b, &st.tile.kv_head, &st.tile.tile,
                    &st.span.first, &st.span.count, &st.span.pos0, &st.span.lo, &st.span.hi, &st.span.sinks,
                    &st.span.units, &st.span.sink_units, &st.span.gap, &st.u0, &st.u1, &st.slot})
@@ -254,12 +265,13 @@ __device__ __forceinline__ bool walk_piece(const PagedPlan &p, int worker, PlanL
   return finite;
 }
 
-// A worker of the main kernels.
+// A workgroup of the main kernels.
 // kMergeRows: rows of an item's group, kMergeCols: groups that share rows.
-template <int kMergeRows, int kMergeCols, class Part>
-__device__ __forceinline__ void work_piece(const PagedAttnArgs &a, int worker, PlanLds &lds, Part part) {
+template <bool kByXcd, int kMergeRows, int kMergeCols, class Part>
+__device__ __forceinline__ void work_piece(const PagedAttnArgs &a, PlanLds &lds, Part part) {
+  int worker = blockIdx.x;
   MergeItem item = {0, 0, 0, 0, 0, 0};
-  const bool finite = walk_piece(a.plan, worker, lds, &item, part);
+  const bool finite = walk_piece<kByXcd>(a.plan, &worker, lds, &item, part);
   if (threadIdx.x == 0) {
     a.items[worker] = item;
     a.groups[worker] = item.parts > 0 ? (item.tokens * a.group + kMergeRows - 1) / kMergeRows * kMergeCols : 0;
@@ -545,7 +557,7 @@ template <class T, int kD>
 __global__ __launch_bounds__(kT, kSmall.workers / 256) void paged_small_kernel(const PagedAttnArgs a) {
   __shared__ __attribute__((aligned(16))) SmallLds<T, kD> lds;
   __shared__ PlanLds plan;
-  work_piece<1, 1>(a, blockIdx.x, plan, [&](const PieceStep &st, Line) { return attn_small<T, kD>(a, st.tile, st.span, st.u0, st.u1, st.slot, lds); });
+  work_piece<false, 1, 1>(a, plan, [&](const PieceStep &st, Line) { return attn_small<T, kD>(a, st.tile, st.span, st.u0, st.u1, st.slot, lds); });
 }
 
 // ---- tiles of up to 128 rows ------------------------------------------------------------
@@ -821,9 +833,7 @@ template <class T, int kD>
 __global__ __launch_bounds__(kT, kLarge.workers / 256) void paged_large_kernel(const PagedAttnArgs a) {
   __shared__ __attribute__((aligned(16))) LargeLds<kD> lds;
   __shared__ PlanLds plan;
-  // consecutive pieces to one XCD: they share K and V
-  const int worker = (blockIdx.x & 7) * (a.plan.workers >> 3) + (blockIdx.x >> 3);
-  work_piece<32, kD / 32>(a, worker, plan, [&](const PieceStep &st, Line) {
+  work_piece<true, 32, kD / 32>(a, plan, [&](const PieceStep &st, Line) {
     return attn_large<T, kD>(a, st.tile, st.span, st.u0, st.u1, st.slot, lds);
   });
 }
@@ -894,11 +904,11 @@ __device__ __forceinline__ void scan_items(const PagedAttnArgs &a, MergeLds &lds
 // The flagged workers' tiles.
 template <class T, int kD>
 __device__ __forceinline__ void redo_tiles(const PagedAttnArgs &a, MergeLds &lds, int flagged) {
-  const int w = blockIdx.x;
+  int w = blockIdx.x;
   if (flagged == 0) return;
   __syncthreads();  // lds.prefix is read
   MergeItem unused;
-  walk_piece(a.plan, w, lds.plan, &unused, [&](const PieceStep &st, Line piece) {
+  walk_piece<false>(a.plan, &w, lds.plan, &unused, [&](const PieceStep &st, Line piece) {
     if (st.slot >= 0)  // a cut tile is the first flagged worker's
       for (int j = plan_first(st.tile, w, piece, w * piece); j < w; j++)
         if (a.redo[j] != 0) return true;
