@@ -374,3 +374,76 @@ def test_tensors_that_overlap(ctx):
             "work buffer overlaps x")
     for b in (big, small, index):
         b.free()
+
+
+# ---- chunks announced as long ----------------------------------------------------------
+
+LONG = 100000
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("heads,kv_heads,d,page", [(16, 8, 128, 16), (4, 4, 64, 32), (6, 2, 128, 64), (7, 1, 64, 128), (128, 1, 64, 16)])
+@pytest.mark.parametrize("new,lengths", [([1], [1]), ([300, 0, 2], [300, 9, 900]), ([33, 140, 257, 20], [100, 1500, 257, 3000])])
+def test_long_chunks(ctx, dtype, heads, kv_heads, d, page, new, lengths):
+    if heads == 128 and sum(new) > 400:
+        new, lengths = [33, 20], [100, 700]
+    paged.check_attention(paged.Case(ctx, sum(new) + d, dtype, new, lengths, heads, kv_heads, d, page, first_row=2), max_new=LONG)
+
+
+@pytest.mark.parametrize("heads,kv_heads,d", [(8, 4, 128), (6, 2, 64)])
+@pytest.mark.parametrize("window,sinks", [(1, 0), (1, 1), (7, 4), (64, 64), (100, 130), (5000, 4)])
+def test_long_chunks_with_windows(ctx, heads, kv_heads, d, window, sinks):
+    c = paged.Case(ctx, window + sinks, "bf16", [350, 20, 1], [900, 333, 1], heads, kv_heads, d, 16)
+    paged.check_attention(c, window=window, sinks=sinks, max_new=LONG)
+
+
+def test_long_chunks_with_bad_pages(ctx):
+    new = [300, 9, 2, 30]
+    c = paged.Case(ctx, 5, "f16", new, [900, 90, 20, 120], 4, 2, 64, 16)
+    c.table[0, 0] = -1
+    c.table[0, 3] = c.num_pages
+    c.table[0, 4] = np.iinfo(np.int32).min
+    c.table[0, 42] = np.iinfo(np.int32).max
+    c.table[1, :] = -7
+    c.lengths[2] = 1
+    c.table[3, 1:7] = 1 << 30
+    paged.check_attention(c, max_new=LONG)
+    paged.check_attention(c, window=20, sinks=3, max_new=LONG)
+
+
+@pytest.mark.parametrize("window", [0, 40])
+@pytest.mark.parametrize("dtype,bad", [("f16", np.nan), ("bf16", np.inf)])
+def test_long_chunks_leave_unseen_places(ctx, dtype, bad, window):
+    c = paged.Case(ctx, 9, dtype, [270, 3], [350, 71], 4, 2, 128, 32)
+    keep = np.zeros((c.num_pages, c.page), bool)
+    for b in range(c.batch):
+        p = np.arange(c.lengths[b])
+        if window:
+            p = p[p > c.lengths[b] - c.new[b] - window]
+        keep[c.table[b, p // c.page], p % c.page] = True
+    for bits in (c.k, c.v):
+        x = paged.from16(bits, dtype).astype(np.float32)
+        x[~keep[:, None, :, None] & np.ones(x.shape, bool)] = bad
+        bits[:] = paged.to16(x, dtype)
+    paged.check_attention(c, window=window, max_new=LONG)
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+def test_long_chunks_with_later_tokens_that_are_not_finite(ctx, dtype):
+    c = paged.Case(ctx, 11, dtype, [280, 5], [300, 50], 4, 2, 64, 16)
+    page, at = c.table[0, 200 // 16], 200 % 16
+    for bits, bad in ((c.k, np.inf), (c.v, np.nan)):
+        x = paged.from16(bits, dtype).astype(np.float32)
+        x[page, :, at, :3] = bad
+        bits[:] = paged.to16(x, dtype)
+    q, got = paged.run_attention(c, max_new=LONG)
+    ref, tol = paged.attention_oracle(c, paged.from16(q, dtype), 0, 0, 64 ** -0.5)
+    out = paged.from16(got, dtype)
+    for rows in (slice(0, 180), slice(280, 285)):
+        assert (np.abs(out[rows] - ref[rows]) <= tol[rows]).all()
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+def test_long_chunks_with_large_scores(ctx, dtype):
+    paged.check_attention(paged.Case(ctx, 13, dtype, [260], [600], 4, 2, 128, 16, scale=30.0), scale=1.0, max_new=LONG)
+    paged.check_attention(paged.Case(ctx, 14, dtype, [40], [9000], 4, 2, 64, 16), max_new=LONG)
