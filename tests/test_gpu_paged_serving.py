@@ -447,3 +447,37 @@ def test_long_chunks_with_later_tokens_that_are_not_finite(ctx, dtype):
 def test_long_chunks_with_large_scores(ctx, dtype):
     paged.check_attention(paged.Case(ctx, 13, dtype, [260], [600], 4, 2, 128, 16, scale=30.0), scale=1.0, max_new=LONG)
     paged.check_attention(paged.Case(ctx, 14, dtype, [40], [9000], 4, 2, 64, 16), max_new=LONG)
+
+
+@pytest.mark.parametrize("new", [[1, 1, 1], [40, 200, 9]])
+def test_starts_and_lengths_that_are_not_theirs(ctx, new):
+    # whatever the device holds there, only rows of out and pages of the cache are written
+    c = paged.Case(ctx, 31, "f16", new, [300, 300, 300], 4, 2, 64, 16, rows_behind=3)
+    kv = c.upload()
+    nbytes = c.tokens * 4 * 64 * 2
+    guarded = ctx.alloc(3 * nbytes)
+    out = guarded.view(nbytes, nbytes)
+    dq = ctx.upload(paged.to16(c.rng.normal(0, 1, (c.tokens, 4, 64)), "f16"))
+    qkv = ctx.upload(paged.to16(c.rng.normal(0, 1, (c.tokens, 8, 64)), "f16"))
+    gain = ctx.upload(np.ones(64, np.float32))
+    work = ctx.alloc(ctx.attn_paged_workspace(kv, c.tokens, 4, max(new)))
+    rng = np.random.default_rng(32)
+    ends = np.array([0, 1, -1, c.tokens, c.tokens + 1, 7, np.iinfo(np.int32).max, np.iinfo(np.int32).min], np.int64)
+    for _ in range(30):
+        c.buffers[3].copy_from_host(rng.choice(np.append(ends, 300), 3).astype(np.int32))
+        c.buffers[4].copy_from_host(rng.choice(ends, 4).astype(np.int32))
+        ctx.memset(guarded, 0x5a)
+        ctx.attn_paged(kv, dq, out, c.tokens, 4, max(new), 0.125, work, int(rng.choice([0, 50])), 4)
+        ctx.sync()
+        host = guarded.to_host()
+        assert (host[:nbytes] == 0x5a).all() and (host[2 * nbytes:] == 0x5a).all()
+        assert (c.buffers[0].to_host() == c.k).all() and (c.buffers[1].to_host() == c.v).all()
+        ctx.qk_norm_rope_paged(kv, qkv, gain, gain, out, c.tokens, 4, EPS, THETA)
+        ctx.sync()
+        host = guarded.to_host()
+        assert (host[:nbytes] == 0x5a).all() and (host[2 * nbytes:] == 0x5a).all()
+        for b, bits in zip(c.buffers[:2], (c.k, c.v)):
+            b.copy_from_host(bits)
+    for b in (guarded, dq, qkv, gain, work):
+        b.free()
+    c.free()
