@@ -10,7 +10,7 @@
 // q, K or V, or in places of V that only some of a tile's rows see.
 //
 // Softmax runs over the positions in order with a running maximum, in base 2:
-// s = q.k scale log2(e), weights 2^(s - max) (times 2^14 in fp16).
+// s = q.k scale log2(e), weights 2^(s - max) (times 2^7 in fp16).
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
