@@ -493,8 +493,8 @@ SH_API int sh_attn_decode_f16_noalloc(sh_ctx *ctx, const float *q, const uint16_
  * are taken within 0 .. tokens and ascending, lengths within 0 .. max_pages *
  * page_size; a position whose table entry is no page (not 0 .. num_pages - 1)
  * is seen by no token and not stored. page_size: a power of two, 16..65536;
- * max_pages * page_size at most 2^28, and (tokens + batch) * kv_heads * (max_pages
- * * page_size + 512) at most 2^52. */
+ * max_pages * page_size at most 2^28, (tokens + batch) * kv_heads * (max_pages *
+ * page_size + 512) at most 2^52, and a pool at most 2^62 bytes. */
 typedef struct sh_paged_kv {
   uint16_t *k, *v; /* [num_pages][kv_heads][page_size][head_dim], 16-byte aligned */
   const int32_t *page_table; /* [batch][max_pages] */

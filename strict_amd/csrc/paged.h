@@ -24,6 +24,7 @@ namespace sh {
 
 constexpr int kMaxPagedTokens = 1 << 22, kMaxPagedBatch = 1 << 16, kMaxPagedKvHeads = 1 << 10;
 constexpr int kMaxPagedPositions = 1 << 28;  // max_pages * page_size
+constexpr double kMaxPoolBytes = 4611686018427387904.0;  // 2^62: sizes and ends of pools in 64 bits
 
 SH_HD int clamp_int(int v, int lo, int hi) { return v < lo ? lo : v > hi ? hi : v; }
 
@@ -324,6 +325,9 @@ inline const char *check_paged_sizes(const sh_paged_kv *kv, int tokens, int head
   // (what an attention call may cost: kMaxLine, in tiles of one token)
   if (((double)tokens + kv->batch) * kv->kv_heads * ((double)kv->max_pages * kv->page_size + 512.0) > kMaxLine)
     return "(tokens + batch) * kv_heads * (max_pages * page_size + 512) exceeds 2^52";
+  // (exact in fp64 for the head sizes there are: 31 and 10 bits, and powers of two)
+  if ((double)kv->num_pages * kv->kv_heads * kv->page_size * kv->head_dim * 2.0 > kMaxPoolBytes)
+    return "num_pages * kv_heads * page_size * head_dim exceeds 2^61 (a pool of 2^62 bytes)";
   return nullptr;
 }
 

@@ -1,0 +1,34 @@
+"""Calls of the paged operators and of sampling that are refused before anything is
+launched: sizes whose products leave 64 bits, tensors over one another."""
+import numpy as np
+import pytest
+
+import strict_amd
+import test_gpu_paged as paged
+from strict_amd import PagedKV
+
+pytestmark = pytest.mark.gpu
+
+
+def refused(call, text):
+    with pytest.raises(strict_amd.StrictHipError) as e:
+        call()
+    assert e.value.status == strict_amd.SH_ERR_INVALID_ARGUMENT and text in e.value.message, e.value.message
+
+
+@pytest.mark.parametrize("num_pages", [1 << 30, (1 << 30) + 1, (1 << 28) + 1])
+def test_pools_past_64_bits(ctx, num_pages):
+    # (their sizes come round to nothing, to one page of 16 GiB and to little more than 2^62)
+    c = paged.Case(ctx, 1, "f16", [1], [20], 1, 1, 128, 16)
+    c.upload()
+    kv = PagedKV(*c.buffers, batch=1, max_pages=1, num_pages=num_pages, page_size=65536, kv_heads=1024, head_dim=128)
+    rows = ctx.upload(np.zeros((3 * 1024, 128), np.int16))
+    q, out = (ctx.upload(np.zeros((1024, 128), np.int16)) for _ in range(2))
+    gain = ctx.upload(np.ones(128, np.float32))
+    work = ctx.alloc(1 << 20)
+    refused(lambda: ctx.attn_paged_workspace(kv, 1, 1024, 1), "num_pages")
+    refused(lambda: ctx.attn_paged(kv, q, out, 1, 1024, 1, 1.0, work), "num_pages")
+    refused(lambda: ctx.qk_norm_rope_paged(kv, rows, gain, gain, q, 1, 1024, 1e-6, 1e4), "num_pages")
+    for b in (rows, q, out, gain, work):
+        b.free()
+    c.free()
