@@ -532,7 +532,7 @@ SH_API int sh_qk_norm_rope_paged_bf16(sh_ctx *ctx, const sh_paged_kv *kv, const 
  * heads / kv_heads <= 128, 0 < scale <= 2^127. max_new: the most new tokens of any sequence;
  * the kernel and the work buffer are chosen by it, more are computed as well. The
  * work buffer (16-byte aligned) holds at least what sh_attn_paged_workspace
- * says for the same sizes. */
+ * says for the same sizes. It and out overlap nothing else of the call. */
 SH_API int sh_attn_paged_workspace(const sh_paged_kv *kv, int tokens, int heads, int max_new,
                                    size_t *bytes);
 SH_API int sh_attn_paged_f16(sh_ctx *ctx, const sh_paged_kv *kv, const uint16_t *q, uint16_t *out,

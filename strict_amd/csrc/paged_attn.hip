@@ -1144,8 +1144,11 @@ int attn_paged(sh_ctx *ctx, const sh_paged_kv *kv, const uint16_t *q, uint16_t *
     return fail(SH_ERR_INVALID_ARGUMENT, "the work buffer must be 16-byte aligned");
   const size_t pool = paged_pool_bytes(kv);
   if (ranges_overlap(workspace, need, q, bytes) || ranges_overlap(workspace, need, out, bytes) ||
-      ranges_overlap(workspace, need, kv->k, pool) || ranges_overlap(workspace, need, kv->v, pool))
+      ranges_overlap(workspace, need, kv->k, pool) || ranges_overlap(workspace, need, kv->v, pool) ||
+      overlaps_index(kv, workspace, need))
     return fail(SH_ERR_INVALID_ARGUMENT, "the work buffer overlaps a tensor of the call");
+  if (overlaps_index(kv, out, bytes))
+    return fail(SH_ERR_INVALID_ARGUMENT, "out overlaps the page table, lengths or starts");
   if (ranges_overlap(out, bytes, kv->k, pool) || ranges_overlap(out, bytes, kv->v, pool))
     return fail(SH_ERR_INVALID_ARGUMENT, "out overlaps the cache");
   PagedAttnArgs a;

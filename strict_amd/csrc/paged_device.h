@@ -68,4 +68,12 @@ inline int check_paged_pointers(sh_ctx *ctx, const sh_paged_kv *kv) {
   return SH_OK;
 }
 
+// Whether [p, p + bytes), which a call writes, lies over what it reads to find its way:
+// workgroups that read it before and after would not divide the call alike.
+inline bool overlaps_index(const sh_paged_kv *kv, const void *p, size_t bytes) {
+  const size_t batch = kv->batch;
+  return ranges_overlap(p, bytes, kv->page_table, batch * kv->max_pages * 4) ||
+         ranges_overlap(p, bytes, kv->lengths, batch * 4) || ranges_overlap(p, bytes, kv->starts, (batch + 1) * 4);
+}
+
 }  // namespace sh

@@ -32,3 +32,31 @@ def test_pools_past_64_bits(ctx, num_pages):
     for b in (rows, q, out, gain, work):
         b.free()
     c.free()
+
+
+def test_attention_over_its_own_index(ctx):
+    # out or the work buffer over the page table, the lengths or the starts: at their first and last bytes
+    c = paged.Case(ctx, 2, "f16", [1], [20], 4, 2, 64, 16)
+    c.upload()
+    need = ctx.attn_paged_workspace(c.kv, c.tokens, 4, 1)
+    nbytes = c.tokens * 4 * 64 * 2
+    q, out = ctx.alloc(nbytes), ctx.alloc(nbytes)
+    for which, text, size in (("out", "page table, lengths or starts", nbytes), ("work", "work buffer overlaps", need)):
+        area = ctx.alloc(size + 64)
+        for i in (2, 3, 4):
+            index = c.buffers[i]
+            for at in (0, 16 + size - 4):  # the index before the written range's start, and at its end
+                buffers = list(c.buffers)
+                buffers[i] = area.view(at, index.nbytes) if at else area.view(16 - index.nbytes + 4, index.nbytes)
+                kv = PagedKV(*buffers, batch=1, max_pages=c.max_pages, num_pages=c.num_pages, page_size=16, kv_heads=2,
+                             head_dim=64)
+                over = area.view(16, size)
+                args = (kv, q, over if which == "out" else out, c.tokens, 4, 1, 1.0)
+                work = ctx.alloc(need) if which == "out" else over
+                refused(lambda: ctx.attn_paged(*args, work), text)
+                if which == "out":
+                    work.free()
+        area.free()
+    q.free()
+    out.free()
+    c.free()
