@@ -510,8 +510,8 @@ typedef struct sh_paged_kv {
  * theta^(-2i / head_dim) in fp64; q to q[tokens][heads][head_dim], k and v (as
  * it is) to their pages. fp16 or bf16, rounded once. A token before position 0
  * is rotated by its negative position and not stored. head_dim 64 or 128; qkv
- * and q 16-byte aligned, ld a multiple of 8; q must not overlap qkv. Two tokens
- * of one page row (a page in two tables) leave either's values. */
+ * and q 16-byte aligned, ld a multiple of 8; q and the pages overlap nothing else of
+ * the call. Two tokens of one page row (a page in two tables) leave either's values. */
 SH_API int sh_qk_norm_rope_paged_f16(sh_ctx *ctx, const sh_paged_kv *kv, const uint16_t *qkv,
                                      const float *q_gain, const float *k_gain, uint16_t *q,
                                      int tokens, int heads, int ld, float eps, float theta);

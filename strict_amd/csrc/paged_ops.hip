@@ -171,6 +171,13 @@ int norm_rope(sh_ctx *ctx, const sh_paged_kv *kv, const uint16_t *qkv, const flo
   if (ranges_overlap(kv->k, pool, q, q_bytes) || ranges_overlap(kv->v, pool, q, q_bytes) ||
       ranges_overlap(kv->k, pool, qkv, in_bytes) || ranges_overlap(kv->v, pool, qkv, in_bytes))
     return fail(SH_ERR_INVALID_ARGUMENT, "the cache overlaps q or qkv");
+  const size_t gain_bytes = (size_t)d * 4;
+  const auto over_inputs = [&](const void *p, size_t bytes) {
+    return overlaps_index(kv, p, bytes) || ranges_overlap(p, bytes, q_gain, gain_bytes) ||
+           ranges_overlap(p, bytes, k_gain, gain_bytes);
+  };
+  if (over_inputs(q, q_bytes) || over_inputs(kv->k, pool) || over_inputs(kv->v, pool))
+    return fail(SH_ERR_INVALID_ARGUMENT, "q or the cache overlaps the page table, lengths, starts or gains");
   NormRopeArgs a;
   a.qkv = qkv;
   a.q_gain = q_gain;

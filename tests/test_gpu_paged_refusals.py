@@ -60,3 +60,30 @@ def test_attention_over_its_own_index(ctx):
     q.free()
     out.free()
     c.free()
+
+
+def test_head_norms_over_their_own_index(ctx):
+    # q or a pool over the page table, the lengths, the starts or a gain
+    c = paged.Case(ctx, 3, "f16", [1], [20], 4, 2, 64, 16)
+    c.upload()
+    nbytes, pool = c.tokens * 4 * 64 * 2, c.buffers[0].nbytes
+    q, qkv, gain = ctx.alloc(nbytes), ctx.alloc(c.tokens * 8 * 64 * 2), ctx.upload(np.ones(64, np.float32))
+    for which, size in (("q", nbytes), ("k", pool), ("v", pool)):
+        area = ctx.alloc(size + 512)
+        over = area.view(256, size)
+        for i in (2, 3, 4, "q_gain", "k_gain"):
+            index_bytes = c.buffers[i].nbytes if isinstance(i, int) else 256
+            for at in (256 - index_bytes + 4, 256 + size - 4):
+                index = area.view(at, index_bytes)
+                buffers = [b if j != i else index for j, b in enumerate(c.buffers)]
+                if which in "kv":
+                    buffers["kv".index(which)] = over
+                gains = [index if i == name else gain for name in ("q_gain", "k_gain")]
+                kv = PagedKV(*buffers, batch=1, max_pages=c.max_pages, num_pages=c.num_pages, page_size=16, kv_heads=2,
+                             head_dim=64)
+                refused(lambda: ctx.qk_norm_rope_paged(kv, qkv, *gains, over if which == "q" else q, c.tokens, 4, 1e-6, 1e4),
+                        "overlaps the page table, lengths, starts or gains")
+        area.free()
+    for b in (q, qkv, gain):
+        b.free()
+    c.free()
