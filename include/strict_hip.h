@@ -548,7 +548,7 @@ SH_API int sh_attn_paged_bf16(sh_ctx *ctx, const sh_paged_kv *kv, const uint16_t
  * 0 .. num_pages - 1 is skipped. A page may be the source of several; the dst
  * pages are distinct and none of them a source of another. pool 16-byte aligned,
  * page_bytes and plane_stride multiples of 16, plane_stride >= num_pages *
- * page_bytes. */
+ * page_bytes; src and dst do not lie in the pools. */
 SH_API int sh_pages_copy(sh_ctx *ctx, void *pool, int planes, size_t plane_stride, int num_pages,
                          size_t page_bytes, const int32_t *src, const int32_t *dst, int count);
 

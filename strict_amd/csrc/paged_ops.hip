@@ -267,6 +267,8 @@ SH_API int sh_pages_copy(sh_ctx *ctx, void *pool, int planes, size_t plane_strid
       (rc = check_range(ctx, dst, (size_t)count * 4, "dst")))
     return rc;
   if (reinterpret_cast<uintptr_t>(pool) & 15) return fail(SH_ERR_INVALID_ARGUMENT, "pool must be 16-byte aligned");
+  if (ranges_overlap(pool, extent, src, (size_t)count * 4) || ranges_overlap(pool, extent, dst, (size_t)count * 4))
+    return fail(SH_ERR_INVALID_ARGUMENT, "src or dst lies in the pools");
   const uint32_t vectors = (uint32_t)(page_bytes / 16);
   const int chunks = (int)((vectors + kT * kCopyVectors - 1) / (kT * kCopyVectors));
   const long long blocks = (long long)count * chunks;

@@ -87,3 +87,21 @@ def test_head_norms_over_their_own_index(ctx):
     for b in (q, qkv, gain):
         b.free()
     c.free()
+
+
+def test_page_numbers_in_the_pool(ctx):
+    planes, num, page_bytes, count = 2, 5, 32, 3
+    extent = planes * num * page_bytes
+    area = ctx.alloc(extent + 256)
+    other = ctx.upload(np.zeros(count, np.int32))
+    pool = area.view(128, extent)
+    for at in (128 - 4 * count + 4, 128 + extent - 4):
+        inside = area.view(at, 4 * count)
+        for src, dst in ((inside, other), (other, inside)):
+            refused(lambda: ctx.pages_copy(pool, planes, num, page_bytes, src, dst, count), "in the pools")
+    ctx.memset(area, 0xff)  # (page numbers that are none)
+    for at in (128 - 4 * count, 128 + extent):
+        ctx.pages_copy(pool, planes, num, page_bytes, area.view(at, 4 * count), area.view(at, 4 * count), count)
+    ctx.sync()
+    area.free()
+    other.free()
