@@ -570,7 +570,8 @@ SH_API int sh_pages_copy(sh_ctx *ctx, void *pool, int planes, size_t plane_strid
  * fp64 exponentials, and their sums exact: a token below 2^-43 of the likeliest
  * is not drawn, and results do not depend on any order. n <= 2^20, rows <= 2^16.
  * The work buffer (16-byte aligned) holds at least what
- * sh_sample_workspace says for the same sizes. */
+ * sh_sample_workspace says for the same sizes. It and index overlap nothing else of
+ * the call. */
 SH_API int sh_sample_workspace(int rows, int n, size_t *bytes);
 SH_API int sh_sample_f32(sh_ctx *ctx, const float *x, int rows, int n, int ld,
                          const float *temperature, const int32_t *top_k, const float *top_p,

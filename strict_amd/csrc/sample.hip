@@ -30,6 +30,7 @@
 #include <cmath>
 
 #include "common.h"
+#include "paged.h"
 #include "sample.h"
 
 namespace sh {
@@ -917,9 +918,19 @@ SH_API int sh_sample_f32(sh_ctx *ctx, const float *x, int rows, int n, int ld, c
   if ((rc = check_range(ctx, workspace, need, "workspace"))) return rc;
   if (reinterpret_cast<uintptr_t>(workspace) & 15)
     return fail(SH_ERR_INVALID_ARGUMENT, "the work buffer must be 16-byte aligned");
-  const uintptr_t w0 = reinterpret_cast<uintptr_t>(workspace), x0 = reinterpret_cast<uintptr_t>(x);
-  if (n > kList && w0 < x0 + ((size_t)(rows - 1) * ld + n) * 4 && x0 < w0 + need)
+  // what a call writes (rows that the list holds use no work buffer) lies over nothing that it reads
+  const size_t x_bytes = ((size_t)(rows - 1) * ld + n) * 4;
+  if (n > kList && ranges_overlap(workspace, need, x, x_bytes))
     return fail(SH_ERR_INVALID_ARGUMENT, "the work buffer overlaps x");
+  const auto over_parameters = [&](const void *p, size_t bytes) {
+    for (const void *of : {(const void *)temperature, (const void *)top_k, (const void *)top_p, (const void *)min_p, (const void *)u})
+      if (of && ranges_overlap(p, bytes, of, per_row)) return true;
+    return false;
+  };
+  if (n > kList && (over_parameters(workspace, need) || ranges_overlap(workspace, need, index, per_row)))
+    return fail(SH_ERR_INVALID_ARGUMENT, "the work buffer overlaps index, u or a row's parameters");
+  if (ranges_overlap(index, per_row, x, x_bytes) || over_parameters(index, per_row))
+    return fail(SH_ERR_INVALID_ARGUMENT, "index overlaps x, u or a row's parameters");
   SampleArgs a;
   a.x = x;
   a.temperature = temperature;

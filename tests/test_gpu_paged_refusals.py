@@ -105,3 +105,44 @@ def test_page_numbers_in_the_pool(ctx):
     ctx.sync()
     area.free()
     other.free()
+
+
+def test_sampling_over_its_own_parameters(ctx):
+    # the work buffer over index, u or a parameter, index over these or over x
+    rows, n = 3, 3000
+    need = ctx.sample_workspace(rows, n)
+    names = ["x", "temperature", "top_k", "top_p", "min_p", "u", "index"]
+    own = {name: ctx.upload(np.zeros(rows, np.float32)) for name in names[1:]}
+    own["x"] = ctx.upload(np.zeros((rows, n), np.float32))
+    work, area = ctx.alloc(need), ctx.alloc(need + 256)
+
+    def call(n=n, work=work, **other):
+        b = {**own, **other}
+        ctx.sample(b["x"], rows, n, b["temperature"], b["top_k"], b["top_p"], b["min_p"], b["u"], b["index"], work)
+
+    for name in names[1:]:
+        for at in (128 - 4 * rows + 4, 128 + need - 4):
+            refused(lambda: call(work=area.view(128, need), **{name: area.view(at, 4 * rows)}), "work buffer overlaps index")
+    # index over another, of rows short and long
+    for short in (n, 100):
+        for name in names[1:6]:
+            for at in (-4 * rows + 4, 4 * rows - 4):
+                refused(lambda: call(short, index=area.view(128 + at, 4 * rows), **{name: area.view(128, 4 * rows)}),
+                        "index overlaps x")
+        for at in (-4 * rows + 4, 4 * rows * short - 4):
+            refused(lambda: call(short, index=area.view(128 + at, 4 * rows), x=area.view(128, 4 * rows * short)),
+                    "index overlaps x")
+    # what is only read may be shared
+    call(temperature=own["u"], top_p=own["u"], min_p=own["u"])
+    ctx.sync()
+    for b in [work, area, *own.values()]:
+        b.free()
+
+
+def test_logits_past_their_allocation(ctx):
+    x, u, index = ctx.upload(np.zeros((2, 3000), np.float32)), ctx.upload(np.zeros(2, np.float32)), ctx.empty(2, np.int32)
+    work = ctx.alloc(ctx.sample_workspace(2, 3000))
+    refused(lambda: ctx.sample(x, 2, 3000, None, None, None, None, u, index, work, 3001), "x (")
+    refused(lambda: ctx.sample(x, 2, 3000, None, None, None, None, u, index, work, 3001), "is not inside an allocation")
+    for b in (x, u, index, work):
+        b.free()
