@@ -605,11 +605,12 @@ __global__ __launch_bounds__(kT) void sample_gather_kernel(const SampleArgs a) {
   }
   if (mode == kDigits) return;
   const int begin = split * a.chunk, end = min(begin + a.chunk, a.n);
-  // below this value no token is in the bins up to `bin` (a bin's width and a half
-  // more than y's roundings could make of it): most of the row is passed over by it
+  // below this value no token is in the bins up to `bin` (by the bins' own factor, which
+  // temperatures below 2^-126 meet the limit of; half a bin is more than the roundings of
+  // t could make of it): most of the row is passed over by it
   const float least = mode == kAll || (r.k == 0 && bin == kBins - 1)
                           ? -INFINITY
-                          : (float)((double)r.m - (bin + 1.5) / (kBinsPerUnit * r.inv_t));
+                          : (float)((double)r.m - (bin + 1.5) / (0.5 * kBinsPerUnit * (double)r.inv_2t));
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
   for (int i0 = begin + wave * kRun; i0 < end; i0 += kT / 64 * kRun) {
     unsigned long long sum = 0;
