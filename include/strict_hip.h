@@ -526,13 +526,14 @@ SH_API int sh_qk_norm_rope_paged_bf16(sh_ctx *ctx, const sh_paged_kv *kv, const 
  * over p <= pos, with window > 0 only those with p > pos - window or p < sinks
  * (window 0: all). A row that sees nothing gets zeros; what stands in places
  * that a row does not see, NaN and infinities included, does not reach it; a
- * score of -infinity has no weight. q, out [tokens][heads][head_dim] in the
- * cache's type, 16-byte aligned, not overlapping; fp32 scores, softmax and sums,
- * the weights rounded to the type for the product with v. head_dim 64 or 128,
- * heads / kv_heads <= 128, 0 < scale <= 2^127. max_new: the most new tokens of any sequence;
- * the kernel and the work buffer are chosen by it, more are computed as well. The
- * work buffer (16-byte aligned) holds at least what sh_attn_paged_workspace
- * says for the same sizes. It and out overlap nothing else of the call. */
+ * q . k of -infinity (or below -2^108) has no weight, one of +infinity makes the row
+ * NaN; with the scale, products may leave fp32's range. q, out [tokens][heads][head_dim] in the
+ * cache's type, 16-byte aligned; fp32 scores, softmax and sums, the weights rounded
+ * to the type for the product with v. head_dim 64 or 128, heads / kv_heads <= 128,
+ * 0 < scale <= 2^127. max_new: the most new tokens of any sequence; the kernel and
+ * the work buffer are chosen by it, more are computed as well. The work buffer
+ * (16-byte aligned) holds at least what sh_attn_paged_workspace says for the same
+ * sizes. It and out overlap nothing else of the call. */
 SH_API int sh_attn_paged_workspace(const sh_paged_kv *kv, int tokens, int heads, int max_new,
                                    size_t *bytes);
 SH_API int sh_attn_paged_f16(sh_ctx *ctx, const sh_paged_kv *kv, const uint16_t *q, uint16_t *out,

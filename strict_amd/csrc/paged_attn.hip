@@ -6,8 +6,9 @@
 // that lies in one piece is written to the output; one cut between pieces leaves
 // a part in each of its workgroups' slots (V sums, maximum and sum of weights
 // per row), and a second kernel merges the parts. That kernel also works out again,
-// in fp32 without matrix products, what came out not finite: infinities and NaN in
-// q, K or V, or in places of V that only some of a tile's rows see.
+// in fp32 without matrix products, what came out not finite (infinities and NaN in
+// q, K or V, or in places of V that only some of a tile's rows see) and rows whose
+// largest score is beyond kMaxScore.
 //
 // Softmax runs over the positions in order with a running maximum, in base 2:
 // s = q.k scale log2(e), weights 2^(s - max) (times 2^7 in fp16).
@@ -46,10 +47,11 @@ struct PagedAttnArgs {
   PagedPlan plan;
   MergeItem *items;  // [workers]
   int *groups;       // [workers]: rows to merge of the worker's item, in groups
-  int *redo;         // [workers]: 1: some of the worker's results are not finite
+  int *redo;         // [workers]: 1: some of the worker's results are to be worked out again
   float *slots;      // [2 workers][rows of a tile * (d + 2)]
   int heads, group, group_inv, max_pages, num_pages, page_shift, tile_rows;
   float scale_log2;
+  float no_score;    // a row's maximum that says it has no scores: -infinity or NaN (none)
 };
 
 // Token of a tile's row (r <= 255, group <= 128: exact), and its row of heads in q
@@ -92,6 +94,19 @@ __device__ __forceinline__ void store_value(const PagedAttnArgs &a, const PagedT
 
 __device__ __forceinline__ float exp2_weight(float x) { return __builtin_amdgcn_exp2f(x); }
 
+// The maximum is q.k scale rounded to fp32, the weights are 2 to the power of the
+// unrounded products less that: all of a row are off by one factor, which the division
+// takes out again, of up to 2^(half a step of the maximum). Up to 2^22 that is a quarter
+// and no more. At 2^30 it is 2^32: weights overflow, or all come to 0.
+// -infinity is the maximum of a row that sees nothing, or whose products are below
+// fp32's range: with scales of up to 2^20 only those of q.k below -2^108. With larger
+// ones a row of it is worked out again. (To ask what a row sees, where its sums are
+// written, was 1 us of 35 for 8 sequences of up to 333 tokens, and so was a branch.)
+constexpr float kMaxScore = 4194304.0f, kPlainScale = 1048576.0f;
+__device__ __forceinline__ bool score_fits(const PagedAttnArgs &a, float m) {
+  return __builtin_fabsf(m) < kMaxScore || m == a.no_score;
+}
+
 // What a token at position `pos` sees of the positions from p on: i of them on if
 // i <= last and (i >= first or i < sinks). (As limits of i, which the compiler has as
 // constants: as positions it would keep all of them in registers.)
@@ -102,9 +117,10 @@ struct Sees {
   __device__ __forceinline__ bool operator()(int i) const { return i <= last && (i >= first || i < sinks); }
 };
 
-// A tile in fp32, a wave per row, a lane per position of 64:
-// whatever the values are. A score of -infinity, and a weight that is 0 in fp32,
-// adds nothing. Slow: for tiles whose sums by MFMA are not finite.
+// A tile in fp32, a wave per row, a lane per position of 64: whatever the values are.
+// The maximum is q.k's, the scale taken after it is subtracted, so that the largest
+// weight is 1 however large the scores. A score of -infinity, and a weight that is 0 in
+// fp32, adds nothing. Slow: for tiles that the matrix products cannot do.
 template <class T, int kD>
 __device__ void attn_exact(const PagedAttnArgs &a, const PagedTile &t, const TileSpan &s) {
   typedef typename T::Value Value;
@@ -129,15 +145,14 @@ __device__ void attn_exact(const PagedAttnArgs &a, const PagedTile &t, const Til
           at = (((((long long)max(page, 0) * a.plan.kv_heads + t.kv_head) << a.page_shift) +
                  (p & ((1 << a.page_shift) - 1))) * kD);
         }
-        float sc = -INFINITY;
+        float dot = -INFINITY;
         if (seen) {
-          float dot = 0.0f;
+          dot = 0.0f;
           for (int c = 0; c < kD; c++) dot = fmaf((float)q[c], (float)kp[at + c], dot);
-          sc = dot * a.scale_log2;
         }
-        const float top = fmaxf(m, wave_max(sc));
-        const float w = sc == -INFINITY ? 0.0f : exp2_weight(sc - top + T::kWeightLog2);
-        const float c = top == m ? 1.0f : exp2_weight(m - top);
+        const float top = fmaxf(m, wave_max(dot));
+        const float w = dot == -INFINITY ? 0.0f : exp2_weight((dot - top) * a.scale_log2);
+        const float c = top == m ? 1.0f : exp2_weight((m - top) * a.scale_log2);
         l = l * c + wave_sum(w);
         m = top;
 #pragma unroll
@@ -234,7 +249,7 @@ __device__ __forceinline__ int worker_by_xcd(const PagedPlan &p, Line total, Lin
 }
 
 // A worker's piece, step by step: part(step), which says whether its results are
-// finite. Returns whether all are. kByXcd: *worker is to be found.
+// sound: finite, of scores that fit. Returns whether all are. kByXcd: *worker is to be found.
 template <bool kByXcd, class Part>
 __device__ __forceinline__ bool walk_piece(const PagedPlan &p, int *worker, PlanLds &lds, MergeItem *item, Part part) {
   const int per = (p.batch + kT - 1) / kT;
@@ -246,7 +261,7 @@ __device__ __forceinline__ bool walk_piece(const PagedPlan &p, int *worker, Plan
   const int me = kByXcd ? uniform(worker_by_xcd(p, total, piece)) : *worker;
   *worker = me;
   const Line x0 = me * piece, end = uniform(fmin(x0 + piece, total));
-  bool finite = true;
+  bool sound = true;
   Line x = x0;
   while (uniform(x < end ? 1 : 0)) {
     const int i = uniform(find_part(lds, x)), b = plan_part_first(p, i, per);
@@ -260,9 +275,9 @@ __device__ __forceinline__ bool walk_piece(const PagedPlan &p, int *worker, Plan
     st.more = uniform(st.more ? 1 : 0) != 0;
     x = uniform(t.begin + t.cost);
     if (!st.more) break;
-    if (st.run && !part(st, piece)) finite = false;
+    if (st.run && !part(st, piece)) sound = false;
   }
-  return finite;
+  return sound;
 }
 
 // A workgroup of the main kernels.
@@ -271,11 +286,11 @@ template <bool kByXcd, int kMergeRows, int kMergeCols, class Part>
 __device__ __forceinline__ void work_piece(const PagedAttnArgs &a, PlanLds &lds, Part part) {
   int worker = blockIdx.x;
   MergeItem item = {0, 0, 0, 0, 0, 0};
-  const bool finite = walk_piece<kByXcd>(a.plan, &worker, lds, &item, part);
+  const bool sound = walk_piece<kByXcd>(a.plan, &worker, lds, &item, part);
   if (threadIdx.x == 0) {
     a.items[worker] = item;
     a.groups[worker] = item.parts > 0 ? (item.tokens * a.group + kMergeRows - 1) / kMergeRows * kMergeCols : 0;
-    a.redo[worker] = finite ? 0 : 1;
+    a.redo[worker] = sound ? 0 : 1;
   }
 }
 
@@ -543,7 +558,7 @@ __device__ __forceinline__ bool attn_small(const PagedAttnArgs &a, const PagedTi
     for (int dt = 0; dt < kDT; dt++) *reinterpret_cast<f32x4 *>(&lds.acc[wave][r16][16 * dt + 4 * grp]) = acc[dt];
   }
   lds_barrier();
-  bool finite = true;
+  bool sound = true;
   for (int i = tid; i < rows * kD; i += kT) {
     const int r = i / kD, dim = i % kD;
     float m = lds.stat[0][r][0];
@@ -556,14 +571,14 @@ __device__ __forceinline__ bool attn_small(const PagedAttnArgs &a, const PagedTi
       sum = fmaf(f, lds.acc[w][r][dim], sum);
       l = fmaf(f, lds.stat[w][r][1], l);
     }
-    finite = finite && __builtin_fabsf(sum) < INFINITY && l < INFINITY;
+    sound = sound && score_fits(a, m) && __builtin_fabsf(sum) < INFINITY && l < INFINITY;
     store_value<T, kD>(a, t, s, slot, r, dim, sum, l);
     if (slot >= 0 && dim == 0) {
       slot_stats<kD>(a, slot, r)[0] = m;
       slot_stats<kD>(a, slot, r)[1] = l;
     }
   }
-  return !__syncthreads_or(finite ? 0 : 1);
+  return !__syncthreads_or(sound ? 0 : 1);
 }
 
 template <class T, int kD>
@@ -811,9 +826,9 @@ __device__ __forceinline__ bool attn_large(const PagedAttnArgs &a, const PagedTi
       }
   }
   l_run += __shfl_xor(l_run, 32, 64);
-  bool finite = true;
+  bool sound = true;
   const bool there = 32 * wave + n32 < rows;
-  if (there) finite = l_run < INFINITY;
+  if (there) sound = score_fits(a, m_run) && l_run < INFINITY;
   const float inv = l_run == 0.0f ? 0.0f : 1.0f / l_run;
   uint16_t *op = a.out + head_row(a, t.seq.row0 + s.first, t.kv_head, row) * kD;
 #pragma unroll
@@ -822,7 +837,7 @@ __device__ __forceinline__ bool attn_large(const PagedAttnArgs &a, const PagedTi
     for (int i = 0; i < 4; i++) {
       const f32x4 x = {acc[db][4 * i], acc[db][4 * i + 1], acc[db][4 * i + 2], acc[db][4 * i + 3]};
 #pragma unroll
-      for (int e = 0; e < 4; e++) finite = finite && (!there || __builtin_fabsf(x[e]) < INFINITY);
+      for (int e = 0; e < 4; e++) sound = sound && (!there || __builtin_fabsf(x[e]) < INFINITY);
       if (slot >= 0) {
         if (active) *slot_large<kD>(a, slot, wave, db, i) = x;
       } else if (there) {
@@ -834,7 +849,7 @@ __device__ __forceinline__ bool attn_large(const PagedAttnArgs &a, const PagedTi
     slot_stats<kD>(a, slot, row)[0] = m_run;
     slot_stats<kD>(a, slot, row)[1] = l_run;
   }
-  return !__syncthreads_or(finite ? 0 : 1);
+  return !__syncthreads_or(sound ? 0 : 1);
 }
 
 template <class T, int kD>
@@ -853,7 +868,7 @@ __global__ __launch_bounds__(kT, kLarge.workers / 256) void paged_large_kernel(c
 // sum over the workers' items): of small tiles a row, whose parts, perhaps spread over
 // all workers, are taken by 8 waves, 8 at once in each; of large tiles, of two or three
 // parts mostly, 32 rows by 32 dims a wave, as the main kernel's lanes held them.
-// Tiles with a part that is not finite are left to workgroup w of the first such
+// Tiles with a part that is not sound are left to workgroup w of the first such
 // worker w, which works them out in fp32, and its whole tiles too.
 struct MergeLds {
   union {
@@ -957,12 +972,12 @@ __global__ __launch_bounds__(kMergeT) void paged_merge_small_kernel(const PagedA
       // part, and for those that are not there, was 2 us of 9)
       const int mine = j0 + kWaves * lane;
       float my_m = -INFINITY, my_l = 0.0f;
-      int not_finite = 0;
+      int again = 0;
       if (lane < kStep && mine < it.parts) {
         const f32x2 stat = *reinterpret_cast<const f32x2 *>(slot_stats<kD>(a, part_slot(it, mine), r));
         my_m = stat.x;
         my_l = stat.y;
-        not_finite = a.redo[it.first_worker + mine];
+        again = a.redo[it.first_worker + mine];
       }
 #pragma unroll
       for (int u = 0; u < kStep; u++) {
@@ -971,7 +986,7 @@ __global__ __launch_bounds__(kMergeT) void paged_merge_small_kernel(const PagedA
         if (j < it.parts)
           x[u] = *reinterpret_cast<const Dims *>(slot_of<kD>(a, part_slot(it, j)) + r * kD + lane * kDims);
       }
-      redo = redo || __any(not_finite != 0);
+      redo = redo || __any(again != 0);
       float m[kStep], l[kStep], t = top;
 #pragma unroll
       for (int u = 0; u < kStep; u++) {
@@ -1166,6 +1181,7 @@ int attn_paged(sh_ctx *ctx, const sh_paged_kv *kv, const uint16_t *q, uint16_t *
   const Variant v = variant_of(a.group, max_new);
   a.tile_rows = v.rows;
   a.scale_log2 = scale * 1.44269504f;
+  a.no_score = a.scale_log2 <= kPlainScale ? -INFINITY : NAN;
   PagedPlan &p = a.plan;
   p.starts = kv->starts;
   p.lengths = kv->lengths;

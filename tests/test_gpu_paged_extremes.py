@@ -1,0 +1,85 @@
+"""Attention over pages where fp32 runs out: scores far beyond the exponent's range,
+values whose sums do. What the rows are is known, or as in test_gpu_paged.py."""
+import numpy as np
+import pytest
+
+import test_gpu_paged as paged
+
+pytestmark = pytest.mark.gpu
+
+
+def pointed(seed, ctx, dtype, new, lengths, at, size=1.0):
+    """A case whose query rows all point where position `at` of each sequence's k does:
+    its product with them is 250 size^2 or more, of the others no more than a third of that."""
+    c = paged.Case(ctx, seed, dtype, new, lengths, 4, 2, 128, 16)
+    way = c.rng.choice([-1.0, 1.0], 128)
+    k = paged.from16(c.k, dtype)
+    for b, p in enumerate(at):
+        k[c.table[b, p // 16], :, p % 16] = 2 * way
+    c.k[:] = paged.to16(k * size, dtype)
+    q = way * (1 + np.abs(c.rng.normal(0, 0.2, (c.tokens, 4, 128)))) * size
+    return c, paged.to16(q, dtype)
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("new,lengths,at", [([1, 1], [600, 40], [123, 39]), ([40, 3], [600, 90], [7, 80]),
+                                            ([1], [9000], [4321])])
+@pytest.mark.parametrize("log2", [14, 18, 22, 26, 30, 36, 60, 119, 126])
+def test_one_score_far_above_the_others(ctx, dtype, new, lengths, at, log2):
+    # (by 100 times the scale and more: the others have no weight)
+    c, q = pointed(log2, ctx, dtype, new, lengths, at)
+    _, got = paged.run_attention(c, q=q, scale=float(np.float32(c.rng.uniform(1, 2) * 2.0 ** log2)))
+    for b, p in enumerate(at):
+        v = c.v[c.table[b, p // 16], :, p % 16].repeat(2, 0)
+        assert (got[c.starts[b]:c.starts[b] + new[b]] == v).all(), b
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("new,lengths,at", [([1, 1], [600, 40], [123, 39]), ([40, 3], [600, 90], [7, 80])])
+@pytest.mark.parametrize("log2", [16, 30, 119, 126])
+def test_the_least_of_large_negative_scores(ctx, dtype, new, lengths, at, log2):
+    # (products with the scale below fp32's range among them)
+    c, q = pointed(log2, ctx, dtype, new, lengths, at)
+    way = np.sign(paged.from16(q, dtype)[0, 0])
+    k = np.broadcast_to(-2 * way, c.k.shape).copy()
+    for b, p in enumerate(at):
+        k[c.table[b, p // 16], :, p % 16] = -way
+    c.k[:] = paged.to16(k, dtype)
+    _, got = paged.run_attention(c, q=q, scale=float(np.float32(c.rng.uniform(1, 2) * 2.0 ** log2)))
+    for b, p in enumerate(at):
+        v = c.v[c.table[b, p // 16], :, p % 16].repeat(2, 0)
+        assert (got[c.starts[b]:c.starts[b] + new[b]] == v).all(), b
+
+
+@pytest.mark.parametrize("new,lengths,at", [([1], [700], [123]), ([40], [700], [600])])
+@pytest.mark.parametrize("dtype,size", [("f16", 2.0 ** 10), ("f16", 2.0 ** 13), ("bf16", 2.0 ** 18), ("bf16", 2.0 ** 55)])
+def test_large_queries_and_keys(ctx, dtype, size, new, lengths, at):
+    c, q = pointed(int(np.log2(size)), ctx, dtype, new, lengths, at, size)
+    _, got = paged.run_attention(c, q=q)
+    v = c.v[c.table[0, at[0] // 16], :, at[0] % 16].repeat(2, 0)
+    assert (got[c.starts[0]:c.starts[0] + new[0]] == v).all()
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("new,lengths", [([1], [600]), ([40], [600])])
+@pytest.mark.parametrize("base", [-2.0 ** 23, -2.0 ** 19, 2.0 ** 12, 2.0 ** 19, 2.0 ** 22, 2.0 ** 23])
+def test_close_scores_far_from_zero(ctx, dtype, new, lengths, base):
+    # whole numbers base + 0 .. 9, exact in fp32: the weights are those of 0 .. 9
+    c = paged.Case(ctx, 5, dtype, new, lengths, 4, 2, 64, 16)
+    some = c.rng.integers(0, 10, c.k.shape[:3])
+    k = np.zeros(c.k.shape)
+    k[..., 0], k[..., 1] = some, 64
+    c.k[:] = paged.to16(k, dtype)
+    q = np.zeros((c.tokens, 4, 64))
+    q[..., 0], q[..., 1] = 1, base / 64
+    ones = np.zeros((c.tokens, 4, 64))
+    ones[..., 0] = 1
+    if abs(base) / 64 > 60000:  # (fp16)
+        k[..., 1:9], q[..., 1:9] = 64, base / 512
+        c.k[:] = paged.to16(k, dtype)
+    _, got = paged.run_attention(c, q=paged.to16(q, dtype), scale=1.0)
+    c.k[:] = paged.to16(np.where(np.arange(64) == 0, k, 0), dtype)
+    ref, tol = paged.attention_oracle(c, ones, 0, 0, 1.0)
+    out = paged.from16(got, dtype)
+    n = sum(new)
+    assert (np.abs(out - ref)[:n] <= tol[:n]).all()
