@@ -676,7 +676,7 @@ __device__ __forceinline__ bool attn_large(const PagedAttnArgs &a, const PagedTi
         ".Lpaged_load%=:"
         ::"v"(k_off ^ (64 * u)), "v"(v_off), "s"(k_from + u * 1024), "s"(v_from + u * 1024),
         "s"(k_lds + to + u * 1024), "s"(v_lds + to + u * 1024), "s"(uniform(really))
-        : "memory", "scc");
+        : "memory", "scc", "m0");
   };
 
   float m_run = -INFINITY, l_run = 0.0f;
