@@ -7,8 +7,8 @@
 // a part in each of its workgroups' slots (V sums, maximum and sum of weights
 // per row), and a second kernel merges the parts. That kernel also works out again,
 // in fp32 without matrix products, what came out not finite (infinities and NaN in
-// q, K or V, or in places of V that only some of a tile's rows see) and rows whose
-// largest score is beyond kMaxScore.
+// q, K or V, or in places of V that only some of a tile's rows see), sums beyond kMaxSum
+// and rows whose largest score is beyond kMaxScore.
 //
 // Softmax runs over the positions in order with a running maximum, in base 2:
 // s = q.k scale log2(e), weights 2^(s - max) (times 2^7 in fp16).
@@ -107,6 +107,11 @@ __device__ __forceinline__ bool score_fits(const PagedAttnArgs &a, float m) {
   return __builtin_fabsf(m) < kMaxScore || m == a.no_score;
 }
 
+// V sums that leave room for those of all parts (bf16 values of 2^64 and more reach it):
+// beyond, the mean may be in fp32's range where the sums are not.
+constexpr float kMaxSum = 0x1p100f;
+__device__ __forceinline__ bool sum_fits(float x) { return __builtin_fabsf(x) < kMaxSum; }
+
 // What a token at position `pos` sees of the positions from p on: i of them on if
 // i <= last and (i >= first or i < sinks). (As limits of i, which the compiler has as
 // constants: as positions it would keep all of them in registers.)
@@ -119,8 +124,9 @@ struct Sees {
 
 // A tile in fp32, a wave per row, a lane per position of 64: whatever the values are.
 // The maximum is q.k's, the scale taken after it is subtracted, so that the largest
-// weight is 1 however large the scores. A score of -infinity, and a weight that is 0 in
-// fp32, adds nothing. Slow: for tiles that the matrix products cannot do.
+// weight is 1 however large the scores; the V sums are those of weights divided by their
+// sum so far, and so no larger than the values. A score of -infinity, and a weight that
+// is 0 in fp32, adds nothing. Slow: for tiles that the matrix products cannot do.
 template <class T, int kD>
 __device__ void attn_exact(const PagedAttnArgs &a, const PagedTile &t, const TileSpan &s) {
   typedef typename T::Value Value;
@@ -153,12 +159,14 @@ __device__ void attn_exact(const PagedAttnArgs &a, const PagedTile &t, const Til
         const float top = fmaxf(m, wave_max(dot));
         const float w = dot == -INFINITY ? 0.0f : exp2_weight((dot - top) * a.scale_log2);
         const float c = top == m ? 1.0f : exp2_weight((m - top) * a.scale_log2);
-        l = l * c + wave_sum(w);
+        const float before = l * c;
+        l = before + wave_sum(w);
         m = top;
+        const float kept = l == 0.0f ? 0.0f : before / l, part = l == 0.0f ? 0.0f : w / l;
 #pragma unroll
-        for (int j = 0; j < kDims; j++) acc[j] *= c;
+        for (int j = 0; j < kDims; j++) acc[j] *= kept;
         for (int i = 0; i < 64; i++) {
-          const float wi = __shfl(w, i, 64);
+          const float wi = __shfl(part, i, 64);
           const long long ai = __shfl(at, i, 64);
           if (wi == 0.0f) continue;
 #pragma unroll
@@ -167,7 +175,7 @@ __device__ void attn_exact(const PagedAttnArgs &a, const PagedTile &t, const Til
       }
     }
 #pragma unroll
-    for (int j = 0; j < kDims; j++) store_value<T, kD>(a, t, s, -1, r, lane + 64 * j, acc[j], l);
+    for (int j = 0; j < kDims; j++) store_value<T, kD>(a, t, s, -1, r, lane + 64 * j, acc[j], 1.0f);
   }
 }
 
@@ -249,7 +257,7 @@ __device__ __forceinline__ int worker_by_xcd(const PagedPlan &p, Line total, Lin
 }
 
 // A worker's piece, step by step: part(step), which says whether its results are
-// sound: finite, of scores that fit. Returns whether all are. kByXcd: *worker is to be found.
+// sound: finite, of sums and scores that fit. Returns whether all are. kByXcd: *worker is to be found.
 template <bool kByXcd, class Part>
 __device__ __forceinline__ bool walk_piece(const PagedPlan &p, int *worker, PlanLds &lds, MergeItem *item, Part part) {
   const int per = (p.batch + kT - 1) / kT;
@@ -571,7 +579,7 @@ __device__ __forceinline__ bool attn_small(const PagedAttnArgs &a, const PagedTi
       sum = fmaf(f, lds.acc[w][r][dim], sum);
       l = fmaf(f, lds.stat[w][r][1], l);
     }
-    sound = sound && score_fits(a, m) && __builtin_fabsf(sum) < INFINITY && l < INFINITY;
+    sound = sound && score_fits(a, m) && sum_fits(sum) && l < INFINITY;
     store_value<T, kD>(a, t, s, slot, r, dim, sum, l);
     if (slot >= 0 && dim == 0) {
       slot_stats<kD>(a, slot, r)[0] = m;
@@ -837,7 +845,7 @@ __device__ __forceinline__ bool attn_large(const PagedAttnArgs &a, const PagedTi
     for (int i = 0; i < 4; i++) {
       const f32x4 x = {acc[db][4 * i], acc[db][4 * i + 1], acc[db][4 * i + 2], acc[db][4 * i + 3]};
 #pragma unroll
-      for (int e = 0; e < 4; e++) sound = sound && (!there || __builtin_fabsf(x[e]) < INFINITY);
+      for (int e = 0; e < 4; e++) sound = sound && (!there || sum_fits(x[e]));
       if (slot >= 0) {
         if (active) *slot_large<kD>(a, slot, wave, db, i) = x;
       } else if (there) {

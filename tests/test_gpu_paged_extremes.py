@@ -83,3 +83,15 @@ def test_close_scores_far_from_zero(ctx, dtype, new, lengths, base):
     out = paged.from16(got, dtype)
     n = sum(new)
     assert (np.abs(out - ref)[:n] <= tol[:n]).all()
+
+
+@pytest.mark.parametrize("new,lengths", [([1, 1], [600, 40]), ([40, 9], [600, 300]), ([1], [20000])])
+@pytest.mark.parametrize("top", [2.0 ** 110, 2.0 ** 122, 2.0 ** 125])
+def test_values_whose_sums_leave_the_range(ctx, new, lengths, top):
+    c = paged.Case(ctx, 7, "bf16", new, lengths, 4, 2, 128, 16)
+    c.v[:] = paged.to16(np.clip(paged.from16(c.v, "bf16"), -7, 7) * top, "bf16")
+    paged.check_attention(c)
+    c.v[:] = paged.to16(np.full(c.v.shape, 2.0 ** 127), "bf16")
+    _, got = paged.run_attention(c)
+    n = sum(new)
+    assert (got[:n] == paged.to16([2.0 ** 127], "bf16")).all()
