@@ -529,7 +529,7 @@ SH_API int sh_qk_norm_rope_paged_bf16(sh_ctx *ctx, const sh_paged_kv *kv, const 
  * q . k of -infinity (or below -2^108) has no weight, one of +infinity makes the row
  * NaN; with the scale, products may leave fp32's range. q, out [tokens][heads][head_dim] in the
  * cache's type, 16-byte aligned; fp32 scores, softmax and sums, the weights rounded
- * to the type for the product with v. head_dim 64 or 128, heads / kv_heads <= 128,
+ * to the type before the sums. head_dim 64 or 128, heads / kv_heads <= 128,
  * 0 < scale <= 2^127. max_new: the most new tokens of any sequence; the kernel and
  * the work buffer are chosen by it, more are computed as well. The work buffer
  * (16-byte aligned) holds at least what sh_attn_paged_workspace says for the same

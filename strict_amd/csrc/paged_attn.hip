@@ -11,7 +11,12 @@
 // and rows whose largest score is beyond kMaxScore.
 //
 // Softmax runs over the positions in order with a running maximum, in base 2:
-// s = q.k scale log2(e), weights 2^(s - max) (times 2^7 in fp16).
+// s = q.k scale log2(e), weights 2^(s - max) (times 2^7 in fp16). The weights are
+// rounded to 16 bits for the product with V (whose matrix instructions take both
+// operands so; those of fp32 run at a sixteenth of the rate): 8,192 bf16 tokens are then
+// off by 2.2e-3 of their size where the rounding of the results alone makes 1.6e-3.
+// Their sum is that of the rounded ones: what the roundings of many equal weights have
+// in common goes out with the division.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -518,10 +523,10 @@ __device__ __forceinline__ bool attn_small(const PagedAttnArgs &a, const PagedTi
     for (int tt = 0; tt < kBlocks; tt++)
 #pragma unroll
       for (int e = 0; e < 4; e++) {
-        const float w = exp2_weight(fmaf(sc[tt][e], a.scale_log2, -off));
-        p[tt / 2][(tt & 1) * 4 + e] = (Value)w;
-        ls += w;
+        p[tt / 2][(tt & 1) * 4 + e] = (Value)exp2_weight(fmaf(sc[tt][e], a.scale_log2, -off));
       }
+#pragma unroll
+    for (int i = 0; i < kBlocks / 2; i++) ls = T::sum8(p[i], ls);
     l_run = l_run * corr + ls;  // this lane's positions; the groups are summed at the end
 #pragma unroll
     for (int dt = 0; dt < kDT; dt++)
@@ -814,11 +819,10 @@ __device__ __forceinline__ bool attn_large(const PagedAttnArgs &a, const PagedTi
     for (int sb = 0; sb < 2; sb++)
 #pragma unroll
       for (int i = 0; i < 16; i++) {
-        const float w = exp2_weight(fmaf(sc[sb][i], a.scale_log2, -off));
-        p[2 * sb + i / 8][i % 8] = (Value)w;
-        ls += w;
+        p[2 * sb + i / 8][i % 8] = (Value)exp2_weight(fmaf(sc[sb][i], a.scale_log2, -off));
       }
-    l_run += ls;
+    ls = T::sum8(p[1], T::sum8(p[0], ls));
+    l_run += ls + T::sum8(p[3], T::sum8(p[2], 0.0f));
     __builtin_amdgcn_sched_barrier(0);
     read_v(2);
     read_v(3);

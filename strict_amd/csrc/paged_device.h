@@ -27,6 +27,14 @@ struct PagedF16 {
   static __device__ __forceinline__ f32x16 mfma32(Vec a, Vec b, f32x16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
   }
+  // sum and the eight values, two at a time (fp16 below the normal range as they are)
+  static __device__ __forceinline__ float sum8(Vec v, float sum) {
+    typedef _Float16 Pair __attribute__((ext_vector_type(2)));
+    const Pair one = {(_Float16)1.0f, (_Float16)1.0f};
+#pragma unroll
+    for (int i = 0; i < 4; i++) sum = __builtin_amdgcn_fdot2(Pair{v[2 * i], v[2 * i + 1]}, one, sum, false);
+    return sum;
+  }
 };
 struct PagedBf16 {
   typedef __bf16 Value;
@@ -37,6 +45,14 @@ struct PagedBf16 {
   }
   static __device__ __forceinline__ f32x16 mfma32(Vec a, Vec b, f32x16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+  }
+  // (each step off by up to 2^-23 of the sum, toward zero)
+  static __device__ __forceinline__ float sum8(Vec v, float sum) {
+    typedef __bf16 Pair __attribute__((ext_vector_type(2)));
+    const Pair one = {(__bf16)1.0f, (__bf16)1.0f};
+#pragma unroll
+    for (int i = 0; i < 4; i++) sum = __builtin_amdgcn_fdot2_f32_bf16(Pair{v[2 * i], v[2 * i + 1]}, one, sum, false);
+    return sum;
   }
 };
 

@@ -95,3 +95,25 @@ def test_values_whose_sums_leave_the_range(ctx, new, lengths, top):
     _, got = paged.run_attention(c)
     n = sum(new)
     assert (got[:n] == paged.to16([2.0 ** 127], "bf16")).all()
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("new,lengths", [([1], [600]), ([1, 1, 1], [1000, 77, 3]), ([40, 9], [600, 300])])
+@pytest.mark.parametrize("d", [64, 128])
+def test_values_that_are_all_alike(ctx, dtype, new, lengths, d):
+    # a mean of one value is that value, whatever the weights are rounded to: sums of at most
+    # 1,000 of them, in fp32 off by less than 2,016 2^-24 = 2^-13, are rounded back to it. One
+    # position's score is above all others', which are one another's: their roundings do not
+    # average out.
+    c = paged.Case(ctx, 6, dtype, new, lengths, 16, 2, d, 16)
+    value = paged.to16(c.rng.uniform(1, 2, (2, 1, d)) * c.rng.choice([-1, 1], (2, 1, d)), dtype)
+    c.v[:] = value
+    k = np.zeros(c.k.shape)
+    for b in range(c.batch):
+        k[c.table[b, 0], :, 0, 0] = 1
+    c.k[:] = paged.to16(k, dtype)
+    q = np.zeros((c.tokens, 16, d))
+    q[..., 0] = c.rng.uniform(0, 3, (c.tokens, 16))
+    _, got = paged.run_attention(c, q=paged.to16(q, dtype), scale=1.0)
+    n = sum(new)
+    assert (got[:n] == value[:, 0].repeat(8, 0)).all()
