@@ -507,7 +507,8 @@ typedef struct sh_paged_kv {
  * values each, rows ld >= (heads + 2 kv_heads) * head_dim values apart: q and k
  * normalised per head, x / sqrt(mean(x^2) + eps) * gain (gains fp32, head_dim
  * values), then rotated by halves at the token's position, angle = position *
- * theta^(-2i / head_dim) in fp64; q to q[tokens][heads][head_dim], k and v (as
+ * theta^(-2i / head_dim) in fp64 (theta 1 or more; less where max_pages * page_size,
+ * and tokens, times theta^(-(head_dim - 2) / head_dim) are at most 2^29); q to q[tokens][heads][head_dim], k and v (as
  * it is) to their pages. fp16 or bf16, rounded once. A token before position 0
  * is rotated by its negative position and not stored. head_dim 64 or 128; qkv
  * and q 16-byte aligned, ld a multiple of 8; q and the pages overlap nothing else of

@@ -331,6 +331,18 @@ inline const char *check_paged_sizes(const sh_paged_kv *kv, int tokens, int head
   return nullptr;
 }
 
+// RoPE's angles, position * theta^(-2i / head_dim) in fp64, are to be below 2^29: there
+// a step of fp64 is 2^-24, fp32's of their cosines, and the quadrant fits an int.
+// Positions reach from -tokens to the capacity; with theta >= 1 no frequency exceeds 1.
+inline const char *check_rope_theta(const sh_paged_kv *kv, int tokens, float theta) {
+  if (!(theta > 0.0f) || !std::isfinite(theta)) return "theta must be positive and finite";
+  const double capacity = (double)kv->max_pages * kv->page_size, reach = capacity > tokens ? capacity : tokens;
+  const double fastest = theta < 1.0f ? std::pow((double)theta, -(kv->head_dim - 2.0) / kv->head_dim) : 1.0;
+  if (reach * fastest > 536870912.0)
+    return "theta: max_pages * page_size (or tokens) * theta^(-(head_dim - 2) / head_dim) exceeds 2^29";
+  return nullptr;
+}
+
 inline bool paged_dim_built(int head_dim) { return head_dim == 64 || head_dim == 128; }
 
 inline size_t paged_pool_bytes(const sh_paged_kv *kv) {

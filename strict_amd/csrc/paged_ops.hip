@@ -26,7 +26,7 @@ struct NormRopeArgs {
   double freq[64];  // theta^(-2i / d)
 };
 
-// cos and sin of an fp64 angle below 2^29 to fp32: reduction by pi / 2 in two
+// cos and sin of an fp64 angle below 2^29 (check_rope_theta) to fp32: reduction by pi / 2 in two
 // parts (Cody and Waite) and Taylor polynomials on [-pi / 4, pi / 4], in fp64.
 __device__ __forceinline__ void cos_sin64(double a, float *c, float *s) {
   const double q = rint(a * 0.63661977236758134308);  // 2 / pi
@@ -153,7 +153,7 @@ int norm_rope(sh_ctx *ctx, const sh_paged_kv *kv, const uint16_t *qkv, const flo
   const int d = kv->head_dim;
   if (!paged_dim_built(d)) return fail(SH_ERR_UNSUPPORTED, "paged head_dim %d (64 or 128 are built)", d);
   if (!(eps >= 0.0f)) return fail(SH_ERR_INVALID_ARGUMENT, "eps must be >= 0");
-  if (!(theta > 0.0f) || !std::isfinite(theta)) return fail(SH_ERR_INVALID_ARGUMENT, "theta must be positive and finite");
+  if (const char *wrong = check_rope_theta(kv, tokens, theta)) return fail(SH_ERR_INVALID_ARGUMENT, "%s", wrong);
   const long long width = ((long long)heads + 2LL * kv->kv_heads) * d;
   if (ld < width || ld % 8 != 0)
     return fail(SH_ERR_INVALID_ARGUMENT, "ld %d must be a multiple of 8 and at least %lld", ld, width);

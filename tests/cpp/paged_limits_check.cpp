@@ -1,5 +1,6 @@
 // Host check of the paged operators' argument checks at their largest sizes
 // (strict_amd/csrc/paged.h).
+#include <cmath>
 #include <cstdint>
 #include <cstdio>
 #include <cstring>
@@ -46,8 +47,25 @@ static void pools() {
         }
 }
 
+static void thetas() {
+  sh_paged_kv kv = sizes(4, 1, 65536, 128);
+  kv.max_pages = 1 << 12;  // 2^28 positions
+  CHECK(!check_rope_theta(&kv, kMaxPagedTokens, 1.0f) && !check_rope_theta(&kv, 1, 1e6f) && !check_rope_theta(&kv, 1, 3.4e38f));
+  for (float theta : {0.0f, -1.0f, INFINITY, NAN, -0.0f}) CHECK(check_rope_theta(&kv, 1, theta));
+  // (2^28 positions: frequencies of up to 2)
+  CHECK(!check_rope_theta(&kv, 1, 0.5f) && check_rope_theta(&kv, 1, 0.25f) && check_rope_theta(&kv, 1, 1e-45f));
+  for (int head_dim : {64, 128})
+    for (int log2 = 1; log2 <= 149; log2++) {  // theta = 2^-log2: 2^(log2 (1 - 2 / head_dim)) times the positions
+      kv.head_dim = head_dim, kv.page_size = 16, kv.max_pages = 1;
+      const double exponent = log2 * (1.0 - 2.0 / head_dim);
+      CHECK((check_rope_theta(&kv, 1, std::ldexp(1.0f, -log2)) != nullptr) == (exponent + 4 > 29));
+      CHECK((check_rope_theta(&kv, 1 << 10, std::ldexp(1.0f, -log2)) != nullptr) == (exponent + 10 > 29));
+    }
+}
+
 int main() {
   pools();
+  thetas();
   std::printf("failures=%lld\n", failures);
   return failures == 0 ? 0 : 1;
 }
