@@ -500,13 +500,16 @@ class Context:
         return n.value
 
     def attn_paged(self, kv: PagedKV, q, out, tokens: int, heads: int, max_new: int, scale: float,
-                   workspace: DeviceVariable, window: int = 0, sinks: int = 0) -> None:
+                   workspace, window: int = 0, sinks: int = 0) -> None:
         """Attention of the new tokens (q, out [tokens, heads, d] in the cache's type)
         over their sequences' pages, causal; window > 0: over the last `window`
-        positions and the first `sinks`. max_new: the most new tokens of a sequence."""
+        positions and the first `sinks`. max_new: the most new tokens of a sequence.
+        workspace: a buffer, or the address of one, of at least attn_paged_workspace's bytes."""
+        size = (workspace.nbytes if isinstance(workspace, DeviceVariable)
+                else self.attn_paged_workspace(kv, tokens, heads, max_new))
         f = self._l.sh_attn_paged_f16 if kv.dtype == "f16" else self._l.sh_attn_paged_bf16
         _check(f(self.handle, kv.address, _ptr(q), _ptr(out), tokens, heads, max_new, window, sinks,
-                 scale, _ptr(workspace), workspace.nbytes))
+                 scale, _ptr(workspace), size))
 
     def pages_copy(self, pool, planes: int, num_pages: int, page_bytes: int, src, dst, count: int,
                    plane_stride: int | None = None) -> None:
@@ -522,12 +525,14 @@ class Context:
         return size.value
 
     def sample(self, logits, rows: int, n: int, temperature, top_k, top_p, min_p, u, index,
-               workspace: DeviceVariable, ld: int | None = None) -> None:
+               workspace, ld: int | None = None) -> None:
         """index[r] = a token drawn from logits [rows, n] (rows ld apart) by each row's
-        temperature, top-k, top-p, min-p (device arrays or None) and uniform number u."""
+        temperature, top-k, top-p, min-p (device arrays or None) and uniform number u.
+        workspace: a buffer, or the address of one, of at least sample_workspace's bytes."""
+        size = workspace.nbytes if isinstance(workspace, DeviceVariable) else self.sample_workspace(rows, n)
         _check(self._l.sh_sample_f32(self.handle, _ptr(logits), rows, n, n if ld is None else ld,
                                      _ptr(temperature), _ptr(top_k), _ptr(top_p), _ptr(min_p),
-                                     _ptr(u), _ptr(index), _ptr(workspace), workspace.nbytes))
+                                     _ptr(u), _ptr(index), _ptr(workspace), size))
 
 
 class Event:
