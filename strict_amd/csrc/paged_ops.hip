@@ -271,15 +271,17 @@ SH_API int sh_pages_copy(sh_ctx *ctx, void *pool, int planes, size_t plane_strid
     return fail(SH_ERR_INVALID_ARGUMENT, "src or dst lies in the pools");
   const uint32_t vectors = (uint32_t)(page_bytes / 16);
   const int chunks = (int)((vectors + kT * kCopyVectors - 1) / (kT * kCopyVectors));
-  const long long blocks = (long long)count * chunks;
-  if (blocks >= (1LL << 24)) {  // (a launch takes fewer than 2^32 threads)
-    return fail(SH_ERR_INVALID_ARGUMENT, "count * page_bytes exceeds 2^38 bytes a plane");
-  }
-  for (int p0 = 0; p0 < planes;) {
-    const int n = (int)std::min<long long>(planes - p0, std::max(1LL, (1LL << 24) / blocks - 1));
-    pages_copy_kernel<<<dim3((unsigned)blocks, (unsigned)n), kT, 0, stream_of(ctx)>>>(
-        static_cast<uint8_t *>(pool) + p0 * plane_stride, plane_stride, num_pages, vectors, chunks, src, dst);
-    p0 += n;
+  // (a launch takes fewer than 2^32 threads: 2^24 workgroups; a page is 2^17 of them at most)
+  const int most = (1 << 24) - 1;
+  for (int i0 = 0; i0 < count;) {
+    const int pages = std::min(count - i0, most / chunks), blocks = pages * chunks;
+    for (int p0 = 0; p0 < planes;) {
+      const int n = std::min(planes - p0, most / blocks);
+      pages_copy_kernel<<<dim3((unsigned)blocks, (unsigned)n), kT, 0, stream_of(ctx)>>>(
+          static_cast<uint8_t *>(pool) + p0 * plane_stride, plane_stride, num_pages, vectors, chunks, src + i0, dst + i0);
+      p0 += n;
+    }
+    i0 += pages;
   }
   const hipError_t e = hipGetLastError();
   return e == hipSuccess ? SH_OK : hip_fail(e, "pages_copy");

@@ -146,3 +146,26 @@ def test_logits_past_their_allocation(ctx):
     refused(lambda: ctx.sample(x, 2, 3000, None, None, None, None, u, index, work, 3001), "is not inside an allocation")
     for b in (x, u, index, work):
         b.free()
+
+
+@pytest.mark.parametrize("planes", [1, 3])
+def test_more_pages_than_a_launch_has_workgroups(ctx, planes):
+    # 2^24 and more pairs, small pages: all but a few skipped
+    num, page_bytes = (1 << 24) + 100, 16
+    count = num - 5
+    src = np.full(count, -1, np.int32)
+    dst = np.full(count, num, np.int32)
+    some = np.array([0, 1, 70000, (1 << 24) - 2, (1 << 24) - 1, 1 << 24, count - 1])
+    src[some], dst[some] = np.arange(len(some)), num - 1 - np.arange(len(some))
+    pool, s, d = ctx.alloc(planes * num * page_bytes), ctx.upload(src), ctx.upload(dst)
+    ctx.memset(pool, 0)
+    first = np.arange(planes * len(some) * 2, dtype=np.int64).reshape(planes, -1) + 1
+    last = [pool.view((p * num + num - len(some)) * page_bytes, len(some) * page_bytes, np.int64) for p in range(planes)]
+    for p in range(planes):
+        pool.view(p * num * page_bytes, len(some) * page_bytes).copy_from_host(first[p])
+    ctx.pages_copy(pool, planes, num, page_bytes, s, d, count)
+    ctx.sync()
+    for p in range(planes):
+        assert (last[p].to_host().reshape(-1, 2)[::-1] == first[p].reshape(-1, 2)).all()
+    for b in (pool, s, d):
+        b.free()
