@@ -126,7 +126,7 @@ SH_HD Line plan_last(const PagedPlan &p, const PlanSeq &s) {
 
 // (At least total / workers, with room for the roundings.) A piece that is somewhat
 // shorter than the largest tile becomes as long: most tiles then fit one and need no
-// merge. Of 448 tiles of one cost over 512 workers: 87 -> 73 us a call. From 3/8 of it on,
+// merge. Of 392 tiles of about one cost over 512 workers: 87 -> 73 us a call. From 3/8 of it on,
 // 8 sequences of up to 333 tokens: 35 -> 46, 4 of up to 512 65 -> 86.
 SH_HD Line plan_piece(const PagedPlan &p, Line total, Line largest) {
   const Line q = floor(total * p.inv_workers) + 2;

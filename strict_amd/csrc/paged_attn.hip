@@ -131,7 +131,10 @@ struct Sees {
 // The maximum is q.k's, the scale taken after it is subtracted, so that the largest
 // weight is 1 however large the scores; the V sums are those of weights divided by their
 // sum so far, and so no larger than the values. A score of -infinity, and a weight that
-// is 0 in fp32, adds nothing. Slow: for tiles that the matrix products cannot do.
+// is 0 in fp32, adds nothing. For tiles that the matrix products cannot do, and slow:
+// each lane reads a row of K of its own, and a worker with one such tile has all of its
+// tiles done again. A NaN that one of 48 decode rows of up to 4,352 positions sees:
+// 0.11 -> 4.0 ms; one in the last of 8,192 tokens over 12,288 positions: 0.6 -> 285 ms.
 template <class T, int kD>
 __device__ void attn_exact(const PagedAttnArgs &a, const PagedTile &t, const TileSpan &s) {
   typedef typename T::Value Value;
@@ -254,7 +257,7 @@ __device__ __forceinline__ int find_part(const PlanLds &lds, Line x) {
 
 // The worker that a workgroup is, if workgroups of one XCD are to be consecutive
 // workers, which share K and V. Of fewer pieces than workers each XCD takes an eighth
-// (448 tiles on 512: 66.4 -> 64.0 us a call; 8 sequences of up to 200 tokens 28 -> 27).
+// (392 tiles on 512: 66.4 -> 64.0 us a call; 8 sequences of up to 200 tokens 28 -> 27).
 __device__ __forceinline__ int worker_by_xcd(const PagedPlan &p, Line total, Line piece) {
   const int used = min((int)plan_div(total + piece - 1, piece), p.workers), per = (used + 7) >> 3;
   const int xcd = blockIdx.x & 7, i = blockIdx.x >> 3;
@@ -376,7 +379,8 @@ __device__ __forceinline__ void scale_if(f32x16 (&x)[4], float f, int really) {
 //    LDS rows as it is and comes back by transposing reads.
 // A unit's 16-position blocks lie in one page each (pages of 16 and more).
 // 48 ragged sequences of up to 4,352 positions (626 MB of bf16): 101 us here and 6 in
-// the merge, 6.2 TB/s of a copy's 6.4.
+// the merge, 6.2 TB/s of a copy's 6.4. 16 of up to 16,000 positions 134 us a call, with a
+// window of 1,024 and 4 sinks 25.
 template <int kD>
 constexpr int kSmallUnit = 32 * 128 / kD;
 
@@ -610,9 +614,9 @@ __global__ __launch_bounds__(kT, kSmall.workers / 256) void paged_small_kernel(c
 //  - scores as K x q, 32 x 32 positions and rows, K fragments from LDS;
 //  - V sums as V^T x P with the k slots numbered as P has them (slot (h, e) of 16
 //    positions: 4 h + e for e < 4, 8 + 4 h + e - 4 after that), V by transposing reads.
-// 8,192 tokens over 12,288 positions, 16 heads of 128 (550 GFLOP): 600 us, 917 TFLOP/s,
-// where a large product reaches 1,228; matrix cores busy 41 % of the time, vector units
-// (the softmax) 40 %, mostly in turn.
+// 8,192 tokens over 12,288 positions, 16 heads of 128 (550 GFLOP): 590 to 620 us a call
+// with the merge, 890 to 930 TFLOP/s, where a large product reaches 1,228; matrix cores
+// busy 41 % of the time, vector units (the softmax) 40 %, mostly in turn.
 constexpr int kLargeUnit = 64;
 constexpr float kSlack = 8.0f;
 
@@ -1113,10 +1117,13 @@ __global__ __launch_bounds__(kT) void paged_merge_large_kernel(const PagedAttnAr
 
 // ---- the entry points ---------------------------------------------------------------
 
-// Small tiles where every sequence's new tokens fit one. (Small and large, us a call, 16
-// sequences of up to 4,096 positions, 8 KV heads of 2 query heads: of 2 tokens 42 and 55,
-// 8 tokens, which is 16 rows, 55 and 59, 16 tokens 87 and 60. 48 sequences of one token
-// 110 and 135.)
+// Small tiles where every sequence's new tokens fit one: a second one reads K and V again,
+// a large one has idle waves. (Small and large, us a call, 16 sequences of up to 4,096
+// positions, 8 KV heads of 1, 2, 4 or 8 query heads: 16 rows a KV head 52 - 57 and
+// 54 - 59, 32 rows 76 - 87 and 57 - 59, 64 rows 124 - 154 and 61 - 63. 2 KV heads of 16: 16
+// rows 27 and 34, 32 rows 34 and 34, 64 rows 46 and 36. 48 sequences of one token of 2 heads
+// 110 and 135. Of more than 16 query heads a KV head one token is more than a small tile:
+// 17 to 32 heads 34, 128 heads 39.)
 Variant variant_of(int group, int max_new) {
   return group <= kSmall.rows && (long long)group * max_new <= kSmall.rows ? kSmall : kLarge;
 }

@@ -8,9 +8,12 @@
 //
 // Rows of up to 2,048 logits, which the list holds: one kernel, one workgroup a row (64
 // rows of 2,048 logits 23 us, by the four kernels 34; of 1,000 20 and 24). Longer ones in
-// four kernels over (row, split), bound by the weights' arithmetic (200 rows of 151,936:
-// max 19 us, the HBM rate; bins 29, gather 29, draw 27 from the last-level cache; one row
-// of 50,257 16 us, four launches):
+// four kernels over (row, split). 200 rows of 151,936: max 19 us, the HBM rate; bins 25
+// where top-k ends the selection (an LDS atomic a logit), 44 where top-p does (a weight in
+// fp64, too); gather 28 at top-k 50, 35 at 1,000, 47 to 54 where most logits are weighed;
+// draw, whose steps wait for each other in one workgroup a row, 7 at top-k 50, 18 at
+// 1,000, 20 at top-p 0.95, 27 where rows have several of them. One row of 50,257: 16.5 to
+// 18 us, four launches.
 //   max     the splits' largest values; clears the row's histogram
 //   bins    count of the tokens by t in bins of 1/46, or their weight, where top-p is
 //           without top-k; other rows pass
@@ -23,7 +26,8 @@
 //           in it the token that u falls on
 // A list that would not hold the bin's tokens, or top-p after a top-k of more than
 // the list holds: the draw kernel finds the last kept key by its digits, reading
-// the row once per digit.
+// the row once per digit: a cliff (200 rows of 151,936 at temperature 40: top-k 50,000 or
+// top-p 0.5 1.1 ms, top-k 50,000 with top-p 0.9 2.0; one row 0.6 and 1.1).
 #include <hip/hip_runtime.h>
 
 #include <algorithm>

@@ -123,7 +123,8 @@ class PageTable:
 class PagedCache:
     """K and V of `layers` layers in pages on a context's device, for up to `rows`
     sequences of up to max_pages pages each. Every method is ordered on the
-    context's stream."""
+    context's stream; `step`, and `compact` where it moves pages, upload tables from
+    the host and wait for the stream, and are not to be captured."""
 
     def __init__(self, ctx: Context, layers: int, kv_heads: int, head_dim: int, *, rows: int,
                  max_pages: int, num_pages: int, page_size: int = 64, dtype: str = "f16"):
