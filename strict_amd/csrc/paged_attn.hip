@@ -99,17 +99,14 @@ __device__ __forceinline__ void store_value(const PagedAttnArgs &a, const PagedT
 
 __device__ __forceinline__ float exp2_weight(float x) { return __builtin_amdgcn_exp2f(x); }
 
-// The maximum is q.k scale rounded to fp32, the weights are 2 to the power of the
-// unrounded products less that: all of a row are off by one factor, which the division
-// takes out again, of up to 2^(half a step of the maximum). Up to 2^22 that is a quarter
-// and no more. At 2^30 it is 2^32: weights overflow, or all come to 0.
-// -infinity is the maximum of a row that sees nothing, or whose products are below
-// fp32's range: with scales of up to 2^20 only those of q.k below -2^108. With larger
-// ones a row of it is worked out again. (To ask what a row sees, where its sums are
+// A row's maximum fits. -infinity is that of a row that sees nothing, or whose products
+// are below fp32's range: with scales of up to 2^20 only those of q.k below -2^108. With
+// larger ones a row of it is worked out again. (To ask what a row sees, where its sums are
 // written, was 1 us of 35 for 8 sequences of up to 333 tokens, and so was a branch.)
-constexpr float kMaxScore = 4194304.0f, kPlainScale = 1048576.0f;
+constexpr float kPlainScale = 0x1p20f;
+template <class T>
 __device__ __forceinline__ bool score_fits(const PagedAttnArgs &a, float m) {
-  return __builtin_fabsf(m) < kMaxScore || m == a.no_score;
+  return __builtin_fabsf(m) < T::kMaxScore || m == a.no_score;
 }
 
 // V sums that leave room for those of all parts (bf16 values of 2^64 and more reach it):
@@ -588,7 +585,7 @@ __device__ __forceinline__ bool attn_small(const PagedAttnArgs &a, const PagedTi
       sum = fmaf(f, lds.acc[w][r][dim], sum);
       l = fmaf(f, lds.stat[w][r][1], l);
     }
-    sound = sound && score_fits(a, m) && sum_fits(sum) && l < INFINITY;
+    sound = sound && score_fits<T>(a, m) && sum_fits(sum) && l < INFINITY;
     store_value<T, kD>(a, t, s, slot, r, dim, sum, l);
     if (slot >= 0 && dim == 0) {
       slot_stats<kD>(a, slot, r)[0] = m;
@@ -844,7 +841,7 @@ __device__ __forceinline__ bool attn_large(const PagedAttnArgs &a, const PagedTi
   l_run += __shfl_xor(l_run, 32, 64);
   bool sound = true;
   const bool there = 32 * wave + n32 < rows;
-  if (there) sound = score_fits(a, m_run) && l_run < INFINITY;
+  if (there) sound = score_fits<T>(a, m_run) && l_run < INFINITY;
   const float inv = l_run == 0.0f ? 0.0f : 1.0f / l_run;
   uint16_t *op = a.out + head_row(a, t.seq.row0 + s.first, t.kv_head, row) * kD;
 #pragma unroll

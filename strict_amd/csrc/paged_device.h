@@ -17,10 +17,15 @@ typedef float f32x16 __attribute__((ext_vector_type(16)));
 // (bf16's range is fp32's, so its weights need no scale; fp16 weights are kept
 // 2^7 times as large, which leaves those down to 2^-21 normal and those of a
 // maximum that lags behind by up to 2^8 finite.)
+// kMaxScore: a row's maximum is q.k scale rounded to fp32, its weights are 2 to the power
+// of the unrounded products less that: all are off by one factor, which the division
+// takes out again, of up to 2^(half a step of the maximum). Below 2^24 that is 2^(1/2): the
+// weights of fp16 stay below 2^15.5, and the maximum less 7 is exact. Below 2^30 it is
+// 2^32, which bf16's range has room for. Beyond, weights overflow or all come to 0.
 struct PagedF16 {
   typedef _Float16 Value;
   typedef pf16x8 Vec;
-  static constexpr float kWeightLog2 = 7.0f;
+  static constexpr float kWeightLog2 = 7.0f, kMaxScore = 0x1p24f;
   static __device__ __forceinline__ f32x4 mfma16(Vec a, Vec b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
   }
@@ -39,7 +44,7 @@ struct PagedF16 {
 struct PagedBf16 {
   typedef __bf16 Value;
   typedef pbf16x8 Vec;
-  static constexpr float kWeightLog2 = 0.0f;
+  static constexpr float kWeightLog2 = 0.0f, kMaxScore = 0x1p30f;
   static __device__ __forceinline__ f32x4 mfma16(Vec a, Vec b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
   }

@@ -24,7 +24,7 @@ def pointed(seed, ctx, dtype, new, lengths, at, size=1.0):
 @pytest.mark.parametrize("dtype", ["f16", "bf16"])
 @pytest.mark.parametrize("new,lengths,at", [([1, 1], [600, 40], [123, 39]), ([40, 3], [600, 90], [7, 80]),
                                             ([1], [9000], [4321])])
-@pytest.mark.parametrize("log2", [14, 18, 22, 26, 30, 36, 60, 119, 126])
+@pytest.mark.parametrize("log2", [14, 16, 18, 20, 21, 22, 26, 30, 36, 60, 119, 126])
 def test_one_score_far_above_the_others(ctx, dtype, new, lengths, at, log2):
     # (by 100 times the scale and more: the others have no weight)
     c, q = pointed(log2, ctx, dtype, new, lengths, at)
@@ -58,6 +58,22 @@ def test_large_queries_and_keys(ctx, dtype, size, new, lengths, at):
     _, got = paged.run_attention(c, q=q)
     v = c.v[c.table[0, at[0] // 16], :, at[0] % 16].repeat(2, 0)
     assert (got[c.starts[0]:c.starts[0] + new[0]] == v).all()
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("new,lengths", [([1, 1], [600, 5]), ([40, 3], [600, 90]), ([1], [20000])])
+@pytest.mark.parametrize("log2", [-40, 0, 8, 12, 13, 14, 15, 16, 19, 20, 21, 22, 26, 40, 100, 118, 126])
+def test_equal_scores_far_from_zero(ctx, dtype, new, lengths, log2):
+    # about 300 times the scale, and less that: means of the values
+    for sign in (1, -1):
+        c, q = pointed(log2 + 50, ctx, dtype, new, lengths, [0] * len(new))
+        way = np.sign(paged.from16(q, dtype)[0, 0])
+        c.k[:] = paged.to16(np.broadcast_to(sign * 2 * way, c.k.shape), dtype)
+        _, got = paged.run_attention(c, q=q, scale=float(np.float32(c.rng.uniform(1, 2) * 2.0 ** log2)))
+        c.k[:] = 0
+        ref, tol = paged.attention_oracle(c, paged.from16(q, dtype), 0, 0, 1.0)
+        n = sum(new)
+        assert (np.abs(paged.from16(got, dtype) - ref)[:n] <= tol[:n]).all(), sign
 
 
 @pytest.mark.parametrize("dtype", ["f16", "bf16"])
