@@ -8,6 +8,7 @@ copied when one of them appends to it. The reference has no counterpart.
 from __future__ import annotations
 
 import heapq
+import operator
 
 import numpy as np
 
@@ -45,6 +46,7 @@ class PageTable:
         plan, need = [], 0
         for row, n in new.items():
             self._check(row)
+            n = operator.index(n)
             if n < 0:
                 raise ValueError("a negative number of tokens")
             pages, length = self.pages[row], self.lengths[row]
@@ -164,7 +166,7 @@ class PagedCache:
     def step(self, new) -> int:
         """Prepares a step of new[row] new tokens for the rows named (their rows in
         the step's tensors follow the rows' order); returns how many there are."""
-        new = dict(new)
+        new = {row: operator.index(n) for row, n in dict(new).items()}
         self._copy(self.table.extend(new))
         self._upload(new)
         return sum(new.values())
