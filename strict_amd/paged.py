@@ -134,17 +134,26 @@ class PagedCache:
         self.table = PageTable(rows, max_pages, num_pages, page_size)
         self.page_bytes = kv_heads * page_size * head_dim * 2
         plane = num_pages * self.page_bytes
-        self.pool = ctx.alloc(layers * 2 * plane)  # [layer][k, v][page]
-        self.table_buf = ctx.empty((rows, max_pages), np.int32)
-        self.lengths = ctx.empty(rows, np.int32)
-        self.starts = ctx.empty(rows + 1, np.int32)
-        self.moves = ctx.empty((2, num_pages), np.int32)
-        self.kv = [PagedKV(self.pool.ptr + 2 * i * plane, self.pool.ptr + (2 * i + 1) * plane,
-                           self.table_buf, self.lengths, self.starts, batch=rows,
-                           max_pages=max_pages, num_pages=num_pages, page_size=page_size,
-                           kv_heads=kv_heads, head_dim=head_dim, dtype=dtype)
-                   for i in range(layers)]  # a layer's view, for the operators
-        self._upload({})
+        self.buffers = []
+        try:
+            self.pool = self._keep(ctx.alloc(layers * 2 * plane))  # [layer][k, v][page]
+            self.table_buf = self._keep(ctx.empty((rows, max_pages), np.int32))
+            self.lengths = self._keep(ctx.empty(rows, np.int32))
+            self.starts = self._keep(ctx.empty(rows + 1, np.int32))
+            self.moves = self._keep(ctx.empty((2, num_pages), np.int32))
+            self.kv = [PagedKV(self.pool.ptr + 2 * i * plane, self.pool.ptr + (2 * i + 1) * plane,
+                               self.table_buf, self.lengths, self.starts, batch=rows,
+                               max_pages=max_pages, num_pages=num_pages, page_size=page_size,
+                               kv_heads=kv_heads, head_dim=head_dim, dtype=dtype)
+                       for i in range(layers)]  # a layer's view, for the operators
+            self._upload({})
+        except BaseException:
+            self.dispose()
+            raise
+
+    def _keep(self, buffer):
+        self.buffers.append(buffer)
+        return buffer
 
     def _copy(self, pairs) -> None:
         if pairs:
@@ -185,7 +194,7 @@ class PagedCache:
         return len(moves)
 
     def dispose(self) -> None:
-        for b in (self.pool, self.table_buf, self.lengths, self.starts, self.moves):
+        for b in self.buffers:
             b.free()
 
     def __enter__(self):

@@ -77,3 +77,26 @@ def test_steps_count_in_any_whole_type(cache):
     ctx.sent.clear()
     assert c.step({0: np.uint8(200), 1: np.uint8(100)}) == 300
     assert ctx.sent[-1].tolist() == [0, 200, 300] and ctx.sent[-2].tolist() == [200, 100]
+
+
+@pytest.mark.parametrize("allocations", range(5))
+def test_a_cache_that_finds_no_memory_keeps_none(cache, allocations):
+    ctx = Host(allocations)
+    with pytest.raises(MemoryError):
+        cache(ctx, 2, 1, 64, rows=2, max_pages=4, num_pages=8, page_size=16)
+    assert ctx.held == []
+
+
+def test_a_cache_of_no_type_keeps_no_memory():
+    from strict_amd.paged import PagedCache
+    ctx = Host()
+    with pytest.raises(ValueError):
+        PagedCache(ctx, 2, 1, 64, rows=2, max_pages=4, num_pages=8, page_size=16, dtype="f32")
+    assert ctx.held == []
+
+
+def test_a_cache_gives_back_what_it_took(cache):
+    ctx = Host()
+    with cache(ctx, 2, 1, 64, rows=2, max_pages=4, num_pages=8, page_size=16):
+        assert len(ctx.held) == 5
+    assert ctx.held == []
