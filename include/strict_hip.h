@@ -508,11 +508,12 @@ typedef struct sh_paged_kv {
  * normalised per head, x / sqrt(mean(x^2) + eps) * gain (gains fp32, head_dim
  * values), then rotated by halves at the token's position, angle = position *
  * theta^(-2i / head_dim) in fp64 (theta 1 or more; less where max_pages * page_size,
- * and tokens, times theta^(-(head_dim - 2) / head_dim) are at most 2^29); q to q[tokens][heads][head_dim], k and v (as
- * it is) to their pages. fp16 or bf16, rounded once. A token before position 0
- * is rotated by its negative position and not stored. head_dim 64 or 128; qkv
- * and q 16-byte aligned, ld a multiple of 8; q and the pages overlap nothing else of
- * the call. Two tokens of one page row (a page in two tables) leave either's values. */
+ * and tokens, times theta^(-(head_dim - 2) / head_dim) are at most 2^29); q to
+ * q[tokens][heads][head_dim], k and v (as it is) to their pages. fp16 or bf16,
+ * rounded once. A token before position 0 is rotated by its negative position and
+ * not stored. head_dim 64 or 128; qkv and q 16-byte aligned, ld a multiple of 8; q
+ * and the pages overlap nothing else of the call. Two tokens of one page row (a page
+ * in two tables) leave either's values. */
 SH_API int sh_qk_norm_rope_paged_f16(sh_ctx *ctx, const sh_paged_kv *kv, const uint16_t *qkv,
                                      const float *q_gain, const float *k_gain, uint16_t *q,
                                      int tokens, int heads, int ld, float eps, float theta);
@@ -528,13 +529,15 @@ SH_API int sh_qk_norm_rope_paged_bf16(sh_ctx *ctx, const sh_paged_kv *kv, const 
  * (window 0: all). A row that sees nothing gets zeros; what stands in places
  * that a row does not see, NaN and infinities included, does not reach it; a
  * q . k of -infinity (or below -2^108) has no weight, one of +infinity makes the row
- * NaN; with the scale, products may leave fp32's range. q, out [tokens][heads][head_dim] in the
- * cache's type, 16-byte aligned; fp32 scores, softmax and sums, the weights rounded
- * to the type before the sums. head_dim 64 or 128, heads / kv_heads <= 128,
- * 0 < scale <= 2^127. max_new: the most new tokens of any sequence; the kernel and
- * the work buffer are chosen by it, more are computed as well. The work buffer
- * (16-byte aligned) holds at least what sh_attn_paged_workspace says for the same
- * sizes. It and out overlap nothing else of the call. */
+ * NaN; with the scale, products may leave fp32's range. Rows with scores of 2^24
+ * (bf16 2^30) and more, or with values that are not finite, take some hundred times
+ * as long. q, out [tokens][heads][head_dim] in the cache's type, 16-byte aligned;
+ * fp32 scores, softmax and sums, the weights rounded to the type before the sums.
+ * head_dim 64 or 128, heads / kv_heads <= 128, 0 < scale <= 2^127. max_new: the most
+ * new tokens of any sequence; the kernel and the work buffer are chosen by it, more
+ * are computed as well. The work buffer (16-byte aligned) holds at least what
+ * sh_attn_paged_workspace says for the same sizes. It and out overlap nothing else
+ * of the call. */
 SH_API int sh_attn_paged_workspace(const sh_paged_kv *kv, int tokens, int heads, int max_new,
                                    size_t *bytes);
 SH_API int sh_attn_paged_f16(sh_ctx *ctx, const sh_paged_kv *kv, const uint16_t *q, uint16_t *out,

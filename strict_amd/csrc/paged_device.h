@@ -51,7 +51,7 @@ struct PagedBf16 {
   static __device__ __forceinline__ f32x16 mfma32(Vec a, Vec b, f32x16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
   }
-  // (each step off by up to 2^-23 of the sum, toward zero)
+  // (a step may be off by 2^-23 of the sum)
   static __device__ __forceinline__ float sum8(Vec v, float sum) {
     typedef __bf16 Pair __attribute__((ext_vector_type(2)));
     const Pair one = {(__bf16)1.0f, (__bf16)1.0f};

@@ -133,3 +133,19 @@ def test_values_that_are_all_alike(ctx, dtype, new, lengths, d):
     _, got = paged.run_attention(c, q=paged.to16(q, dtype), scale=1.0)
     n = sum(new)
     assert (got[:n] == value[:, 0].repeat(8, 0)).all()
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("new,lengths", [([1], [20000]), ([40], [20000])])
+@pytest.mark.parametrize("above", [4.0, 10.0, 16.0])
+def test_many_small_weights(ctx, dtype, new, lengths, above):
+    # one position far above the others, whose weights (in fp16 below the normal range) carry the values
+    c = paged.Case(ctx, 8, dtype, new, lengths, 4, 2, 64, 16)
+    k, v = np.zeros(c.k.shape), np.ones(c.v.shape)
+    at = c.table[0, 9000 // 16], 9000 % 16
+    k[at[0], :, at[1], 0] = above
+    v[at[0], :, at[1]] = 0
+    c.k[:], c.v[:] = paged.to16(k, dtype), paged.to16(v, dtype)
+    q = np.zeros((c.tokens, 4, 64))
+    q[..., 0] = 1
+    paged.check_attention(c, q=paged.to16(q, dtype), scale=1.0)
