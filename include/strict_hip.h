@@ -547,6 +547,55 @@ SH_API int sh_attn_paged_bf16(sh_ctx *ctx, const sh_paged_kv *kv, const uint16_t
                               int tokens, int heads, int max_new, int window, int sinks,
                               float scale, void *workspace, size_t workspace_bytes);
 
+/* The same cache in 8 bits: a page of sh_paged8_page_bytes bytes holds its rows of k
+ * [kv_heads][page_size][head_dim] and of v alike as OCP E4M3 bytes, then a scale byte
+ * for each row, [2][kv_heads][page_size] (k, v): a byte stands for its value times
+ * 2^(scale - 127), of scale 255 for NaN. Sizes as above; sh_pages_copy copies such pages. */
+typedef struct sh_paged_kv8 {
+  uint8_t *pages; /* [num_pages] of sh_paged8_page_bytes, 16-byte aligned */
+  const int32_t *page_table; /* [batch][max_pages] */
+  const int32_t *lengths;    /* [batch] */
+  const int32_t *starts;     /* [batch + 1] */
+  int batch, max_pages, num_pages, page_size, kv_heads, head_dim;
+} sh_paged_kv8;
+
+/* Bytes of a page (a multiple of 32); only the sizes of `kv` are read. */
+SH_API int sh_paged8_page_bytes(const sh_paged_kv8 *kv, size_t *bytes);
+
+/* sh_qk_norm_rope_paged_* into such pages (the same q). A row of k or v is stored with
+ * the smallest scale 2^e, e >= -127, for which its largest value is at most 448 * 2^e,
+ * each value rounded once, to the nearest E4M3 (half way: to the even one); k is worked
+ * out in fp64 until then, to 2^-36 of its row's size. Values beyond 1.875 * 2^15 (bf16
+ * 2^127), which the type of q does not hold, count as that; infinities and NaN are
+ * stored as NaN and leave the rest of their row as it would be. Two tokens of one page
+ * row (a page in two tables) leave values of no meaning there. */
+SH_API int sh_qk_norm_rope_paged8_f16(sh_ctx *ctx, const sh_paged_kv8 *kv, const uint16_t *qkv,
+                                      const float *q_gain, const float *k_gain, uint16_t *q,
+                                      int tokens, int heads, int ld, float eps, float theta);
+SH_API int sh_qk_norm_rope_paged8_bf16(sh_ctx *ctx, const sh_paged_kv8 *kv, const uint16_t *qkv,
+                                       const float *q_gain, const float *k_gain, uint16_t *q,
+                                       int tokens, int heads, int ld, float eps, float theta);
+
+/* The rows of the call's new tokens read back: k, v [tokens][kv_heads][head_dim], the
+ * values that the pages' bytes stand for in fp16 or bf16 (rounded where they leave its
+ * range). Rows of no sequence, and of positions below 0 or without a page, are left as
+ * they are. k and v 16-byte aligned; they overlap nothing else of the call. */
+SH_API int sh_paged8_read_f16(sh_ctx *ctx, const sh_paged_kv8 *kv, uint16_t *k, uint16_t *v,
+                              int tokens);
+SH_API int sh_paged8_read_bf16(sh_ctx *ctx, const sh_paged_kv8 *kv, uint16_t *k, uint16_t *v,
+                               int tokens);
+
+/* sh_attn_paged_* over such pages, with k and v as sh_paged8_read_* gives them. Scores,
+ * weights, sums and what a row sees are as there, and so are the arguments. */
+SH_API int sh_attn_paged8_workspace(const sh_paged_kv8 *kv, int tokens, int heads, int max_new,
+                                    size_t *bytes);
+SH_API int sh_attn_paged8_f16(sh_ctx *ctx, const sh_paged_kv8 *kv, const uint16_t *q,
+                              uint16_t *out, int tokens, int heads, int max_new, int window,
+                              int sinks, float scale, void *workspace, size_t workspace_bytes);
+SH_API int sh_attn_paged8_bf16(sh_ctx *ctx, const sh_paged_kv8 *kv, const uint16_t *q,
+                               uint16_t *out, int tokens, int heads, int max_new, int window,
+                               int sinks, float scale, void *workspace, size_t workspace_bytes);
+
 /* Pages src[i] to pages dst[i], i < count, in each of `planes` pools (the K and V
  * pools of every layer) at pool + p * plane_stride bytes, num_pages pages of
  * page_bytes each. src and dst are device int32; a pair with a number outside

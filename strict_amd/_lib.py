@@ -109,6 +109,11 @@ class PagedKv(ctypes.Structure):
     ]
 
 
+class PagedKv8(ctypes.Structure):
+    """sh_paged_kv8: the same in pages of 8-bit values."""
+    _fields_ = [("pages", ctypes.c_void_p)] + PagedKv._fields_[2:]
+
+
 _P = ctypes.c_void_p
 _PP = ctypes.POINTER(ctypes.c_void_p)
 _I = ctypes.c_int
@@ -200,6 +205,14 @@ SIGNATURES = {
     "sh_attn_paged_workspace": (_I, [_P, _I, _I, _I, ctypes.POINTER(_SZ)]),
     "sh_attn_paged_f16": (_I, [_P, _P, _P, _P, _I, _I, _I, _I, _I, _F, _P, _SZ]),
     "sh_attn_paged_bf16": (_I, [_P, _P, _P, _P, _I, _I, _I, _I, _I, _F, _P, _SZ]),
+    "sh_paged8_page_bytes": (_I, [_P, ctypes.POINTER(_SZ)]),
+    "sh_qk_norm_rope_paged8_f16": (_I, [_P, _P, _P, _P, _P, _P, _I, _I, _I, _F, _F]),
+    "sh_qk_norm_rope_paged8_bf16": (_I, [_P, _P, _P, _P, _P, _P, _I, _I, _I, _F, _F]),
+    "sh_paged8_read_f16": (_I, [_P, _P, _P, _P, _I]),
+    "sh_paged8_read_bf16": (_I, [_P, _P, _P, _P, _I]),
+    "sh_attn_paged8_workspace": (_I, [_P, _I, _I, _I, ctypes.POINTER(_SZ)]),
+    "sh_attn_paged8_f16": (_I, [_P, _P, _P, _P, _I, _I, _I, _I, _I, _F, _P, _SZ]),
+    "sh_attn_paged8_bf16": (_I, [_P, _P, _P, _P, _I, _I, _I, _I, _I, _F, _P, _SZ]),
     "sh_pages_copy": (_I, [_P, _P, _I, _SZ, _I, _SZ, _P, _P, _I]),
     "sh_sample_workspace": (_I, [_I, _I, ctypes.POINTER(_SZ)]),
     "sh_sample_f32": (_I, [_P, _P, _I, _I, _I, _P, _P, _P, _P, _P, _P, _P, _SZ]),

@@ -349,6 +349,24 @@ inline size_t paged_pool_bytes(const sh_paged_kv *kv) {
   return (size_t)kv->num_pages * kv->kv_heads * kv->page_size * kv->head_dim * 2;
 }
 
+// ---- pages of 8-bit values ------------------------------------------------------------
+//
+// A page: k [kv_heads][page_size][head_dim], v alike, then their scales
+// [2][kv_heads][page_size], a byte each, so that a copy of a page takes all of it. A
+// multiple of 32 bytes, as page_size is one of 16.
+inline size_t paged8_page_bytes(const sh_paged_kv8 *kv) {
+  return (size_t)kv->kv_heads * kv->page_size * 2 * ((size_t)kv->head_dim + 1);
+}
+// (Of sizes that check_paged_sizes takes: at most 1 + 1 / head_dim times 2^62 bytes.)
+inline size_t paged8_pool_bytes(const sh_paged_kv8 *kv) { return (size_t)kv->num_pages * paged8_page_bytes(kv); }
+
+// The cache's sizes and index tensors as those of one of 16-bit values without pools.
+inline sh_paged_kv paged8_index(const sh_paged_kv8 *kv) {
+  sh_paged_kv i = {nullptr,   nullptr,       kv->page_table, kv->lengths,   kv->starts,  kv->batch,
+                   kv->max_pages, kv->num_pages, kv->page_size,  kv->kv_heads, kv->head_dim};
+  return i;
+}
+
 // The same of sh_pages_copy.
 inline const char *check_pages_copy(int planes, size_t plane_stride, int num_pages, size_t page_bytes,
                                     int count) {

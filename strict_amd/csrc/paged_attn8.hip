@@ -1,0 +1,640 @@
+// Attention of new tokens over a KV cache in pages of 8-bit values (sh_attn_paged8_*): the
+// kernels that read such pages. How a call is divided, the merge and the tiles that
+// matrix products cannot do are those of 16-bit pages (paged_attn.h).
+//
+// A byte times its row's power of two is a value of the 16-bit type but for that type's
+// range, so the products, the softmax and their roundings are the same; only half the
+// bytes are read.
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+#include <cmath>
+
+#include "common.h"
+#include "paged.h"
+#include "paged_attn.h"
+#include "paged_device.h"
+
+namespace sh {
+namespace {
+
+struct Attn8Args : PagedAttnArgs {
+  const uint8_t *pages;
+  size_t page_bytes, v_at, v_scale_at;  // of a page: its bytes, the first row of V, the scales of V after those of K
+};
+
+// Pages of 8-bit values as attn_exact reads them.
+template <class T>
+struct Pages8 {
+  typedef T Type;
+  typedef Attn8Args Args;
+  struct Row {
+    long long at;  // of the row of K
+    float k_scale, v_scale;
+  };
+  template <int kD>
+  static __device__ __forceinline__ Row row(const Args &a, int page, int kv_head, int in_page) {
+    const size_t first = (size_t)page * a.page_bytes, r = ((size_t)kv_head << a.page_shift) + in_page;
+    const uint8_t *scale = a.pages + first + 2 * a.v_at + r;
+    return Row{(long long)(first + r * kD), e8m0_scale(scale[0]), e8m0_scale(scale[a.v_scale_at])};
+  }
+  static __device__ __forceinline__ Row row_of_lane(Row r, int lane) {
+    return Row{__shfl(r.at, lane, 64), __shfl(r.k_scale, lane, 64), __shfl(r.v_scale, lane, 64)};
+  }
+  static __device__ __forceinline__ float value(uint32_t byte, float scale) {
+    return (float)__builtin_bit_cast(typename T::Pair, from_e4m3<T>(byte, scale).x)[0];
+  }
+  static __device__ __forceinline__ float k(const Args &a, Row r, int c) { return value(a.pages[r.at + c], r.k_scale); }
+  static __device__ __forceinline__ float v(const Args &a, Row r, int c) {
+    return value(a.pages[r.at + (long long)a.v_at + c], r.v_scale);
+  }
+};
+
+// ---- tiles of up to 16 rows ------------------------------------------------------------
+//
+// As the kernel of 16-bit pages (paged_attn.hip), bound by the bytes of K and V: each
+// wave takes units of 64 positions (128 at head_dim 64) by itself, twice as many as there
+// for the same bytes in flight. What differs is how the values come to the products:
+//  - K fragments straight from memory, 16 bytes of position lane % 16 per lane, which are
+//    those of two products (of the 64 dims that four lanes hold, each product takes the
+//    8 of each lane's half: q is read in the same order);
+//  - V as 16-bit values to LDS rows, where a lane's 16 bytes have one scale.
+// Both are converted with their scale in one instruction for two values.
+template <int kD>
+constexpr int kSmallUnit8 = 64 * 128 / kD;
+
+template <class T, int kD>
+struct SmallLds8 {
+  union {
+    uint8_t v[4][kSmallUnit8<kD> * kD * 2];
+    float acc[4][kSmall.rows][kD];
+  };
+  float stat[4][kSmall.rows][2];
+};
+
+template <class T, int kD>
+__device__ __forceinline__ bool attn_small8(const Attn8Args &a, const PagedTile &t, const TileSpan &s, int u0,
+                                           int u1, int slot, SmallLds8<T, kD> &lds) {
+  typedef typename T::Vec Vec;
+  typedef typename T::Value Value;
+  constexpr int kUnit = kSmallUnit8<kD>, kBlocks = kUnit / 16, kKL = kD / 64, kDT = kD / 16;
+  constexpr int kRow = kD * 2, kChunks = kD / 16, kVLoads = kUnit * kChunks / 64, kVRows = 64 / kChunks;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int r16 = lane & 15, grp = lane >> 4, rows = s.count * a.group;
+  const int row = min(r16, rows - 1), my_pos = s.pos0 + token_of(a, row);
+  const uint16_t *qp = a.q + head_row(a, t.seq.row0 + s.first, t.kv_head, row) * kD + grp * 16;
+  const int *table = a.table + (size_t)t.b * a.max_pages;
+  const int last_pos = s.pos0 + s.count - 1, page_mask = (1 << a.page_shift) - 1;
+  Vec q[2 * kKL];
+#pragma unroll
+  for (int kk = 0; kk < 2 * kKL; kk++) q[kk] = *reinterpret_cast<const Vec *>(qp + 64 * (kk / 2) + 8 * (kk % 2));
+
+  // the table entry of block lane % kBlocks of unit j
+  auto entry = [&](int j) __attribute__((always_inline)) {
+    const int p = span_position(s, kUnit, min(j, u1 - 1)) + 16 * (lane % kBlocks);
+    return table[min(p >> a.page_shift, a.max_pages - 1)];
+  };
+  u32x4 kr[kBlocks][kKL], vr[kVLoads];
+  uint32_t ks[kBlocks], vs[kVLoads];  // the scales of the lane's rows
+  size_t base[kBlocks], scales[kBlocks];  // of the blocks' first rows of K; bad: no page
+  auto place = [&](int j, int entries, unsigned *bad) __attribute__((always_inline)) {
+    const int p = span_position(s, kUnit, j);
+    *bad = 0;
+#pragma unroll
+    for (int tt = 0; tt < kBlocks; tt++) {
+      const int page = paged_page(__builtin_amdgcn_readlane(entries, tt), a.num_pages);
+      if (page < 0) *bad |= 1u << tt;
+      const size_t at = (size_t)max(page, 0) * a.page_bytes;
+      const size_t row = ((size_t)t.kv_head << a.page_shift) + ((p + 16 * tt) & page_mask);
+      base[tt] = at + row * kD;
+      scales[tt] = at + 2 * a.v_at + row;
+    }
+  };
+  auto load_k = [&]() __attribute__((always_inline)) {
+#pragma unroll
+    for (int tt = 0; tt < kBlocks; tt++) {
+#pragma unroll
+      for (int c = 0; c < kKL; c++)
+        kr[tt][c] = *reinterpret_cast<const u32x4 *>(a.pages + base[tt] + (r16 * kD + grp * 16 + 64 * c));
+      ks[tt] = a.pages[scales[tt] + r16];
+    }
+  };
+  auto load_v = [&]() __attribute__((always_inline)) {
+#pragma unroll
+    for (int u = 0; u < kVLoads; u++) {
+      const int block = u * kVRows / 16, r = u * kVRows % 16 + lane / kChunks;
+      vr[u] = __builtin_nontemporal_load(
+          reinterpret_cast<const u32x4 *>(a.pages + (base[block] + a.v_at) + (r * kD + (lane % kChunks) * 16)));
+      vs[u] = a.pages[scales[block] + a.v_scale_at + r];
+    }
+  };
+
+  float m_run = -INFINITY, l_run = 0.0f;
+  f32x4 acc[kDT];
+#pragma unroll
+  for (int dt = 0; dt < kDT; dt++) acc[dt] = f32x4{0.f, 0.f, 0.f, 0.f};
+  uint8_t *vl = lds.v[wave];
+  // chunk c of row r lies at c ^ f(r): a transposing read's 32 lanes (8 rows, 2
+  // chunks each) then hit 64 banks, and so do 16 lanes that write every other chunk
+  auto swz = [](int r) { return kD == 128 ? 2 * (r & 7) + (r & 1) : 2 * ((r >> 1) & 3) + ((r >> 1) & 1); };
+  const int ti = (lane >> 2) & 3, tq = lane & 3;
+  int v_at[kDT];  // (f repeats every 8 rows)
+  const int v_row = lane / kChunks, v_to = v_row * kRow + (((2 * (lane % kChunks)) ^ swz(v_row)) * 16);
+#pragma unroll
+  for (int dt = 0; dt < kDT; dt++) {
+    const int r = 4 * grp + ti;
+    v_at[dt] = r * kRow + (((2 * dt + (tq >> 1)) ^ swz(r)) * 16) + (tq & 1) * 8;
+  }
+  auto unit = [&](int j, unsigned bad, unsigned *next_bad, int *entries) __attribute__((always_inline)) {
+    const int p0 = span_position(s, kUnit, j), next = j + 4;
+    f32x4 sc[kBlocks];
+#pragma unroll
+    for (int tt = 0; tt < kBlocks; tt++) sc[tt] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int c = 0; c < kKL; c++)
+#pragma unroll
+      for (int half = 0; half < 2; half++)
+#pragma unroll
+        for (int tt = 0; tt < kBlocks; tt++) {
+          const u32x4 kf = from_e4m3<T>(kr[tt][c][2 * half], kr[tt][c][2 * half + 1], e8m0_scale(ks[tt]));
+          sc[tt] = T::mfma16(__builtin_bit_cast(Vec, kf), q[2 * c + half], sc[tt]);
+        }
+    if (next < u1) {
+      place(next, *entries, next_bad);
+      __builtin_amdgcn_sched_barrier(0);
+      load_k();
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    // every row sees every position
+    const bool plain = bad == 0 && p0 + kUnit <= s.pos0 + 1 &&
+                       (a.plan.window == 0 || p0 > last_pos - a.plan.window || p0 + kUnit <= s.sinks);
+    // V to this wave's LDS rows (LDS works in order: after the last unit's reads);
+    // what no row sees as zeros
+    if (!plain) {
+#pragma unroll
+      for (int u = 0; u < kVLoads; u++)
+        if (((bad >> (u * kVRows / 16)) & 1) || !tile_sees(a, s, p0 + u * kVRows + lane / kChunks)) {
+          vr[u] = u32x4{0, 0, 0, 0};
+          vs[u] = 0;
+        }
+    }
+#pragma unroll
+    for (int u = 0; u < kVLoads; u++) {
+      const float scale = e8m0_scale(vs[u]);
+      uint8_t *to = vl + u * kVRows * kRow;
+      *reinterpret_cast<u32x4 *>(to + v_to) = from_e4m3<T>(vr[u].x, vr[u].y, scale);
+      *reinterpret_cast<u32x4 *>(to + (v_to ^ 16)) = from_e4m3<T>(vr[u].z, vr[u].w, scale);
+    }
+    if (next < u1) {
+      __builtin_amdgcn_sched_barrier(0);
+      load_v();
+      *entries = entry(next + 4);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    float mx = -INFINITY;
+    if (!plain) {
+      const Sees seen(a, s, my_pos, p0 + 4 * grp);
+#pragma unroll
+      for (int tt = 0; tt < kBlocks; tt++)
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+          if (((bad >> tt) & 1) || !seen(16 * tt + e)) sc[tt][e] = -INFINITY;
+    }
+#pragma unroll
+    for (int tt = 0; tt < kBlocks; tt++)
+#pragma unroll
+      for (int e = 0; e < 4; e++) mx = fmaxf(mx, sc[tt][e]);
+    mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
+    mx = fmaxf(mx, __shfl_xor(mx, 32, 64)) * a.scale_log2;
+    const float m = fmaxf(m_run, mx);
+    const float corr = m_run == m ? 1.0f : exp2_weight(m_run - m);
+    m_run = m;
+    // (a row that has seen nothing yet: its weights are exp2(-infinity))
+    const float off = (m == -INFINITY ? 0.0f : m) - T::kWeightLog2;
+    float ls = 0.0f;
+    Vec p[kBlocks / 2];
+#pragma unroll
+    for (int tt = 0; tt < kBlocks; tt++)
+#pragma unroll
+      for (int e = 0; e < 4; e++) {
+        p[tt / 2][(tt & 1) * 4 + e] = (Value)exp2_weight(fmaf(sc[tt][e], a.scale_log2, -off));
+      }
+#pragma unroll
+    for (int i = 0; i < kBlocks / 2; i++) ls = T::sum8(p[i], ls);
+    l_run = l_run * corr + ls;  // this lane's positions; the groups are summed at the end
+#pragma unroll
+    for (int dt = 0; dt < kDT; dt++)
+#pragma unroll
+      for (int e = 0; e < 4; e++) acc[dt][e] *= corr;
+    wait_lds();  // this wave's V rows are in LDS
+#pragma unroll
+    for (int sl = 0; sl < kBlocks / 2; sl++)
+#pragma unroll
+      for (int dt = 0; dt < kDT; dt++) {
+        s16x4 half[2];
+#pragma unroll
+        for (int q2 = 0; q2 < 2; q2++)
+          half[q2] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+              (SH_PAGED_LDS s16x4 *)((SH_PAGED_LDS uint8_t *)vl + v_at[dt] + (32 * sl + 16 * q2) * kRow));
+        const Vec vf = __builtin_bit_cast(Vec, __builtin_shufflevector(half[0], half[1], 0, 1, 2, 3, 4, 5, 6, 7));
+        acc[dt] = T::mfma16(vf, p[sl], acc[dt]);
+      }
+    __atomic_signal_fence(__ATOMIC_SEQ_CST);
+  };
+  if (u0 + wave < u1) {
+    unsigned bad = 0, next_bad = 0;
+    int entries = entry(u0 + wave);
+    place(u0 + wave, entries, &bad);
+    load_k();
+    load_v();
+    entries = entry(u0 + wave + 4);
+    for (int j = u0 + wave; j < u1; j += 4) {
+      unit(j, bad, &next_bad, &entries);
+      bad = next_bad;
+    }
+  }
+  l_run += __shfl_xor(l_run, 16, 64);
+  l_run += __shfl_xor(l_run, 32, 64);
+  if (grp == 0) {
+    lds.stat[wave][r16][0] = m_run;
+    lds.stat[wave][r16][1] = l_run;
+  }
+  lds_barrier();  // every wave's V reads are done: lds.v becomes lds.acc
+  if (r16 < rows) {
+#pragma unroll
+    for (int dt = 0; dt < kDT; dt++) *reinterpret_cast<f32x4 *>(&lds.acc[wave][r16][16 * dt + 4 * grp]) = acc[dt];
+  }
+  lds_barrier();
+  bool sound = true;
+  for (int i = tid; i < rows * kD; i += kT) {
+    const int r = i / kD, dim = i % kD;
+    float m = lds.stat[0][r][0];
+#pragma unroll
+    for (int w = 1; w < 4; w++) m = fmaxf(m, lds.stat[w][r][0]);
+    float sum = 0.0f, l = 0.0f;
+#pragma unroll
+    for (int w = 0; w < 4; w++) {
+      const float f = lds.stat[w][r][0] == m ? 1.0f : exp2_weight(lds.stat[w][r][0] - m);
+      sum = fmaf(f, lds.acc[w][r][dim], sum);
+      l = fmaf(f, lds.stat[w][r][1], l);
+    }
+    sound = sound && score_fits<T>(a, m) && sum_fits(sum) && l < INFINITY;
+    store_value<T, kD>(a, t, s, slot, r, dim, sum, l);
+    if (slot >= 0 && dim == 0) {
+      slot_stats<kD>(a, slot, r)[0] = m;
+      slot_stats<kD>(a, slot, r)[1] = l;
+    }
+  }
+  return !__syncthreads_or(sound ? 0 : 1);
+}
+
+template <class T, int kD>
+__global__ __launch_bounds__(kT, kSmall.workers / 256) void paged8_small_kernel(const Attn8Args a) {
+  __shared__ __attribute__((aligned(16))) SmallLds8<T, kD> lds;
+  __shared__ PlanLds plan;
+  work_piece<false, 1, 1>(a, plan, [&](const PieceStep &st, Line) { return attn_small8<T, kD>(a, st.tile, st.span, st.u0, st.u1, st.slot, lds); });
+}
+
+// ---- tiles of up to 128 rows ------------------------------------------------------------
+//
+// As the kernel of 16-bit pages (paged_attn.hip): four waves of 32 rows share K and V units
+// of 64 positions in LDS, double-buffered, a barrier per unit. Here a wave's 16 positions of
+// a unit go through its registers: requested a unit ahead, converted to 16 bits among the
+// next unit's products of scores (each value once, where fragments of bytes would be
+// converted by all four waves) and written to the other buffer.
+constexpr float kSlack = 8.0f;
+
+template <int kD>
+struct LargeLds8 {
+  uint8_t k[2][kLargeUnit * kD * 2], v[2][kLargeUnit * kD * 2];
+  __attribute__((aligned(16))) unsigned bad[2][4];  // a 16-position block without a page
+};
+
+template <class T, int kD>
+__device__ __forceinline__ bool attn_large8(const Attn8Args &a, const PagedTile &t, const TileSpan &s, int u0,
+                                           int u1, int slot, LargeLds8<kD> &lds) {
+  typedef typename T::Vec Vec;
+  typedef typename T::Value Value;
+  typedef Value Quad __attribute__((ext_vector_type(4)));
+  constexpr int kRow = kD * 2, kChunks = kD / 16, kKK = kD / 16, kDB = kD / 32;
+  constexpr int kLoadRows = 64 / kChunks, kLoads = 16 / kLoadRows;  // of a wave's 16 positions
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int n32 = lane & 31, h = lane >> 5, rows = s.count * a.group;
+  const bool active = 32 * wave < rows;  // (of the wave)
+  const int row = min(32 * wave + n32, rows - 1), my_pos = s.pos0 + token_of(a, row);
+  const int pos_lo = s.pos0 + token_of(a, min(32 * wave, rows - 1));
+  const int pos_hi = s.pos0 + token_of(a, min(32 * wave + 31, rows - 1));
+  const int *table = a.table + (size_t)t.b * a.max_pages;
+  const int page_mask = (1 << a.page_shift) - 1;
+  const uint16_t *qp = a.q + head_row(a, t.seq.row0 + s.first, t.kv_head, row) * kD + h * 8;
+  Vec q[kKK];
+#pragma unroll
+  for (int kk = 0; kk < kKK; kk++) q[kk] = *reinterpret_cast<const Vec *>(qp + 16 * kk);
+
+  // chunk c of row r lies at c ^ f(r): 16 lanes that read one chunk of 16 rows of K
+  // hit all banks, 32 lanes of a transposing read of V (4 rows, 4 chunks each), and 16
+  // that write every other chunk
+  auto swz_k = [](int r) { return kD == 128 ? r & 15 : (r >> 1) & 7; };
+  auto swz_v = [](int r) { return kD == 128 ? 4 * (r & 3) + (r & 1) : 4 * ((r >> 1) & 1) + ((r >> 1) & 1); };
+  const int load_row = lane / kChunks, load_chunk = lane % kChunks;
+  constexpr uint32_t kBuffer = kLargeUnit * kD * 2, kWave = 16 * kRow;
+  // the table entry of this wave's 16 positions of unit j
+  auto entry = [&](int j) __attribute__((always_inline)) {
+    const int p = span_position(s, kLargeUnit, min(j, u1 - 1)) + 16 * wave;
+    return table[min(p >> a.page_shift, a.max_pages - 1)];
+  };
+  // this wave's 16 rows of K and V of unit j, requested; whether there is no page
+  u32x4 kr[kLoads], vr[kLoads];
+  uint32_t ks[kLoads], vs[kLoads];
+  bool none = false;
+  auto request = [&](int j, int e) __attribute__((always_inline)) {
+    const int p = span_position(s, kLargeUnit, j) + 16 * wave;
+    const int page = paged_page(__builtin_amdgcn_readfirstlane(e), a.num_pages);
+    none = page < 0;
+    const size_t row = ((size_t)t.kv_head << a.page_shift) + (p & page_mask);
+    const uint8_t *from = a.pages + (size_t)max(page, 0) * a.page_bytes;
+    const uint8_t *rows = from + row * kD, *scales = from + 2 * a.v_at + row;
+#pragma unroll
+    for (int u = 0; u < kLoads; u++) {
+      kr[u] = *reinterpret_cast<const u32x4 *>(rows + (u * 1024 + lane * 16));
+      vr[u] = *reinterpret_cast<const u32x4 *>(rows + a.v_at + (u * 1024 + lane * 16));
+      ks[u] = scales[u * kLoadRows + load_row];
+      vs[u] = scales[a.v_scale_at + u * kLoadRows + load_row];
+    }
+  };
+  // load u of what was requested for unit j to buffer j & 1; what no row sees is zeros
+  // in V (of K, such scores are masked)
+  auto keep_k = [&](int j, int u) __attribute__((always_inline)) {
+    const int r = u * kLoadRows + load_row, at = wave * kWave + r * kRow + (((2 * load_chunk) ^ swz_k(r)) * 16);
+    const float scale = e8m0_scale(ks[u]);
+    *reinterpret_cast<u32x4 *>(lds.k[j & 1] + at) = from_e4m3<T>(kr[u].x, kr[u].y, scale);
+    *reinterpret_cast<u32x4 *>(lds.k[j & 1] + (at ^ 16)) = from_e4m3<T>(kr[u].z, kr[u].w, scale);
+  };
+  auto keep_v = [&](int j, int u) __attribute__((always_inline)) {
+    const int r = u * kLoadRows + load_row, at = wave * kWave + r * kRow + (((2 * load_chunk) ^ swz_v(r)) * 16);
+    const float scale = e8m0_scale(vs[u]);
+    *reinterpret_cast<u32x4 *>(lds.v[j & 1] + at) = from_e4m3<T>(vr[u].x, vr[u].y, scale);
+    *reinterpret_cast<u32x4 *>(lds.v[j & 1] + (at ^ 16)) = from_e4m3<T>(vr[u].z, vr[u].w, scale);
+  };
+  auto blank = [&](int j) __attribute__((always_inline)) {
+    const int p = span_position(s, kLargeUnit, j) + 16 * wave;
+    if (lane == 0) lds.bad[j & 1][wave] = none ? 1 : 0;
+    if (none || p + 16 > s.hi || (a.plan.window > 0 && p < s.lo && p + 16 > s.sinks)) {
+#pragma unroll
+      for (int u = 0; u < kLoads; u++) {
+        if (none || !tile_sees(a, s, p + u * kLoadRows + load_row)) {
+          vr[u] = u32x4{0, 0, 0, 0};
+          vs[u] = 0;
+        }
+      }
+    }
+  };
+  auto keep = [&](int j) __attribute__((always_inline)) {
+    blank(j);
+#pragma unroll
+    for (int u = 0; u < kLoads; u++) {
+      keep_k(j, u);
+      keep_v(j, u);
+    }
+  };
+
+  float m_run = -INFINITY, l_run = 0.0f;
+  f32x16 acc[kDB];
+#pragma unroll
+  for (int db = 0; db < kDB; db++)
+#pragma unroll
+    for (int i = 0; i < 16; i++) acc[db][i] = 0.0f;
+
+  __syncthreads();  // the last tile's LDS reads are done
+  int entries = 0;
+  if (u0 < u1) {
+    request(u0, entry(u0));
+    entries = entry(u0 + 1);
+    keep(u0);
+    if (u0 + 1 < u1) request(u0 + 1, entries);
+    entries = entry(u0 + 2);
+  }
+  const int ti = (lane >> 2) & 3, tq = lane & 3, side = (lane >> 4) & 1;
+  const int v_at0 = (4 * h + ti) * kRow + (((2 * side + (tq >> 1)) ^ swz_v(4 * h + ti)) * 16) + (tq & 1) * 8;
+  const int k_at0 = n32 * kRow + ((h ^ swz_k(n32)) * 16);
+  if (!active) {  // a wave without rows loads its part
+    for (int j = u0; j < u1; j++) {
+      lds_barrier();
+      if (j + 1 < u1) keep(j + 1);
+      if (j + 2 < u1) request(j + 2, entries);
+      entries = entry(j + 3);
+    }
+  }
+  for (int j = active ? u0 : u1; j < u1; j++) {
+    const int p0 = span_position(s, kLargeUnit, j), buf = j & 1, next = min(j + 1, u1 - 1);
+    lds_barrier();
+    if (j + 1 < u1) blank(next);
+    // Fragments are requested ahead of the products that take them (the compiler left
+    // to itself reads each just before its use), and the next unit's values converted
+    // and written among the products of the scores. (Of the last unit, what there is once
+    // more, to the buffer that nobody reads.)
+    Vec kf[2][kKK];
+    s16x4 vh[4][kDB][2];
+    const int k_at = k_at0 + buf * (int)kBuffer, v_at = v_at0 + buf * (int)kBuffer;
+    auto read_v = [&](int ks) __attribute__((always_inline)) {
+#pragma unroll
+      for (int db = 0; db < kDB; db++)
+#pragma unroll
+        for (int q2 = 0; q2 < 2; q2++)
+          vh[ks][db][q2] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+              (SH_PAGED_LDS s16x4 *)((SH_PAGED_LDS uint8_t *)lds.v[0] + (v_at ^ (64 * db)) + (16 * ks + 8 * q2) * kRow));
+    };
+    auto read_k = [&](int kk) __attribute__((always_inline)) {
+#pragma unroll
+      for (int sb = 0; sb < 2; sb++)
+        kf[sb][kk] = *reinterpret_cast<const Vec *>(lds.k[0] + (k_at ^ (32 * kk)) + 32 * sb * kRow);
+    };
+    constexpr int kAhead = 4;
+#pragma unroll
+    for (int kk = 0; kk < kAhead; kk++) read_k(kk);
+    const u32x4 bad4 = *reinterpret_cast<const u32x4 *>(lds.bad[buf]);
+    __builtin_amdgcn_sched_barrier(0);
+    f32x16 sc[2];
+#pragma unroll
+    for (int sb = 0; sb < 2; sb++)
+#pragma unroll
+      for (int i = 0; i < 16; i++) sc[sb][i] = 0.0f;
+#pragma unroll
+    for (int kk = 0; kk < kKK; kk++) {
+#pragma unroll
+      for (int sb = 0; sb < 2; sb++) sc[sb] = T::mfma32(kf[sb][kk], q[kk], sc[sb]);
+      __builtin_amdgcn_sched_barrier(0);
+      if (kk + kAhead < kKK) read_k(kk + kAhead);
+      if (kk % 4 == 1) keep_k(j + 1, kk / 4);
+      if (kk % 4 == 3) keep_v(j + 1, kk / 4);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    static_assert(kLoads == kKK / 4, "a load of K or V every other step");
+    if (j + 2 < u1) request(j + 2, entries);
+    entries = entry(j + 3);
+    // (a wave in its softmax before one in its products, which take turns)
+    __builtin_amdgcn_s_setprio(1);
+    read_v(0);
+    read_v(1);
+    __builtin_amdgcn_sched_barrier(0);
+    const unsigned bad = __builtin_amdgcn_readfirstlane(bad4.x | (bad4.y << 1) | (bad4.z << 2) | (bad4.w << 3));
+    const bool plain = bad == 0 && p0 + kLargeUnit <= pos_lo + 1 &&
+                       (a.plan.window == 0 || p0 > pos_hi - a.plan.window || p0 + kLargeUnit <= s.sinks);
+    if (!plain) {
+      const Sees seen(a, s, my_pos, p0 + 4 * h);
+#pragma unroll
+      for (int sb = 0; sb < 2; sb++)
+#pragma unroll
+        for (int i = 0; i < 16; i++)
+          if (((bad >> (2 * sb + i / 8)) & 1) || !seen(32 * sb + 8 * (i / 4) + i % 4)) sc[sb][i] = -INFINITY;
+    }
+    float mx = -INFINITY;
+#pragma unroll
+    for (int sb = 0; sb < 2; sb++)
+#pragma unroll
+      for (int i = 0; i < 16; i++) mx = fmaxf(mx, sc[sb][i]);
+    mx = half_max(mx) * a.scale_log2;
+    // the sums are rescaled only once a row's maximum has grown by 2^kSlack: until then
+    // its weights are up to 2^kSlack times as large
+    const int grown = uniform(__any(mx > m_run + kSlack) ? 1 : 0);
+    const float m = grown ? fmaxf(m_run, mx) : m_run;
+    const float corr = m_run == m ? 1.0f : exp2_weight(m_run - m);
+    m_run = m;
+    l_run *= corr;
+    scale_if(acc, corr, grown);
+    // (a row that has seen nothing yet: its weights are exp2(-infinity))
+    const float off = (m_run == -INFINITY ? 0.0f : m_run) - T::kWeightLog2;
+    float ls = 0.0f;
+    Vec p[4];
+#pragma unroll
+    for (int sb = 0; sb < 2; sb++)
+#pragma unroll
+      for (int i = 0; i < 16; i++) {
+        p[2 * sb + i / 8][i % 8] = (Value)exp2_weight(fmaf(sc[sb][i], a.scale_log2, -off));
+      }
+    ls = T::sum8(p[1], T::sum8(p[0], ls));
+    l_run += ls + T::sum8(p[3], T::sum8(p[2], 0.0f));
+    __builtin_amdgcn_sched_barrier(0);
+    read_v(2);
+    read_v(3);
+    __builtin_amdgcn_sched_barrier(0);
+    __builtin_amdgcn_s_setprio(0);
+#pragma unroll
+    for (int ks = 0; ks < 4; ks++)
+#pragma unroll
+      for (int db = 0; db < kDB; db++) {
+        const Vec vf = __builtin_bit_cast(
+            Vec, __builtin_shufflevector(vh[ks][db][0], vh[ks][db][1], 0, 1, 2, 3, 4, 5, 6, 7));
+        acc[db] = T::mfma32(vf, p[ks], acc[db]);
+      }
+  }
+  l_run += __shfl_xor(l_run, 32, 64);
+  bool sound = true;
+  const bool there = 32 * wave + n32 < rows;
+  if (there) sound = score_fits<T>(a, m_run) && l_run < INFINITY;
+  const float inv = l_run == 0.0f ? 0.0f : 1.0f / l_run;
+  uint16_t *op = a.out + head_row(a, t.seq.row0 + s.first, t.kv_head, row) * kD;
+#pragma unroll
+  for (int db = 0; db < kDB; db++)
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      const f32x4 x = {acc[db][4 * i], acc[db][4 * i + 1], acc[db][4 * i + 2], acc[db][4 * i + 3]};
+#pragma unroll
+      for (int e = 0; e < 4; e++) sound = sound && (!there || sum_fits(x[e]));
+      if (slot >= 0) {
+        if (active) *slot_large<kD>(a, slot, wave, db, i) = x;
+      } else if (there) {
+        const Quad o = {(Value)(x[0] * inv), (Value)(x[1] * inv), (Value)(x[2] * inv), (Value)(x[3] * inv)};
+        *reinterpret_cast<Quad *>(op + 32 * db + 8 * i + 4 * h) = o;
+      }
+    }
+  if (slot >= 0 && there && h == 0) {
+    slot_stats<kD>(a, slot, row)[0] = m_run;
+    slot_stats<kD>(a, slot, row)[1] = l_run;
+  }
+  return !__syncthreads_or(sound ? 0 : 1);
+}
+
+template <class T, int kD>
+__global__ __launch_bounds__(kT, kLarge.workers / 256) void paged8_large_kernel(const Attn8Args a) {
+  __shared__ __attribute__((aligned(16))) LargeLds8<kD> lds;
+  __shared__ PlanLds plan;
+  work_piece<true, 32, kD / 32>(a, plan, [&](const PieceStep &st, Line) {
+    return attn_large8<T, kD>(a, st.tile, st.span, st.u0, st.u1, st.slot, lds);
+  });
+}
+
+// ---- the entry points ---------------------------------------------------------------
+
+template <class T, int kD>
+void launch8(hipStream_t st, const Attn8Args &a) {
+  const int workers = a.plan.workers;
+  if (a.tile_rows == kSmall.rows) {
+    paged8_small_kernel<T, kD><<<workers, kT, 0, st>>>(a);
+    paged_merge_small_kernel<Pages8<T>, kD><<<workers, kMergeT, 0, st>>>(a);
+    return;
+  }
+  paged8_large_kernel<T, kD><<<workers, kT, 0, st>>>(a);
+  paged_merge_large_kernel<Pages8<T>, kD><<<std::max(workers, 1024), kT, 0, st>>>(a);
+}
+
+template <class T>
+int attn_paged8(sh_ctx *ctx, const sh_paged_kv8 *kv, const uint16_t *q, uint16_t *out, int tokens, int heads,
+                int max_new, int window, int sinks, float scale, void *workspace, size_t workspace_bytes) {
+  if (!kv) return fail(SH_ERR_INVALID_ARGUMENT, "the paged cache is NULL");
+  const sh_paged_kv index = paged8_index(kv);
+  const AttnCall c = {&index, q, out, tokens, heads, max_new, window, sinks, scale, workspace, workspace_bytes};
+  int rc = check_attn_call(ctx, c);
+  if (rc != SH_OK || tokens == 0 || kv->batch == 0) return rc;
+  if ((rc = check_paged8_pointers(ctx, kv)) || (rc = check_attn_tensors(ctx, c, [&](const void *p, size_t bytes) {
+              return ranges_overlap(p, bytes, kv->pages, paged8_pool_bytes(kv));
+            })))
+    return rc;
+  Attn8Args a;
+  fill_attn_args(c, 64 * 128 / kv->head_dim, &a);
+  a.k = a.v = nullptr;
+  a.pages = kv->pages;
+  a.page_bytes = paged8_page_bytes(kv);
+  a.v_scale_at = (size_t)kv->kv_heads * kv->page_size;
+  a.v_at = a.v_scale_at * kv->head_dim;
+  const hipStream_t st = stream_of(ctx);
+  if (kv->head_dim == 64)
+    launch8<T, 64>(st, a);
+  else
+    launch8<T, 128>(st, a);
+  const hipError_t e = hipGetLastError();
+  return e == hipSuccess ? SH_OK : hip_fail(e, "attn_paged8");
+}
+
+}  // namespace
+}  // namespace sh
+
+using namespace sh;
+
+extern "C" {
+
+SH_API int sh_attn_paged8_workspace(const sh_paged_kv8 *kv, int tokens, int heads, int max_new, size_t *bytes) {
+  if (!bytes) return fail(SH_ERR_INVALID_ARGUMENT, "bytes is NULL");
+  if (!kv) return fail(SH_ERR_INVALID_ARGUMENT, "the paged cache is NULL");
+  const sh_paged_kv index = paged8_index(kv);
+  const int rc = check_attn_sizes(&index, tokens, heads, max_new);
+  if (rc != SH_OK) return rc;
+  *bytes = workspace_of(&index, heads, max_new);
+  return SH_OK;
+}
+
+SH_API int sh_attn_paged8_f16(sh_ctx *ctx, const sh_paged_kv8 *kv, const uint16_t *q, uint16_t *out, int tokens,
+                              int heads, int max_new, int window, int sinks, float scale, void *workspace,
+                              size_t workspace_bytes) {
+  return attn_paged8<PagedF16>(ctx, kv, q, out, tokens, heads, max_new, window, sinks, scale, workspace,
+                               workspace_bytes);
+}
+
+SH_API int sh_attn_paged8_bf16(sh_ctx *ctx, const sh_paged_kv8 *kv, const uint16_t *q, uint16_t *out, int tokens,
+                               int heads, int max_new, int window, int sinks, float scale, void *workspace,
+                               size_t workspace_bytes) {
+  return attn_paged8<PagedBf16>(ctx, kv, q, out, tokens, heads, max_new, window, sinks, scale, workspace,
+                                workspace_bytes);
+}
+
+}  // extern "C"

@@ -1,6 +1,7 @@
 // Device helpers of the operators over a KV cache in pages (paged_ops.hip,
-// paged_attn.hip): the two 16-bit types and their conversions, and the pointer
-// checks that both files' entry points share.
+// paged_attn.hip and their counterparts for pages of 8-bit values): the two 16-bit
+// types and their conversions, those from the 8-bit type, a token's sequence and angles,
+// and the pointer checks that the entry points share.
 #pragma once
 
 #include <hip/hip_runtime.h>
@@ -25,6 +26,8 @@ typedef float f32x16 __attribute__((ext_vector_type(16)));
 struct PagedF16 {
   typedef _Float16 Value;
   typedef pf16x8 Vec;
+  typedef _Float16 Pair __attribute__((ext_vector_type(2)));
+  static constexpr bool kIsF16 = true;
   static constexpr float kWeightLog2 = 7.0f, kMaxScore = 0x1p24f;
   static __device__ __forceinline__ f32x4 mfma16(Vec a, Vec b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
@@ -34,7 +37,6 @@ struct PagedF16 {
   }
   // sum and the eight values, two at a time (fp16 below the normal range as they are)
   static __device__ __forceinline__ float sum8(Vec v, float sum) {
-    typedef _Float16 Pair __attribute__((ext_vector_type(2)));
     const Pair one = {(_Float16)1.0f, (_Float16)1.0f};
 #pragma unroll
     for (int i = 0; i < 4; i++) sum = __builtin_amdgcn_fdot2(Pair{v[2 * i], v[2 * i + 1]}, one, sum, false);
@@ -44,6 +46,8 @@ struct PagedF16 {
 struct PagedBf16 {
   typedef __bf16 Value;
   typedef pbf16x8 Vec;
+  typedef __bf16 Pair __attribute__((ext_vector_type(2)));
+  static constexpr bool kIsF16 = false;
   static constexpr float kWeightLog2 = 0.0f, kMaxScore = 0x1p30f;
   static __device__ __forceinline__ f32x4 mfma16(Vec a, Vec b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
@@ -53,13 +57,31 @@ struct PagedBf16 {
   }
   // (a step may be off by 2^-23 of the sum)
   static __device__ __forceinline__ float sum8(Vec v, float sum) {
-    typedef __bf16 Pair __attribute__((ext_vector_type(2)));
     const Pair one = {(__bf16)1.0f, (__bf16)1.0f};
 #pragma unroll
     for (int i = 0; i < 4; i++) sum = __builtin_amdgcn_fdot2_f32_bf16(Pair{v[2 * i], v[2 * i + 1]}, one, sum, false);
     return sum;
   }
 };
+
+// Four values of OCP E4M3 (a byte each) times a power of two, in the 16-bit type: exact
+// but for what leaves that type's range, rounded as ever. Of `scale` only the exponent
+// counts, as an E8M0 byte in its place would: 0 is 2^-127, 255 gives NaN.
+__device__ __forceinline__ float e8m0_scale(uint32_t byte) { return __builtin_bit_cast(float, byte << 23); }
+template <class T>
+__device__ __forceinline__ u32x2 from_e4m3(uint32_t four, float scale) {
+  if constexpr (T::kIsF16)
+    return u32x2{__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(four, scale, false)),
+                 __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(four, scale, true))};
+  else
+    return u32x2{__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(four, scale, false)),
+                 __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(four, scale, true))};
+}
+template <class T>
+__device__ __forceinline__ u32x4 from_e4m3(uint32_t first, uint32_t second, float scale) {
+  const u32x2 a = from_e4m3<T>(first, scale), b = from_e4m3<T>(second, scale);
+  return u32x4{a.x, a.y, b.x, b.y};
+}
 
 template <class T>
 __device__ __forceinline__ void unpack8(u32x4 bits, float (&x)[8]) {
@@ -74,6 +96,49 @@ __device__ __forceinline__ u32x4 pack8(const float (&x)[8]) {
 #pragma unroll
   for (int e = 0; e < 8; e++) v[e] = (typename T::Value)x[e];
   return __builtin_bit_cast(u32x4, v);
+}
+
+// cos and sin of an fp64 angle below 2^29 (check_rope_theta) to within 2^-38: reduction by
+// pi / 2 in two parts (Cody and Waite) and Taylor polynomials on [-pi / 4, pi / 4], in fp64.
+template <class Real>
+__device__ __forceinline__ void cos_sin64(double a, Real *c, Real *s) {
+  const double q = rint(a * 0.63661977236758134308);  // 2 / pi
+  double r = fma(-q, 1.57079632679489655800, a);      // pi / 2 as the nearest double
+  r = fma(-q, 6.12323399573676603587e-17, r);         // and the rest
+  const double z = r * r;
+  // to r^13 / 13! and r^12 / 12!: the next terms are below 2^-38
+  double ps = fma(z, 1.60590438368216145994e-10, -2.50521083854417187751e-8);
+  ps = fma(z, ps, 2.75573192239858906526e-6);
+  ps = fma(z, ps, -1.98412698412698412698e-4);
+  ps = fma(z, ps, 8.33333333333333333333e-3);
+  ps = fma(z, ps, -1.66666666666666666667e-1);
+  const double sr = fma(r * z, ps, r);
+  double pc = fma(z, 2.08767569878680989792e-9, -2.75573192239858906526e-7);
+  pc = fma(z, pc, 2.48015873015873015873e-5);
+  pc = fma(z, pc, -1.38888888888888888889e-3);
+  pc = fma(z, pc, 4.16666666666666666667e-2);
+  pc = fma(z, pc, -5.0e-1);
+  const double cr = fma(z, pc, 1.0);
+  const int k = (int)q & 3;
+  const double sd = (k & 1) ? cr : sr, cd = (k & 1) ? sr : cr;
+  *s = (Real)((k & 2) ? -sd : sd);
+  *c = (Real)((k == 1 || k == 2) ? -cd : cd);
+}
+
+// The sequence that row `row` belongs to: the last b with starts[b] <= row (b =
+// batch: behind the last, -1: before the first). A wave looks at 64 values at a
+// time; batches of up to 63 take one round.
+__device__ __forceinline__ int find_seq(const int *__restrict__ starts, int batch, int row) {
+  const int lane = threadIdx.x & 63;
+  int lo = 0, n = batch + 1;  // the answer is in lo - 1 .. lo + n - 1
+  while (true) {
+    const int step = (n + 63) / 64, at = lane * step;
+    const int below = __popcll(__ballot(at < n && starts[lo + min(at, n - 1)] <= row));
+    if (below == 0) return lo - 1;  // (lo > 0 only after starts[lo] <= row was seen)
+    lo += (below - 1) * step;
+    n = min(step, n - (below - 1) * step);
+    if (step == 1) return lo;
+  }
 }
 
 inline int check_paged_pointers(sh_ctx *ctx, const sh_paged_kv *kv) {
@@ -95,6 +160,18 @@ inline bool overlaps_index(const sh_paged_kv *kv, const void *p, size_t bytes) {
   const size_t batch = kv->batch;
   return ranges_overlap(p, bytes, kv->page_table, batch * kv->max_pages * 4) ||
          ranges_overlap(p, bytes, kv->lengths, batch * 4) || ranges_overlap(p, bytes, kv->starts, (batch + 1) * 4);
+}
+
+inline int check_paged8_pointers(sh_ctx *ctx, const sh_paged_kv8 *kv) {
+  int rc;
+  if ((rc = check_range(ctx, kv->pages, paged8_pool_bytes(kv), "pages")) ||
+      (rc = check_range(ctx, kv->page_table, (size_t)kv->batch * kv->max_pages * 4, "page_table")) ||
+      (rc = check_range(ctx, kv->lengths, (size_t)kv->batch * 4, "lengths")) ||
+      (rc = check_range(ctx, kv->starts, ((size_t)kv->batch + 1) * 4, "starts")))
+    return rc;
+  if (reinterpret_cast<uintptr_t>(kv->pages) & 15)
+    return fail(SH_ERR_INVALID_ARGUMENT, "pages must be 16-byte aligned");
+  return SH_OK;
 }
 
 }  // namespace sh

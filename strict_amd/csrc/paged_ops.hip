@@ -26,48 +26,6 @@ struct NormRopeArgs {
   double freq[64];  // theta^(-2i / d)
 };
 
-// cos and sin of an fp64 angle below 2^29 (check_rope_theta) to fp32: reduction by pi / 2 in two
-// parts (Cody and Waite) and Taylor polynomials on [-pi / 4, pi / 4], in fp64.
-__device__ __forceinline__ void cos_sin64(double a, float *c, float *s) {
-  const double q = rint(a * 0.63661977236758134308);  // 2 / pi
-  double r = fma(-q, 1.57079632679489655800, a);      // pi / 2 as the nearest double
-  r = fma(-q, 6.12323399573676603587e-17, r);         // and the rest
-  const double z = r * r;
-  // to r^13 / 13! and r^12 / 12!: the next terms are below 2^-38
-  double ps = fma(z, 1.60590438368216145994e-10, -2.50521083854417187751e-8);
-  ps = fma(z, ps, 2.75573192239858906526e-6);
-  ps = fma(z, ps, -1.98412698412698412698e-4);
-  ps = fma(z, ps, 8.33333333333333333333e-3);
-  ps = fma(z, ps, -1.66666666666666666667e-1);
-  const double sr = fma(r * z, ps, r);
-  double pc = fma(z, 2.08767569878680989792e-9, -2.75573192239858906526e-7);
-  pc = fma(z, pc, 2.48015873015873015873e-5);
-  pc = fma(z, pc, -1.38888888888888888889e-3);
-  pc = fma(z, pc, 4.16666666666666666667e-2);
-  pc = fma(z, pc, -5.0e-1);
-  const double cr = fma(z, pc, 1.0);
-  const int k = (int)q & 3;
-  const double sd = (k & 1) ? cr : sr, cd = (k & 1) ? sr : cr;
-  *s = (float)((k & 2) ? -sd : sd);
-  *c = (float)((k == 1 || k == 2) ? -cd : cd);
-}
-
-// The sequence that row `row` belongs to: the last b with starts[b] <= row (b =
-// batch: behind the last, -1: before the first). A wave looks at 64 values at a
-// time; batches of up to 63 take one round.
-__device__ __forceinline__ int find_seq(const int *__restrict__ starts, int batch, int row) {
-  const int lane = threadIdx.x & 63;
-  int lo = 0, n = batch + 1;  // the answer is in lo - 1 .. lo + n - 1
-  while (true) {
-    const int step = (n + 63) / 64, at = lane * step;
-    const int below = __popcll(__ballot(at < n && starts[lo + min(at, n - 1)] <= row));
-    if (below == 0) return lo - 1;  // (lo > 0 only after starts[lo] <= row was seen)
-    lo += (below - 1) * step;
-    n = min(step, n - (below - 1) * step);
-    if (step == 1) return lo;
-  }
-}
-
 // A wave takes 4 * kHeadsAt heads of one token: q heads, then k, then v. A head is
 // d / 16 lanes wide, 8 values of its first half and the 8 that rotate with them in
 // each lane, all loads requested at once. The factors, one pair of them per lane,

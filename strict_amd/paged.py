@@ -12,7 +12,7 @@ import operator
 
 import numpy as np
 
-from . import Context, PagedKV
+from . import Context, PagedKV, PagedKV8
 
 
 class OutOfPages(RuntimeError):
@@ -124,27 +124,37 @@ class PageTable:
 
 class PagedCache:
     """K and V of `layers` layers in pages on a context's device, for up to `rows`
-    sequences of up to max_pages pages each. Every method is ordered on the
+    sequences of up to max_pages pages each: as 16-bit values of `dtype`, or with bits=8
+    quantised as they are written (E4M3 with a power of two for each row), `dtype` being
+    that of the activations. Every method is ordered on the
     context's stream; `step`, and `compact` where it moves pages, upload tables from
     the host and wait for the stream, and are not to be captured."""
 
     def __init__(self, ctx: Context, layers: int, kv_heads: int, head_dim: int, *, rows: int,
-                 max_pages: int, num_pages: int, page_size: int = 64, dtype: str = "f16"):
+                 max_pages: int, num_pages: int, page_size: int = 64, dtype: str = "f16", bits: int = 16):
+        if bits not in (8, 16):
+            raise ValueError(f"{bits} bits: 8 or 16")
         self.ctx, self.layers = ctx, layers
         self.table = PageTable(rows, max_pages, num_pages, page_size)
-        self.page_bytes = kv_heads * page_size * head_dim * 2
+        if bits == 16:
+            self.page_bytes = kv_heads * page_size * head_dim * 2
+            self.planes = 2 * layers  # [layer][k, v][page]
+        else:
+            self.page_bytes = PagedKV8.page_bytes(kv_heads, page_size, head_dim)
+            self.planes = layers  # [layer][page]
         plane = num_pages * self.page_bytes
         self.buffers = []
         try:
-            self.pool = self._keep(ctx.alloc(layers * 2 * plane))  # [layer][k, v][page]
+            self.pool = self._keep(ctx.alloc(self.planes * plane))
             self.table_buf = self._keep(ctx.empty((rows, max_pages), np.int32))
             self.lengths = self._keep(ctx.empty(rows, np.int32))
             self.starts = self._keep(ctx.empty(rows + 1, np.int32))
             self.moves = self._keep(ctx.empty((2, num_pages), np.int32))
-            self.kv = [PagedKV(self.pool.ptr + 2 * i * plane, self.pool.ptr + (2 * i + 1) * plane,
-                               self.table_buf, self.lengths, self.starts, batch=rows,
-                               max_pages=max_pages, num_pages=num_pages, page_size=page_size,
-                               kv_heads=kv_heads, head_dim=head_dim, dtype=dtype)
+            kind, planes = (PagedKV, 2) if bits == 16 else (PagedKV8, 1)
+            self.kv = [kind(*(self.pool.ptr + (planes * i + j) * plane for j in range(planes)),
+                            self.table_buf, self.lengths, self.starts, batch=rows,
+                            max_pages=max_pages, num_pages=num_pages, page_size=page_size,
+                            kv_heads=kv_heads, head_dim=head_dim, dtype=dtype)
                        for i in range(layers)]  # a layer's view, for the operators
             self._upload({})
         except BaseException:
@@ -162,7 +172,7 @@ class PagedCache:
             at_src, at_dst = self.moves.view(0, 4 * num), self.moves.view(4 * num, 4 * num)
             at_src.copy_from_host(src)
             at_dst.copy_from_host(dst)
-            self.ctx.pages_copy(self.pool, 2 * self.layers, num, self.page_bytes, at_src, at_dst,
+            self.ctx.pages_copy(self.pool, self.planes, num, self.page_bytes, at_src, at_dst,
                                 len(pairs))
 
     def _upload(self, new) -> None:
