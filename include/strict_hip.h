@@ -417,6 +417,38 @@ SH_API int sh_pack_e4m3_tiles(sh_ctx *ctx, const uint8_t *q, int N, int K, uint8
 SH_API int sh_gemv_w8a16(sh_ctx *ctx, const uint16_t *x, const uint8_t *w_tiled,
                          const float *scales, float *y, int batch, int K, int N);
 
+/* 4-bit weights as OCP MX has them: E2M1 values (0, 0.5, 1, 1.5, 2, 3, 4, 6 and their
+ * negatives; the sign above the three bits of the size) with a power of two for each 32 of
+ * a row, of an E8M0 byte: 2^(byte - 127), 255 a NaN. */
+
+/* A device fp32 matrix W[N][K] in that form: q[n * K / 2 + k / 2], the even k in the low
+ * four bits, scales[n * K / 32 + k / 32]. The smallest scale 2^e, e >= -127, for which the
+ * largest of the 32 is at most 6 * 2^e; values to the nearest, half way to the even code. 32
+ * with one that is not finite get the scale 255. K a multiple of 32, at most 2^24, N
+ * at most 2^28 (of all calls of this form); W and q 16-byte aligned. */
+SH_API int sh_quantize_e2m1(sh_ctx *ctx, const float *W, int N, int K, uint8_t *q,
+                            uint8_t *scales);
+
+/* Such a matrix in the layout that sh_gemv_w4a16_* reads (16-row x 128-column tiles in MFMA
+ * operand order, what is missing of one filled up with zeros), of sh_e2m1_tiles_bytes bytes.
+ * q 4-byte, tiled 16-byte aligned. */
+SH_API int sh_e2m1_tiles_bytes(int N, int K, size_t *bytes);
+SH_API int sh_pack_e2m1_tiles(sh_ctx *ctx, const uint8_t *q, const uint8_t *scales, int N, int K,
+                              uint8_t *tiled);
+
+/* W4A16 GEMV / skinny GEMM: y[b * ldy + n] = sum_k x[b * ldx + k] * w[n][k] for b < batch
+ * (1..64); x fp16 or bf16, fp32 accumulation of exact products, y of x's type (rounded once)
+ * or fp32. Weights and scales of any values; a row with a scale of 255 gives NaN. ldx a multiple of 8 and at least K, ldy at least N; x and
+ * w_tiled 16-byte aligned. y overlaps neither. */
+SH_API int sh_gemv_w4a16_f16(sh_ctx *ctx, const uint16_t *x, int ldx, const uint8_t *w_tiled,
+                             uint16_t *y, int ldy, int batch, int K, int N);
+SH_API int sh_gemv_w4a16_bf16(sh_ctx *ctx, const uint16_t *x, int ldx, const uint8_t *w_tiled,
+                              uint16_t *y, int ldy, int batch, int K, int N);
+SH_API int sh_gemv_w4a16_f16_f32(sh_ctx *ctx, const uint16_t *x, int ldx, const uint8_t *w_tiled,
+                                 float *y, int ldy, int batch, int K, int N);
+SH_API int sh_gemv_w4a16_bf16_f32(sh_ctx *ctx, const uint16_t *x, int ldx, const uint8_t *w_tiled,
+                                  float *y, int ldy, int batch, int K, int N);
+
 /* ---- typed ops: decoder building blocks ---------------------------------------
  * No reference counterpart (Strict has no LLM path): the operations of the
  * GPT-2 and Qwen3 decoders, which the model runners below fuse into their
@@ -631,6 +663,41 @@ SH_API int sh_sample_f32(sh_ctx *ctx, const float *x, int rows, int n, int ld,
                          const float *temperature, const int32_t *top_k, const float *top_p,
                          const float *min_p, const float *u, int32_t *index, void *workspace,
                          size_t workspace_bytes);
+
+/* Rules on rows of logits, as a sampler's user sets them; all pointers are device memory,
+ * any group of them NULL: no such rule. Values outside their ranges do no harm: lengths are
+ * taken within 0 .. max_tokens, prompts within 0 .. the length, bias_starts within 0 ..
+ * bias_count and ascending; tokens outside 0 .. n - 1 name nothing. */
+typedef struct sh_logit_rules {
+  const int32_t *tokens;  /* [rows][max_tokens]: the tokens of each row so far */
+  const int32_t *lengths; /* [rows]: how many (needed with tokens) */
+  const int32_t *prompts; /* [rows]: how many of the first are the prompt; NULL: none */
+  int max_tokens;
+  const float *repetition, *frequency, *presence; /* [rows]; NULL: 1, 0, 0 */
+  const int32_t *bias_starts; /* [rows + 1]: row r's biases are bias_starts[r] .. [r + 1] - 1 */
+  const int32_t *bias_tokens; /* [bias_count] */
+  const float *bias_values;   /* [bias_count] */
+  int bias_count;
+  const uint32_t *masks;  /* [num_masks][(n + 31) / 32]: token i allowed where bit i % 32 of word i / 32 is set */
+  const int32_t *mask_of; /* [rows]: the row's mask; outside 0 .. num_masks - 1: none */
+  int num_masks;
+} sh_logit_rules;
+
+/* y[r * ldy + i] = x[r * ldx + i] (x fp32, fp16 or bf16) by the rules, in this order, each
+ * step rounded to fp32:
+ *   a token of the row's: x > 0 ? x / repetition : x * repetition (repetition 0 or less,
+ *   infinite or NaN: 1);
+ *   a token c > 0 times behind the prompt: less (frequency * c + presence) (NaN: 0);
+ *   a token with a bias: plus that (of several the last in the list);
+ *   a token that the row's mask leaves out: -infinity.
+ * Nothing allocated, nothing waited for. rows <= 2^16, n <= 2^20. y is x itself (fp32, ldy
+ * = ldx) or overlaps nothing of the call; the rows' gaps are left as they are. */
+SH_API int sh_adjust_logits_f32(sh_ctx *ctx, const float *x, int ldx, float *y, int ldy, int rows,
+                                int n, const sh_logit_rules *rules);
+SH_API int sh_adjust_logits_f16(sh_ctx *ctx, const uint16_t *x, int ldx, float *y, int ldy,
+                                int rows, int n, const sh_logit_rules *rules);
+SH_API int sh_adjust_logits_bf16(sh_ctx *ctx, const uint16_t *x, int ldx, float *y, int ldy,
+                                 int rows, int n, const sh_logit_rules *rules);
 
 /* ---- LLM decode (model runners) ------------------------------------------------
  * No reference counterpart. The models: GPT-2 (measured as GPT-2 small, fp16

@@ -33,7 +33,7 @@ from ._lib import (SH_ERR_COMPILE, SH_ERR_INVALID_ARGUMENT, SH_ERR_NO_DEVICE, SH
 __all__ = [
     "StrictHipError", "CompileError", "Context", "DeviceVariable", "RuntimeCompiler",
     "KernelFunction", "Module", "Kernel", "device_count", "SAXPY_SOURCE", "PagedKV",
-    "PagedKV8",
+    "PagedKV8", "LogitRules",
     "ADD", "SUBTRACT", "MULTIPLY", "DIVIDE", "BLUR_CONFIG", "BLUR_REFERENCE",
     "BRIGHTNESS_ALL_CHANNELS",
 ]
@@ -187,6 +187,24 @@ class PagedKV8:
         n = ctypes.c_size_t(0)
         _check(_lib.load().sh_paged8_page_bytes(ctypes.byref(kv), ctypes.byref(n)))
         return n.value
+
+
+class LogitRules:
+    """Rules on rows of logits (sh_logit_rules), device arrays or None: tokens
+    [rows, max_tokens] with lengths and prompts [rows]; repetition, frequency and presence
+    [rows]; bias_tokens and bias_values [bias_count] with bias_starts [rows + 1]; masks
+    [num_masks, (n + 31) // 32] of bits with mask_of [rows]."""
+
+    def __init__(self, *, tokens=None, max_tokens: int = 0, lengths=None, prompts=None,
+                 repetition=None, frequency=None, presence=None, bias_starts=None,
+                 bias_tokens=None, bias_values=None, bias_count: int = 0, masks=None,
+                 mask_of=None, num_masks: int = 0):
+        # kept alive with the struct
+        self.buffers = (tokens, lengths, prompts, repetition, frequency, presence, bias_starts,
+                        bias_tokens, bias_values, masks, mask_of)
+        p = [_ptr(b) for b in self.buffers]
+        self.struct = _lib.LogitRules(*p[:3], max_tokens, *p[3:9], bias_count, *p[9:], num_masks)
+        self.address = ctypes.byref(self.struct)
 
 
 class RuntimeCompiler:
@@ -472,6 +490,29 @@ class Context:
         _check(self._l.sh_gemv_w8a16(self.handle, _ptr(x), _ptr(w_tiled), _ptr(scales), _ptr(y),
                                      batch, k, n))
 
+    def quantize_e2m1(self, w, q, scales, n: int, k: int) -> None:
+        """fp32 W [n, k] as 4-bit values, two a byte, with an E8M0 scale for 32 of a row."""
+        _check(self._l.sh_quantize_e2m1(self.handle, _ptr(w), n, k, _ptr(q), _ptr(scales)))
+
+    def e2m1_tiles_bytes(self, n: int, k: int) -> int:
+        """Bytes of the layout that gemv_w4a16 reads."""
+        size = ctypes.c_size_t(0)
+        _check(self._l.sh_e2m1_tiles_bytes(n, k, ctypes.byref(size)))
+        return size.value
+
+    def pack_e2m1_tiles(self, q, scales, tiled, n: int, k: int) -> None:
+        _check(self._l.sh_pack_e2m1_tiles(self.handle, _ptr(q), _ptr(scales), n, k, _ptr(tiled)))
+
+    def gemv_w4a16(self, x, w_tiled, y, batch: int, k: int, n: int, dtype: str = "f16",
+                   out: str = "f32", ldx: int | None = None, ldy: int | None = None) -> None:
+        """y[b] = W x[b] for packed 4-bit weights; x [batch, k] of dtype "f16" or "bf16"
+        (rows ldx apart), y [batch, n] (ldy) fp32 or, where `out` is dtype, of that type."""
+        if dtype not in ("f16", "bf16") or out not in ("f32", dtype):
+            raise ValueError(f"dtype {dtype!r} and out {out!r}: 'f16' or 'bf16', and 'f32' or the same")
+        f = getattr(self._l, f"sh_gemv_w4a16_{dtype}" + ("_f32" if out == "f32" else ""))
+        _check(f(self.handle, _ptr(x), k if ldx is None else ldx, _ptr(w_tiled), _ptr(y),
+                 n if ldy is None else ldy, batch, k, n))
+
     # -- decoder building blocks (fp32 device buffers) --
     def rmsnorm(self, x, gain, y, rows: int, n: int, eps: float) -> None:
         """y = (x * fp32(1 / sqrt(mean(x^2) + eps))) * gain, per row of n."""
@@ -555,6 +596,16 @@ class Context:
         _check(self._l.sh_pages_copy(self.handle, _ptr(pool), planes,
                                      num_pages * page_bytes if plane_stride is None else plane_stride,
                                      num_pages, page_bytes, _ptr(src), _ptr(dst), count))
+
+    def adjust_logits(self, x, y, rows: int, n: int, rules: LogitRules, dtype: str = "f32",
+                      ldx: int | None = None, ldy: int | None = None) -> None:
+        """y [rows, n] fp32 = logits x of dtype "f32", "f16" or "bf16" by the rules; y may
+        be x where that is fp32."""
+        if dtype not in ("f32", "f16", "bf16"):
+            raise ValueError(f"dtype {dtype!r}: 'f32', 'f16' or 'bf16'")
+        _check(getattr(self._l, f"sh_adjust_logits_{dtype}")(
+            self.handle, _ptr(x), n if ldx is None else ldx, _ptr(y), n if ldy is None else ldy, rows,
+            n, rules.address))
 
     def sample_workspace(self, rows: int, n: int) -> int:
         """Bytes of the work buffer sample takes at these sizes."""

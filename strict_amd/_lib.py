@@ -114,6 +114,26 @@ class PagedKv8(ctypes.Structure):
     _fields_ = [("pages", ctypes.c_void_p)] + PagedKv._fields_[2:]
 
 
+class LogitRules(ctypes.Structure):
+    """sh_logit_rules: penalties, biases and masks of rows of logits."""
+    _fields_ = [
+        ("tokens", ctypes.c_void_p),
+        ("lengths", ctypes.c_void_p),
+        ("prompts", ctypes.c_void_p),
+        ("max_tokens", ctypes.c_int),
+        ("repetition", ctypes.c_void_p),
+        ("frequency", ctypes.c_void_p),
+        ("presence", ctypes.c_void_p),
+        ("bias_starts", ctypes.c_void_p),
+        ("bias_tokens", ctypes.c_void_p),
+        ("bias_values", ctypes.c_void_p),
+        ("bias_count", ctypes.c_int),
+        ("masks", ctypes.c_void_p),
+        ("mask_of", ctypes.c_void_p),
+        ("num_masks", ctypes.c_int),
+    ]
+
+
 _P = ctypes.c_void_p
 _PP = ctypes.POINTER(ctypes.c_void_p)
 _I = ctypes.c_int
@@ -192,6 +212,13 @@ SIGNATURES = {
     "sh_quantize_e4m3": (_I, [_P, _P, _I, _I, _P, _P]),
     "sh_pack_e4m3_tiles": (_I, [_P, _P, _I, _I, _P]),
     "sh_gemv_w8a16": (_I, [_P, _P, _P, _P, _P, _I, _I, _I]),
+    "sh_quantize_e2m1": (_I, [_P, _P, _I, _I, _P, _P]),
+    "sh_e2m1_tiles_bytes": (_I, [_I, _I, ctypes.POINTER(_SZ)]),
+    "sh_pack_e2m1_tiles": (_I, [_P, _P, _P, _I, _I, _P]),
+    "sh_gemv_w4a16_f16": (_I, [_P, _P, _I, _P, _P, _I, _I, _I, _I]),
+    "sh_gemv_w4a16_bf16": (_I, [_P, _P, _I, _P, _P, _I, _I, _I, _I]),
+    "sh_gemv_w4a16_f16_f32": (_I, [_P, _P, _I, _P, _P, _I, _I, _I, _I]),
+    "sh_gemv_w4a16_bf16_f32": (_I, [_P, _P, _I, _P, _P, _I, _I, _I, _I]),
     "sh_rmsnorm_f32": (_I, [_P, _P, _P, _P, _I, _I, _F]),
     "sh_layernorm_f32": (_I, [_P, _P, _P, _P, _P, _I, _I, _F]),
     "sh_rope_f32": (_I, [_P, _P, _P, _I, _I, _I, _F]),
@@ -216,6 +243,9 @@ SIGNATURES = {
     "sh_pages_copy": (_I, [_P, _P, _I, _SZ, _I, _SZ, _P, _P, _I]),
     "sh_sample_workspace": (_I, [_I, _I, ctypes.POINTER(_SZ)]),
     "sh_sample_f32": (_I, [_P, _P, _I, _I, _I, _P, _P, _P, _P, _P, _P, _P, _SZ]),
+    "sh_adjust_logits_f32": (_I, [_P, _P, _I, _P, _I, _I, _I, _P]),
+    "sh_adjust_logits_f16": (_I, [_P, _P, _I, _P, _I, _I, _I, _P]),
+    "sh_adjust_logits_bf16": (_I, [_P, _P, _I, _P, _I, _I, _I, _P]),
     "sh_llm_create": (_I, [_P, ctypes.POINTER(LlmConfig), _PP]),
     "sh_llm_destroy": (_I, [_P]),
     "sh_llm_init_random": (_I, [_P, ctypes.c_uint64, _F]),
