@@ -149,8 +149,6 @@ class PagedKV:
     [batch, max_pages], lengths [batch] (new tokens included) and starts
     [batch + 1] (rows of the new tokens), all int32 on the device."""
 
-    symbol = "paged"  # in the names of the operators that take it
-
     def __init__(self, k, v, page_table, lengths, starts, *, batch: int, max_pages: int,
                  num_pages: int, page_size: int, kv_heads: int, head_dim: int, dtype: str = "f16"):
         if dtype not in ("f16", "bf16"):
@@ -158,6 +156,9 @@ class PagedKV:
         self.dtype = dtype
         self.kv_heads, self.head_dim = kv_heads, head_dim
         self.buffers = (k, v, page_table, lengths, starts)  # kept alive with the struct
+        l = _lib.load()
+        self.append = getattr(l, f"sh_qk_norm_rope_paged_{dtype}")  # the operators for this cache
+        self.attend, self.workspace = getattr(l, f"sh_attn_paged_{dtype}"), l.sh_attn_paged_workspace
         self.struct = _lib.PagedKv(*(_ptr(b) for b in self.buffers), batch, max_pages, num_pages,
                                    page_size, kv_heads, head_dim)
         self.address = ctypes.byref(self.struct)
@@ -167,8 +168,6 @@ class PagedKV8:
     """The same in 8 bits (sh_paged_kv8): pages [num_pages, page_bytes] that hold E4M3
     rows of k and v and a scale byte for each; dtype: that of q and the output."""
 
-    symbol = "paged8"
-
     def __init__(self, pages, page_table, lengths, starts, *, batch: int, max_pages: int,
                  num_pages: int, page_size: int, kv_heads: int, head_dim: int, dtype: str = "f16"):
         if dtype not in ("f16", "bf16"):
@@ -176,6 +175,10 @@ class PagedKV8:
         self.dtype = dtype
         self.kv_heads, self.head_dim = kv_heads, head_dim
         self.buffers = (pages, page_table, lengths, starts)  # kept alive with the struct
+        l = _lib.load()
+        self.append = getattr(l, f"sh_qk_norm_rope_paged8_{dtype}")
+        self.attend, self.workspace = getattr(l, f"sh_attn_paged8_{dtype}"), l.sh_attn_paged8_workspace
+        self.read = getattr(l, f"sh_paged8_read_{dtype}")
         self.struct = _lib.PagedKv8(*(_ptr(b) for b in self.buffers), batch, max_pages, num_pages,
                                     page_size, kv_heads, head_dim)
         self.address = ctypes.byref(self.struct)
@@ -554,29 +557,24 @@ class Context:
 
 
     # -- a KV cache in pages, and sampling --
-    def _paged(self, operator: str, kv):
-        """The operator for the kind of cache and the type of q."""
-        return getattr(self._l, f"sh_{operator.format(kv.symbol)}_{kv.dtype}")
-
     def qk_norm_rope_paged(self, kv: PagedKV | PagedKV8, qkv, q_gain, k_gain, q, tokens: int,
                            heads: int, eps: float, theta: float, ld: int | None = None) -> None:
         """Rows q | k | v of a linear: q and k normalised per head and rotated at the
         tokens' positions, q to q [tokens, heads, d], k and v to their pages (those of a
         PagedKV8 quantised)."""
-        _check(self._paged("qk_norm_rope_{}", kv)(
+        _check(kv.append(
             self.handle, kv.address, _ptr(qkv), _ptr(q_gain), _ptr(k_gain), _ptr(q), tokens, heads,
             (heads + 2 * kv.kv_heads) * kv.head_dim if ld is None else ld, eps, theta))
 
     def paged_read(self, kv: PagedKV8, k, v, tokens: int) -> None:
         """The rows of the call's new tokens read back from the pages: k, v
         [tokens, kv_heads, d] of the values that the bytes stand for."""
-        _check(self._paged("{}_read", kv)(self.handle, kv.address, _ptr(k), _ptr(v), tokens))
+        _check(kv.read(self.handle, kv.address, _ptr(k), _ptr(v), tokens))
 
     def attn_paged_workspace(self, kv: PagedKV | PagedKV8, tokens: int, heads: int, max_new: int) -> int:
         """Bytes of the work buffer attn_paged takes at these sizes."""
         n = ctypes.c_size_t(0)
-        _check(getattr(self._l, f"sh_attn_{kv.symbol}_workspace")(kv.address, tokens, heads, max_new,
-                                                                 ctypes.byref(n)))
+        _check(kv.workspace(kv.address, tokens, heads, max_new, ctypes.byref(n)))
         return n.value
 
     def attn_paged(self, kv: PagedKV | PagedKV8, q, out, tokens: int, heads: int, max_new: int,
@@ -587,8 +585,8 @@ class Context:
         workspace: a buffer, or the address of one, of at least attn_paged_workspace's bytes."""
         size = (workspace.nbytes if isinstance(workspace, DeviceVariable)
                 else self.attn_paged_workspace(kv, tokens, heads, max_new))
-        _check(self._paged("attn_{}", kv)(self.handle, kv.address, _ptr(q), _ptr(out), tokens, heads,
-                                          max_new, window, sinks, scale, _ptr(workspace), size))
+        _check(kv.attend(self.handle, kv.address, _ptr(q), _ptr(out), tokens, heads, max_new, window,
+                         sinks, scale, _ptr(workspace), size))
 
     def pages_copy(self, pool, planes: int, num_pages: int, page_bytes: int, src, dst, count: int,
                    plane_stride: int | None = None) -> None:
