@@ -7,7 +7,7 @@
 
 namespace sh {
 
-constexpr int kMaxGemv4Batch = 64, kMaxGemv4N = 1 << 28, kMaxGemv4K = 1 << 24;
+constexpr int kMaxGemv4Batch = 64, kMaxGemv4N = 1 << 28, kMaxGemv4K = 1 << 24, kMaxGemv4Ldx = 1 << 25;
 
 // The layout that the products read: tiles of 16 rows by 128 columns, columns first, as
 // the matrix instructions take them: lane l's 16 bytes are row l % 16, dword j of them
@@ -32,7 +32,8 @@ inline const char *check_e2m1_sizes(int N, int K) {
 inline const char *check_gemv4_sizes(int batch, int K, int N, int ldx, int ldy) {
   if (batch < 1 || batch > kMaxGemv4Batch) return "batch must be 1..64";
   if (const char *wrong = check_e2m1_sizes(N, K)) return wrong;
-  if (ldx < K || ldx % 8 != 0) return "ldx must be a multiple of 8 and at least K";
+  // (64 rows' bytes in 32 bits)
+  if (ldx < K || ldx % 8 != 0 || ldx > kMaxGemv4Ldx) return "ldx must be a multiple of 8, at least K and at most 2^25";
   if (ldy < N) return "ldy must be at least N";
   return nullptr;
 }

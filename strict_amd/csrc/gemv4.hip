@@ -6,6 +6,8 @@
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
+#include <cstddef>
+#include <type_traits>
 
 #include "common.h"
 #include "gemv4.h"
@@ -128,82 +130,70 @@ __device__ __forceinline__ typename T::Vec from_e2m1(uint32_t eight, float scale
   return __builtin_bit_cast(typename T::Vec, v);
 }
 
+// The nearest exponent with which every weight is a normal number of the type.
+template <class T>
+__device__ __forceinline__ uint32_t normal_exponent(uint32_t exponent) {
+  constexpr uint32_t kLeast = T::kIsF16 ? kF16Least : kBf16Least, kMost = T::kIsF16 ? kF16Most : kBf16Most;
+  return min(max(exponent, kLeast << 23), kMost << 23);
+}
+
 // What a wave has of a step: kR tiles of weights, their scales, and the activations.
-template <int kR, int kM>
+template <int kR>
 struct Gemv4Step {
-  u32x4 w[kR], x[kM][4];
+  u32x4 w[kR], x[4];
   uint32_t s[kR];
 };
 
-// A workgroup takes kR tiles of rows; its waves share the columns, step by step of 128 in
-// turn, and add up in LDS in their order. Activations are the rows of the products, weights
-// the columns, so that a lane's results are of one row of weights: 16 kM rows of x, row b
-// in the product's row 4 (b % 4) + b / 4, so that up to 4 of them need one register (kI)
-// and up to 8 two. Where a scale leaves the type's normal numbers (kExact), weights are
-// converted with the nearest that does not, and each group's sum is multiplied by the rest.
-template <class T, int kR, int kM, int kI, bool kExact>
-__device__ __forceinline__ void gemv4_sum(const Gemv4Args &a, f32x4 (&acc)[kR][kM]) {
+// Up to 16 rows of activations. A workgroup takes kR tiles of rows; its waves share the
+// columns, step by step of 128 in turn, and add up in LDS in their order. Activations are
+// the rows of the products, weights the columns, so that a lane's results are of one row of
+// weights; row b of x is the product's row 4 (b % 4) + b / 4, so that up to 4 of them need
+// one register (kI) and up to 8 two. Where a scale leaves the type's normal numbers
+// (kExact), weights are converted with the nearest that does not, and each group's sum is
+// multiplied by the rest. Bound by the weights' bytes.
+template <class T, int kR, int kI, bool kExact>
+__device__ __forceinline__ void gemv4_sum(const Gemv4Args &a, f32x4 (&acc)[kR]) {
   typedef typename T::Vec Vec;
   const int lane = threadIdx.x & 63, r16 = lane & 15, grp = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
-  const uint16_t *x[kM];
-#pragma unroll
-  for (int m = 0; m < kM; m++) {
-    const int b = 16 * m + 4 * (r16 & 3) + (r16 >> 2);
-    x[m] = a.x + (size_t)min(b, a.batch - 1) * a.ldx + grp * 8;
-  }
+  const uint16_t *x = a.x + (size_t)min(4 * (r16 & 3) + (r16 >> 2), a.batch - 1) * a.ldx + grp * 8;
   size_t first[kR];
 #pragma unroll
   for (int r = 0; r < kR; r++) first[r] = (size_t)min((int)blockIdx.x * kR + r, a.row_tiles - 1) * a.col_tiles;
-  auto load = [&](int t, Gemv4Step<kR, kM> &s) __attribute__((always_inline)) {
+  auto load = [&](int t, Gemv4Step<kR> &s) __attribute__((always_inline)) {
 #pragma unroll
     for (int r = 0; r < kR; r++) {
       s.w[r] = __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(a.w + (first[r] + t) * 1024 + lane * 16));
       s.s[r] = *reinterpret_cast<const uint32_t *>(a.scales + (first[r] + t) * 64 + r16 * 4);
     }
 #pragma unroll
-    for (int m = 0; m < kM; m++)
-#pragma unroll
-      for (int j = 0; j < 4; j++)
-        s.x[m][j] = *reinterpret_cast<const u32x4 *>(x[m] + min(128 * t + 32 * j, a.K - 32));
+    for (int j = 0; j < 4; j++) s.x[j] = *reinterpret_cast<const u32x4 *>(x + min(128 * t + 32 * j, a.K - 32));
   };
-  auto multiply = [&](int t, Gemv4Step<kR, kM> &s) __attribute__((always_inline)) {
+  auto multiply = [&](int t, Gemv4Step<kR> &s) __attribute__((always_inline)) {
     if (128 * t + 128 > a.K) {  // columns behind the last: zeros, whatever x has there
 #pragma unroll
-      for (int m = 0; m < kM; m++)
-#pragma unroll
-        for (int j = 1; j < 4; j++)
-          if (128 * t + 32 * j >= a.K) s.x[m][j] = u32x4{0, 0, 0, 0};
+      for (int j = 1; j < 4; j++)
+        if (128 * t + 32 * j >= a.K) s.x[j] = u32x4{0, 0, 0, 0};
     }
 #pragma unroll
     for (int j = 0; j < 4; j++)
 #pragma unroll
       for (int r = 0; r < kR; r++) {
-        uint32_t exponent = (j == 3 ? s.s[r] >> 1 : s.s[r] << (23 - 8 * j)) & 0x7f800000u, rest = 127u << 23;
+        const uint32_t exponent = (j == 3 ? s.s[r] >> 1 : s.s[r] << (23 - 8 * j)) & 0x7f800000u;
+        const uint32_t normal = kExact ? normal_exponent<T>(exponent) : exponent;
+        const Vec w = from_e2m1<T>(s.w[r][j], __builtin_bit_cast(float, normal)), xv = __builtin_bit_cast(Vec, s.x[j]);
         if constexpr (kExact) {
-          constexpr uint32_t kLeast = T::kIsF16 ? kF16Least : kBf16Least, kMost = T::kIsF16 ? kF16Most : kBf16Most;
-          const uint32_t normal = min(max(exponent, kLeast << 23), kMost << 23);
-          rest += exponent - normal;
-          exponent = normal;
-        }
-        const Vec w = from_e2m1<T>(s.w[r][j], __builtin_bit_cast(float, exponent));
+          const f32x4 d = T::mfma16(xv, w, f32x4{0.f, 0.f, 0.f, 0.f});
+          const float rest = __builtin_bit_cast(float, (127u << 23) + exponent - normal);
 #pragma unroll
-        for (int m = 0; m < kM; m++) {
-          const Vec xv = __builtin_bit_cast(Vec, s.x[m][j]);
-          if constexpr (kExact) {
-            const f32x4 d = T::mfma16(xv, w, f32x4{0.f, 0.f, 0.f, 0.f});
-            const float scale = __builtin_bit_cast(float, rest);
-#pragma unroll
-            for (int i = 0; i < kI; i++) acc[r][m][i] = fmaf(d[i], scale, acc[r][m][i]);
-          } else {
-            acc[r][m] = T::mfma16(xv, w, acc[r][m]);
-          }
+          for (int i = 0; i < kI; i++) acc[r][i] = fmaf(d[i], rest, acc[r][i]);
+        } else {
+          acc[r] = T::mfma16(xv, w, acc[r]);
         }
       }
   };
   int t = wave;
-  if (t >= a.col_tiles) return;
-  Gemv4Step<kR, kM> now, next;
+  Gemv4Step<kR> now, next;
   load(t, now);
   for (; t + waves < a.col_tiles; t += waves) {
     load(t + waves, next);
@@ -213,11 +203,11 @@ __device__ __forceinline__ void gemv4_sum(const Gemv4Args &a, f32x4 (&acc)[kR][k
   multiply(t, now);
 }
 
-constexpr int kMaxWaves = 8;
+constexpr int kMaxWaves = 16;
 
-template <class T, int kR, int kM, int kI, class Out>
-__global__ __launch_bounds__(64 * kMaxWaves) void gemv4_kernel(const Gemv4Args a) {
-  extern __shared__ __attribute__((aligned(16))) float parts[];  // [waves - 1][kR][kM][kI][64]
+template <class T, int kR, int kI, class Out>
+__global__ __launch_bounds__(64 * (kR == 1 ? kMaxWaves : 8)) void gemv4_kernel(const Gemv4Args a) {
+  extern __shared__ __attribute__((aligned(16))) float parts[];  // [waves - 1][kR][kI][64]
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
   uint32_t flags[kR], any = 0;
 #pragma unroll
@@ -225,23 +215,19 @@ __global__ __launch_bounds__(64 * kMaxWaves) void gemv4_kernel(const Gemv4Args a
     flags[r] = a.flags[min((int)blockIdx.x * kR + r, a.row_tiles - 1)];
     any |= flags[r];
   }
-  f32x4 acc[kR][kM];
+  f32x4 acc[kR];
 #pragma unroll
-  for (int r = 0; r < kR; r++)
-#pragma unroll
-    for (int m = 0; m < kM; m++) acc[r][m] = f32x4{0.f, 0.f, 0.f, 0.f};
+  for (int r = 0; r < kR; r++) acc[r] = f32x4{0.f, 0.f, 0.f, 0.f};
   if (any & (T::kIsF16 ? 1u << 16 : 1u << 17))
-    gemv4_sum<T, kR, kM, kI, true>(a, acc);
+    gemv4_sum<T, kR, kI, true>(a, acc);
   else
-    gemv4_sum<T, kR, kM, kI, false>(a, acc);
+    gemv4_sum<T, kR, kI, false>(a, acc);
   if (wave > 0) {
-    float *to = parts + (wave - 1) * (kR * kM * kI * 64) + lane;
+    float *to = parts + (wave - 1) * (kR * kI * 64) + lane;
 #pragma unroll
     for (int r = 0; r < kR; r++)
 #pragma unroll
-      for (int m = 0; m < kM; m++)
-#pragma unroll
-        for (int i = 0; i < kI; i++) to[((r * kM + m) * kI + i) * 64] = acc[r][m][i];
+      for (int i = 0; i < kI; i++) to[(r * kI + i) * 64] = acc[r][i];
   }
   if (waves > 1) __syncthreads();
   if (wave > 0) return;
@@ -249,34 +235,241 @@ __global__ __launch_bounds__(64 * kMaxWaves) void gemv4_kernel(const Gemv4Args a
 #pragma unroll
   for (int r = 0; r < kR; r++)
 #pragma unroll
-    for (int m = 0; m < kM; m++)
-#pragma unroll
-      for (int i = 0; i < kI; i++) {
-        float sum = acc[r][m][i];
-        for (int w = 1; w < waves; w++) sum += parts[(w - 1) * (kR * kM * kI * 64) + ((r * kM + m) * kI + i) * 64 + lane];
-        if ((flags[r] >> (lane & 15)) & 1) sum = NAN;
-        const long long n = ((long long)blockIdx.x * kR + r) * 16 + (lane & 15);
-        const int b = 16 * m + 4 * i + (lane >> 4);
-        if (n < a.N && b < a.batch) y[b * a.ldy + n] = (Out)sum;
-      }
+    for (int i = 0; i < kI; i++) {
+      float sum = acc[r][i];
+      for (int w = 1; w < waves; w++) sum += parts[(w - 1) * (kR * kI * 64) + (r * kI + i) * 64 + lane];
+      if ((flags[r] >> (lane & 15)) & 1) sum = NAN;
+      const long long n = ((long long)blockIdx.x * kR + r) * 16 + (lane & 15);
+      const int b = 4 * i + (lane >> 4);
+      if (n < a.N && b < a.batch) y[b * a.ldy + n] = (Out)sum;
+    }
 }
 
-template <class T, int kR, int kM, int kI, class Out>
+// ---- more rows of activations -----------------------------------------------------------
+//
+// From some rows on the activations are what a CU reads most of, each wave for its own
+// tiles. Here a workgroup of 8 waves goes through 4 tiles of rows in chunks of 2 steps of
+// 128 columns: activations (8 kX rows), weights and scales of a chunk go straight to LDS,
+// the next chunks' in flight meanwhile, a barrier a chunk. A wave takes a tile of one step
+// for all rows of activations, so that each weight is converted once; the two steps' sums
+// are added up in LDS. Workgroups take groups of tiles in turn, their loads going on from
+// one group to the next.
+//
+// In LDS a row's 16 bytes c lie at c ^ (row % 16) of the row, so that 16 lanes that read
+// one place of 16 rows hit all banks.
+constexpr int kTiles = 4, kSteps = 2;
+
+template <int kX>
+struct Gemv4Lds {
+  static constexpr int kM = (kX + 1) / 2;
+  struct Chunk {
+    uint8_t x[8 * kX * kSteps * 256], w[kTiles * kSteps * 1024];
+    uint32_t s[kTiles * kSteps * 16];
+  };
+  float parts[kTiles][kM * 4][64];
+  static constexpr int kFit = (int)((160 * 1024 - sizeof(parts)) / sizeof(Chunk)), kRing = kFit < 4 ? kFit : 4;
+  Chunk chunk[kRing];
+};
+
+// 16 (4) bytes for each lane, from `from` and the lane's offset, to LDS in the lanes' order.
+// (Inline asm: through the compiler's builtin every later LDS read would wait for all loads
+// in flight.)
+__device__ __forceinline__ void load_lds16(const void *from, uint32_t offset, uint32_t to) {
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(offset), "s"(from), "s"(to)
+               : "memory", "m0");
+}
+__device__ __forceinline__ void load_lds4(const void *from, uint32_t offset, uint32_t to) {
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dword %0, %1" ::"v"(offset), "s"(from), "s"(to)
+               : "memory", "m0");
+}
+// Until at most kLeft of the wave's loads are in flight.
+template <int kLeft>
+__device__ __forceinline__ void wait_loads() {
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kLeft) : "memory");
+}
+__device__ __forceinline__ void gemv4_barrier() {
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
+#define SH_GEMV4_LDS __attribute__((address_space(3)))
+// A word through the scalar cache (a vector load's wait would be for the chunks in flight).
+__device__ __forceinline__ uint32_t constant_word(const uint32_t *p) {
+  return *(const __attribute__((address_space(4))) uint32_t *)p;
+}
+
+template <class T, int kX, class Out>
+__global__ __launch_bounds__(512) void gemv4_rows_kernel(const Gemv4Args a) {
+  typedef Gemv4Lds<kX> Lds;
+  typedef typename Lds::Chunk Chunk;
+  typedef typename T::Vec Vec;
+  constexpr int kM = Lds::kM, kRing = Lds::kRing, kRow = kSteps * 256, kPlaces = kSteps * 16;
+  constexpr int kXSlots = 4 * kX, kXLoads = (kXSlots + 7) / 8, kLoads = kXLoads + 2;  // (of the wave; KiB of x)
+  static_assert(kRing >= 2 && (kRing - 1) * kLoads <= 63, "chunks in flight, and what vmcnt counts");
+  __shared__ __attribute__((aligned(16))) Lds lds;
+  const int lane = threadIdx.x & 63, r16 = lane & 15, grp = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), mine = wave % kTiles, step = wave / kTiles;
+  const int groups = (a.row_tiles + kTiles - 1) / kTiles, chunks = (a.col_tiles + kSteps - 1) / kSteps;
+  const int items = (groups - (int)blockIdx.x + (int)gridDim.x - 1) / (int)gridDim.x * chunks;
+  const uint32_t base = (uint32_t)(uintptr_t)(SH_GEMV4_LDS Chunk *)lds.chunk;
+
+  // the next item (a group's chunk) of this workgroup, requested into the next buffer;
+  // behind the last the last again, which nobody reads, so that as many loads are in flight
+  int next_group = blockIdx.x, next_chunk = 0, next_buf = 0;
+  uint32_t x_row[kXLoads], x_col[kXLoads];  // bytes of the lane's row from x, of its columns from the chunk's first
+#pragma unroll
+  for (int u = 0; u < kXLoads; u++) {
+    const int at = min(wave + 8 * u, kXSlots - 1) * 64 + lane, row = at / kPlaces;
+    x_row[u] = (uint32_t)min(row, a.batch - 1) * ((uint32_t)a.ldx * 2);
+    x_col[u] = 16 * (at % kPlaces ^ (row & 15));
+  }
+  auto request = [&]() __attribute__((always_inline)) {
+    const int t0 = next_chunk * kSteps, first = next_group * kTiles;
+    const uint32_t to = base + next_buf * (uint32_t)sizeof(Chunk), x_last = (uint32_t)(a.K - 8 - 128 * t0) * 2;
+    const uint8_t *x = reinterpret_cast<const uint8_t *>(a.x) + (size_t)t0 * 256;
+#pragma unroll
+    for (int u = 0; u < kXLoads; u++)
+      load_lds16(x, x_row[u] + min(x_col[u], x_last), to + offsetof(Chunk, x) + min(wave + 8 * u, kXSlots - 1) * 1024);
+    const int tile = min(first + mine, a.row_tiles - 1), t = min(t0 + step, a.col_tiles - 1);
+    load_lds16(a.w + ((size_t)tile * a.col_tiles + t) * 1024, lane * 16, to + offsetof(Chunk, w) + wave * 1024);
+    // (scales: half of the waves two tiles' two steps each, the others the same)
+    const int s_tile = min(first + mine / 2 * 2, a.row_tiles - 1), s_one = min(s_tile + 1, a.row_tiles - 1) - s_tile;
+    const int s_step = min(t0 + (grp & 1), a.col_tiles - 1);
+    load_lds4(a.scales + (size_t)s_tile * a.col_tiles * 64, ((uint32_t)((grp >> 1) * s_one) * a.col_tiles + s_step) * 64 + r16 * 4,
+              to + offsetof(Chunk, s) + mine / 2 * 256);
+    next_buf = next_buf + 1 == kRing ? 0 : next_buf + 1;
+    if (next_chunk + 1 < chunks)
+      next_chunk++;
+    else if (next_group + (int)gridDim.x < groups) {
+      next_chunk = 0;
+      next_group += gridDim.x;
+    }
+  };
+
+  f32x4 acc[kM];
+  int x_at[kM];
+#pragma unroll
+  for (int m = 0; m < kM; m++) {
+    acc[m] = f32x4{0.f, 0.f, 0.f, 0.f};
+    const int row = min(16 * m + r16, 8 * kX - 1);
+    x_at[m] = row * kRow + step * 256 + ((grp ^ (row & 15)) * 16);
+  }
+  auto compute = [&](const Chunk &c, int t, bool exact) __attribute__((always_inline)) {
+    u32x4 x[4][kM];
+    const u32x4 w = *reinterpret_cast<const u32x4 *>(c.w + wave * 1024 + lane * 16);
+    const uint32_t s = c.s[mine * 32 + step * 16 + r16];
+#pragma unroll
+    for (int j = 0; j < 4; j++)
+#pragma unroll
+      for (int m = 0; m < kM; m++) x[j][m] = *reinterpret_cast<const u32x4 *>(c.x + (x_at[m] ^ (64 * j)));
+    if (128 * t + 128 > a.K) {  // columns behind the last: zeros, whatever x has there
+#pragma unroll
+      for (int j = 1; j < 4; j++)
+#pragma unroll
+        for (int m = 0; m < kM; m++)
+          if (128 * t + 32 * j >= a.K) x[j][m] = u32x4{0, 0, 0, 0};
+    }
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+      const uint32_t exponent = (j == 3 ? s >> 1 : s << (23 - 8 * j)) & 0x7f800000u;
+      const uint32_t normal = exact ? normal_exponent<T>(exponent) : exponent;
+      const Vec wv = from_e2m1<T>(w[j], __builtin_bit_cast(float, normal));
+#pragma unroll
+      for (int m = 0; m < kM; m++) {
+        const Vec xv = __builtin_bit_cast(Vec, x[j][m]);
+        if (exact) {
+          const f32x4 d = T::mfma16(xv, wv, f32x4{0.f, 0.f, 0.f, 0.f});
+          const float rest = __builtin_bit_cast(float, (127u << 23) + exponent - normal);
+#pragma unroll
+          for (int i = 0; i < 4; i++) acc[m][i] = fmaf(d[i], rest, acc[m][i]);
+        } else {
+          acc[m] = T::mfma16(xv, wv, acc[m]);
+        }
+      }
+    }
+  };
+
+#pragma unroll
+  for (int i = 0; i < kRing - 1; i++) request();
+  int group = blockIdx.x, chunk = 0, buf = 0;
+  uint32_t flags = 0;
+  for (int item = 0; item < items; item++) {
+    const int t = chunk * kSteps + step;
+    if (chunk == 0) flags = constant_word(a.flags + min(group * kTiles + mine, a.row_tiles - 1));
+    wait_loads<(kRing - 2) * kLoads>();
+    gemv4_barrier();  // every wave's part of the chunk is here, and the last chunk is read
+    request();
+    if (t < a.col_tiles) {
+      if (flags & (T::kIsF16 ? 1u << 16 : 1u << 17))
+        compute(lds.chunk[buf], t, true);
+      else
+        compute(lds.chunk[buf], t, false);
+    }
+    buf = buf + 1 == kRing ? 0 : buf + 1;
+    if (++chunk < chunks) continue;
+    chunk = 0;
+    if (step == 1) {
+#pragma unroll
+      for (int m = 0; m < kM; m++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) lds.parts[mine][4 * m + i][lane] = acc[m][i];
+    }
+    gemv4_barrier();  // (the parts are read before the next group's last chunk is)
+    if (step == 0) {
+      Out *y = static_cast<Out *>(a.y);
+      const long long n = ((long long)group * kTiles + mine) * 16 + r16;
+#pragma unroll
+      for (int m = 0; m < kM; m++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+          const float sum = (flags >> r16) & 1 ? NAN : acc[m][i] + lds.parts[mine][4 * m + i][lane];
+          const int b = 16 * m + 4 * grp + i;
+          if (n < a.N && b < a.batch) y[b * a.ldy + n] = (Out)sum;
+        }
+    }
+#pragma unroll
+    for (int m = 0; m < kM; m++) acc[m] = f32x4{0.f, 0.f, 0.f, 0.f};
+    group += gridDim.x;
+  }
+  wait_loads<0>();  // (nothing is to arrive in LDS that is another workgroup's)
+}
+
+// Tiles of rows for a workgroup and waves for its columns. Few rows of weights: one, and
+// waves as long as each has a step (us for one row of x, one tile of each 8 waves and four:
+// 1,024 x 2,048 4.2 and 4.6, 4,096 x 4,096 4.7 and 6.8; 12,289 x 8,160 17 and 12.1). Many: four,
+// with a step or two in flight for a wave: one tile of a wave is too little to hide a
+// load's time (151,936 x 1,024: waves of 1, 2, 4 and 8 steps 23, 15.1, 15.7 and 15.8), and from 5
+// rows of x on, which each wave reads, longer ones (16 rows: 22.3 us with 4 waves, 20.4 with
+// one; 12,289 x 8,160 19.8 with 8, 18.0 with 4).
+template <class T, int kI, class Out>
 hipError_t launch_gemv4(hipStream_t st, const Gemv4Args &a) {
-  const int groups = (a.row_tiles + kR - 1) / kR;
-  const int waves = std::max(1, std::min({kMaxWaves, a.col_tiles, 8192 / groups}));
-  gemv4_kernel<T, kR, kM, kI, Out><<<groups, 64 * waves, (size_t)(waves - 1) * kR * kM * kI * 256, st>>>(a);
+  if (a.row_tiles < 512) {
+    const int waves = std::min(kMaxWaves, a.col_tiles);
+    gemv4_kernel<T, 1, kI, Out><<<a.row_tiles, 64 * waves, (size_t)(waves - 1) * kI * 256, st>>>(a);
+  } else {
+    const int waves = kI == 1 ? std::max(1, std::min(8, a.col_tiles / 2)) : std::max(1, std::min(4, a.col_tiles / 8));
+    gemv4_kernel<T, 4, kI, Out><<<(a.row_tiles + 3) / 4, 64 * waves, (size_t)(waves - 1) * 4 * kI * 256, st>>>(a);
+  }
+  return hipGetLastError();
+}
+
+template <class T, int kX, class Out>
+hipError_t launch_gemv4_rows(hipStream_t st, const Gemv4Args &a) {
+  const int groups = (a.row_tiles + kTiles - 1) / kTiles;
+  gemv4_rows_kernel<T, kX, Out><<<std::min(groups, 256), 512, 0, st>>>(a);
   return hipGetLastError();
 }
 
 template <class T, class Out>
 hipError_t launch_gemv4_batch(hipStream_t st, const Gemv4Args &a) {
-  if (a.batch <= 4) return launch_gemv4<T, 2, 1, 1, Out>(st, a);
-  if (a.batch <= 8) return launch_gemv4<T, 2, 1, 2, Out>(st, a);
-  if (a.batch <= 16) return launch_gemv4<T, 2, 1, 4, Out>(st, a);
-  if (a.batch <= 32) return launch_gemv4<T, 2, 2, 4, Out>(st, a);
-  if (a.batch <= 48) return launch_gemv4<T, 2, 3, 4, Out>(st, a);
-  return launch_gemv4<T, 2, 4, 4, Out>(st, a);
+  if (a.batch <= 4) return launch_gemv4<T, 1, Out>(st, a);
+  if (a.batch <= 8) return launch_gemv4<T, 2, Out>(st, a);
+  if (a.batch <= 16) return launch_gemv4<T, 4, Out>(st, a);
+  if (a.batch <= 24) return launch_gemv4_rows<T, 3, Out>(st, a);
+  if (a.batch <= 32) return launch_gemv4_rows<T, 4, Out>(st, a);
+  if (a.batch <= 40) return launch_gemv4_rows<T, 5, Out>(st, a);
+  if (a.batch <= 48) return launch_gemv4_rows<T, 6, Out>(st, a);
+  return launch_gemv4_rows<T, 8, Out>(st, a);
 }
 
 template <class T, class Out>

@@ -120,7 +120,8 @@ def test_products(ctx, dtype, out, n, k, batch):
     check(run(ctx, code, scale, x, dtype, out), code, scale, x, dtype, out)
 
 
-@pytest.mark.parametrize("n,k,batch", [(151_936 // 8, 1024, 1), (40_000, 96, 3), (16, 65_536, 2), (3000, 8160, 37)])
+@pytest.mark.parametrize("n,k,batch", [(151_936 // 8, 1024, 1), (40_000, 96, 3), (16, 65_536, 2), (3000, 8160, 37), (40_000, 96, 9),
+                                       (20_001, 1184, 40), (40_000, 160, 48), (40_000, 160, 64), (40_000, 96, 20), (70_000, 544, 6)])
 def test_products_of_large_matrices(ctx, n, k, batch):
     rng = np.random.default_rng(n)
     code, scale = random_weights(rng, n, k)
