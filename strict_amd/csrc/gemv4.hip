@@ -434,17 +434,18 @@ __global__ __launch_bounds__(512) void gemv4_rows_kernel(const Gemv4Args a) {
   wait_loads<0>();  // (nothing is to arrive in LDS that is another workgroup's)
 }
 
-// Tiles of rows for a workgroup and waves for its columns. Few rows of weights: one, and
-// waves as long as each has a step (us for one row of x, one tile of each 8 waves and four:
-// 1,024 x 2,048 4.2 and 4.6, 4,096 x 4,096 4.7 and 6.8; 12,289 x 8,160 17 and 12.1). Many: four,
-// with a step or two in flight for a wave: one tile of a wave is too little to hide a
-// load's time (151,936 x 1,024: waves of 1, 2, 4 and 8 steps 23, 15.1, 15.7 and 15.8), and from 5
-// rows of x on, which each wave reads, longer ones (16 rows: 22.3 us with 4 waves, 20.4 with
-// one; 12,289 x 8,160 19.8 with 8, 18.0 with 4).
+// Tiles of rows for a workgroup and waves for its columns (measured in us).
+// Few tiles, or little in all: one, and as many waves as there are steps, from 5 rows of x
+// on, which each wave reads, 4 where the tiles fill the card. (One row of x by 4,096 x
+// 4,096: one tile and 8 waves 4.7, four 6.8; 8 rows by 16,384 x 1,024: one tile and 4 waves 5.6,
+// 16 waves 6.4, four tiles 7.6; one row by 8,192 x 4,096 6.9 and 7.1.)
+// More: four, with a few steps for a wave. (One row by 12,289 x 8,160: one tile 17.0, four
+// 12.1; by 151,936 x 1,024 with one step a wave 23, 2 15.1, 4 15.7, 8 15.8; 16 rows by the same
+// 2 steps 22.3, 8 20.4, by 12,289 x 8,160 with 8 waves 19.8, 4 18.0.)
 template <class T, int kI, class Out>
 hipError_t launch_gemv4(hipStream_t st, const Gemv4Args &a) {
-  if (a.row_tiles < 512) {
-    const int waves = std::min(kMaxWaves, a.col_tiles);
+  if (a.row_tiles < 512 || (long long)a.row_tiles * a.col_tiles <= 8192) {
+    const int waves = std::min(kI > 1 && a.row_tiles >= 256 ? 4 : kMaxWaves, a.col_tiles);
     gemv4_kernel<T, 1, kI, Out><<<a.row_tiles, 64 * waves, (size_t)(waves - 1) * kI * 256, st>>>(a);
   } else {
     const int waves = kI == 1 ? std::max(1, std::min(8, a.col_tiles / 2)) : std::max(1, std::min(4, a.col_tiles / 8));
