@@ -673,7 +673,7 @@ typedef struct sh_logit_rules {
   const int32_t *tokens;  /* [rows][max_tokens]: the tokens of each row so far */
   const int32_t *lengths; /* [rows]: how many (needed with tokens) */
   const int32_t *prompts; /* [rows]: how many of the first are the prompt; NULL: none */
-  int max_tokens;
+  int max_tokens; /* at most 2^29 */
   const float *repetition, *frequency, *presence; /* [rows]; NULL: 1, 0, 0 */
   const int32_t *bias_starts; /* [rows + 1]: row r's biases are bias_starts[r] .. [r + 1] - 1 */
   const int32_t *bias_tokens; /* [bias_count] */

@@ -46,15 +46,28 @@ __device__ __forceinline__ TokenPlace token_place(const int *starts, const int *
 // The largest value that E4M3 times a power of two and the 16-bit type both hold: 1.875
 // times the type's largest power of two.
 template <class T>
-constexpr double kLargest8 = T::kIsF16 ? 0x1.ep15 : 0x1.ep127;
+constexpr float kLargest8 = T::kIsF16 ? 0x1.ep15f : 0x1.ep127f;
 
-// The exponent of a row whose largest finite magnitude is `most` (of its kLanes lanes),
-// 448 = 1.75 * 2^8.
-__device__ __forceinline__ int row_exponent(double most) {
-  const uint64_t bits = __builtin_bit_cast(uint64_t, most);
-  const int e = (int)(bits >> 52) - 1023 - 8 + ((bits & 0xfffffffffffffull) > 0xc000000000000ull ? 1 : 0);
-  return max(e, -127);
+// A magnitude in 64 bits as a key that orders as it does: its upper word, and whether there
+// is anything in the lower one. 20 bits behind the point and that bit are what rounding to
+// E4M3's 3, half way to even, can depend on.
+__device__ __forceinline__ uint32_t size_key(double y) {
+  const uint64_t bits = __builtin_bit_cast(uint64_t, y);
+  return ((uint32_t)(bits >> 32) << 1) | min((uint32_t)bits, 1u);
 }
+// The exponent of the scale of a row whose largest key is `most`: 448 = 1.75 * 2^8.
+__device__ __forceinline__ int row_exponent(uint32_t most) {
+  return max((int)(most >> 21) - 1023 - 8 + ((most & 0x1fffff) > 0x180000 ? 1 : 0), -127);
+}
+// Its value times 2^-exponent in fp32, the key's last bit in the fraction. (What is far below
+// E4M3's smallest comes to 0.)
+__device__ __forceinline__ float key_value(double y, uint32_t key, int exponent) {
+  const uint32_t sign = (uint32_t)(__builtin_bit_cast(uint64_t, y) >> 32) & 0x80000000u;
+  return __builtin_bit_cast(float, ((uint32_t)max((int)(key - ((uint32_t)(1023 - 127 + exponent) << 21)), 0) << 2) | sign);
+}
+
+// 2^e, e of -126 .. 127.
+__device__ __forceinline__ float exponent_value(int e) { return __builtin_bit_cast(float, (uint32_t)(127 + e) << 23); }
 
 // To fp32 with the last bit set where something was cut off: rounding that to fewer bits
 // by at least two gives what rounding the fp64 value at once would.
@@ -71,15 +84,41 @@ __device__ __forceinline__ uint32_t to_e4m3(float a, float b, float c, float d) 
   return __builtin_bit_cast(uint32_t, r);
 }
 
-// A wave takes 4 * kHeadsAt heads of one token: q heads, then k, then v. A head is
+// Of kLanes (4 or 8) lanes that follow each other: by lane moves, a fraction of the time of
+// LDS permutes.
+template <int kCtrl>
+__device__ __forceinline__ uint32_t lane_move(uint32_t v) {
+  return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, kCtrl, 0xf, 0xf, false);
+}
+template <int kCtrl>
+__device__ __forceinline__ float lane_move(float v) {
+  return __builtin_bit_cast(float, lane_move<kCtrl>(__builtin_bit_cast(uint32_t, v)));
+}
+template <int kCtrl>
+__device__ __forceinline__ double lane_move(double v) {
+  const uint64_t u = __builtin_bit_cast(uint64_t, v);
+  return __builtin_bit_cast(double, ((uint64_t)lane_move<kCtrl>((uint32_t)(u >> 32)) << 32) | lane_move<kCtrl>((uint32_t)u));
+}
+template <int kLanes, class V, class Op>
+__device__ __forceinline__ V over_lanes(V v, Op op) {
+  v = op(v, lane_move<0xb1>(v));                              // lane ^ 1
+  v = op(v, lane_move<0x4e>(v));                              // lane ^ 2
+  if constexpr (kLanes == 8) v = op(v, lane_move<0x141>(v));  // 7 - lane: the other four
+  return v;
+}
+
+// A wave takes kSteps * kHeadsAt heads of one token: q heads, then k, then v. A head is
 // d / 16 lanes wide, 8 values of its first half and the 8 that rotate with them in each
 // lane, all loads requested at once. q's arithmetic is that of the 16-bit cache's
 // operator. k is normalised and rotated in fp64 (which has fp32's rate here) so that its
 // bytes do not depend on the order of sums: in fp32 one value in 10^6 comes out a step of
-// E4M3, 6 % of it, off.
-template <class T, int kD>
+// E4M3, 6 % of it, off. (Quantised in fp64 too, v as well, and with sums by LDS permutes:
+// 41 us for 9,312 tokens of 16 and 8 heads of 128 and not 28.5, 8.2 us for 3 and not 3.5.)
+// Bound by the bytes: those 9,312 are 172 MB, 6.0 TB/s. (Stores of pages that the caches
+// need not keep take as long, and reading the rows back 14.6 us and not 13.)
+template <class T, int kD, int kSteps>
 __global__ __launch_bounds__(kT) void norm_rope8_kernel(const NormRope8Args a) {
-  constexpr int kLanes = kD / 16, kHeadsAt = 64 / kLanes, kSteps = 4, kHalf = kD / 2;
+  constexpr int kLanes = kD / 16, kHeadsAt = 64 / kLanes, kHalf = kD / 2;
   __shared__ double2 factors[kT / 64][kHalf];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const long long unit = (long long)blockIdx.x * (kT / 64) + wave;
@@ -137,57 +176,106 @@ __global__ __launch_bounds__(kT) void norm_rope8_kernel(const NormRope8Args a) {
     if (h >= all || p.page < 0) continue;
     const bool is_k = h < a.heads + a.kv_heads;
     const int kv_head = h - a.heads - (is_k ? 0 : a.kv_heads);
-    double y1[8], y2[8], most = 0.0;
-#pragma unroll
-    for (int e = 0; e < 8; e++) {
-      y1[e] = x1[e];
-      y2[e] = x2[e];
-    }
+    int exponent = 0;
+    bool plain;  // nothing beyond the largest, or not finite, in the lane: x1, x2 are scaled
     if (is_k) {
-      double ss = 0.0;
+      double y1[8], y2[8], ss = 0.0;
 #pragma unroll
-      for (int e = 0; e < 8; e++) ss = fma(y1[e], y1[e], fma(y2[e], y2[e], ss));
-#pragma unroll
-      for (int off = 1; off < kLanes; off *= 2) ss += __shfl_xor(ss, off, 64);
+      for (int e = 0; e < 8; e++) {
+        y1[e] = x1[e];
+        y2[e] = x2[e];
+        ss = fma(y1[e], y1[e], fma(y2[e], y2[e], ss));
+      }
+      ss = over_lanes<kLanes>(ss, [](double m, double n) { return m + n; });
       const double inv = 1.0 / sqrt(ss * (1.0 / kD) + a.eps);
       const float *gain = a.k_gain + part * 8;
+      uint32_t key1[8], key2[8], most = 0;
 #pragma unroll
       for (int e = 0; e < 8; e++) {
         const double2 f = factors[wave][part * 8 + e];
-        const double z1 = y1[e] * inv * gain[e], z2 = y2[e] * inv * gain[e + kHalf];
-        y1[e] = z1 * f.x - z2 * f.y;
-        y2[e] = z2 * f.x + z1 * f.y;
+        const double z1 = y1[e] * (inv * gain[e]), z2 = y2[e] * (inv * gain[e + kHalf]);
+        y1[e] = fma(z1, f.x, -(z2 * f.y));
+        y2[e] = fma(z2, f.x, z1 * f.y);
+        key1[e] = size_key(y1[e]);
+        key2[e] = size_key(y2[e]);
+        most = max(most, max(key1[e], key2[e]));
+      }
+      most = over_lanes<kLanes>(most, [](uint32_t m, uint32_t n) { return max(m, n); });
+      plain = most <= size_key((double)kLargest8<T>);
+      if (plain) {
+        exponent = row_exponent(most);
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+          x1[e] = key_value(y1[e], key1[e], exponent);
+          x2[e] = key_value(y2[e], key2[e], exponent);
+        }
+      } else {  // (to fp32 for what follows: the last bit stands for all that is cut off)
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+          x1[e] = to_odd(y1[e]);
+          x2[e] = to_odd(y2[e]);
+        }
+      }
+    } else {
+      float most = 0.0f;
+#pragma unroll
+      for (int e = 0; e < 8; e++) most = fmaxf(most, fmaxf(__builtin_fabsf(x1[e]), __builtin_fabsf(x2[e])));
+      most = over_lanes<kLanes>(most, [](float m, float n) { return fmaxf(m, n); });
+      plain = most <= kLargest8<T>;
+      if (plain) {
+        exponent = row_exponent(size_key((double)most));
+        const float to_row = exponent_value(-exponent);
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+          x1[e] *= to_row;
+          x2[e] *= to_row;
+        }
       }
     }
-    // (infinities become NaN, which fmax and the format's rounding pass over and keep)
+    if (!plain) {  // infinities become NaN, which the maximum passes over and the format keeps
+      float most = 0.0f;
 #pragma unroll
-    for (int e = 0; e < 8; e++) {
-      for (double *y : {&y1[e], &y2[e]}) {
-        const double size = fabs(*y);
-        if (size == INFINITY)
-          *y = NAN;
-        else if (size > kLargest8<T>)
-          *y = copysign(kLargest8<T>, *y);
-        most = fmax(most, fabs(*y));
+      for (int e = 0; e < 8; e++) {
+        for (float *y : {&x1[e], &x2[e]}) {
+          const float size = __builtin_fabsf(*y);
+          *y = size == INFINITY ? NAN : size > kLargest8<T> ? copysignf(kLargest8<T>, *y) : *y;
+          most = fmaxf(most, __builtin_fabsf(*y));
+        }
       }
-    }
+      most = over_lanes<kLanes>(most, [](float m, float n) { return fmaxf(m, n); });
+      exponent = row_exponent(size_key((double)most));
+      const float to_row = exponent_value(-exponent);
 #pragma unroll
-    for (int off = 1; off < kLanes; off *= 2) most = fmax(most, __shfl_xor(most, off, 64));
-    const int exponent = row_exponent(most);
-    const double to_row = __builtin_bit_cast(double, (uint64_t)(1023 - exponent) << 52);  // 2^-exponent
-    float z1[8], z2[8];
-#pragma unroll
-    for (int e = 0; e < 8; e++) {
-      z1[e] = to_odd(y1[e] * to_row);
-      z2[e] = to_odd(y2[e] * to_row);
+      for (int e = 0; e < 8; e++) {
+        x1[e] *= to_row;
+        x2[e] *= to_row;
+      }
     }
     const size_t at = ((size_t)kv_head << a.page_shift) + in_page;
     uint8_t *to = page + (is_k ? 0 : v_at) + at * kD + part * 8;
-    const u32x2 b1 = {to_e4m3(z1[0], z1[1], z1[2], z1[3]), to_e4m3(z1[4], z1[5], z1[6], z1[7])};
-    const u32x2 b2 = {to_e4m3(z2[0], z2[1], z2[2], z2[3]), to_e4m3(z2[4], z2[5], z2[6], z2[7])};
+    const u32x2 b1 = {to_e4m3(x1[0], x1[1], x1[2], x1[3]), to_e4m3(x1[4], x1[5], x1[6], x1[7])};
+    const u32x2 b2 = {to_e4m3(x2[0], x2[1], x2[2], x2[3]), to_e4m3(x2[4], x2[5], x2[6], x2[7])};
     *reinterpret_cast<u32x2 *>(to) = b1;
     *reinterpret_cast<u32x2 *>(to + kHalf) = b2;
     if (part == 0) page[2 * v_at + (is_k ? 0 : (size_t)a.kv_heads << a.page_shift) + at] = (uint8_t)(exponent + 127);
+  }
+}
+
+template <class T, int kD>
+void launch_norm_rope8(hipStream_t st, NormRope8Args &a) {
+  constexpr int kHeadsAt = 64 / (kD / 16);
+  const int all = a.heads + 2 * a.kv_heads;
+  const auto grid = [&](int steps) {
+    a.chunks = (all + steps * kHeadsAt - 1) / (steps * kHeadsAt);
+    return (unsigned)(((long long)a.tokens * a.chunks + kT / 64 - 1) / (kT / 64));
+  };
+  // of few tokens a step each, side by side
+  if ((long long)a.tokens * all <= 2048LL * kHeadsAt) {
+    const unsigned blocks = grid(1);
+    norm_rope8_kernel<T, kD, 1><<<blocks, kT, 0, st>>>(a);
+  } else {
+    const unsigned blocks = grid(4);
+    norm_rope8_kernel<T, kD, 4><<<blocks, kT, 0, st>>>(a);
   }
 }
 
@@ -246,14 +334,10 @@ int norm_rope8(sh_ctx *ctx, const sh_paged_kv8 *kv, const uint16_t *qkv, const f
   a.ld = ld;
   a.eps = eps;
   for (int i = 0; i < d / 2; i++) a.freq[i] = std::pow((double)theta, -2.0 * i / d);
-  const int per_unit = 4 * (64 / (d / 16));
-  a.chunks = (heads + 2 * kv->kv_heads + per_unit - 1) / per_unit;
-  const long long units = (long long)tokens * a.chunks;
-  const unsigned grid = (unsigned)((units + kT / 64 - 1) / (kT / 64));
   if (d == 64)
-    norm_rope8_kernel<T, 64><<<grid, kT, 0, stream_of(ctx)>>>(a);
+    launch_norm_rope8<T, 64>(stream_of(ctx), a);
   else
-    norm_rope8_kernel<T, 128><<<grid, kT, 0, stream_of(ctx)>>>(a);
+    launch_norm_rope8<T, 128>(stream_of(ctx), a);
   const hipError_t e = hipGetLastError();
   return e == hipSuccess ? SH_OK : hip_fail(e, "qk_norm_rope_paged8");
 }

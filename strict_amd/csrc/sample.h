@@ -10,6 +10,7 @@ namespace sh {
 
 constexpr int kMaxSampleN = 1 << 20;
 constexpr int kMaxSampleRows = 1 << 16;
+constexpr int kMaxRuleTokens = 1 << 29;
 
 // nullptr, or what is wrong.
 inline const char *check_sample_sizes(int rows, int n, int ld) {
@@ -23,7 +24,7 @@ inline const char *check_logits_sizes(int rows, int n, int ldx, int ldy, const s
   if (const char *wrong = check_sample_sizes(rows, n, ldx)) return wrong;
   if (ldy < n) return "ldy must be at least n";
   if (r->tokens && !r->lengths) return "tokens need lengths";
-  if (r->tokens && r->max_tokens < 0) return "max_tokens must not be negative";
+  if (r->tokens && (r->max_tokens < 0 || r->max_tokens > kMaxRuleTokens)) return "max_tokens must be 0..2^29";
   if (r->bias_starts && r->bias_count < 0) return "bias_count must not be negative";
   if (r->bias_starts && r->bias_count > 0 && (!r->bias_tokens || !r->bias_values))
     return "bias_starts needs bias_tokens and bias_values";
