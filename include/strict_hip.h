@@ -598,7 +598,8 @@ SH_API int sh_paged8_page_bytes(const sh_paged_kv8 *kv, size_t *bytes);
 /* sh_qk_norm_rope_paged_* into such pages (the same q). A row of k or v is stored with
  * the smallest scale 2^e, e >= -127, for which its largest value is at most 448 * 2^e,
  * each value rounded once, to the nearest E4M3 (half way: to the even one); k is worked
- * out in fp64 until then, to 2^-36 of its row's size. Values beyond 1.875 * 2^15 (bf16
+ * out in fp64 until then (to 2^-36 of its row's size, beyond position 2^15 to a step of its
+ * angles). Values beyond 1.875 * 2^15 (bf16
  * 2^127), which the type of q does not hold, count as that; infinities and NaN are
  * stored as NaN and leave the rest of their row as it would be. Two tokens of one page
  * row (a page in two tables) leave values of no meaning there. */

@@ -72,13 +72,13 @@ def device_count() -> int:
     return n.value
 
 
-def _ptr(x) -> ctypes.c_void_p:
+def _ptr(x) -> int | None:
+    """The address of a buffer, an address, or None, as ctypes takes it for a pointer (a
+    c_void_p around it would cost 0.15 us for each argument of a call)."""
     if isinstance(x, DeviceVariable):
-        return ctypes.c_void_p(x.ptr)
-    if isinstance(x, int):
-        return ctypes.c_void_p(x)
-    if x is None:
-        return ctypes.c_void_p(0)
+        return x.ptr
+    if x is None or isinstance(x, int):
+        return x
     raise TypeError(f"expected a DeviceVariable or device address, got {type(x).__name__}")
 
 
@@ -333,6 +333,11 @@ class Context:
         self.handle = ctypes.c_void_p(0)
         _check(self._l.sh_create(device, ctypes.byref(self.handle)))
         self.device = device
+        l = self._l  # operators by their types
+        self._gemv_w4a16 = {("f16", "f16"): l.sh_gemv_w4a16_f16, ("f16", "f32"): l.sh_gemv_w4a16_f16_f32,
+                            ("bf16", "bf16"): l.sh_gemv_w4a16_bf16, ("bf16", "f32"): l.sh_gemv_w4a16_bf16_f32}
+        self._adjust_logits = {"f32": l.sh_adjust_logits_f32, "f16": l.sh_adjust_logits_f16,
+                               "bf16": l.sh_adjust_logits_bf16}
 
     # -- lifetime --
     def dispose(self) -> None:
@@ -510,9 +515,9 @@ class Context:
                    out: str = "f32", ldx: int | None = None, ldy: int | None = None) -> None:
         """y[b] = W x[b] for packed 4-bit weights; x [batch, k] of dtype "f16" or "bf16"
         (rows ldx apart), y [batch, n] (ldy) fp32 or, where `out` is dtype, of that type."""
-        if dtype not in ("f16", "bf16") or out not in ("f32", dtype):
+        f = self._gemv_w4a16.get((dtype, out))
+        if f is None:
             raise ValueError(f"dtype {dtype!r} and out {out!r}: 'f16' or 'bf16', and 'f32' or the same")
-        f = getattr(self._l, f"sh_gemv_w4a16_{dtype}" + ("_f32" if out == "f32" else ""))
         _check(f(self.handle, _ptr(x), k if ldx is None else ldx, _ptr(w_tiled), _ptr(y),
                  n if ldy is None else ldy, batch, k, n))
 
@@ -599,9 +604,10 @@ class Context:
                       ldx: int | None = None, ldy: int | None = None) -> None:
         """y [rows, n] fp32 = logits x of dtype "f32", "f16" or "bf16" by the rules; y may
         be x where that is fp32."""
-        if dtype not in ("f32", "f16", "bf16"):
+        f = self._adjust_logits.get(dtype)
+        if f is None:
             raise ValueError(f"dtype {dtype!r}: 'f32', 'f16' or 'bf16'")
-        _check(getattr(self._l, f"sh_adjust_logits_{dtype}")(
+        _check(f(
             self.handle, _ptr(x), n if ldx is None else ldx, _ptr(y), n if ldy is None else ldy, rows,
             n, rules.address))
 

@@ -333,7 +333,13 @@ int norm_rope8(sh_ctx *ctx, const sh_paged_kv8 *kv, const uint16_t *qkv, const f
   a.kv_heads = kv->kv_heads;
   a.ld = ld;
   a.eps = eps;
-  for (int i = 0; i < d / 2; i++) a.freq[i] = std::pow((double)theta, -2.0 * i / d);
+  // (a power for each took a third of the call's time on the host)
+  double eights[8];
+  for (int i = 0; i < d / 16; i++) eights[i] = std::pow((double)theta, -16.0 * i / d);
+  for (int j = 0; j < 8; j++) {
+    const double one = std::pow((double)theta, -2.0 * j / d);
+    for (int i = 0; i < d / 16; i++) a.freq[8 * i + j] = eights[i] * one;
+  }
   if (d == 64)
     launch_norm_rope8<T, 64>(stream_of(ctx), a);
   else
