@@ -437,10 +437,11 @@ SH_API int sh_pack_e2m1_tiles(sh_ctx *ctx, const uint8_t *q, const uint8_t *scal
                               uint8_t *tiled);
 
 /* W4A16 GEMV / skinny GEMM: y[b * ldy + n] = sum_k x[b * ldx + k] * w[n][k] for b < batch
- * (1..64); x fp16 or bf16, fp32 accumulation of exact products, y of x's type (rounded once)
- * or fp32. Weights and scales of any values; a row with a scale of 255 gives NaN. ldx a multiple of 8, at least K and at
- * most 2^25, ldy at least N; x and
- * w_tiled 16-byte aligned. y overlaps neither. */
+ * (1..64); x fp16 or bf16, fp32 accumulation of exact products (a sum's size leaves fp32's
+ * range where its terms' sizes add up beyond it), y of x's type (rounded once) or fp32.
+ * Weights and scales of any values; a row with a scale of 255 gives NaN. ldx a multiple of
+ * 8, at least K and at most 2^25, ldy at least N; x and w_tiled 16-byte aligned. y overlaps
+ * neither. */
 SH_API int sh_gemv_w4a16_f16(sh_ctx *ctx, const uint16_t *x, int ldx, const uint8_t *w_tiled,
                              uint16_t *y, int ldy, int batch, int K, int N);
 SH_API int sh_gemv_w4a16_bf16(sh_ctx *ctx, const uint16_t *x, int ldx, const uint8_t *w_tiled,
