@@ -295,6 +295,25 @@ __global__ __launch_bounds__(kT, kSmall.workers / 256) void paged8_small_kernel(
   work_piece<false, 1, 1>(a, plan, [&](const PieceStep &st, Line) { return attn_small8<T, kD>(a, st.tile, st.span, st.u0, st.u1, st.slot, lds); });
 }
 
+// A call whose tiles are not cut: nothing is left to merge, and a workgroup does again
+// itself what is not sound.
+template <class T, int kD>
+__global__ __launch_bounds__(kT, kSmall.workers / 256) void paged8_whole_kernel(const Attn8Args a) {
+  __shared__ __attribute__((aligned(16))) SmallLds8<T, kD> lds;
+  __shared__ PlanLds plan;
+  int worker = blockIdx.x;
+  MergeItem unused;
+  if (walk_piece<false, true>(a.plan, &worker, plan, &unused, [&](const PieceStep &st, Line) {
+        return attn_small8<T, kD>(a, st.tile, st.span, st.u0, st.u1, -1, lds);
+      }))
+    return;
+  __syncthreads();  // the plan is read
+  walk_piece<false, true>(a.plan, &worker, plan, &unused, [&](const PieceStep &st, Line) {
+    attn_exact<Pages8<T>, kD>(a, st.tile, st.span);
+    return true;
+  });
+}
+
 // ---- tiles of up to 128 rows ------------------------------------------------------------
 //
 // As the kernel of 16-bit pages (paged_attn.hip): four waves of 32 rows share K and V units
@@ -566,8 +585,24 @@ __global__ __launch_bounds__(kT, kLarge.workers / 256) void paged8_large_kernel(
 
 // ---- the entry points ---------------------------------------------------------------
 
+// Tiles of up to 16 rows whose sequences have at most two units for each of the four waves
+// (512 positions at head_dim 128) are not cut: what is cut needs a merge, whose launch takes
+// longer than the positions do. A decode row each over 128, 512 and 1,024 positions at most,
+// cut and not, us a call: 1 sequence of 8 KV heads of 128 13.0 and 7.1, 13.2 and 9.8, 13.7
+// and 14.0; 4 of 2 17.1 and 9.2, 16.6 and 11.5, 16.7 and 14.9; 16 of 8 15.3 and 12.9, 18.8
+// and 19.1, 20.8 and 26.7; 48 of 8 19.4 and 14.5, 24.6 and 23.9, 30.6 and 34.0. Of heads of
+// 64, 1 sequence of 12 over 1,024 13.5 and 10.2, 64 of 12 38.1 and 34.8. (Tiles of up to 128
+// rows gain nothing: 8 sequences of 128 new tokens 13.3 and 18.5.)
 template <class T, int kD>
-void launch8(hipStream_t st, const Attn8Args &a) {
+void launch8(hipStream_t st, Attn8Args &a) {
+  if (a.tile_rows == kSmall.rows && a.plan.capacity <= 8 * kSmallUnit8<kD>) {
+    PagedPlan &p = a.plan;  // a worker per tile, and a few
+    const int tile = p.capacity + p.per_tile + kTileFixedCost;
+    p.workers = plan_workers(p.batch, p.kv_heads, p.tokens, p.capacity, p.per_tile, tile, kSmall.workers);
+    p.inv_workers = 1.0 / p.workers;
+    paged8_whole_kernel<T, kD><<<p.workers, kT, 0, st>>>(a);
+    return;
+  }
   const int workers = a.plan.workers;
   if (a.tile_rows == kSmall.rows) {
     paged8_small_kernel<T, kD><<<workers, kT, 0, st>>>(a);

@@ -348,6 +348,44 @@ def test_one_long_sequence_among_short_ones(ctx):
     paged.check_attention(Case8(ctx, 15, "bf16", [1] * 9, [30000] + [5] * 8, 8, 1, 128, 64))
 
 
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("heads,kv_heads,d", [(16, 8, 128), (12, 12, 64), (15, 1, 128), (8, 4, 64)])
+@pytest.mark.parametrize("positions,new", [(256, [1] * 9), (512, [1, 0, 1, 1]), (512, [8, 3, 1, 15, 0, 2]), (528, [1, 2, 1]), (1024, [1, 1])])
+@pytest.mark.parametrize("window,sinks", [(0, 0), (50, 3)])
+def test_short_caches(ctx, dtype, heads, kv_heads, d, positions, new, window, sinks):
+    # tables of up to 512 positions at head_dim 128 and 1,024 at 64, and longer ones
+    rng = np.random.default_rng(positions + heads)
+    lengths = [int(rng.integers(max(n, 1), positions - 15)) for n in new]
+    lengths[0] = positions - 16  # (a Case's tables have a page more)
+    c = Case8(ctx, positions + d, dtype, new, lengths, heads, kv_heads, d, 16)
+    assert c.max_pages * c.page == positions
+    paged.check_attention(c, window=window, sinks=sinks)
+    if new[0] > 1:  # more tokens than positions: the first ones see nothing
+        c.lengths[0], c.lengths[1] = 5, 0
+        paged.check_attention(c, window=window, sinks=sinks)
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("d", [64, 128])
+def test_not_numbers_and_large_scores_in_short_caches(ctx, dtype, d):
+    # 700 tiles for at most 512 workgroups: those that share one with a NaN stay right
+    lengths = [3 + 17 * i % 180 for i in range(350)]
+    c = Case8(ctx, d, dtype, [1] * 350, lengths, 4, 2, d, 16)
+    assert c.max_pages * c.page <= 256
+    page, at = c.table[17, 0], 2
+    c.kb[page, 0, at, 3] = 127
+    page, at = c.table[40, 0], 1
+    c.vs[page, 1, at] = 255
+    q, got = paged.run_attention(c)
+    ref, tol = paged.attention_oracle(c, from16(q, dtype), 0, 0, d ** -0.5)
+    out, sound = from16(got, dtype)[:350], np.ones((350, 4), bool)
+    sound[17, :2] = sound[40, 2:] = False
+    assert np.isnan(out[~sound]).all()
+    assert (np.abs(out - ref[:350]) <= tol[:350])[sound].all()
+    large = Case8(ctx, d + 1, dtype, [1, 2, 1], [100, 60, 2], 4, 2, d, 16, scale=1.0)
+    paged.check_attention(large, scale=300.0)
+
+
 @pytest.mark.parametrize("group", [17, 128])
 def test_many_query_heads(ctx, group):
     paged.check_attention(Case8(ctx, 16, "f16", [3, 1], [120, 300], group, 1, 64, 16))
