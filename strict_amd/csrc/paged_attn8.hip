@@ -585,25 +585,28 @@ __global__ __launch_bounds__(kT, kLarge.workers / 256) void paged8_large_kernel(
 
 // ---- the entry points ---------------------------------------------------------------
 
-// Tiles of up to 16 rows whose sequences have at most two units for each of the four waves
-// (512 positions at head_dim 128) are not cut: what is cut needs a merge, whose launch takes
+// Tiles of up to 16 rows that see at most two units for each of the four waves (512
+// positions at head_dim 128) are not cut: what is cut needs a merge, whose launch takes
 // longer than the positions do. A decode row each over 128, 512 and 1,024 positions at most,
 // cut and not, us a call: 1 sequence of 8 KV heads of 128 13.0 and 7.1, 13.2 and 9.8, 13.7
 // and 14.0; 4 of 2 17.1 and 9.2, 16.6 and 11.5, 16.7 and 14.9; 16 of 8 15.3 and 12.9, 18.8
 // and 19.1, 20.8 and 26.7; 48 of 8 19.4 and 14.5, 24.6 and 23.9, 30.6 and 34.0. Of heads of
-// 64, 1 sequence of 12 over 1,024 13.5 and 10.2, 64 of 12 38.1 and 34.8. (Tiles of up to 128
+// 64, 1 sequence of 12 over 1,024 13.5 and 10.2, 64 of 12 38.1 and 34.8. With a window of
+// 256 of up to 4,096 positions, 16 of 8 KV heads of 128 20.0 and 12.0. (Tiles of up to 128
 // rows gain nothing: 8 sequences of 128 new tokens 13.3 and 18.5.)
 template <class T, int kD>
 void launch8(hipStream_t st, Attn8Args &a) {
-  if (a.tile_rows == kSmall.rows && a.plan.capacity <= 8 * kSmallUnit8<kD>) {
-    PagedPlan &p = a.plan;  // a worker per tile, and a few
-    const int tile = p.capacity + p.per_tile + kTileFixedCost;
-    p.workers = plan_workers(p.batch, p.kv_heads, p.tokens, p.capacity, p.per_tile, tile, kSmall.workers);
+  PagedPlan &p = a.plan;
+  const int seen = p.window > 0 ? (int)std::min((long long)p.sinks + p.window, (long long)p.capacity) : p.capacity;
+  if (a.tile_rows == kSmall.rows && seen <= 8 * kSmallUnit8<kD>) {
+    // a worker per tile, and a few
+    const int tile = seen + p.per_tile + kTileFixedCost;
+    p.workers = plan_workers(p.batch, p.kv_heads, p.tokens, seen, p.per_tile, tile, kSmall.workers);
     p.inv_workers = 1.0 / p.workers;
     paged8_whole_kernel<T, kD><<<p.workers, kT, 0, st>>>(a);
     return;
   }
-  const int workers = a.plan.workers;
+  const int workers = p.workers;
   if (a.tile_rows == kSmall.rows) {
     paged8_small_kernel<T, kD><<<workers, kT, 0, st>>>(a);
     paged_merge_small_kernel<Pages8<T>, kD><<<workers, kMergeT, 0, st>>>(a);

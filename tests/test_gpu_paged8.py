@@ -262,6 +262,13 @@ def test_window_and_sinks(ctx, heads, kv_heads, d, new, window, sinks):
                           window=window, sinks=sinks)
 
 
+@pytest.mark.parametrize("heads,kv_heads,d", [(8, 4, 128), (6, 2, 64)])
+@pytest.mark.parametrize("window,sinks", [(500, 12), (500, 13), (1000, 24), (1024, 300)])
+def test_long_windows_and_sinks(ctx, heads, kv_heads, d, window, sinks):
+    paged.check_attention(Case8(ctx, window + sinks, "f16", [1, 2, 1, 0, 1], [3000, 1030, 600, 5, 1], heads, kv_heads, d, 16),
+                          window=window, sinks=sinks)
+
+
 @pytest.mark.parametrize("new", [[1, 1, 1, 1], [40, 9, 2, 30]])
 def test_rows_that_see_nothing_and_bad_pages(ctx, new):
     c = Case8(ctx, 5, "f16", new, [200, 90, 20, 120], 4, 2, 64, 16)
