@@ -198,15 +198,20 @@ class LogitRules:
     [rows]; bias_tokens and bias_values [bias_count] with bias_starts [rows + 1]; masks
     [num_masks, (n + 31) // 32] of bits with mask_of [rows]."""
 
-    def __init__(self, *, tokens=None, max_tokens: int = 0, lengths=None, prompts=None,
+    def __init__(self, *, tokens=None, max_tokens: int | None = None, lengths=None, prompts=None,
                  repetition=None, frequency=None, presence=None, bias_starts=None,
-                 bias_tokens=None, bias_values=None, bias_count: int = 0, masks=None,
-                 mask_of=None, num_masks: int = 0):
+                 bias_tokens=None, bias_values=None, bias_count: int | None = None, masks=None,
+                 mask_of=None, num_masks: int | None = None):
+        for array, size, name in ((tokens, max_tokens, "tokens need max_tokens"),
+                                  (bias_starts, bias_count, "bias_starts needs bias_count"),
+                                  (masks, num_masks, "masks need num_masks")):
+            if array is not None and size is None:
+                raise ValueError(name)
         # kept alive with the struct
         self.buffers = (tokens, lengths, prompts, repetition, frequency, presence, bias_starts,
                         bias_tokens, bias_values, masks, mask_of)
         p = [_ptr(b) for b in self.buffers]
-        self.struct = _lib.LogitRules(*p[:3], max_tokens, *p[3:9], bias_count, *p[9:], num_masks)
+        self.struct = _lib.LogitRules(*p[:3], max_tokens or 0, *p[3:9], bias_count or 0, *p[9:], num_masks or 0)
         self.address = ctypes.byref(self.struct)
 
 
@@ -574,6 +579,8 @@ class Context:
     def paged_read(self, kv: PagedKV8, k, v, tokens: int) -> None:
         """The rows of the call's new tokens read back from the pages: k, v
         [tokens, kv_heads, d] of the values that the bytes stand for."""
+        if not isinstance(kv, PagedKV8):
+            raise TypeError("paged_read takes a PagedKV8")
         _check(kv.read(self.handle, kv.address, _ptr(k), _ptr(v), tokens))
 
     def attn_paged_workspace(self, kv: PagedKV | PagedKV8, tokens: int, heads: int, max_new: int) -> int:
