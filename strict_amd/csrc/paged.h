@@ -306,20 +306,6 @@ SH_HD PieceStep plan_step(const PagedPlan &p, const PagedTile &t, Line piece, in
   return r;
 }
 
-// The step at point x of a piece from x0 on in a call whose tiles are not cut: a tile is
-// the worker's in whose piece it begins.
-SH_HD PieceStep plan_step_whole(const PagedPlan &p, const PagedTile &t, Line x0, Line x) {
-  PieceStep r;
-  r.tile = t;
-  r.span = plan_span(p, t);
-  r.more = x < t.begin + t.cost;
-  r.u0 = 0;
-  r.u1 = r.span.units;
-  r.slot = -1;
-  r.run = r.span.count > 0 && t.begin >= x0;
-  return r;
-}
-
 // ---- argument checks that need no device -------------------------------------------
 
 // nullptr, or what is wrong with the cache's sizes.

@@ -288,8 +288,7 @@ __device__ __forceinline__ int worker_by_xcd(const PagedPlan &p, Line total, Lin
 
 // A worker's piece, step by step: part(step), which says whether its results are
 // sound: finite, of sums and scores that fit. Returns whether all are. kByXcd: *worker is to be found.
-// kWhole: no tile is cut (*item is not written).
-template <bool kByXcd, bool kWhole = false, class Part>
+template <bool kByXcd, class Part>
 __device__ __forceinline__ bool walk_piece(const PagedPlan &p, int *worker, PlanLds &lds, MergeItem *item, Part part) {
   const int per = (p.batch + kT - 1) / kT;
   scan_costs(p, per, lds);
@@ -305,7 +304,7 @@ __device__ __forceinline__ bool walk_piece(const PagedPlan &p, int *worker, Plan
   while (uniform(x < end ? 1 : 0)) {
     const int i = uniform(find_part(lds, x)), b = plan_part_first(p, i, per);
     const PagedTile t = plan_locate(p, per == 1 ? lds.seqs[b] : plan_sequence(p, b), i, per, lds.prefix[i], x);
-    PieceStep st = kWhole ? plan_step_whole(p, t, x0, x) : plan_step(p, t, piece, me, x0, x, item);
+    PieceStep st = plan_step(p, t, piece, me, x0, x, item);
     for (int *v : {&st.tile.seq.row0, &st.tile.seq.n, &st.tile.seq.len, &st.tile.b, &st.tile.kv_head, &st.tile.tile,
                    &st.span.first, &st.span.count, &st.span.pos0, &st.span.lo, &st.span.hi, &st.span.sinks,
                    &st.span.units, &st.span.sink_units, &st.span.gap, &st.u0, &st.u1, &st.slot})

@@ -1,6 +1,6 @@
 // Attention of new tokens over a KV cache in pages of 8-bit values (sh_attn_paged8_*): the
-// kernels that read such pages. How a call is divided, the merge and the tiles that
-// matrix products cannot do are those of 16-bit pages (paged_attn.h).
+// kernels that read such pages. How a call of many positions is divided, the merge and the
+// tiles that matrix products cannot do are those of 16-bit pages (paged_attn.h).
 //
 // A byte times its row's power of two is a value of the 16-bit type but for that type's
 // range, so the products, the softmax and their roundings are the same; only half the
@@ -295,23 +295,32 @@ __global__ __launch_bounds__(kT, kSmall.workers / 256) void paged8_small_kernel(
   work_piece<false, 1, 1>(a, plan, [&](const PieceStep &st, Line) { return attn_small8<T, kD>(a, st.tile, st.span, st.u0, st.u1, st.slot, lds); });
 }
 
-// A call whose tiles are not cut: nothing is left to merge, and a workgroup does again
-// itself what is not sound.
+// The sequence's tile without a place on the line (its units are all one workgroup's).
+__device__ __forceinline__ PagedTile whole_tile(const Attn8Args &a, int b, int kv_head) {
+  PagedTile t;
+  t.seq = plan_seq(a.plan, b);
+  for (int *v : {&t.seq.row0, &t.seq.n, &t.seq.len}) *v = uniform(*v);
+  t.b = b;
+  t.kv_head = kv_head;
+  t.tile = 0;
+  t.begin = t.cost = 0;
+  return t;
+}
+
+// A call whose tiles are not cut: a workgroup a sequence and KV head (of as many new tokens
+// as were announced one tile), nothing to plan and nothing to merge. What is not sound it
+// does again.
 template <class T, int kD>
-__global__ __launch_bounds__(kT, kSmall.workers / 256) void paged8_whole_kernel(const Attn8Args a) {
+__global__ __launch_bounds__(kT, kSmall.workers / 256) void paged8_small_whole_kernel(const Attn8Args a) {
   __shared__ __attribute__((aligned(16))) SmallLds8<T, kD> lds;
-  __shared__ PlanLds plan;
-  int worker = blockIdx.x;
-  MergeItem unused;
-  if (walk_piece<false, true>(a.plan, &worker, plan, &unused, [&](const PieceStep &st, Line) {
-        return attn_small8<T, kD>(a, st.tile, st.span, st.u0, st.u1, -1, lds);
-      }))
-    return;
-  __syncthreads();  // the plan is read
-  walk_piece<false, true>(a.plan, &worker, plan, &unused, [&](const PieceStep &st, Line) {
-    attn_exact<Pages8<T>, kD>(a, st.tile, st.span);
-    return true;
-  });
+  for (int b = blockIdx.y; b < a.plan.batch; b += gridDim.y) {
+    PagedTile t = whole_tile(a, b, blockIdx.x);
+    const int tiles = plan_tiles(a.plan, t.seq);
+    for (; t.tile < tiles; t.tile++) {
+      const TileSpan s = plan_span(a.plan, t);
+      if (!attn_small8<T, kD>(a, t, s, 0, s.units, -1, lds)) attn_exact<Pages8<T>, kD>(a, t, s);
+    }
+  }
 }
 
 // ---- tiles of up to 128 rows ------------------------------------------------------------
@@ -583,37 +592,123 @@ __global__ __launch_bounds__(kT, kLarge.workers / 256) void paged8_large_kernel(
   });
 }
 
+// Sum of lanes 0 .. own, at most `most`, by lane moves as in wave_scan_line.
+__device__ __forceinline__ int scan_most(int v, int most) {
+  const auto add = [&](int moved) { v = min(v + moved, most); };
+  add(__builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false));
+  add(__builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false));
+  add(__builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false));
+  add(__builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false));
+  add(__builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false));
+  add(__builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false));
+  return v;
+}
+
+// The sequence of tile `at` of all sequences' tiles, fewer than `most`, and how many of its
+// tiles come behind that; -1: there is no such tile. The longest come first: of up to 64
+// sequences the last tile of each, then the last but one, and so on; of more, sequence by
+// sequence. A wave looks at 64 numbers at once.
+constexpr int kMaxWholeBatch = 4096;
+__device__ __forceinline__ int find_tile(const PagedPlan &p, int at, int most, int *back) {
+  const int lane = threadIdx.x & 63, per = (p.batch + 63) / 64;
+  const auto tiles = [&](int b) {
+    const int from = clamp_int(p.starts[b], 0, p.tokens), end = clamp_int(p.starts[b + 1], from, p.tokens);
+    return (end - from + p.per_tile - 1) / p.per_tile;
+  };
+  if (per == 1) {
+    const int mine = lane < p.batch ? tiles(lane) : 0;
+    // tiles with fewer than n behind them
+    const auto behind = [&](int n) { return __builtin_amdgcn_readlane(scan_most(min(mine, n), most), 63); };
+    int n = 0, end = most;  // behind(n) <= at < behind(end)
+    if (behind(end) <= at) return -1;
+    while (end - n > 1) {
+      const int mid = (n + end) / 2;
+      if (behind(mid) <= at)
+        n = mid;
+      else
+        end = mid;
+    }
+    *back = n;
+    const int which = at - behind(n);  // (with all lanes)
+    const uint64_t those = __ballot(mine > n);
+    const int rank = (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(those >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)those, 0));
+    return __builtin_ctzll(__ballot(mine > n && rank == which));
+  }
+  int first = 0;
+  for (int step = per;; step = 1) {  // a 64th of the sequences in each lane, then one
+    int sum = 0;
+    for (int i = 0; i < step; i++) {
+      const int b = first + lane * step + i;
+      if (b < p.batch && (step == per || lane < per)) sum = min(sum + tiles(b), most);
+    }
+    const int up_to = scan_most(sum, most);
+    const int before = __popcll(__ballot(up_to <= at));
+    if (before == 64) return -1;
+    at -= before == 0 ? 0 : __builtin_amdgcn_readlane(up_to, before - 1);
+    first += before * step;
+    if (step == 1) break;
+  }
+  *back = at;
+  return first;
+}
+
+// A call whose tiles are not cut: a workgroup a tile. (With places between the sequences that have no tile, so that no sums were
+// needed, 16 sequences of 256 new tokens took 67 us and not 49: which CU a workgroup goes to
+// is settled by its number, and some had two rounds.)
+template <class T, int kD>
+__global__ __launch_bounds__(kT, kLarge.workers / 256) void paged8_large_whole_kernel(const Attn8Args a, int most) {
+  __shared__ __attribute__((aligned(16))) LargeLds8<kD> lds;
+  for (int tile = blockIdx.y; tile < most; tile += gridDim.y) {
+    int back = 0;
+    const int b = uniform(find_tile(a.plan, tile, most, &back));
+    if (b < 0) return;
+    PagedTile t = whole_tile(a, b, blockIdx.x);
+    t.tile = plan_tiles(a.plan, t.seq) - 1 - uniform(back);
+    const TileSpan s = plan_span(a.plan, t);
+    if (!attn_large8<T, kD>(a, t, s, 0, s.units, -1, lds)) attn_exact<Pages8<T>, kD>(a, t, s);
+  }
+}
+
 // ---- the entry points ---------------------------------------------------------------
 
-// Tiles of up to 16 rows that see at most two units for each of the four waves (512
-// positions at head_dim 128) are not cut: what is cut needs a merge, whose launch takes
-// longer than the positions do. A decode row each over 128, 512 and 1,024 positions at most,
-// cut and not, us a call: 1 sequence of 8 KV heads of 128 13.0 and 7.1, 13.2 and 9.8, 13.7
-// and 14.0; 4 of 2 17.1 and 9.2, 16.6 and 11.5, 16.7 and 14.9; 16 of 8 15.3 and 12.9, 18.8
-// and 19.1, 20.8 and 26.7; 48 of 8 19.4 and 14.5, 24.6 and 23.9, 30.6 and 34.0. Of heads of
-// 64, 1 sequence of 12 over 1,024 13.5 and 10.2, 64 of 12 38.1 and 34.8. With a window of
-// 256 of up to 4,096 positions, 16 of 8 KV heads of 128 20.0 and 12.0. (Tiles of up to 128
-// rows gain nothing: 8 sequences of 128 new tokens 13.3 and 18.5.)
+// Where tiles see few positions they are not cut: to plan the pieces takes 4 us, and the
+// merge, a launch that reads all parts, 4 to 50. Up to 16 units (1,024 positions, of 16-row
+// tiles at head_dim 64 2,048) always, up to 32 where there are tiles for every CU, so that
+// a long one matters less. Cut and not, us a call:
+// - a token each, 16-row tiles: 1 sequence of 8 KV heads of 128 over 128 positions 13.1 and
+//   5.6, 512 13.3 and 8.5, 1,024 13.7 and 12.5, 2,048 13.7 and 19.1; 48 of them over up to
+//   256 22.1 and 10.5, 1,024 30.6 and 23.0, 2,048 42.1 and 37.4, 4,096 69.6 and 68.9; 64 of
+//   12 KV heads of 64 over up to 512 29.5 and 19.9, 2,048 47.5 and 41.2; a window of 256 of
+//   up to 4,096, 16 of 8 KV heads of 128 20.0 and 11.0;
+// - chunks, 128-row tiles: 8 prompts of 512 of 12 KV heads of 64 36.7 and 20.5, 1 of 1,024 23.6
+//   and 25.8; of 8 KV heads of 128, 512 new tokens after 512 29.8 and 32.8, after 1,536 40 and
+//   56, 16 times 256 after up to 768 88 and 51, 4 prompts of 2,048 149 and 106, 4 of 4,096 408
+//   and 322, but 40 times 64 after up to 4,032 122 and 145; 63 single tokens and a prompt of
+//   1,024 83 and 58.
+// (Eight waves for a 16-row tile: as long, a CU reads no faster. Tiles not cut but on planned
+// pieces: 1 sequence over 128 7.1, 16 14.4, 8 prompts of 512 38.)
 template <class T, int kD>
-void launch8(hipStream_t st, Attn8Args &a) {
-  PagedPlan &p = a.plan;
-  const int seen = p.window > 0 ? (int)std::min((long long)p.sinks + p.window, (long long)p.capacity) : p.capacity;
-  if (a.tile_rows == kSmall.rows && seen <= 8 * kSmallUnit8<kD>) {
-    // a worker per tile, and a few
-    const int tile = seen + p.per_tile + kTileFixedCost;
-    p.workers = plan_workers(p.batch, p.kv_heads, p.tokens, seen, p.per_tile, tile, kSmall.workers);
-    p.inv_workers = 1.0 / p.workers;
-    paged8_whole_kernel<T, kD><<<p.workers, kT, 0, st>>>(a);
+void launch8(hipStream_t st, const Attn8Args &a) {
+  const PagedPlan &p = a.plan;
+  const bool small = a.tile_rows == kSmall.rows;
+  const long long seen = p.window > 0 ? std::min((long long)p.sinks + p.window, (long long)p.capacity) : p.capacity;
+  const long long tiles = (long long)std::max(p.batch, p.tokens / p.per_tile) * p.kv_heads;
+  if ((small || p.batch <= kMaxWholeBatch) && seen <= (tiles >= 256 ? 32 : 16) * p.unit) {
+    if (small) {
+      paged8_small_whole_kernel<T, kD><<<dim3(p.kv_heads, std::min(p.batch, 32768)), kT, 0, st>>>(a);
+    } else {
+      const int most = p.batch + p.tokens / p.per_tile;
+      paged8_large_whole_kernel<T, kD><<<dim3(p.kv_heads, std::min(most, 32768)), kT, 0, st>>>(a, most);
+    }
     return;
   }
-  const int workers = p.workers;
-  if (a.tile_rows == kSmall.rows) {
-    paged8_small_kernel<T, kD><<<workers, kT, 0, st>>>(a);
-    paged_merge_small_kernel<Pages8<T>, kD><<<workers, kMergeT, 0, st>>>(a);
-    return;
+  if (small) {
+    paged8_small_kernel<T, kD><<<p.workers, kT, 0, st>>>(a);
+    paged_merge_small_kernel<Pages8<T>, kD><<<p.workers, kMergeT, 0, st>>>(a);
+  } else {
+    paged8_large_kernel<T, kD><<<p.workers, kT, 0, st>>>(a);
+    paged_merge_large_kernel<Pages8<T>, kD><<<std::max(p.workers, 1024), kT, 0, st>>>(a);
   }
-  paged8_large_kernel<T, kD><<<workers, kT, 0, st>>>(a);
-  paged_merge_large_kernel<Pages8<T>, kD><<<std::max(workers, 1024), kT, 0, st>>>(a);
 }
 
 template <class T>

@@ -355,6 +355,63 @@ def test_one_long_sequence_among_short_ones(ctx):
     paged.check_attention(Case8(ctx, 15, "bf16", [1] * 9, [30000] + [5] * 8, 8, 1, 128, 64))
 
 
+# Tables of 300 pages more than are used: sequences that could be long, whose tiles are cut.
+WIDE = dict(page=16, extra_entries=300)
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("heads,kv_heads,d", [(16, 8, 128), (12, 12, 64), (15, 1, 128), (4, 4, 64)])
+@pytest.mark.parametrize("new,lengths", [([1] * 7, [777, 1, 64, 65, 128, 300, 2129]), ([130], [130]), ([33, 0, 1, 200], [500, 40, 1, 201]),
+                                         ([5, 64, 17, 128], [5, 64, 900, 2500])])
+def test_wide_tables(ctx, dtype, heads, kv_heads, d, new, lengths):
+    paged.check_attention(Case8(ctx, sum(new) + d, dtype, new, lengths, heads, kv_heads, d, first_row=2, **WIDE))
+
+
+@pytest.mark.parametrize("new", [[1, 1, 1, 1], [40, 9, 2, 30]])
+@pytest.mark.parametrize("window,sinks", [(0, 0), (20, 3), (5000, 5)])
+def test_bad_pages_in_wide_tables(ctx, new, window, sinks):
+    c = Case8(ctx, 5, "bf16", new, [200, 90, 20, 120], 4, 2, 128, **WIDE)
+    c.table[0, [0, 3, 4]] = -1, c.num_pages, np.iinfo(np.int32).min
+    c.table[1, :] = -7
+    c.lengths[2] = min(2, new[2] - 1) if new[2] > 1 else 0
+    c.table[3, 1:7] = 1 << 30
+    paged.check_attention(c, window=window, sinks=sinks)
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("new", [[1, 1], [40, 5]])
+@pytest.mark.parametrize("extra", [1, 300])
+@pytest.mark.parametrize("d", [64, 128])
+def test_not_numbers_that_rows_see(ctx, dtype, new, extra, d):
+    # the last token's k and v are NaN: tokens before it and other sequences must not notice
+    c = Case8(ctx, 11, dtype, new, [90, 50], 4, 2, d, 16, extra_entries=extra)
+    page, at = c.table[0, 89 // 16], 89 % 16
+    c.kb[page, :, at, :3] = 127
+    c.vs[page, :, at] = 255
+    q, got = paged.run_attention(c)
+    ref, tol = paged.attention_oracle(c, from16(q, dtype), 0, 0, d ** -0.5)
+    out, last = from16(got, dtype), new[0] - 1
+    for rows in (slice(0, last), slice(new[0], sum(new))):
+        assert (np.abs(out[rows] - ref[rows]) <= tol[rows]).all()
+    assert np.isnan(out[last]).all()
+
+
+@pytest.mark.parametrize("lengths,new,max_new", [([300, 50, 700], [100, 3, 1], 1), ([300, 50, 700], [100, 3, 300], 33)])
+@pytest.mark.parametrize("extra", [1, 300])
+def test_more_tokens_than_announced(ctx, lengths, new, max_new, extra):
+    paged.check_attention(Case8(ctx, 14, "f16", new, lengths, 6, 2, 128, 16, extra_entries=extra), max_new=max_new)
+
+
+@pytest.mark.parametrize("batch,lengths,most", [(70, (0, 60), 40), (700, (0, 60), 30), (200, (100, 500), 3)])
+@pytest.mark.parametrize("extra", [1, 300])
+def test_many_ragged_chunks(ctx, batch, lengths, most, extra):
+    rng = np.random.default_rng(batch)
+    lengths = [int(l) for l in rng.integers(*lengths, batch)]
+    new = [min(l, int(rng.integers(0, most + 1))) for l in lengths]
+    new[batch // 2], lengths[batch // 2] = 300, 310  # one prompt among them
+    paged.check_attention(Case8(ctx, batch, "bf16", new, lengths, 4, 1, 64, 16, first_row=5, extra_entries=extra))
+
+
 @pytest.mark.parametrize("dtype", ["f16", "bf16"])
 @pytest.mark.parametrize("heads,kv_heads,d", [(16, 8, 128), (12, 12, 64), (15, 1, 128), (8, 4, 64)])
 @pytest.mark.parametrize("positions,new", [(256, [1] * 9), (512, [1, 0, 1, 1]), (512, [8, 3, 1, 15, 0, 2]), (528, [1, 2, 1]), (1024, [1, 1])])
