@@ -672,9 +672,9 @@ __global__ __launch_bounds__(kT, kLarge.workers / 256) void paged8_large_whole_k
 // ---- the entry points ---------------------------------------------------------------
 
 // Where tiles see few positions they are not cut: to plan the pieces takes 4 us, and the
-// merge, a launch that reads all parts, 4 to 50. Up to 16 units (1,024 positions, of 16-row
-// tiles at head_dim 64 2,048) always, up to 32 where there are tiles for every CU, so that
-// a long one matters less. Cut and not, us a call:
+// merge, a launch that reads all parts, 4 to 50. Up to 18 units (tables of 1,024 positions
+// and some pages more, of 16-row tiles at head_dim 64 of 2,048) always, up to 34 where there
+// are tiles for every CU, so that a long one matters less. Cut and not, us a call:
 // - a token each, 16-row tiles: 1 sequence of 8 KV heads of 128 over 128 positions 13.1 and
 //   5.6, 512 13.3 and 8.5, 1,024 13.7 and 12.5, 2,048 13.7 and 19.1; 48 of them over up to
 //   256 22.1 and 10.5, 1,024 30.6 and 23.0, 2,048 42.1 and 37.4, 4,096 69.6 and 68.9; 64 of
@@ -693,7 +693,7 @@ void launch8(hipStream_t st, const Attn8Args &a) {
   const bool small = a.tile_rows == kSmall.rows;
   const long long seen = p.window > 0 ? std::min((long long)p.sinks + p.window, (long long)p.capacity) : p.capacity;
   const long long tiles = (long long)std::max(p.batch, p.tokens / p.per_tile) * p.kv_heads;
-  if ((small || p.batch <= kMaxWholeBatch) && seen <= (tiles >= 256 ? 32 : 16) * p.unit) {
+  if ((small || p.batch <= kMaxWholeBatch) && seen <= (tiles >= 256 ? 34 : 18) * p.unit) {
     if (small) {
       paged8_small_whole_kernel<T, kD><<<dim3(p.kv_heads, std::min(p.batch, 32768)), kT, 0, st>>>(a);
     } else {

@@ -414,10 +414,11 @@ def test_many_ragged_chunks(ctx, batch, lengths, most, extra):
 
 @pytest.mark.parametrize("dtype", ["f16", "bf16"])
 @pytest.mark.parametrize("heads,kv_heads,d", [(16, 8, 128), (12, 12, 64), (15, 1, 128), (8, 4, 64)])
-@pytest.mark.parametrize("positions,new", [(256, [1] * 9), (512, [1, 0, 1, 1]), (512, [8, 3, 1, 15, 0, 2]), (528, [1, 2, 1]), (1024, [1, 1])])
+@pytest.mark.parametrize("positions,new", [(256, [1] * 9), (512, [1, 0, 1, 1]), (512, [8, 3, 1, 15, 0, 2]), (528, [1, 2, 1]), (1024, [1, 1]),
+                                           (1152, [1, 40]), (1168, [40, 1]), (2304, [1, 3])])
 @pytest.mark.parametrize("window,sinks", [(0, 0), (50, 3)])
 def test_short_caches(ctx, dtype, heads, kv_heads, d, positions, new, window, sinks):
-    # tables of up to 512 positions at head_dim 128 and 1,024 at 64, and longer ones
+    # tables of up to 1,152 positions (16-row tiles at head_dim 64: 2,304), and longer ones
     rng = np.random.default_rng(positions + heads)
     lengths = [int(rng.integers(max(n, 1), positions - 15)) for n in new]
     lengths[0] = positions - 16  # (a Case's tables have a page more)
