@@ -22,7 +22,8 @@ constexpr int kT = 256;
 // ---- quantisation and layout ---------------------------------------------------------
 
 // A thread a group: the smallest scale 2^e, e >= -127, for which its largest value is at
-// most 6 * 2^e = 1.5 * 2^(e + 2), each value to the nearest (half way: the even one).
+// most 6 * 2^e = 1.5 * 2^(e + 2), each value to the nearest (half way: the even one). Bound
+// by the bytes: 151,936 x 1,024 125 us (705 MB, 5.6 TB/s).
 __global__ __launch_bounds__(kT) void quantize_e2m1_kernel(const float *__restrict__ W, size_t groups, uint8_t *q,
                                                            uint8_t *scales) {
   const size_t g = (size_t)blockIdx.x * kT + threadIdx.x;
@@ -61,15 +62,21 @@ __global__ __launch_bounds__(kT) void quantize_e2m1_kernel(const float *__restri
 // Scales 2^e with which every weight but 0 (0.5 to 6 times it) is a normal number.
 constexpr int kF16Least = 127 - 13, kF16Most = 127 + 13, kBf16Least = 127 - 125, kBf16Most = 127 + 125;
 
-// A wave takes 16 rows. A group of zeros gets the scale 1, whatever its own.
-__global__ __launch_bounds__(64) void pack_e2m1_kernel(const uint8_t *__restrict__ q, const uint8_t *__restrict__ scales,
+constexpr int kPackT = 1024;
+
+// A workgroup takes 16 rows, its waves their tiles in turn. A group of zeros gets the scale 1,
+// whatever its own. (12,289 x 8,160 34 us, 4,096 x 4,096 11; a wave for 16 rows 122 and 36.)
+__global__ __launch_bounds__(kPackT) void pack_e2m1_kernel(const uint8_t *__restrict__ q, const uint8_t *__restrict__ scales,
                                                        int N, int K, int col_tiles, uint8_t *w, uint32_t *tile_scales,
                                                        uint32_t *tile_flags) {
-  const int lane = threadIdx.x, r16 = lane & 15, grp = lane >> 4;
+  __shared__ uint32_t row_flags;
+  const int lane = threadIdx.x & 63, r16 = lane & 15, grp = lane >> 4, waves = blockDim.x >> 6;
   const size_t tile = blockIdx.x, row = tile * 16 + r16;
+  if (threadIdx.x == 0) row_flags = 0;
+  __syncthreads();
   const bool there = row < (size_t)N;
   bool nan = false, no_f16 = false, no_bf16 = false;
-  for (size_t t = 0; t < (size_t)col_tiles; t++) {
+  for (size_t t = threadIdx.x >> 6; t < (size_t)col_tiles; t += waves) {
     u32x4 code = {0, 0, 0, 0};
     uint32_t scale = 0;
 #pragma unroll
@@ -99,7 +106,9 @@ __global__ __launch_bounds__(64) void pack_e2m1_kernel(const uint8_t *__restrict
   }
   const uint32_t nans = (uint32_t)__ballot(nan) & 0xffffu;
   const uint32_t flags = nans | (__any(no_f16) ? 1u << 16 : 0) | (__any(no_bf16) ? 1u << 17 : 0);
-  if (lane == 0) tile_flags[tile] = flags;
+  if (lane == 0 && flags != 0) atomicOr(&row_flags, flags);
+  __syncthreads();
+  if (threadIdx.x == 0) tile_flags[tile] = row_flags;
 }
 
 // ---- the products ----------------------------------------------------------------------
@@ -564,7 +573,9 @@ SH_API int sh_pack_e2m1_tiles(sh_ctx *ctx, const uint8_t *q, const uint8_t *scal
     return fail(SH_ERR_INVALID_ARGUMENT, "q must be 4-byte and tiled 16-byte aligned");
   if (ranges_overlap(tiled, at.bytes(), q, groups * 16) || ranges_overlap(tiled, at.bytes(), scales, groups))
     return fail(SH_ERR_INVALID_ARGUMENT, "tiled overlaps q or scales");
-  pack_e2m1_kernel<<<(unsigned)at.row_tiles, 64, 0, stream_of(ctx)>>>(
+  // (a launch takes fewer than 2^32 threads)
+  const int waves = (int)std::min<size_t>(std::min<size_t>(at.col_tiles, kPackT / 64), ((size_t)1 << 25) / at.row_tiles);
+  pack_e2m1_kernel<<<(unsigned)at.row_tiles, 64 * waves, 0, stream_of(ctx)>>>(
       q, scales, N, K, (int)at.col_tiles, tiled, reinterpret_cast<uint32_t *>(tiled + at.scales_at()),
       reinterpret_cast<uint32_t *>(tiled + at.flags_at()));
   const hipError_t e = hipGetLastError();
