@@ -355,6 +355,16 @@ def test_one_long_sequence_among_short_ones(ctx):
     paged.check_attention(Case8(ctx, 15, "bf16", [1] * 9, [30000] + [5] * 8, 8, 1, 128, 64))
 
 
+@pytest.mark.parametrize("batch", [63, 64, 65, 4095, 4096, 4097])
+def test_batches_of_chunks(ctx, batch):
+    # (those of more than 4,096 sequences are cut)
+    rng = np.random.default_rng(batch)
+    lengths = [int(l) for l in rng.integers(0, 6, batch)]
+    new = [min(l, int(rng.integers(0, 4))) for l in lengths]
+    lengths[0], new[0], lengths[-1], new[-1] = 40, 37, 70, 66
+    paged.check_attention(Case8(ctx, batch, "f16", new, lengths, 4, 1, 64, 16), max_new=66)
+
+
 # Tables of 300 pages more than are used: sequences that could be long, whose tiles are cut.
 WIDE = dict(page=16, extra_entries=300)
 

@@ -184,10 +184,11 @@ def test_a_server(ctx, dtype, heads, kv_heads, d, page):
     m.dispose()
 
 
-def test_captured_steps(hip):
+@pytest.mark.parametrize("max_pages", [20, 300])  # (tiles of the second are cut)
+def test_captured_steps(hip, max_pages):
     # replays with other values, eager steps of another model in between, two graphs of one work buffer
     with strict_amd.Context(0) as ctx:
-        make = lambda seed, new: (Model(ctx, seed, "f16", 4, 2, 64, 700, 40, rows=3, max_pages=20, num_pages=70, page_size=16), new)  # noqa: E731
+        make = lambda seed, new: (Model(ctx, seed, "f16", 4, 2, 64, 700, 40, rows=3, max_pages=max_pages, num_pages=70, page_size=16), new)  # noqa: E731
         models = [make(3, {0: 1, 1: 1, 2: 1}), make(4, {0: 30, 2: 5})]
         for m, new in models:
             m.cache.step({0: 20, 1: 13, 2: 7})
@@ -277,10 +278,12 @@ def test_long_chunks_with_windows_and_bad_pages(ctx, heads, kv_heads, d, window,
     paged.check_attention(c, max_new=LONG)
 
 
-@pytest.mark.parametrize("new", [[1, 1, 1], [40, 200, 9]])
-def test_starts_and_lengths_that_are_not_theirs(ctx, new):
+@pytest.mark.parametrize("extra", [1, 300])
+@pytest.mark.parametrize("new", [[1, 1, 1], [40, 200, 9], [3] * 130, [40] * 70])
+def test_starts_and_lengths_that_are_not_theirs(ctx, new, extra):
     # whatever the device holds there, only rows of the results and pages of the cache are written
-    c = paged8.Case8(ctx, 31, "f16", new, [300, 300, 300], 4, 2, 64, 16, rows_behind=3)
+    n = len(new)
+    c = paged8.Case8(ctx, 31, "f16", new, [300] * n, 4, 2, 64, 16, rows_behind=3, extra_entries=extra)
     c.upload()
     nbytes, pool = c.tokens * 4 * 64 * 2, c.buffers[0].nbytes
     guarded, pages = ctx.alloc(3 * nbytes), ctx.alloc(pool + 2048)
@@ -293,8 +296,8 @@ def test_starts_and_lengths_that_are_not_theirs(ctx, new):
     rng = np.random.default_rng(32)
     ends = np.array([0, 1, -1, c.tokens, c.tokens + 1, 7, np.iinfo(np.int32).max, np.iinfo(np.int32).min], np.int64)
     for _ in range(20):
-        c.buffers[2].copy_from_host(rng.choice(np.append(ends, 300), 3).astype(np.int32))
-        c.buffers[3].copy_from_host(rng.choice(ends, 4).astype(np.int32))
+        c.buffers[2].copy_from_host(rng.choice(np.append(ends, 300), n).astype(np.int32))
+        c.buffers[3].copy_from_host(rng.choice(ends, n + 1).astype(np.int32))
         ctx.memset(guarded, 0x5a)
         ctx.memset(pages, 0x5a)
         pages.view(1024, pool).copy_from_host(c.bytes())
