@@ -337,21 +337,34 @@ __global__ __launch_bounds__(kT, kSmall.workers / 256) void paged8_small_whole_k
 // 638.)
 constexpr float kSlack = 8.0f;
 
-template <int kD>
+//
+// kHalves 2: eight waves, four for the first half of the units and four for the others,
+// whose sums are joined in LDS at the end.
+template <int kD, int kHalves>
 struct LargeLds8 {
-  uint8_t k[2][kLargeUnit * kD * 2], v[2][kLargeUnit * kD * 2];
-  __attribute__((aligned(16))) unsigned bad[2][4];  // a 16-position block without a page
+  union {
+    struct {
+      uint8_t k[2 * kHalves][kLargeUnit * kD * 2], v[2 * kHalves][kLargeUnit * kD * 2];
+    };
+    f32x4 acc[4][kD / 8][64];  // of the other half: [wave][four sums][lane]
+  };
+  __attribute__((aligned(16))) unsigned bad[2 * kHalves][4];  // a 16-position block without a page
+  float stat[4][2][64];
 };
 
-template <class T, int kD>
-__device__ __forceinline__ bool attn_large8(const Attn8Args &a, const PagedTile &t, const TileSpan &s, int u0,
-                                           int u1, int slot, LargeLds8<kD> &lds) {
+template <class T, int kD, int kHalves>
+__device__ __forceinline__ bool attn_large8(const Attn8Args &a, const PagedTile &t, const TileSpan &s, int first,
+                                           int end, int slot, LargeLds8<kD, kHalves> &lds) {
   typedef typename T::Vec Vec;
   typedef typename T::Value Value;
   typedef Value Quad __attribute__((ext_vector_type(4)));
   constexpr int kRow = kD * 2, kChunks = kD / 16, kKK = kD / 16, kDB = kD / 32;
   constexpr int kLoadRows = 64 / kChunks, kLoads = 16 / kLoadRows;  // of a wave's 16 positions
-  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int lane = threadIdx.x & 63, half = kHalves == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x >> 8);
+  const int wave = __builtin_amdgcn_readfirstlane((threadIdx.x >> 6) & 3);
+  const int middle = kHalves == 1 ? end : first + (end - first + 1) / 2;
+  const int u0 = half == 0 ? first : middle, u1 = half == 0 ? middle : end;
+  const auto buffer = [&](int j) { return 2 * half + (j & 1); };
   const int n32 = lane & 31, h = lane >> 5, rows = s.count * a.group;
   const bool active = 32 * wave < rows;  // (of the wave)
   const int row = min(32 * wave + n32, rows - 1), my_pos = s.pos0 + token_of(a, row);
@@ -395,23 +408,23 @@ __device__ __forceinline__ bool attn_large8(const Attn8Args &a, const PagedTile 
       vs[u] = scales[a.v_scale_at + u * kLoadRows + load_row];
     }
   };
-  // load u of what was requested for unit j to buffer j & 1; what no row sees is zeros
+  // load u of what was requested for unit j to its buffer; what no row sees is zeros
   // in V (of K, such scores are masked)
   auto keep_k = [&](int j, int u) __attribute__((always_inline)) {
     const int r = u * kLoadRows + load_row, at = wave * kWave + r * kRow + (((2 * load_chunk) ^ swz_k(r)) * 16);
     const float scale = e8m0_scale(ks[u]);
-    *reinterpret_cast<u32x4 *>(lds.k[j & 1] + at) = from_e4m3<T>(kr[u].x, kr[u].y, scale);
-    *reinterpret_cast<u32x4 *>(lds.k[j & 1] + (at ^ 16)) = from_e4m3<T>(kr[u].z, kr[u].w, scale);
+    *reinterpret_cast<u32x4 *>(lds.k[buffer(j)] + at) = from_e4m3<T>(kr[u].x, kr[u].y, scale);
+    *reinterpret_cast<u32x4 *>(lds.k[buffer(j)] + (at ^ 16)) = from_e4m3<T>(kr[u].z, kr[u].w, scale);
   };
   auto keep_v = [&](int j, int u) __attribute__((always_inline)) {
     const int r = u * kLoadRows + load_row, at = wave * kWave + r * kRow + (((2 * load_chunk) ^ swz_v(r)) * 16);
     const float scale = e8m0_scale(vs[u]);
-    *reinterpret_cast<u32x4 *>(lds.v[j & 1] + at) = from_e4m3<T>(vr[u].x, vr[u].y, scale);
-    *reinterpret_cast<u32x4 *>(lds.v[j & 1] + (at ^ 16)) = from_e4m3<T>(vr[u].z, vr[u].w, scale);
+    *reinterpret_cast<u32x4 *>(lds.v[buffer(j)] + at) = from_e4m3<T>(vr[u].x, vr[u].y, scale);
+    *reinterpret_cast<u32x4 *>(lds.v[buffer(j)] + (at ^ 16)) = from_e4m3<T>(vr[u].z, vr[u].w, scale);
   };
   auto blank = [&](int j) __attribute__((always_inline)) {
     const int p = span_position(s, kLargeUnit, j) + 16 * wave;
-    if (lane == 0) lds.bad[j & 1][wave] = none ? 1 : 0;
+    if (lane == 0) lds.bad[buffer(j)][wave] = none ? 1 : 0;
     if (none || p + 16 > s.hi || (a.plan.window > 0 && p < s.lo && p + 16 > s.sinks)) {
 #pragma unroll
       for (int u = 0; u < kLoads; u++) {
@@ -459,7 +472,7 @@ __device__ __forceinline__ bool attn_large8(const Attn8Args &a, const PagedTile 
     }
   }
   for (int j = active ? u0 : u1; j < u1; j++) {
-    const int p0 = span_position(s, kLargeUnit, j), buf = j & 1, next = min(j + 1, u1 - 1);
+    const int p0 = span_position(s, kLargeUnit, j), buf = buffer(j), next = min(j + 1, u1 - 1);
     lds_barrier();
     if (j + 1 < u1) blank(next);
     // Fragments are requested ahead of the products that take them (the compiler left
@@ -562,8 +575,36 @@ __device__ __forceinline__ bool attn_large8(const Attn8Args &a, const PagedTile 
       }
   }
   l_run += __shfl_xor(l_run, 32, 64);
+  if constexpr (kHalves == 2) {
+    if (u1 - u0 < middle - first) lds_barrier();  // (the others had a unit more)
+    lds_barrier();  // K and V are read
+    if (half == 1 && active) {
+#pragma unroll
+      for (int db = 0; db < kDB; db++)
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+          lds.acc[wave][4 * db + i][lane] = f32x4{acc[db][4 * i], acc[db][4 * i + 1], acc[db][4 * i + 2], acc[db][4 * i + 3]};
+      lds.stat[wave][0][lane] = m_run;
+      lds.stat[wave][1][lane] = l_run;
+    }
+    lds_barrier();
+    if (half == 0 && active) {
+      const float other_m = lds.stat[wave][0][lane], other_l = lds.stat[wave][1][lane], m = fmaxf(m_run, other_m);
+      const float mine = m_run == m ? 1.0f : exp2_weight(m_run - m), other = other_m == m ? 1.0f : exp2_weight(other_m - m);
+      m_run = m;
+      l_run = fmaf(other_l, other, l_run * mine);
+#pragma unroll
+      for (int db = 0; db < kDB; db++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+          const f32x4 x = lds.acc[wave][4 * db + i][lane];
+#pragma unroll
+          for (int e = 0; e < 4; e++) acc[db][4 * i + e] = fmaf(x[e], other, acc[db][4 * i + e] * mine);
+        }
+    }
+  }
   bool sound = true;
-  const bool there = 32 * wave + n32 < rows;
+  const bool there = half == 0 && 32 * wave + n32 < rows;
   if (there) sound = score_fits<T>(a, m_run) && l_run < INFINITY;
   const float inv = l_run == 0.0f ? 0.0f : 1.0f / l_run;
   uint16_t *op = a.out + head_row(a, t.seq.row0 + s.first, t.kv_head, row) * kD;
@@ -590,10 +631,10 @@ __device__ __forceinline__ bool attn_large8(const Attn8Args &a, const PagedTile 
 
 template <class T, int kD>
 __global__ __launch_bounds__(kT, kLarge.workers / 256) void paged8_large_kernel(const Attn8Args a) {
-  __shared__ __attribute__((aligned(16))) LargeLds8<kD> lds;
+  __shared__ __attribute__((aligned(16))) LargeLds8<kD, 1> lds;
   __shared__ PlanLds plan;
   work_piece<true, 32, kD / 32>(a, plan, [&](const PieceStep &st, Line) {
-    return attn_large8<T, kD>(a, st.tile, st.span, st.u0, st.u1, st.slot, lds);
+    return attn_large8<T, kD, 1>(a, st.tile, st.span, st.u0, st.u1, st.slot, lds);
   });
 }
 
@@ -660,9 +701,9 @@ __device__ __forceinline__ int find_tile(const PagedPlan &p, int at, int most, i
 // A call whose tiles are not cut: a workgroup a tile. (With places between the sequences that have no tile, so that no sums were
 // needed, 16 sequences of 256 new tokens took 67 us and not 49: which CU a workgroup goes to
 // is settled by its number, and some had two rounds.)
-template <class T, int kD>
-__global__ __launch_bounds__(kT, kLarge.workers / 256) void paged8_large_whole_kernel(const Attn8Args a, int most) {
-  __shared__ __attribute__((aligned(16))) LargeLds8<kD> lds;
+template <class T, int kD, int kHalves>
+__global__ __launch_bounds__(kHalves * kT, 2) void paged8_large_whole_kernel(const Attn8Args a, int most) {
+  __shared__ __attribute__((aligned(16))) LargeLds8<kD, kHalves> lds;
   for (int tile = blockIdx.y; tile < most; tile += gridDim.y) {
     int back = 0;
     const int b = uniform(find_tile(a.plan, tile, most, &back));
@@ -670,7 +711,7 @@ __global__ __launch_bounds__(kT, kLarge.workers / 256) void paged8_large_whole_k
     PagedTile t = whole_tile(a, b, blockIdx.x);
     t.tile = plan_tiles(a.plan, t.seq) - 1 - uniform(back);
     const TileSpan s = plan_span(a.plan, t);
-    if (!attn_large8<T, kD>(a, t, s, 0, s.units, -1, lds)) attn_exact<Pages8<T>, kD>(a, t, s);
+    if (!attn_large8<T, kD, kHalves>(a, t, s, 0, s.units, -1, lds)) attn_exact<Pages8<T>, kD>(a, t, s);
   }
 }
 
@@ -690,6 +731,11 @@ __global__ __launch_bounds__(kT, kLarge.workers / 256) void paged8_large_whole_k
 //   56, 16 times 256 after up to 768 88 and 51, 4 prompts of 2,048 149 and 106, 4 of 4,096 408
 //   and 322, but 40 times 64 after up to 4,032 122 and 145; 63 single tokens and a prompt of
 //   1,024 83 and 58.
+// Two halves of a workgroup share a 128-row tile's units where there can be no more tiles than
+// CUs and there are units enough for the join. One and two halves: 1 prompt of 1,024 of 12 KV
+// heads of 64 25.9 and 21.3, 4 of up to 633 19.9 and 17.9, 8 of 1,024 41.5 and 50.0; of 8 KV
+// heads of 128, 512 new tokens after 512 32.7 and 28.3, 1 prompt of 256 14.6 and 15.0, of 512
+// 20.7 and 19.6. (8 ragged prompts of up to 333 over 1,024, some 250 tiles of 64: 29 and 36.)
 // (Eight waves for a 16-row tile: as long, a CU reads no faster. Tiles not cut but on planned
 // pieces: 1 sequence over 128 7.1, 16 14.4, 8 prompts of 512 38.)
 template <class T, int kD>
@@ -703,7 +749,11 @@ void launch8(hipStream_t st, const Attn8Args &a) {
       paged8_small_whole_kernel<T, kD><<<dim3(p.kv_heads, std::min(p.batch, 32768)), kT, 0, st>>>(a);
     } else {
       const int most = p.batch + p.tokens / p.per_tile;
-      paged8_large_whole_kernel<T, kD><<<dim3(p.kv_heads, std::min(most, 32768)), kT, 0, st>>>(a, most);
+      const dim3 grid(p.kv_heads, std::min(most, 32768));
+      if ((long long)most * p.kv_heads <= 256 && seen > 4 * p.unit)
+        paged8_large_whole_kernel<T, kD, 2><<<grid, 2 * kT, 0, st>>>(a, most);
+      else
+        paged8_large_whole_kernel<T, kD, 1><<<grid, kT, 0, st>>>(a, most);
     }
     return;
   }

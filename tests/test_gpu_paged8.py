@@ -355,6 +355,16 @@ def test_one_long_sequence_among_short_ones(ctx):
     paged.check_attention(Case8(ctx, 15, "bf16", [1] * 9, [30000] + [5] * 8, 8, 1, 128, 64))
 
 
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("heads,kv_heads,d", [(8, 8, 128), (12, 12, 64)])
+@pytest.mark.parametrize("window,sinks", [(0, 0), (300, 5)])
+def test_tiles_for_every_cu(ctx, dtype, heads, kv_heads, d, window, sinks):
+    rng = np.random.default_rng(heads)
+    new = [int(n) for n in rng.integers(1, 140, 12)] + [18] * 22
+    lengths = [n + int(rng.integers(0, 520 - n)) for n in new]
+    paged.check_attention(Case8(ctx, d, dtype, new, lengths, heads, kv_heads, d, 32), window=window, sinks=sinks)
+
+
 @pytest.mark.parametrize("batch", [63, 64, 65, 4095, 4096, 4097])
 def test_batches_of_chunks(ctx, batch):
     # (those of more than 4,096 sequences are cut)
