@@ -267,7 +267,8 @@ __global__ __launch_bounds__(64 * (kR == 1 ? kMaxWaves : 8)) void gemv4_kernel(c
 // alone add 14 (the activations once for every workgroup, 117 MB from L2, beside 53 MB of
 // weights), LDS reads and products 16. With the kernel above (four tiles a wave) 31.5, 64
 // rows 44 against 34. (A wave for two tiles and half of the rows: 30.6; for four tiles and 16
-// rows, each weight converted three times: 36; LDS read a chunk ahead of the products: 33.)
+// rows, each weight converted three times: 36; LDS read a chunk ahead of the products: 33;
+// two, four or five chunks ahead and not three: within 4 %.)
 //
 // In LDS a row's 16 bytes c lie at c ^ (row % 16) of the row, so that 16 lanes that read
 // one place of 16 rows hit all banks.
