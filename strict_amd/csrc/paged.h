@@ -343,6 +343,12 @@ inline const char *check_rope_theta(const sh_paged_kv *kv, int tokens, float the
   return nullptr;
 }
 
+// RoPE's frequencies, theta^(-2i / head_dim) for i < head_dim / 2: a power each, as a product
+// of two powers is another value, and the angles of far positions then steps of fp32 off.
+inline void rope_frequencies(float theta, int head_dim, double *freq) {
+  for (int i = 0; i < head_dim / 2; i++) freq[i] = std::pow((double)theta, -2.0 * i / head_dim);
+}
+
 inline bool paged_dim_built(int head_dim) { return head_dim == 64 || head_dim == 128; }
 
 inline size_t paged_pool_bytes(const sh_paged_kv *kv) {

@@ -125,6 +125,29 @@ __device__ __forceinline__ void cos_sin64(double a, Real *c, Real *s) {
   *c = (Real)((k == 1 || k == 2) ? -cd : cd);
 }
 
+// A lane's part of a head, kD / 16 lanes wide: y = x / sqrt(mean x^2 + eps) * gain, rotated
+// by halves, with factor(e) the cosine and sine of pair e. Which products are fused is
+// written out, so that every operator that takes this gives the same bits: left to the
+// compiler, one value in 10^4 came out a step of fp16 off between two kernels. (The last
+// one's rounding to fp16 is that instruction's own, one rounding and not two: the Makefile
+// has these files compiled so that it is everywhere.)
+template <int kD, class Factor>
+__device__ __forceinline__ void head_norm_rope(float (&x1)[8], float (&x2)[8], const float *gain, float eps, Factor factor) {
+  float ss = 0.0f;
+#pragma unroll
+  for (int e = 0; e < 8; e++) ss = fmaf(x1[e], x1[e], fmaf(x2[e], x2[e], ss));
+#pragma unroll
+  for (int off = 1; off < kD / 16; off *= 2) ss += __shfl_xor(ss, off, 64);
+  const float inv = 1.0f / sqrtf(fmaf(ss, 1.0f / kD, eps));
+#pragma unroll
+  for (int e = 0; e < 8; e++) {
+    const float2 f = factor(e);
+    const float y1 = x1[e] * inv * gain[e], y2 = x2[e] * inv * gain[e + kD / 2];
+    x1[e] = fmaf(y1, f.x, -(y2 * f.y));
+    x2[e] = fmaf(y2, f.x, y1 * f.y);
+  }
+}
+
 // The sequence that row `row` belongs to: the last b with starts[b] <= row (b =
 // batch: behind the last, -1: before the first). A wave looks at 64 values at a
 // time; batches of up to 63 take one round.

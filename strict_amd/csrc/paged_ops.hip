@@ -70,23 +70,12 @@ __global__ __launch_bounds__(kT) void norm_rope_kernel(const NormRopeArgs a) {
   for (int u = 0; u < kSteps; u++) {
     const int h = h0 + u * kHeadsAt + sub;
     const bool is_q = h < a.heads, is_k = !is_q && h < a.heads + a.kv_heads;
-    float x1[8], x2[8], ss = 0.0f;
-    unpack8<T>(lo[u], x1);
-    unpack8<T>(hi[u], x2);
-#pragma unroll
-    for (int e = 0; e < 8; e++) ss = fmaf(x1[e], x1[e], fmaf(x2[e], x2[e], ss));
-#pragma unroll
-    for (int off = 1; off < kLanes; off *= 2) ss += __shfl_xor(ss, off, 64);
-    const float inv = 1.0f / sqrtf(ss * (1.0f / kD) + a.eps);
-    const float *gain = (is_q ? a.q_gain : a.k_gain) + part * 8;
     u32x4 o1 = lo[u], o2 = hi[u];
     if (is_q || is_k) {
-#pragma unroll
-      for (int e = 0; e < 8; e++) {
-        const float y1 = x1[e] * inv * gain[e], y2 = x2[e] * inv * gain[e + kHalf];
-        x1[e] = y1 * f[e].x - y2 * f[e].y;
-        x2[e] = y2 * f[e].x + y1 * f[e].y;
-      }
+      float x1[8], x2[8];
+      unpack8<T>(lo[u], x1);
+      unpack8<T>(hi[u], x2);
+      head_norm_rope<kD>(x1, x2, (is_q ? a.q_gain : a.k_gain) + part * 8, a.eps, [&](int e) { return f[e]; });
       o1 = pack8<T>(x1);
       o2 = pack8<T>(x2);
     }
@@ -155,7 +144,7 @@ int norm_rope(sh_ctx *ctx, const sh_paged_kv *kv, const uint16_t *qkv, const flo
   a.kv_heads = kv->kv_heads;
   a.ld = ld;
   a.eps = eps;
-  for (int i = 0; i < d / 2; i++) a.freq[i] = std::pow((double)theta, -2.0 * i / d);
+  rope_frequencies(theta, d, a.freq);
   const int per_unit = 4 * (64 / (d / 16));
   a.chunks = (heads + 2 * kv->kv_heads + per_unit - 1) / per_unit;
   const long long units = (long long)tokens * a.chunks;

@@ -109,10 +109,10 @@ __device__ __forceinline__ V over_lanes(V v, Op op) {
 
 // A wave takes kSteps * kHeadsAt heads of one token: q heads, then k, then v. A head is
 // d / 16 lanes wide, 8 values of its first half and the 8 that rotate with them in each
-// lane, all loads requested at once. q's arithmetic is that of the 16-bit cache's
-// operator. k is normalised and rotated in fp64 (which has fp32's rate here) so that its
-// bytes do not depend on the order of sums: in fp32 one value in 10^6 comes out a step of
-// E4M3, 6 % of it, off. (Quantised in fp64 too, v as well, and with sums by LDS permutes:
+// lane, all loads requested at once. q is worked out as for the 16-bit cache, bit for bit. k
+// is normalised and rotated in fp64 (which has fp32's rate here) so that its bytes do not
+// depend on the order of sums: in fp32 one value in 10^6 comes out a step of E4M3, 6 % of
+// it, off. (Quantised in fp64 too, v as well, and with sums by LDS permutes:
 // 41 us for 9,312 tokens of 16 and 8 heads of 128 and not 28.5, 8.2 us for 3 and not 3.5.)
 // Bound by the bytes: those 9,312 are 172 MB, 6.0 TB/s. (Stores of pages that the caches
 // need not keep take as long, and reading the rows back 14.6 us and not 13.)
@@ -153,21 +153,10 @@ __global__ __launch_bounds__(kT) void norm_rope8_kernel(const NormRope8Args a) {
     unpack8<T>(lo[u], x1);
     unpack8<T>(hi[u], x2);
     if (h < a.heads) {
-      float ss = 0.0f;
-#pragma unroll
-      for (int e = 0; e < 8; e++) ss = fmaf(x1[e], x1[e], fmaf(x2[e], x2[e], ss));
-#pragma unroll
-      for (int off = 1; off < kLanes; off *= 2) ss += __shfl_xor(ss, off, 64);
-      const float inv = 1.0f / sqrtf(ss * (1.0f / kD) + a.eps);
-      const float *gain = a.q_gain + part * 8;
-#pragma unroll
-      for (int e = 0; e < 8; e++) {
+      head_norm_rope<kD>(x1, x2, a.q_gain + part * 8, a.eps, [&](int e) {
         const double2 f = factors[wave][part * 8 + e];
-        const float c = (float)f.x, s = (float)f.y;
-        const float y1 = x1[e] * inv * gain[e], y2 = x2[e] * inv * gain[e + kHalf];
-        x1[e] = y1 * c - y2 * s;
-        x2[e] = y2 * c + y1 * s;
-      }
+        return make_float2((float)f.x, (float)f.y);
+      });
       uint16_t *to = a.q + ((size_t)row * a.heads + h) * kD + part * 8;
       __builtin_nontemporal_store(pack8<T>(x1), reinterpret_cast<u32x4 *>(to));
       __builtin_nontemporal_store(pack8<T>(x2), reinterpret_cast<u32x4 *>(to + kHalf));
@@ -333,13 +322,7 @@ int norm_rope8(sh_ctx *ctx, const sh_paged_kv8 *kv, const uint16_t *qkv, const f
   a.kv_heads = kv->kv_heads;
   a.ld = ld;
   a.eps = eps;
-  // (a power for each took a third of the call's time on the host)
-  double eights[8];
-  for (int i = 0; i < d / 16; i++) eights[i] = std::pow((double)theta, -16.0 * i / d);
-  for (int j = 0; j < 8; j++) {
-    const double one = std::pow((double)theta, -2.0 * j / d);
-    for (int i = 0; i < d / 16; i++) a.freq[8 * i + j] = eights[i] * one;
-  }
+  rope_frequencies(theta, d, a.freq);
   if (d == 64)
     launch_norm_rope8<T, 64>(stream_of(ctx), a);
   else
