@@ -306,6 +306,74 @@ SH_HD PieceStep plan_step(const PagedPlan &p, const PagedTile &t, Line piece, in
   return r;
 }
 
+// ---- a workgroup a tile -------------------------------------------------------------
+//
+// Calls whose tiles are not cut: the tiles of all sequences are numbered through, and a
+// workgroup finds the one of its number by itself, a wave looking at 64 numbers at once.
+// W is that wave: each(f) and map(v, f) have f of each lane (and its value), scan the sums
+// of lanes 0 .. own, at most kMaxTiles, read the value of a lane, ballot the lanes whose
+// value f takes, nth the n-th of such lanes (on the device registers and lane moves; on the
+// host arrays, so that the search is checked there for any starts).
+constexpr int kMaxWholeBatch = 4096;
+constexpr int kMaxTiles = (1 << 30) - 1;  // (two such sums fit an int)
+
+SH_HD int plan_tiles_of(const PagedPlan &p, int b) {
+  const int from = clamp_int(p.starts[b], 0, p.tokens), end = clamp_int(p.starts[b + 1], from, p.tokens);
+  return (end - from + p.per_tile - 1) / p.per_tile;
+}
+
+// The sequence of tile `at` (0 or more), how many of its tiles come behind that, and how
+// many tiles there are in all; -1: fewer than that. The longest come first: of up to 64 sequences the
+// last tile of each, then the last but one, and so on; of more, up to kMaxWholeBatch,
+// sequence by sequence. (Sequences whose starts are out of order may have more tiles together
+// than all tokens make.)
+template <class W>
+SH_HD int find_tile(const PagedPlan &p, int at, int *back, int *total) {
+  typedef typename W::Int Int;
+  const int per = (p.batch + 63) / 64;
+  if (per == 1) {
+    const Int mine = W::each([&](int lane) { return lane < p.batch ? plan_tiles_of(p, lane) : 0; });
+    // tiles with fewer than n behind them
+    const auto behind = [&](int n) { return W::read(W::scan(W::map(mine, [&](int t) { return t < n ? t : n; })), 63); };
+    int n = 0, end = p.tokens / p.per_tile + 1;  // behind(n) <= at < behind(end): no sequence has more tiles than that
+    *total = behind(end);
+    if (*total <= at) return -1;
+    while (end - n > 1) {
+      const int mid = (n + end) / 2;
+      if (behind(mid) <= at)
+        n = mid;
+      else
+        end = mid;
+    }
+    *back = n;
+    const int which = at - behind(n);
+    return W::nth(W::ballot(mine, [&](int t) { return t > n; }), which);
+  }
+  int first = 0;
+  for (int step = per;; step = 1) {  // a 64th of the sequences in each lane, then one
+    const Int up_to = W::scan(W::each([&](int lane) {
+      int sum = 0;
+      for (int i = 0; i < step; i++) {
+        const int b = first + lane * step + i;
+        if (b < p.batch && (step == per || lane < per)) {
+          sum += plan_tiles_of(p, b);
+          sum = sum < kMaxTiles ? sum : kMaxTiles;
+        }
+      }
+      return sum;
+    }));
+    if (step == per) *total = W::read(up_to, 63);
+    const uint64_t before = W::ballot(up_to, [&](int t) { return t <= at; });
+    if (before == ~(uint64_t)0) return -1;
+    const int lane = __builtin_popcountll(before);  // (sums ascend)
+    at -= lane == 0 ? 0 : W::read(up_to, lane - 1);
+    first += lane * step;
+    if (step == 1) break;
+  }
+  *back = at;
+  return first;
+}
+
 // ---- argument checks that need no device -------------------------------------------
 
 // nullptr, or what is wrong with the cache's sizes.

@@ -638,75 +638,47 @@ __global__ __launch_bounds__(kT, kLarge.workers / 256) void paged8_large_kernel(
   });
 }
 
-// Sum of lanes 0 .. own, at most `most`, by lane moves as in wave_scan_line.
-__device__ __forceinline__ int scan_most(int v, int most) {
-  const auto add = [&](int moved) { v = min(v + moved, most); };
-  add(__builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false));
-  add(__builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false));
-  add(__builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false));
-  add(__builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false));
-  add(__builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false));
-  add(__builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false));
-  return v;
-}
-
-// The sequence of tile `at` of all sequences' tiles, fewer than `most`, and how many of its
-// tiles come behind that; -1: there is no such tile. The longest come first: of up to 64
-// sequences the last tile of each, then the last but one, and so on; of more, sequence by
-// sequence. A wave looks at 64 numbers at once.
-constexpr int kMaxWholeBatch = 4096;
-__device__ __forceinline__ int find_tile(const PagedPlan &p, int at, int most, int *back) {
-  const int lane = threadIdx.x & 63, per = (p.batch + 63) / 64;
-  const auto tiles = [&](int b) {
-    const int from = clamp_int(p.starts[b], 0, p.tokens), end = clamp_int(p.starts[b + 1], from, p.tokens);
-    return (end - from + p.per_tile - 1) / p.per_tile;
-  };
-  if (per == 1) {
-    const int mine = lane < p.batch ? tiles(lane) : 0;
-    // tiles with fewer than n behind them
-    const auto behind = [&](int n) { return __builtin_amdgcn_readlane(scan_most(min(mine, n), most), 63); };
-    int n = 0, end = most;  // behind(n) <= at < behind(end)
-    if (behind(end) <= at) return -1;
-    while (end - n > 1) {
-      const int mid = (n + end) / 2;
-      if (behind(mid) <= at)
-        n = mid;
-      else
-        end = mid;
-    }
-    *back = n;
-    const int which = at - behind(n);  // (with all lanes)
-    const uint64_t those = __ballot(mine > n);
+// find_tile's wave. Sums by lane moves as in wave_scan_line.
+struct DeviceWave {
+  typedef int Int;
+  template <class F>
+  static __device__ __forceinline__ Int each(F f) {
+    return f((int)(threadIdx.x & 63));
+  }
+  template <class F>
+  static __device__ __forceinline__ Int map(Int v, F f) {
+    return f(v);
+  }
+  static __device__ __forceinline__ Int scan(Int v) {
+    const auto add = [&](int moved) { v = min(v + moved, kMaxTiles); };
+    add(__builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false));
+    add(__builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false));
+    add(__builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false));
+    add(__builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false));
+    add(__builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false));
+    add(__builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false));
+    return v;
+  }
+  static __device__ __forceinline__ int read(Int v, int lane) { return __builtin_amdgcn_readlane(v, lane); }
+  template <class F>
+  static __device__ __forceinline__ uint64_t ballot(Int v, F f) {
+    return __ballot(f(v));
+  }
+  static __device__ __forceinline__ int nth(uint64_t those, int n) {
     const int rank = (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(those >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)those, 0));
-    return __builtin_ctzll(__ballot(mine > n && rank == which));
+    return __builtin_ctzll(__ballot((those >> (threadIdx.x & 63) & 1) != 0 && rank == n));
   }
-  int first = 0;
-  for (int step = per;; step = 1) {  // a 64th of the sequences in each lane, then one
-    int sum = 0;
-    for (int i = 0; i < step; i++) {
-      const int b = first + lane * step + i;
-      if (b < p.batch && (step == per || lane < per)) sum = min(sum + tiles(b), most);
-    }
-    const int up_to = scan_most(sum, most);
-    const int before = __popcll(__ballot(up_to <= at));
-    if (before == 64) return -1;
-    at -= before == 0 ? 0 : __builtin_amdgcn_readlane(up_to, before - 1);
-    first += before * step;
-    if (step == 1) break;
-  }
-  *back = at;
-  return first;
-}
+};
 
-// A call whose tiles are not cut: a workgroup a tile. (With places between the sequences that have no tile, so that no sums were
-// needed, 16 sequences of 256 new tokens took 67 us and not 49: which CU a workgroup goes to
-// is settled by its number, and some had two rounds.)
+// A call whose tiles are not cut: a workgroup a tile. (With places between the sequences that
+// have no tile, so that no sums were needed, 16 sequences of 256 new tokens took 67 us and not
+// 49: which CU a workgroup goes to is settled by its number, and some had two rounds.)
 template <class T, int kD, int kHalves>
-__global__ __launch_bounds__(kHalves * kT, 2) void paged8_large_whole_kernel(const Attn8Args a, int most) {
+__global__ __launch_bounds__(kHalves * kT, 2) void paged8_large_whole_kernel(const Attn8Args a) {
   __shared__ __attribute__((aligned(16))) LargeLds8<kD, kHalves> lds;
-  for (int tile = blockIdx.y; tile < most; tile += gridDim.y) {
+  for (int tile = blockIdx.y, total = tile + 1; tile < total; tile += gridDim.y) {
     int back = 0;
-    const int b = uniform(find_tile(a.plan, tile, most, &back));
+    const int b = uniform(find_tile<DeviceWave>(a.plan, tile, &back, &total));
     if (b < 0) return;
     PagedTile t = whole_tile(a, b, blockIdx.x);
     t.tile = plan_tiles(a.plan, t.seq) - 1 - uniform(back);
@@ -748,12 +720,12 @@ void launch8(hipStream_t st, const Attn8Args &a) {
     if (small) {
       paged8_small_whole_kernel<T, kD><<<dim3(p.kv_heads, std::min(p.batch, 32768)), kT, 0, st>>>(a);
     } else {
-      const int most = p.batch + p.tokens / p.per_tile;
+      const int most = p.batch + p.tokens / p.per_tile;  // tiles (of starts in order; any others are found too)
       const dim3 grid(p.kv_heads, std::min(most, 32768));
       if ((long long)most * p.kv_heads <= 256 && seen > 4 * p.unit)
-        paged8_large_whole_kernel<T, kD, 2><<<grid, 2 * kT, 0, st>>>(a, most);
+        paged8_large_whole_kernel<T, kD, 2><<<grid, 2 * kT, 0, st>>>(a);
       else
-        paged8_large_whole_kernel<T, kD, 1><<<grid, kT, 0, st>>>(a, most);
+        paged8_large_whole_kernel<T, kD, 1><<<grid, kT, 0, st>>>(a);
     }
     return;
   }
