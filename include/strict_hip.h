@@ -531,7 +531,7 @@ SH_API int sh_attn_decode_f16_noalloc(sh_ctx *ctx, const float *q, const uint16_
  * page_size + 512) at most 2^52, and a pool at most 2^62 bytes. */
 typedef struct sh_paged_kv {
   uint16_t *k, *v; /* [num_pages][kv_heads][page_size][head_dim], 16-byte aligned */
-  const int32_t *page_table; /* [batch][max_pages] */
+  const int32_t *page_table; /* [batch][max_pages], 4-byte aligned, as the next two */
   const int32_t *lengths;    /* [batch] */
   const int32_t *starts;     /* [batch + 1] */
   int batch, max_pages, num_pages, page_size, kv_heads, head_dim;
@@ -587,7 +587,7 @@ SH_API int sh_attn_paged_bf16(sh_ctx *ctx, const sh_paged_kv *kv, const uint16_t
  * 2^(scale - 127), of scale 255 for NaN. Sizes as above; sh_pages_copy copies such pages. */
 typedef struct sh_paged_kv8 {
   uint8_t *pages; /* [num_pages] of sh_paged8_page_bytes, 16-byte aligned */
-  const int32_t *page_table; /* [batch][max_pages] */
+  const int32_t *page_table; /* [batch][max_pages], 4-byte aligned, as the next two */
   const int32_t *lengths;    /* [batch] */
   const int32_t *starts;     /* [batch + 1] */
   int batch, max_pages, num_pages, page_size, kv_heads, head_dim;

@@ -164,13 +164,25 @@ __device__ __forceinline__ int find_seq(const int *__restrict__ starts, int batc
   }
 }
 
+// The page table, lengths and starts lie in the context's memory, and so that whole integers
+// are read: loads at places which a wave shares leave the address's last two bits out.
+inline int check_paged_index(sh_ctx *ctx, const sh_paged_kv *kv) {
+  int rc;
+  if ((rc = check_range(ctx, kv->page_table, (size_t)kv->batch * kv->max_pages * 4, "page_table")) ||
+      (rc = check_range(ctx, kv->lengths, (size_t)kv->batch * 4, "lengths")) ||
+      (rc = check_range(ctx, kv->starts, ((size_t)kv->batch + 1) * 4, "starts")))
+    return rc;
+  if ((reinterpret_cast<uintptr_t>(kv->page_table) | reinterpret_cast<uintptr_t>(kv->lengths) |
+       reinterpret_cast<uintptr_t>(kv->starts)) & 3)
+    return fail(SH_ERR_INVALID_ARGUMENT, "page_table, lengths and starts must be 4-byte aligned");
+  return SH_OK;
+}
+
 inline int check_paged_pointers(sh_ctx *ctx, const sh_paged_kv *kv) {
   int rc;
   const size_t pool = paged_pool_bytes(kv);
   if ((rc = check_range(ctx, kv->k, pool, "k pages")) || (rc = check_range(ctx, kv->v, pool, "v pages")) ||
-      (rc = check_range(ctx, kv->page_table, (size_t)kv->batch * kv->max_pages * 4, "page_table")) ||
-      (rc = check_range(ctx, kv->lengths, (size_t)kv->batch * 4, "lengths")) ||
-      (rc = check_range(ctx, kv->starts, ((size_t)kv->batch + 1) * 4, "starts")))
+      (rc = check_paged_index(ctx, kv)))
     return rc;
   if ((reinterpret_cast<uintptr_t>(kv->k) | reinterpret_cast<uintptr_t>(kv->v)) & 15)
     return fail(SH_ERR_INVALID_ARGUMENT, "k and v pages must be 16-byte aligned");
@@ -187,10 +199,8 @@ inline bool overlaps_index(const sh_paged_kv *kv, const void *p, size_t bytes) {
 
 inline int check_paged8_pointers(sh_ctx *ctx, const sh_paged_kv8 *kv) {
   int rc;
-  if ((rc = check_range(ctx, kv->pages, paged8_pool_bytes(kv), "pages")) ||
-      (rc = check_range(ctx, kv->page_table, (size_t)kv->batch * kv->max_pages * 4, "page_table")) ||
-      (rc = check_range(ctx, kv->lengths, (size_t)kv->batch * 4, "lengths")) ||
-      (rc = check_range(ctx, kv->starts, ((size_t)kv->batch + 1) * 4, "starts")))
+  const sh_paged_kv index = paged8_index(kv);
+  if ((rc = check_range(ctx, kv->pages, paged8_pool_bytes(kv), "pages")) || (rc = check_paged_index(ctx, &index)))
     return rc;
   if (reinterpret_cast<uintptr_t>(kv->pages) & 15)
     return fail(SH_ERR_INVALID_ARGUMENT, "pages must be 16-byte aligned");
