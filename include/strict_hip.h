@@ -633,8 +633,8 @@ SH_API int sh_attn_paged8_bf16(sh_ctx *ctx, const sh_paged_kv8 *kv, const uint16
 
 /* Pages src[i] to pages dst[i], i < count, in each of `planes` pools (the K and V
  * pools of every layer) at pool + p * plane_stride bytes, num_pages pages of
- * page_bytes each. src and dst are device int32; a pair with a number outside
- * 0 .. num_pages - 1 is skipped. A page may be the source of several; the dst
+ * page_bytes each. src and dst are device int32, 4-byte aligned; a pair with a number
+ * outside 0 .. num_pages - 1 is skipped. A page may be the source of several; the dst
  * pages are distinct and none of them a source of another. pool 16-byte aligned,
  * page_bytes and plane_stride multiples of 16, plane_stride >= num_pages *
  * page_bytes; src and dst do not lie in the pools. */
@@ -658,7 +658,7 @@ SH_API int sh_pages_copy(sh_ctx *ctx, void *pool, int planes, size_t plane_strid
  * of nothing else gives -1. Weights are 42-bit fractions of the largest, from
  * fp64 exponentials, and their sums exact: a token below 2^-43 of the likeliest
  * is not drawn, and results do not depend on any order. n <= 2^20, rows <= 2^16.
- * The work buffer (16-byte aligned) holds at least what
+ * The rows' parameters are 4-byte aligned. The work buffer (16-byte aligned) holds at least what
  * sh_sample_workspace says for the same sizes. It and index overlap nothing else of
  * the call. */
 SH_API int sh_sample_workspace(int rows, int n, size_t *bytes);

@@ -214,6 +214,8 @@ SH_API int sh_pages_copy(sh_ctx *ctx, void *pool, int planes, size_t plane_strid
       (rc = check_range(ctx, dst, (size_t)count * 4, "dst")))
     return rc;
   if (reinterpret_cast<uintptr_t>(pool) & 15) return fail(SH_ERR_INVALID_ARGUMENT, "pool must be 16-byte aligned");
+  if ((reinterpret_cast<uintptr_t>(src) | reinterpret_cast<uintptr_t>(dst)) & 3)  // (scalar loads)
+    return fail(SH_ERR_INVALID_ARGUMENT, "src and dst must be 4-byte aligned");
   if (ranges_overlap(pool, extent, src, (size_t)count * 4) || ranges_overlap(pool, extent, dst, (size_t)count * 4))
     return fail(SH_ERR_INVALID_ARGUMENT, "src or dst lies in the pools");
   const uint32_t vectors = (uint32_t)(page_bytes / 16);

@@ -923,6 +923,10 @@ SH_API int sh_sample_f32(sh_ctx *ctx, const float *x, int rows, int n, int ld, c
   if ((rc = check_range(ctx, workspace, need, "workspace"))) return rc;
   if (reinterpret_cast<uintptr_t>(workspace) & 15)
     return fail(SH_ERR_INVALID_ARGUMENT, "the work buffer must be 16-byte aligned");
+  // (a row's values by scalar loads, which leave the last two bits of an address out; NULL is aligned)
+  if ((reinterpret_cast<uintptr_t>(temperature) | reinterpret_cast<uintptr_t>(top_k) | reinterpret_cast<uintptr_t>(top_p) |
+       reinterpret_cast<uintptr_t>(min_p) | reinterpret_cast<uintptr_t>(u)) & 3)
+    return fail(SH_ERR_INVALID_ARGUMENT, "temperature, top_k, top_p, min_p and u must be 4-byte aligned");
   // what a call writes (rows that the list holds use no work buffer) lies over nothing that it reads
   const size_t x_bytes = ((size_t)(rows - 1) * ld + n) * 4;
   if (n > kList && ranges_overlap(workspace, need, x, x_bytes))

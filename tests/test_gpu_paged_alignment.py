@@ -1,4 +1,4 @@
-"""Calls of the paged operators whose 32-bit arrays do not lie at multiples of 4 bytes are
+"""Calls of the paged operators and of sampling whose 32-bit arrays do not lie at multiples of 4 bytes are
 refused: loads at places that a wave shares would read the integers at the multiple before."""
 import numpy as np
 import pytest
@@ -43,3 +43,30 @@ def test_index(ctx, bits, off):
     for b in (q, out, k, v, qkv, gain, work):
         b.free()
     c.free()
+
+
+@pytest.mark.parametrize("off", [1, 2, 3])
+def test_page_numbers(ctx, off):
+    pool, numbers, area = ctx.alloc(5 * 32), ctx.upload(np.zeros(3, np.int32)), ctx.alloc(32)
+    for src, dst in ((area.ptr + off, numbers), (numbers, area.ptr + off)):
+        refused(lambda: ctx.pages_copy(pool, 1, 5, 32, src, dst, 3), "4-byte aligned")
+    for b in (pool, numbers, area):
+        b.free()
+
+
+@pytest.mark.parametrize("off", [1, 2, 3])
+@pytest.mark.parametrize("n", [50, 5000])
+def test_sampling_parameters(ctx, off, n):
+    rows = 3
+    x, index, area = ctx.upload(np.zeros((rows, n), np.float32)), ctx.alloc(4 * rows), ctx.alloc(64)
+    own = {name: ctx.upload(np.zeros(rows, np.float32)) for name in ("temperature", "top_k", "top_p", "min_p", "u")}
+    work = ctx.alloc(ctx.sample_workspace(rows, n))
+    for name in own:
+        b = {**own, name: area.ptr + off}
+        refused(lambda: ctx.sample(x, rows, n, b["temperature"], b["top_k"], b["top_p"], b["min_p"], b["u"], index, work),
+                "4-byte aligned")
+    ctx.sample(x, rows, n, None, None, None, None, own["u"], index, work)
+    ctx.sync()
+    assert (index.to_host(np.int32, (rows,)) == 0).all()
+    for b in (x, index, area, work, *own.values()):
+        b.free()
