@@ -44,7 +44,7 @@ __global__ __launch_bounds__(kT) void quantize_e2m1_kernel(const float *__restri
   }
   const uint32_t bits = __builtin_bit_cast(uint32_t, most);
   const int e = max((int)(bits >> 23) - 127 - 2 + ((bits & 0x7fffff) > 0x400000 ? 1 : 0), -127);
-  const float to_group = __builtin_bit_cast(float, e == 127 ? 0x400000u : (uint32_t)(127 - e) << 23);  // 2^-e
+  const float to_group = __builtin_bit_cast(float, (uint32_t)(127 - e) << 23);  // 2^-e, e of -127 .. 126
   u32x4 code;
 #pragma unroll
   for (int i = 0; i < 4; i++) {
@@ -263,12 +263,16 @@ __global__ __launch_bounds__(64 * (kR == 1 ? kMaxWaves : 8)) void gemv4_kernel(c
 // for all rows of activations, so that each weight is converted once; the two steps' sums
 // are added up in LDS. Workgroups take groups of tiles in turn, their loads going on from
 // one group to the next.
-// 37 rows by 12,289 x 8,160: 28 us, of which 7 remain without loads and products; loads
-// alone add 14 (the activations once for every workgroup, 117 MB from L2, beside 53 MB of
-// weights), LDS reads and products 16. With the kernel above (four tiles a wave) 31.5, 64
-// rows 44 against 34. (A wave for two tiles and half of the rows: 30.6; for four tiles and 16
-// rows, each weight converted three times: 36; LDS read a chunk ahead of the products: 33;
-// two, four or five chunks ahead and not three: within 4 %.)
+// 37 rows by 12,289 x 8,160: 26 us a call. The kernel alone took 28 when it was taken apart: 7
+// remained without loads and products, loads alone added 14 (the activations once for every
+// workgroup, 117 MB from L2, beside 53 MB of weights), LDS reads and products 16. With the
+// kernel above (four tiles a wave) 31.5, 64 rows 44 against 34. (A wave for two tiles and half
+// of the rows: 30.6; for four tiles and 16 rows, each weight converted three times: 36; LDS
+// read a chunk ahead of the products: 33; two or four chunks ahead and not three: within 4 %.)
+// From 17 rows on, as the kernel above takes no more than 16. Of few tiles of rows most CUs
+// have none, and a call takes what calls of 16 rows each would: 16, 17, 32 and 64 rows by
+// 4,096 x 4,096 (64 workgroups) 6.3, 11.7, 11.8 and 16.6 us, by 1,024 x 16,384 (16) 18.7, 38, 38
+// and 55; of many by 151,936 x 1,024 18.5, 31, 31 and 46.
 //
 // In LDS a row's 16 bytes c lie at c ^ (row % 16) of the row, so that 16 lanes that read
 // one place of 16 rows hit all banks.
