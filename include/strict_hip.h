@@ -596,7 +596,7 @@ typedef struct sh_paged_kv8 {
 /* Bytes of a page (a multiple of 32); only the sizes of `kv` are read. */
 SH_API int sh_paged8_page_bytes(const sh_paged_kv8 *kv, size_t *bytes);
 
-/* sh_qk_norm_rope_paged_* into such pages (the same q). A row of k or v is stored with
+/* sh_qk_norm_rope_paged_* into such pages (the same q, bit for bit). A row of k or v is stored with
  * the smallest scale 2^e, e >= -127, for which its largest value is at most 448 * 2^e,
  * each value rounded once, to the nearest E4M3 (half way: to the even one); k is worked
  * out in fp64 until then (to 2^-36 of its row's size, beyond position 2^15 to a step of its

@@ -332,9 +332,9 @@ __global__ __launch_bounds__(kT, kSmall.workers / 256) void paged8_small_whole_k
 // a unit go through its registers: requested a unit ahead, converted to 16 bits among the
 // next unit's products of scores (each value once, where fragments of bytes would be
 // converted by all four waves) and written to the other buffer. Bound by the products and the
-// softmax's vector work beside them: 8,192 tokens of 16 heads over 12,288 positions 627 us,
-// 880 TFLOP/s, with a merge of 16. (Units requested two ahead, or among other products: 629 to
-// 638.)
+// softmax's vector work beside them: 8,192 tokens of 16 heads over 12,288 positions take 627 to
+// 640 us at best, 860 to 880 TFLOP/s, and a merge of 16; a call 631 to 659 us, 834 to 871. (Units
+// requested two ahead, or among other products: 629 to 638 where this took 627 to 631.)
 constexpr float kSlack = 8.0f;
 
 //

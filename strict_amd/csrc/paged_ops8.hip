@@ -342,7 +342,8 @@ struct Read8Args {
 };
 
 // A wave takes 4 * kRowsAt of a token's 2 kv_heads rows, k first; a row is d / 16 lanes
-// wide. Bound by the bytes and its start: 9,312 tokens of 8 heads of 128 (57 MB) 13 us.
+// wide. 9,312 tokens of 8 heads of 128 (57 MB) take 13 us, 4.4 TB/s: of fewer rows than a wave
+// has places (there 16 of 32) the others' loads repeat the last row.
 template <class T, int kD>
 __global__ __launch_bounds__(kT) void read8_kernel(const Read8Args a) {
   constexpr int kLanes = kD / 16, kRowsAt = 64 / kLanes, kSteps = 4;
